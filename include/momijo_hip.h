@@ -511,6 +511,96 @@ int32_t mj_mlp_w8a16_h(const uint16_t *x, const int8_t *Wg, const float *sg,
                        const int8_t *Wu, const float *su, const int8_t *Wd, const float *sd,
                        uint16_t *h, uint16_t *y, int64_t M, int64_t K, int64_t I, int64_t H);
 
+/* ---- feed-forward block --------------------------------------------------
+ * Operators of a transformer's feed-forward block, forward and backward (no
+ * reference counterpart; Linear, the activations and the elementwise product
+ * compose them there).  Device pointers only.  Scratch memory is the caller's:
+ * these calls allocate nothing, take no library workspace and can be captured
+ * into a HIP graph. */
+#define MJ_F32 0
+#define MJ_BF16 1
+#define MJ_NORM_RMS 0
+#define MJ_NORM_LAYER 1
+
+/* Dropout with a mask from a counter-based generator, never stored:
+ *   y[e] = keep(e) ? x[e] * 65536 / (65536 - T) : 0
+ * T = round(65536 p), at least 1 for p > 0 and at most 65535 for p < 1.  Element
+ * e = 8 b + i is kept where 16-bit half i (low half of word i / 2 for even i) of
+ * Philox4x32-10 of counter words (b, b >> 32, counter, counter >> 32) with key
+ * `seed` is >= T.  A dropped element gives 0 whatever it holds; p = 1 drops all,
+ * p = 0 copies.  The backward pass is the same call on dy.  state (or NULL): a
+ * device array {seed, counter}, whose seed replaces `seed` and whose counter is
+ * added to `counter`, so a captured graph can draw a new mask each replay.  x and
+ * y may be the same array. */
+int32_t mj_dropout(int32_t dtype, const void *x, void *y, int64_t n, float p, uint64_t seed,
+                   uint64_t counter, const uint64_t *state, void *stream);
+
+/* The norms around a residual sum, rows of `dim` (at most 16384):
+ *   c = norm(b) wp + bp (c = b without wp)
+ *   y = scale x + dropout(gate c)
+ *   n = norm(y) wn + bn (computed from the unrounded y; with wn)
+ * norm(v) = v / sqrt(mean(v^2) + eps) (MJ_NORM_RMS) or (v - mean) / sqrt(var + eps)
+ * (MJ_NORM_LAYER), in fp32.  x, b, gate, y, n have element type dtype; scale, wp,
+ * bp, wn, bn are fp32 [dim].  Every operand but x may be NULL (b NULL: y = scale
+ * x); gate has gate_rows rows, each for rows / gate_rows rows of x.  y may be NULL.
+ * Dropout as mj_dropout over the [rows, dim] array.  stats (or NULL) takes what the
+ * backward needs: fp32 [4][rows]. */
+int32_t mj_residual_norm(int32_t dtype, int32_t norm, const void *x, const void *b,
+                         const void *gate, int64_t gate_rows, const float *scale, const float *wp,
+                         const float *bp, const float *wn, const float *bn, float eps, float p,
+                         uint64_t seed, uint64_t counter, const uint64_t *state, void *y, void *n,
+                         float *stats, int64_t rows, int64_t dim, void *stream);
+
+/* Bytes of `work` for mj_residual_norm_backward (gate_rows 0: no gate). */
+int64_t mj_residual_norm_work_bytes(int64_t rows, int64_t dim, int64_t gate_rows);
+
+/* Gradients of mj_residual_norm from dy, dn (either may be NULL) and the forward's
+ * arguments and stats.  dx, db, dgate have element type dtype; dscale, dwp, dbp,
+ * dwn, dbn are fp32 [dim]; any may be NULL.  Sums run in a fixed order: the same
+ * inputs give the same bits.  rows == 0 writes nothing. */
+int32_t mj_residual_norm_backward(int32_t dtype, int32_t norm, const void *x, const void *b,
+                                  const void *gate, int64_t gate_rows, const float *scale,
+                                  const float *wp, const float *bp, const float *wn, float p,
+                                  uint64_t seed, uint64_t counter, const uint64_t *state,
+                                  const float *stats, const void *dy, const void *dn, void *dx,
+                                  void *db, void *dgate, float *dscale, float *dwp, float *dbp,
+                                  float *dwn, float *dbn, int64_t rows, int64_t dim, void *work,
+                                  int64_t work_bytes, void *stream);
+
+/* Gated feed-forward block:
+ *   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
+ * x [M,K], Wg and Wu [I,K], Wd [H,I], h [M,I], y [M,H], all contiguous; act is
+ * MJ_EPI_NONE, RELU, GELU_TANH or SILU.
+ * bf16: K, I, H multiples of 8 (zero-pad other widths), 16-byte aligned arrays;
+ * h is rounded to bf16; g, u fp32 [M,I] are written for the backward, or both NULL;
+ * `work` as mj_gated_mlp_work_bytes says (NULL where that is 0).
+ * fp32: any widths; h, g, u are required. */
+int64_t mj_gated_mlp_work_bytes(int64_t M, int64_t K, int64_t I, int64_t H, int32_t backward);
+int32_t mj_gated_mlp_bf16(const uint16_t *x, const uint16_t *Wg, const uint16_t *Wu,
+                          const uint16_t *Wd, int32_t act, uint16_t *h, float *g, float *u,
+                          uint16_t *y, int64_t M, int64_t K, int64_t I, int64_t H, void *work,
+                          int64_t work_bytes, void *stream);
+int32_t mj_gated_mlp_f32(const float *x, const float *Wg, const float *Wu, const float *Wd,
+                         int32_t act, float *h, float *g, float *u, float *y, int64_t M, int64_t K,
+                         int64_t I, int64_t H, void *stream);
+
+/* Gradients of the gated block from dy [M,H] and the forward's h, g, u:
+ *   dh = dy Wd, dg = dh u act'(g), du = dh act(g)
+ *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+ * dg, du [M,I] are scratch (bf16 in the bf16 form); any of dx, dWg, dWu, dWd may be
+ * NULL.  relu'(0) = 0. */
+int32_t mj_gated_mlp_backward_bf16(const uint16_t *x, const uint16_t *Wg, const uint16_t *Wu,
+                                   const uint16_t *Wd, int32_t act, const uint16_t *h,
+                                   const float *g, const float *u, const uint16_t *dy,
+                                   uint16_t *dg, uint16_t *du, uint16_t *dx, uint16_t *dWg,
+                                   uint16_t *dWu, uint16_t *dWd, int64_t M, int64_t K, int64_t I,
+                                   int64_t H, void *work, int64_t work_bytes, void *stream);
+int32_t mj_gated_mlp_backward_f32(const float *x, const float *Wg, const float *Wu, const float *Wd,
+                                  int32_t act, const float *h, const float *g, const float *u,
+                                  const float *dy, float *dg, float *du, float *dx, float *dWg,
+                                  float *dWu, float *dWd, int64_t M, int64_t K, int64_t I,
+                                  int64_t H, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,9 @@ from .tensor import (Tensor, empty_f32, empty_f64, gemm_bf16_nt, gpu_available, 
                      matmul_backward, tensordot)
 from .nn import (Conv2d, Linear, QuantLinear, ReLU, W8A8Linear, W8Linear, W8MLP, quantize_rowwise_int8,
                  quantize_rows_bf16_int8)
+from .block import (Dropout, GatedMLP, ResidualNorm, dropout, dropout_backward, gated_mlp,
+                    gated_mlp_backward, gated_mlp_train, residual_norm, residual_norm_backward,
+                    residual_norm_train)
 from . import autograd, seam, weights
 from .autograd import GradContext, GradTensor
 from .functional import (MinMaxObserver, convert, dequantize_i32_scaled, dequantize_i32_to_f32_add_bias,
@@ -28,6 +31,9 @@ __all__ = [
     "dequantize_i32_scaled",
     "MinMaxObserver", "prepare", "convert", "MomijoHipError", "seam", "weights",
     "autograd", "GradContext", "GradTensor",
+    "GatedMLP", "gated_mlp", "gated_mlp_train", "gated_mlp_backward",
+    "ResidualNorm", "residual_norm", "residual_norm_train", "residual_norm_backward",
+    "Dropout", "dropout", "dropout_backward",
     "EPI_NONE", "EPI_RELU", "EPI_GELU_TANH", "EPI_SILU", "EPI_GELU_TANH_APPROX",
     "EPI_SILU_APPROX", "EPI_RELU_UNARY", "ROUND_RHE", "ROUND_LEGACY",
 ]

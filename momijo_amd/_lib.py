@@ -17,6 +17,8 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "momijo_hip.h")
 MJ_OK, MJ_ERR_ARG, MJ_ERR_SHAPE, MJ_ERR_UNSUPPORTED, MJ_ERR_DEVICE, MJ_ERR_NO_DEVICE, MJ_ERR_ALLOC = range(7)
 EPI_NONE, EPI_RELU, EPI_GELU_TANH, EPI_SILU, EPI_GELU_TANH_APPROX, EPI_SILU_APPROX, EPI_RELU_UNARY = range(7)
 ROUND_RHE, ROUND_LEGACY = 0, 1
+F32, BF16 = 0, 1
+NORM_RMS, NORM_LAYER = 0, 1
 
 _STATUS_NAMES = {
     MJ_ERR_ARG: "invalid argument",
@@ -38,6 +40,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _F = ctypes.c_float
+_U64 = ctypes.c_uint64
 
 # name -> (restype, argtypes); kept in the order of the header
 SIGNATURES = {
@@ -114,6 +117,19 @@ SIGNATURES = {
     "mj_linear_w8a16_h": (_I32, [_P, _P, _P, _P, _I32, _P, _I64, _I64, _I64]),
     "mj_linear_w8a8_h": (_I32, [_P, _P, _P, _P, _I32, _P, _I64, _I64, _I64]),
     "mj_mlp_w8a16_h": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64]),
+    # the feed-forward block
+    "mj_dropout": (_I32, [_I32, _P, _P, _I64, _F, _U64, _U64, _P, _P]),
+    "mj_residual_norm": (_I32, [_I32, _I32, _P, _P, _P, _I64] + [_P] * 5 +
+                         [_F, _F, _U64, _U64] + [_P] * 4 + [_I64, _I64, _P]),
+    "mj_residual_norm_work_bytes": (_I64, [_I64, _I64, _I64]),
+    "mj_residual_norm_backward": (_I32, [_I32, _I32, _P, _P, _P, _I64] + [_P] * 4 +
+                                  [_F, _U64, _U64] + [_P] * 12 + [_I64, _I64, _P, _I64, _P]),
+    "mj_gated_mlp_work_bytes": (_I64, [_I64, _I64, _I64, _I64, _I32]),
+    "mj_gated_mlp_bf16": (_I32, [_P] * 4 + [_I32] + [_P] * 4 + [_I64] * 4 + [_P, _I64, _P]),
+    "mj_gated_mlp_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 4 + [_I64] * 4 + [_P]),
+    "mj_gated_mlp_backward_bf16": (_I32, [_P] * 4 + [_I32] + [_P] * 10 + [_I64] * 4 +
+                                   [_P, _I64, _P]),
+    "mj_gated_mlp_backward_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 10 + [_I64] * 4 + [_P]),
 }
 
 _lib = None

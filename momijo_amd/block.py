@@ -1,0 +1,438 @@
+"""The operators of a transformer's feed-forward block, forward and backward.
+
+``gated_mlp`` is the gated feed-forward layer, ``residual_norm`` the norms
+before and after a block around its residual sum with gate and dropout, and
+``dropout`` a dropout whose mask is drawn from a counter and never stored.
+Each has a ``_train`` form that also returns what its ``_backward`` needs (the
+dropout's backward needs its seed and counter only), and a class that keeps the
+parameters.
+
+Tensors are bfloat16 or Float32 on the current device; leading dimensions are
+rows.  Operands of other strides are copied to contiguous ones first.  The
+kernels run on the current stream, allocate through torch only and can be
+captured into a HIP graph.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .tensor import _ptr, _stream
+
+_DTYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+_NORMS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+_MASK64 = (1 << 64) - 1
+
+
+def _check_type(t: torch.Tensor, name: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on the GPU")
+    return code
+
+
+def _like(t: torch.Tensor, x: torch.Tensor, shape, name: str) -> torch.Tensor:
+    """t as a contiguous tensor of x's type and device and the given shape."""
+    if t.dtype != x.dtype or t.device != x.device:
+        raise TypeError(f"{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+# ------------------------------------------------------------------ dropout
+def _seed_args(seed, device):
+    """(seed, state) of a call: an integer, or a device int64 tensor {seed, counter}."""
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 2 or seed.device != device or \
+                not seed.is_contiguous():
+            raise ValueError("a seed tensor is a contiguous int64 tensor {seed, counter} on the "
+                             "operand's device")
+        return 0, seed
+    return int(seed) & _MASK64, None
+
+
+def dropout(x: torch.Tensor, p: float, seed, counter: int = 0,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x / (1 - p) where the element is kept, else 0.
+
+    The keep mask is a function of (seed, counter, flat element index) alone:
+    another counter gives an independent mask, the same one the same mask.  p
+    is rounded to a multiple of 2^-16 and the scale is exact for that.  ``seed``
+    is an integer or a device int64 tensor {seed, counter}, whose counter is
+    added (a captured graph draws a new mask when the tensor changes).
+    ``out`` may be x."""
+    code = _check_type(x, "x")
+    x = x if x.is_contiguous() else x.contiguous()
+    if out is None:
+        out = torch.empty_like(x)
+    elif out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous() or \
+            out.device != x.device:
+        raise ValueError(f"out must be a contiguous {x.dtype} {list(x.shape)} tensor")
+    s, state = _seed_args(seed, x.device)
+    _lib.call("mj_dropout", code, _ptr(x), _ptr(out), x.numel(), p, s, int(counter) & _MASK64,
+              _ptr(state), _stream())
+    return out
+
+
+def dropout_backward(dy: torch.Tensor, p: float, seed, counter: int = 0,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of ``dropout``'s x: the same mask and scale on dy."""
+    return dropout(dy, p, seed, counter, out)
+
+
+class Dropout:
+    """Dropout(p, seed): each training ``forward`` draws from the next counter;
+    ``backward`` takes the counter that its forward returned."""
+
+    def __init__(self, p: float, seed: int = 0):
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be in [0, 1], got {p}")
+        self.p, self.seed, self.counter = float(p), int(seed), 0
+        self.training = True
+
+    def forward(self, x: torch.Tensor) -> tuple[torch.Tensor, int | None]:
+        """(y, counter); in evaluation (x, None)."""
+        if not self.training or self.p == 0.0:
+            return x, None
+        c = self.counter
+        self.counter += 1
+        return dropout(x, self.p, self.seed, c), c
+
+    def backward(self, dy: torch.Tensor, counter: int | None) -> torch.Tensor:
+        return dy if counter is None else dropout_backward(dy, self.p, self.seed, counter)
+
+
+# ------------------------------------------------------------------ residual norm
+class ResidualNormSaved(NamedTuple):
+    """What residual_norm_backward needs: the operands and the rows' statistics."""
+    x: torch.Tensor
+    branch: torch.Tensor | None
+    gate: torch.Tensor | None
+    scale: torch.Tensor | None
+    post_weight: torch.Tensor | None
+    post_bias: torch.Tensor | None
+    next_weight: torch.Tensor | None
+    next_bias: torch.Tensor | None
+    norm: str
+    p: float
+    seed: int
+    state: torch.Tensor | None
+    counter: int
+    stats: torch.Tensor
+    gate_shape: tuple
+
+
+def _vector(t, x, dim, name):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.device != x.device or t.numel() != dim:
+        raise ValueError(f"{name} must be float32 with {dim} elements on {x.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight, next_bias, norm,
+                   eps, p, seed, counter, train):
+    code = _check_type(x, "x")
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    x = x if x.is_contiguous() else x.contiguous()
+    dim = x.shape[-1]
+    rows = x.numel() // dim if dim else 0
+    if branch is not None:
+        branch = _like(branch, x, x.shape, "branch")
+    gate_rows, gate_shape = 0, ()
+    if gate is not None:
+        gate_shape = tuple(gate.shape)
+        if gate.dim() not in (1, 2) or gate.shape[-1] != dim:
+            raise ValueError(f"gate must be [{dim}] or [groups, {dim}], got {list(gate.shape)}")
+        gate = _like(gate, x, gate.shape, "gate")
+        gate_rows = 1 if gate.dim() == 1 else gate.shape[0]
+    scale = _vector(scale, x, dim, "scale")
+    post_weight = _vector(post_weight, x, dim, "post_weight")
+    post_bias = _vector(post_bias, x, dim, "post_bias")
+    next_weight = _vector(next_weight, x, dim, "next_weight")
+    next_bias = _vector(next_bias, x, dim, "next_bias")
+    s, state = _seed_args(seed, x.device)
+    counter = int(counter) & _MASK64
+    # without a branch and a scale, y is x itself
+    y = x if branch is None and scale is None else torch.empty_like(x)
+    n = torch.empty_like(x) if next_weight is not None else None
+    stats = torch.empty((4, rows), dtype=torch.float32, device=x.device) if train else None
+    if y is not x or n is not None:
+        _lib.call("mj_residual_norm", code, _NORMS[norm], _ptr(x), _ptr(branch), _ptr(gate),
+                  gate_rows, _ptr(scale), _ptr(post_weight), _ptr(post_bias), _ptr(next_weight),
+                  _ptr(next_bias), eps, p, s, counter, _ptr(state), None if y is x else _ptr(y),
+                  _ptr(n), _ptr(stats), rows, dim, _stream())
+    if not train:
+        return y, n, None
+    return y, n, ResidualNormSaved(x, branch, gate, scale, post_weight, post_bias, next_weight,
+                                   next_bias, norm, p, s, state, counter, stats, gate_shape)
+
+
+def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *,
+                  gate: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                  post_weight: torch.Tensor | None = None, post_bias: torch.Tensor | None = None,
+                  next_weight: torch.Tensor | None = None, next_bias: torch.Tensor | None = None,
+                  norm: str = "rms", eps: float = 1e-6, p: float = 0.0, seed=0, counter: int = 0):
+    """(y, n): the norm after a block, its gate, dropout, the residual sum and
+    the norm before the next block, in one pass over the rows of the last
+    dimension:
+
+        y = scale * x + dropout(gate * (norm(branch) * post_weight + post_bias))
+        n = norm(y) * next_weight + next_bias
+
+    A norm is applied where its weight is given (n is None without next_weight);
+    gate and scale default to 1.  Without ``branch`` the call is the norm before
+    the first block: y = scale * x.  ``gate`` is [dim] or [groups, dim] with
+    consecutive rows of equal number in each group; x, branch and gate are of one
+    type, the vectors Float32."""
+    y, n, _ = _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight,
+                             next_bias, norm, eps, p, seed, counter, False)
+    return y, n
+
+
+def residual_norm_train(x: torch.Tensor, branch: torch.Tensor | None = None, *,
+                        gate: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                        post_weight: torch.Tensor | None = None,
+                        post_bias: torch.Tensor | None = None,
+                        next_weight: torch.Tensor | None = None,
+                        next_bias: torch.Tensor | None = None, norm: str = "rms",
+                        eps: float = 1e-6, p: float = 0.0, seed=0, counter: int = 0):
+    """(y, n, saved): residual_norm and what its backward needs.  The operands are
+    kept, not copied: they must not change before the backward."""
+    return _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight, next_bias,
+                          norm, eps, p, seed, counter, True)
+
+
+def residual_norm_backward(dy: torch.Tensor | None, dn: torch.Tensor | None,
+                           saved: ResidualNormSaved) -> dict[str, torch.Tensor]:
+    """The gradients of residual_norm's operands, by their names, from the
+    gradients of y and n (either may be None, for zero).  Those of x, branch and
+    gate have their type, those of the vectors are Float32."""
+    s = saved
+    x = s.x
+    dim, rows = x.shape[-1], s.stats.shape[1]
+    if dy is not None:
+        dy = _like(dy, x, x.shape, "dy")
+    if dn is not None:
+        if s.next_weight is None:
+            raise ValueError("dn given, but the forward had no next norm")
+        dn = _like(dn, x, x.shape, "dn")
+    out = {"x": torch.empty_like(x)}
+    if s.branch is not None:
+        out["branch"] = torch.empty_like(x)
+    if s.gate is not None:
+        out["gate"] = torch.empty_like(s.gate)
+    for name in ("scale", "post_weight", "post_bias", "next_weight", "next_bias"):
+        if getattr(s, name) is not None:
+            out[name] = torch.empty_like(getattr(s, name))
+    if rows == 0 or dim == 0 or (dy is None and dn is None):
+        return {k: v.zero_() for k, v in out.items()}
+    if dn is None:  # nothing reaches the next norm
+        for name in ("next_weight", "next_bias"):
+            if name in out:
+                out[name].zero_()
+    gate_rows = 0 if s.gate is None else s.gate.numel() // dim
+    nbytes = _lib.load().mj_residual_norm_work_bytes(rows, dim, gate_rows)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    at = lambda k: _ptr(out.get(k))  # noqa: E731
+    _lib.call("mj_residual_norm_backward", _DTYPES[x.dtype], _NORMS[s.norm], _ptr(x),
+              _ptr(s.branch), _ptr(s.gate), gate_rows, _ptr(s.scale), _ptr(s.post_weight),
+              _ptr(s.post_bias), _ptr(s.next_weight), s.p, s.seed, s.counter, _ptr(s.state),
+              _ptr(s.stats), _ptr(dy), _ptr(dn), at("x"), at("branch"), at("gate"), at("scale"),
+              at("post_weight"), at("post_bias"), None if dn is None else at("next_weight"),
+              None if dn is None else at("next_bias"), rows, dim, _ptr(work), nbytes, _stream())
+    return out
+
+
+class ResidualNorm:
+    """ResidualNorm(dim, norm, ...): the vectors of residual_norm as Float32
+    parameters (weights 1, biases 0) with its options."""
+
+    def __init__(self, dim: int, norm: str = "rms", *, post: bool = True, next: bool = True,
+                 bias: bool = False, scale: bool = False, eps: float = 1e-6, p: float = 0.0,
+                 seed: int = 0, device=None):
+        device = device or torch.device("cuda", torch.cuda.current_device())
+        ones = lambda on: torch.ones(dim, device=device) if on else None     # noqa: E731
+        zeros = lambda on: torch.zeros(dim, device=device) if on else None   # noqa: E731
+        self.dim, self.norm, self.eps, self.p, self.seed = dim, norm, eps, p, seed
+        self.scale = ones(scale)
+        self.post_weight, self.post_bias = ones(post), zeros(post and bias)
+        self.next_weight, self.next_bias = ones(next), zeros(next and bias)
+        self.counter = 0
+        self.training = True
+
+    def _kw(self, gate, p):
+        return dict(gate=gate, scale=self.scale, post_weight=self.post_weight,
+                    post_bias=self.post_bias, next_weight=self.next_weight,
+                    next_bias=self.next_bias, norm=self.norm, eps=self.eps, p=p, seed=self.seed)
+
+    def forward(self, x, branch, gate=None):
+        """(y, n) without dropout."""
+        return residual_norm(x, branch, **self._kw(gate, 0.0))
+
+    def forward_train(self, x, branch, gate=None):
+        """(y, n, saved); with dropout each call draws from the next counter."""
+        c = self.counter
+        if self.training and self.p > 0.0:
+            self.counter += 1
+        return residual_norm_train(x, branch, counter=c,
+                                   **self._kw(gate, self.p if self.training else 0.0))
+
+    backward = staticmethod(residual_norm_backward)
+
+
+# ------------------------------------------------------------------ gated MLP
+class GatedMLPSaved(NamedTuple):
+    """What gated_mlp_backward needs: the operands (bf16 of widths that are not
+    multiples of 8: their zero-padded copies), h and the fp32 projections g, u."""
+    x: torch.Tensor
+    gate: torch.Tensor
+    up: torch.Tensor
+    down: torch.Tensor
+    h: torch.Tensor
+    g: torch.Tensor
+    u: torch.Tensor
+    act: int
+    rows: tuple   # leading dimensions of x
+    widths: tuple  # K, I, H as given
+
+
+def _pad8(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """t zero-padded to [rows, cols], at a 16-byte aligned address."""
+    if t.shape == (rows, cols) and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    out = torch.empty((rows, cols), dtype=t.dtype, device=t.device)
+    r, c = t.shape
+    if r < rows:
+        out[r:].zero_()
+    if c < cols:
+        out[:r, c:].zero_()
+    out[:r, :c].copy_(t)
+    return out
+
+
+def _cut(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    return t if t.shape == (rows, cols) else t[:rows, :cols].contiguous()
+
+
+def _mlp_operands(x, gate, up, down, act):
+    """x as [M, K] and the weights, checked, contiguous and (bf16) padded."""
+    code = _check_type(x, "x")
+    if x.dim() < 1 or gate.dim() != 2 or down.dim() != 2:
+        raise ValueError("x must have a last dimension, and gate, up, down be 2-D")
+    K, (I, Kw), (H, Iw) = x.shape[-1], gate.shape, down.shape
+    if Kw != K or Iw != I:
+        raise ValueError(f"x has {K} features, gate is {list(gate.shape)}, down {list(down.shape)}")
+    gate = _like(gate, x, gate.shape, "gate")
+    up = _like(up, x, gate.shape, "up")
+    down = _like(down, x, down.shape, "down")
+    x2 = x.reshape(-1, K) if K else x.reshape(x.shape[:-1].numel(), 0)
+    x2 = x2 if x2.is_contiguous() else x2.contiguous()
+    if code == _lib.BF16:
+        Kp, Ip, Hp = K + 7 & ~7, I + 7 & ~7, H + 7 & ~7
+        x2 = _pad8(x2, x2.shape[0], Kp)
+        gate, up, down = _pad8(gate, Ip, Kp), _pad8(up, Ip, Kp), _pad8(down, Hp, Ip)
+    return code, x2, gate, up, down, (K, I, H)
+
+
+def _work(M, K, I, H, backward, device):
+    nbytes = _lib.load().mj_gated_mlp_work_bytes(M, K, I, H, backward)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
+
+
+def _gated_mlp(x, gate, up, down, act, train):
+    code, x2, gate, up, down, widths = _mlp_operands(x, gate, up, down, act)
+    M, K = x2.shape
+    H, I = down.shape
+    dev = x2.device
+    new = lambda cols, dt=x2.dtype: torch.empty((M, cols), dtype=dt, device=dev)  # noqa: E731
+    y, h = new(H), new(I)
+    if code == _lib.F32:
+        g, u = new(I), new(I)
+        _lib.call("mj_gated_mlp_f32", _ptr(x2), _ptr(gate), _ptr(up), _ptr(down), act, _ptr(h),
+                  _ptr(g), _ptr(u), _ptr(y), M, K, I, H, _stream())
+    else:
+        g, u = (new(I, torch.float32), new(I, torch.float32)) if train else (None, None)
+        work, nbytes = _work(M, K, I, H, 0, dev)
+        _lib.call("mj_gated_mlp_bf16", _ptr(x2), _ptr(gate), _ptr(up), _ptr(down), act, _ptr(h),
+                  _ptr(g), _ptr(u), _ptr(y), M, K, I, H, _ptr(work), nbytes, _stream())
+    y = _cut(y, M, widths[2])
+    if x.dim() != 2:
+        y = y.reshape(*x.shape[:-1], widths[2])
+    if not train:
+        return y, None
+    return y, GatedMLPSaved(x2, gate, up, down, h, g, u, act, tuple(x.shape[:-1]), widths)
+
+
+def gated_mlp(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
+              act: int = _lib.EPI_SILU) -> torch.Tensor:
+    """y = (act(x gate^T) * (x up^T)) down^T for x [..., K], gate and up [I, K],
+    down [H, I], all bfloat16 or all Float32; act is EPI_NONE, EPI_RELU,
+    EPI_GELU_TANH or EPI_SILU.  bfloat16 widths that are not multiples of 8 cost
+    zero-padded copies of the operands."""
+    return _gated_mlp(x, gate, up, down, act, False)[0]
+
+
+def gated_mlp_train(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
+                    act: int = _lib.EPI_SILU):
+    """(y, saved): gated_mlp and what its backward needs (h in x's type and the two
+    projections in Float32).  The operands are kept, not copied: they must not
+    change before the backward."""
+    return _gated_mlp(x, gate, up, down, act, True)
+
+
+def gated_mlp_backward(dy: torch.Tensor, saved: GatedMLPSaved):
+    """(dx, dgate, dup, ddown) of gated_mlp from the gradient of y."""
+    s = saved
+    K0, I0, H0 = s.widths
+    x, (M, K), (H, I) = s.x, s.x.shape, s.down.shape
+    dy = _like(dy, x, torch.Size((*s.rows, H0)), "dy").reshape(M, H0)
+    dev = x.device
+    new = lambda r, c: torch.empty((r, c), dtype=x.dtype, device=dev)  # noqa: E731
+    dg, du = new(M, I), new(M, I)
+    dx, dgate, dup, ddown = new(M, K), new(I, K), new(I, K), new(H, I)
+    args = [_ptr(t) for t in (x, s.gate, s.up, s.down)] + [s.act] + \
+        [_ptr(t) for t in (s.h, s.g, s.u)]
+    outs = [_ptr(t) for t in (dg, du, dx, dgate, dup, ddown)]
+    if x.dtype == torch.float32:
+        _lib.call("mj_gated_mlp_backward_f32", *args, _ptr(dy), *outs, M, K, I, H, _stream())
+    else:
+        dy = _pad8(dy, M, H)
+        work, nbytes = _work(M, K, I, H, 1, dev)
+        _lib.call("mj_gated_mlp_backward_bf16", *args, _ptr(dy), *outs, M, K, I, H, _ptr(work),
+                  nbytes, _stream())
+    return (_cut(dx, M, K0).reshape(*s.rows, K0), _cut(dgate, I0, K0), _cut(dup, I0, K0),
+            _cut(ddown, H0, I0))
+
+
+class GatedMLP:
+    """GatedMLP(gate, up, down, act): gated_mlp with its weights."""
+
+    def __init__(self, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
+                 act: int = _lib.EPI_SILU):
+        if gate.dim() != 2 or up.shape != gate.shape or down.dim() != 2 or \
+                down.shape[1] != gate.shape[0]:
+            raise ValueError(f"gate {list(gate.shape)}, up {list(up.shape)} and down "
+                             f"{list(down.shape)} do not fit each other")
+        self.gate, self.up, self.down, self.act = gate, up, down, act
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return gated_mlp(x, self.gate, self.up, self.down, self.act)
+
+    def forward_train(self, x: torch.Tensor):
+        return gated_mlp_train(x, self.gate, self.up, self.down, self.act)
+
+    backward = staticmethod(gated_mlp_backward)
+
+
+__all__ = ["dropout", "dropout_backward", "Dropout", "residual_norm", "residual_norm_train",
+           "residual_norm_backward", "ResidualNorm", "ResidualNormSaved", "gated_mlp",
+           "gated_mlp_train", "gated_mlp_backward", "GatedMLP", "GatedMLPSaved"]

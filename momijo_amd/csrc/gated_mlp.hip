@@ -1,0 +1,676 @@
+// Gated feed-forward block on gfx950 bf16 MFMA, forward and backward:
+//
+//   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
+//   dh = dy Wd, dg = dh u act'(g), du = dh act(g)
+//   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// Every product is one kernel family over tiles of C[m, n] = sum_k A(m, k) B(n, k):
+//  * each operand is either K-contiguous ([rows][k], as x and W in x W^T) or
+//    K-strided ([k][rows]: W in dy W, both operands of dg^T x), so no matrix is
+//    ever transposed in memory.  A K-contiguous stage lies in LDS as rows of 64 k;
+//    a K-strided one as 64 rows of k, whose fragments are read with
+//    ds_read_b64_tr_b16, which hands each lane four k of one column;
+//  * the gate and up projections share one tile: half its B rows are Wg's, half
+//    the same rows of Wu, so a lane holds g and u of the same outputs and writes h
+//    (and g, u in fp32 for the backward) without another pass;
+//  * dh never reaches memory: its tile's epilogue reads g and u and writes dg, du;
+//  * dx sums two products in one accumulator (two K segments), and the three weight
+//    gradients run as one launch.
+//
+// Roundings to bf16: h, dg, du (they feed the next product's matrix cores) and the
+// outputs; g and u are kept in fp32, so that act and act' see unrounded inputs and
+// every gradient carries one rounding of an operand and one of its own.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "common.h"
+#include "gemm_tile.h"
+#include "launch.h"
+
+namespace mj {
+
+typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 bf16x4;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+
+namespace {
+
+// What a tile's accumulators become.
+enum : int {
+  OUT_STORE = 0,  // C = bf16(acc)
+  OUT_PART,       // fp32 partial sums of a K slice
+  OUT_GATE,       // h = act(g) u, optionally g and u in fp32
+  OUT_DGATE,      // dg, du from dh = acc and the stored g, u
+};
+
+struct TileProb {
+  const uint16_t *A[2] = {nullptr, nullptr}, *B[2] = {nullptr, nullptr};  // K segments; gate/up: B[1] = Wu
+  int64_t lda = 0, ldb = 0;
+  int M = 0, N = 0, K = 0, segs = 1;  // K of one segment
+  int tiles_m = 0, tiles_n = 0, first = 0;
+  uint16_t *C = nullptr, *C2 = nullptr;  // C2: du
+  float *F = nullptr, *F2 = nullptr;     // g, u
+  float *part = nullptr;
+  int64_t ldc = 0;                       // of C, C2, F, F2
+};
+
+struct TileArgs {
+  TileProb p[3];
+  int n = 1, tiles = 0, splits = 1, act = 0;
+};
+
+// act(g) and act'(g) (1 + 1e-6 relative, as silu_b16: the results are rounded to bf16).
+// Where the sigmoid saturates its derivative's term is 0, not 0 x overflow.
+__device__ __forceinline__ float act_b16(int act, float g) { return apply_epi_b16(act, g); }
+
+__device__ __forceinline__ float2 act_grad_b16(int act, float g) {
+  if (act == EPI_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
+    const float t = s * (1.0f - s);
+    return make_float2(g * s, s + (t == 0.0f ? 0.0f : g * t));
+  }
+  if (act == EPI_GELU_TANH) {
+    constexpr float c = 0.7978845608028654f, k = 0.044715f;
+    constexpr float a = (float)(-2.0 * 0.7978845608028654 * 1.4426950408889634);
+    const float g2 = g * g;
+    const float s =
+        __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * __builtin_fmaf(g2, a * k, a)));
+    const float t = s * (1.0f - s);
+    return make_float2(g * s, s + (t == 0.0f ? 0.0f : 2.0f * c * g * t * (1.0f + 3.0f * k * g2)));
+  }
+  if (act == EPI_RELU) return make_float2(g > 0.0f ? g : 0.0f, g > 0.0f ? 1.0f : 0.0f);
+  return make_float2(g, 1.0f);
+}
+
+// One operand of a tile: BR rows of a 64-deep stage, NW waves loading 1 KB each a
+// load, LOADS loads a wave.
+//
+// K-contiguous (KC): LDS row r holds 64 k (128 bytes), chunk c of 8 k at
+// c ^ (r / 2 % 8): a load covers 8 rows.
+//
+// K-strided: LDS row k holds BR columns (2 BR bytes) and a load covers 512 / BR of
+// them.  A transposed read serves 32 lanes at a time: 32-byte pieces of the 8 rows
+// {0-3, 8-11} + 4 h + 16 i, which would all start at one bank (rows are a multiple
+// of the 256-byte bank window); XOR-ing the piece with (k % 4) + 4 (k / 8 % 2) gives
+// them 8 different places in the window.  BR = 64: two rows share a window, so two
+// bits (k / 2 % 2, k / 8 % 2) suffice.
+template <int BR, int NW, bool KC>
+struct Operand {
+  static constexpr int LOADS = BR / (8 * NW);
+  static constexpr int STAGE = BR * kBK;  // elements of a stage buffer
+  static constexpr int READS = KC ? 1 : 2;
+  uint32_t off[LOADS];
+  int kc[LOADS];  // KC: the first k of this lane's chunk
+
+  static __device__ __forceinline__ int piece(int k) {
+    return BR == 64 ? ((k >> 1) & 1) | ((k >> 2) & 2) : (k & 3) | ((k >> 1) & 4);
+  }
+
+  // row(r): the memory row of tile row r relative to the resource's base, or -1.
+  template <typename Row>
+  __device__ __forceinline__ void init(int64_t ld, int wave, int lane, Row row) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int blk = i * NW + wave;
+      if constexpr (KC) {
+        const int r = blk * 8 + (lane >> 3);
+        kc[i] = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+        const int src = row(r);
+        off[i] = src >= 0 ? (uint32_t)(src * ld + kc[i]) * 2 : kOobOffset;
+      } else {
+        constexpr int CH = BR / 8;  // 16-byte chunks of an LDS row
+        const int k = blk * (512 / BR) + lane / CH, c = lane % CH;
+        kc[i] = 0;
+        off[i] = (uint32_t)(k * ld + ((((c >> 1) ^ piece(k)) << 1) | (c & 1)) * 8) * 2;
+      }
+    }
+  }
+
+  static __device__ __forceinline__ uint16_t *dst(uint16_t *stage, int i, int wave) {
+    return stage + (i * NW + wave) * 512;
+  }
+
+  // The lane's part of a fragment's LDS address, in elements of the stage: block j
+  // of 16 rows at base ^ (j * 16) (K-strided; j < 8 and base's bits of j clear
+  // before the XOR with the piece) or base + j * 1024 (KC), step ks of 32 k.
+  static __device__ __forceinline__ int lane_base(int row0, int ks, int lane) {
+    const int fr = lane & 15, fh = lane >> 4;
+    if constexpr (KC) return (row0 + fr) * kBK + (((ks * 4 + fh) ^ ((fr >> 1) & 7)) * 8);
+    const int k = 8 * fh + (fr >> 2);
+    return (ks * 32 + k) * BR + ((row0 >> 4) ^ piece(k)) * 16 + (fr & 3) * 4;
+  }
+
+  // Half h of block j's fragment (KC: the whole of it, h = 0).
+  static __device__ __forceinline__ void read(bf16x8 &f, const uint16_t *stage, int base, int j,
+                                              int h) {
+    if constexpr (KC) {
+      f = *(const bf16x8 *)(stage + base + j * 16 * kBK);
+    } else {
+      const bf16x4 v =
+          __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(stage + (base ^ (j * 16)) + h * 4 * BR));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[4 * h + i] = v[i];
+    }
+  }
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_from(const uint16_t *p, int64_t elems) {
+  return make_rsrc(p, elems > 0 ? elems * 2 : 0);
+}
+
+// Which problem, K slice and tile a workgroup computes.  The problems' tiles form
+// one list, of which each XCD takes a contiguous run (neighbouring tiles share
+// operand panels in its L2).
+struct TileAt {
+  int prob, split, m, n;
+};
+__device__ __forceinline__ TileAt locate(const TileArgs &a) {
+  const int total = a.tiles * a.splits, x = blockIdx.x & 7, q = total >> 3, r = total & 7;
+  int logical = x * q + (x < r ? x : r) + ((int)blockIdx.x >> 3);
+  TileAt t;
+  t.split = logical / a.tiles;
+  logical -= t.split * a.tiles;
+  t.prob = 0;
+  if (a.n > 1 && logical >= a.p[1].first) t.prob = 1;
+  if (a.n > 2 && logical >= a.p[2].first) t.prob = 2;
+  const TileProb &p = a.p[t.prob];
+  group_coords(logical - p.first, p.tiles_m, p.tiles_n, 4, t.m, t.n);
+  return t;
+}
+
+// The columns that a lane's block j (of 16) starts at, in the tile's output.
+template <int ACT, int TM, int TN, int WM, int WN>
+__device__ __forceinline__ void out_gate(const TileProb &p, const f32x4 (&acc)[TM][TN], int m0,
+                                         int n0, int wm, int wn, int lane) {
+  constexpr int TH = TN / 2;
+  const int fr = lane & 15, fh = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + wm * WM + i * 16 + fr;
+    uint32_t w[TH][2];
+#pragma unroll
+    for (int j = 0; j < TH; ++j) {
+      const int n = n0 + wn * (WN / 2) + j * 16 + 4 * fh;
+      float h[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h[q] = act_b16(ACT, acc[i][j][q]) * acc[i][j + TH][q];
+      w[j][0] = pack_bf16x2(h[0], h[1]);
+      w[j][1] = pack_bf16x2(h[2], h[3]);
+      if (p.F && m < p.M && n < p.N) {
+        const f32x4 &g = acc[i][j], &u = acc[i][j + TH];
+        *(float4 *)(p.F + (size_t)m * p.ldc + n) = make_float4(g[0], g[1], g[2], g[3]);
+        *(float4 *)(p.F2 + (size_t)m * p.ldc + n) = make_float4(u[0], u[1], u[2], u[3]);
+      }
+    }
+    if constexpr (TH == 2) {
+      const auto a = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+      const auto b = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+      const int n = n0 + wn * (WN / 2) + (fh & 1) * 16 + 8 * (fh >> 1);
+      if (m < p.M && n < p.N)
+        *(uint4 *)(p.C + (size_t)m * p.ldc + n) = make_uint4(a[0], b[0], a[1], b[1]);
+    } else {
+      const int n = n0 + wn * (WN / 2) + 4 * fh;
+      if (m < p.M && n < p.N) *(uint2 *)(p.C + (size_t)m * p.ldc + n) = make_uint2(w[0][0], w[0][1]);
+    }
+  }
+}
+
+template <int ACT, int TM, int TN, int WM, int WN>
+__device__ __forceinline__ void out_dgate(const TileProb &p, const f32x4 (&acc)[TM][TN], int m0,
+                                          int n0, int wm, int wn, int lane) {
+  const int fr = lane & 15, fh = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + wm * WM + i * 16 + fr;
+    uint32_t wg[TN][2], wu[TN][2];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + wn * WN + j * 16 + 4 * fh;
+      float4 g = make_float4(0, 0, 0, 0), u = g;
+      if (m < p.M && n < p.N) {
+        g = *(const float4 *)(p.F + (size_t)m * p.ldc + n);
+        u = *(const float4 *)(p.F2 + (size_t)m * p.ldc + n);
+      }
+      const float gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
+      float dg[4], du[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 a = act_grad_b16(ACT, gv[q]);
+        du[q] = acc[i][j][q] * a.x;
+        dg[q] = acc[i][j][q] * uv[q] * a.y;
+      }
+      wg[j][0] = pack_bf16x2(dg[0], dg[1]);
+      wg[j][1] = pack_bf16x2(dg[2], dg[3]);
+      wu[j][0] = pack_bf16x2(du[0], du[1]);
+      wu[j][1] = pack_bf16x2(du[2], du[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const int n = n0 + wn * WN + (j + (fh & 1)) * 16 + 8 * (fh >> 1);
+      const auto a = __builtin_amdgcn_permlane16_swap(wg[j][0], wg[j + 1][0], false, false);
+      const auto b = __builtin_amdgcn_permlane16_swap(wg[j][1], wg[j + 1][1], false, false);
+      const auto c = __builtin_amdgcn_permlane16_swap(wu[j][0], wu[j + 1][0], false, false);
+      const auto d = __builtin_amdgcn_permlane16_swap(wu[j][1], wu[j + 1][1], false, false);
+      if (m < p.M && n < p.N) {
+        *(uint4 *)(p.C + (size_t)m * p.ldc + n) = make_uint4(a[0], b[0], a[1], b[1]);
+        *(uint4 *)(p.C2 + (size_t)m * p.ldc + n) = make_uint4(c[0], d[0], c[1], d[1]);
+      }
+    }
+  }
+}
+
+// A lane's block (i, j) holds row 16 i + (lane & 15) at columns 16 j + 4 (lane >> 4)
+// + q; pairs of blocks are traded between lane rows so that a lane stores 16 bytes.
+template <int TM, int TN, int WM, int WN>
+__device__ __forceinline__ void out_store(const TileProb &p, const f32x4 (&acc)[TM][TN], int m0,
+                                          int n0, int wm, int wn, int lane) {
+  const int fr = lane & 15, fh = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + wm * WM + i * 16 + fr;
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const f32x4 &x = acc[i][j], &y = acc[i][j + 1];
+      const auto a = __builtin_amdgcn_permlane16_swap(pack_bf16x2(x[0], x[1]),
+                                                      pack_bf16x2(y[0], y[1]), false, false);
+      const auto b = __builtin_amdgcn_permlane16_swap(pack_bf16x2(x[2], x[3]),
+                                                      pack_bf16x2(y[2], y[3]), false, false);
+      const int n = n0 + wn * WN + (j + (fh & 1)) * 16 + 8 * (fh >> 1);
+      if (m < p.M && n < p.N)
+        *(uint4 *)(p.C + (size_t)m * p.ldc + n) = make_uint4(a[0], b[0], a[1], b[1]);
+    }
+  }
+}
+
+template <int TM, int TN, int WM, int WN>
+__device__ __forceinline__ void out_part(const TileProb &p, const f32x4 (&acc)[TM][TN], int m0,
+                                         int n0, int wm, int wn, int lane, int split) {
+  float *part = p.part + (size_t)split * p.M * p.N;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + wm * WM + i * 16 + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + wn * WN + j * 16 + 4 * (lane >> 4);
+      const f32x4 &v = acc[i][j];
+      if (m < p.M && n < p.N)
+        *(float4 *)(part + (size_t)m * p.N + n) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+template <int OUT, int TM, int TN, int WM, int WN>
+__device__ __forceinline__ void tile_out(const TileArgs &a, const TileProb &p,
+                                         const f32x4 (&acc)[TM][TN], int m0, int n0, int wm,
+                                         int wn, int lane, int split) {
+  if constexpr (OUT == OUT_STORE) {
+    out_store<TM, TN, WM, WN>(p, acc, m0, n0, wm, wn, lane);
+  } else if constexpr (OUT == OUT_PART) {
+    out_part<TM, TN, WM, WN>(p, acc, m0, n0, wm, wn, lane, split);
+  } else {
+    switch (a.act) {
+#define MJ_OUT(E)                                                              \
+  if constexpr (OUT == OUT_GATE)                                               \
+    out_gate<E, TM, TN, WM, WN>(p, acc, m0, n0, wm, wn, lane);                 \
+  else                                                                         \
+    out_dgate<E, TM, TN, WM, WN>(p, acc, m0, n0, wm, wn, lane);                \
+  break;
+      case EPI_RELU: MJ_OUT(EPI_RELU)
+      case EPI_GELU_TANH: MJ_OUT(EPI_GELU_TANH)
+      case EPI_SILU: MJ_OUT(EPI_SILU)
+      default: MJ_OUT(EPI_NONE)
+#undef MJ_OUT
+    }
+  }
+}
+
+// Tiles of four waves (2 x 2) on a ring of S 64-deep stages, the direct loads
+// S - 2 stages ahead and a wave's fragments half a stage: the stage's one barrier
+// sits between its two 32-deep steps, where the next stage has landed.
+template <int BM, int BN, int S, bool AKC, bool BKC, int OUT>
+__global__ __launch_bounds__(256) void mlp_ring_kernel(TileArgs args) {
+  constexpr int NW = 4, WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
+  constexpr int BN_OUT = OUT == OUT_GATE ? BN / 2 : BN;
+  using OA = Operand<BM, NW, AKC>;
+  using OB = Operand<BN, NW, BKC>;
+  constexpr int NDMA = OA::LOADS + OB::LOADS, FLY = (S - 3) * NDMA;
+  static_assert(S >= 3 && FLY < 64, "vmcnt range");
+  static_assert(OUT != OUT_GATE || BKC, "gate and up rows are K-contiguous");
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const TileAt at = locate(args);
+  const TileProb &p = args.p[at.prob];
+  const int m0 = at.m * BM, n0 = at.n * BN_OUT;
+  const int nk = (p.K + kBK - 1) / kBK, stages = nk * p.segs;
+  const int per = (stages + args.splits - 1) / args.splits;
+  const int kt0 = at.split * per, kt1 = std::min(kt0 + per, stages);
+
+  OA oa;
+  oa.init(p.lda, wave, lane, [&](int r) { return m0 + r < p.M ? r : -1; });
+  OB ob;
+  ob.init(p.ldb, wave, lane, [&](int r) {
+    if constexpr (OUT == OUT_GATE) r = (r / WN) * (WN / 2) + r % (WN / 2);
+    return n0 + r < p.N ? r : -1;
+  });
+  // whether load i of this wave fetches up rows (gate/up tiles)
+  auto is_up = [&](int i) { return OUT == OUT_GATE && ((i * NW + wave) * 8) % WN >= WN / 2; };
+  // stage kt into its ring buffer; past the slice it reads zeros
+  auto issue = [&](int kt) __attribute__((always_inline)) {
+    const int seg = kt >= nk ? 1 : 0, k0 = (kt - seg * nk) * kBK;
+    const bool in = kt < kt1;
+    uint16_t *as = lds + (kt % S) * (OA::STAGE + OB::STAGE), *bs = as + OA::STAGE;
+    const int ks = OUT == OUT_GATE ? 0 : seg;
+    if constexpr (AKC) {
+      const auto r = rsrc_from(p.A[seg] + (size_t)m0 * p.lda, in ? (int64_t)(p.M - m0) * p.lda : 0);
+#pragma unroll
+      for (int i = 0; i < OA::LOADS; ++i)
+        dma16(r, OA::dst(as, i, wave), k0 + oa.kc[i] < p.K ? oa.off[i] + k0 * 2 : kOobOffset);
+    } else {
+      const auto r = rsrc_from(p.A[seg] + (size_t)k0 * p.lda + m0,
+                               in ? (int64_t)(p.K - k0) * p.lda - m0 : 0);
+#pragma unroll
+      for (int i = 0; i < OA::LOADS; ++i) dma16(r, OA::dst(as, i, wave), oa.off[i]);
+    }
+    if constexpr (BKC) {
+      const int64_t left = in ? (int64_t)(p.N - n0) * p.ldb : 0;
+      const auto r = rsrc_from(p.B[ks] + (size_t)n0 * p.ldb, left);
+      const auto r2 = rsrc_from(p.B[OUT == OUT_GATE ? 1 : ks] + (size_t)n0 * p.ldb, left);
+#pragma unroll
+      for (int i = 0; i < OB::LOADS; ++i) {
+        const uint32_t o = k0 + ob.kc[i] < p.K ? ob.off[i] + k0 * 2 : kOobOffset;
+        if (is_up(i)) dma16(r2, OB::dst(bs, i, wave), o);
+        else dma16(r, OB::dst(bs, i, wave), o);
+      }
+    } else {
+      const auto r = rsrc_from(p.B[ks] + (size_t)k0 * p.ldb + n0,
+                               in ? (int64_t)(p.K - k0) * p.ldb - n0 : 0);
+#pragma unroll
+      for (int i = 0; i < OB::LOADS; ++i) dma16(r, OB::dst(bs, i, wave), ob.off[i]);
+    }
+  };
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  int abase[2], bbase[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    abase[ks] = OA::lane_base(wm * WM, ks, lane);
+    bbase[ks] = OB::lane_base(wn * WN, ks, lane);
+  }
+  bf16x8 fa[2][TM], fb[2][TN];
+  auto read_frags = [&](int kt, int ks) __attribute__((always_inline)) {
+    const uint16_t *as = lds + (kt % S) * (OA::STAGE + OB::STAGE), *bs = as + OA::STAGE;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int h = 0; h < OA::READS; ++h) OA::read(fa[ks][i], as, abase[ks], i, h);
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int h = 0; h < OB::READS; ++h) OB::read(fb[ks][j], bs, bbase[ks], j, h);
+  };
+  auto mma = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[ks][j], fa[ks][i], acc[i][j], 0, 0,
+                                                            0);
+  };
+  // the loads of all but the FLY youngest have landed, in every wave, and every
+  // wave holds the fragments that it read before
+  auto landed = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (FLY & 0xF) | ((FLY >> 4) << 14));  // and lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int s = 0; s < S - 2; ++s) issue(kt0 + s);
+  landed();  // stage kt0
+  issue(kt0 + S - 2);
+  read_frags(kt0, 0);
+  for (int kt = kt0; kt < kt1; ++kt) {
+    read_frags(kt, 1);
+    mma(0);
+    landed();  // stage kt + 1
+    issue(kt + S - 1);
+    read_frags(kt + 1, 0);
+    mma(1);
+  }
+  // loads past the slice must not land in a later workgroup's LDS
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  tile_out<OUT, TM, TN, WM, WN>(args, p, acc, m0, n0, wm, wn, lane, at.split);
+}
+
+// C = bf16(sum of the K slices' partials, in slice order), 8 elements a thread.
+__global__ __launch_bounds__(256) void mlp_reduce_kernel(const float *part, uint16_t *C, int64_t n,
+                                                         int splits) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e >= n) return;
+  float v[8] = {};
+  for (int s = 0; s < splits; ++s) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 q = *(const float4 *)(part + (size_t)s * n + e + 4 * h);
+      v[4 * h] += q.x, v[4 * h + 1] += q.y, v[4 * h + 2] += q.z, v[4 * h + 3] += q.w;
+    }
+  }
+  *(uint4 *)(C + e) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                 pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// ---------------------------------------------------------------- fp32 block
+__device__ __forceinline__ float2 act_grad_f32(int act, float g) {
+  if (act == EPI_SILU) {
+    const float s = sigmoid32(g), t = s * (1.0f - s);
+    return make_float2(g * s, s + (t == 0.0f ? 0.0f : g * t));
+  }
+  if (act == EPI_GELU_TANH) {
+    const float c = 0.7978845608028654f, k = 0.044715f;
+    const float s = sigmoid32(2.0f * c * (g + k * g * g * g)), t = s * (1.0f - s);
+    return make_float2(g * s, s + (t == 0.0f ? 0.0f : 2.0f * c * g * t * (1.0f + 3.0f * k * g * g)));
+  }
+  if (act == EPI_RELU) return make_float2(g > 0.0f ? g : 0.0f, g > 0.0f ? 1.0f : 0.0f);
+  return make_float2(g, 1.0f);
+}
+
+// 4 elements a thread; the last few singly.
+__global__ __launch_bounds__(256) void gate_f32_kernel(int act, const float *g, const float *u,
+                                                       float *h, int64_t n) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e + 4 <= n) {
+    const float4 a = *(const float4 *)(g + e), b = *(const float4 *)(u + e);
+    *(float4 *)(h + e) =
+        make_float4(act_grad_f32(act, a.x).x * b.x, act_grad_f32(act, a.y).x * b.y,
+                    act_grad_f32(act, a.z).x * b.z, act_grad_f32(act, a.w).x * b.w);
+  } else {
+    for (int64_t i = e; i < n; ++i) h[i] = act_grad_f32(act, g[i]).x * u[i];
+  }
+}
+
+__global__ __launch_bounds__(256) void gate_bwd_f32_kernel(int act, const float *g, const float *u,
+                                                           const float *dh, float *dg, float *du,
+                                                           int64_t n) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e + 4 <= n) {
+    const float4 gv = *(const float4 *)(g + e), uv = *(const float4 *)(u + e),
+                 dv = *(const float4 *)(dh + e);
+    const float2 a = act_grad_f32(act, gv.x), b = act_grad_f32(act, gv.y),
+                 c = act_grad_f32(act, gv.z), d = act_grad_f32(act, gv.w);
+    *(float4 *)(dg + e) = make_float4(dv.x * uv.x * a.y, dv.y * uv.y * b.y, dv.z * uv.z * c.y,
+                                      dv.w * uv.w * d.y);
+    *(float4 *)(du + e) = make_float4(dv.x * a.x, dv.y * b.x, dv.z * c.x, dv.w * d.x);
+  } else {
+    for (int64_t i = e; i < n; ++i) {
+      const float2 a = act_grad_f32(act, g[i]);
+      const float d = dh[i];
+      dg[i] = d * u[i] * a.y;
+      du[i] = d * a.x;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launch
+hipError_t raise_lds(const void *kern, size_t bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
+    hipError_t e =
+        hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return e;
+    done.fetch_or(bit, std::memory_order_release);
+  }
+  return hipSuccess;
+}
+
+void set_tiles(TileArgs &a, int bm, int bn_out) {
+  a.tiles = 0;
+  for (int i = 0; i < a.n; ++i) {
+    a.p[i].tiles_m = (a.p[i].M + bm - 1) / bm;
+    a.p[i].tiles_n = (a.p[i].N + bn_out - 1) / bn_out;
+    a.p[i].first = a.tiles;
+    a.tiles += a.p[i].tiles_m * a.p[i].tiles_n;
+  }
+}
+
+template <int BM, int BN, int S, bool AKC, bool BKC, int OUT>
+hipError_t launch_ring(TileArgs a, hipStream_t stream) {
+  constexpr size_t lds = size_t(S) * (BM + BN) * kBK * sizeof(uint16_t);
+  static_assert(lds <= 160 * 1024, "LDS budget");
+  auto kern = mlp_ring_kernel<BM, BN, S, AKC, BKC, OUT>;
+  static std::atomic<uint64_t> done{0};
+  if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
+  set_tiles(a, BM, OUT == OUT_GATE ? BN / 2 : BN);
+  const int64_t grid = (int64_t)a.tiles * a.splits;
+  if (grid == 0) return hipSuccess;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, a);
+  return hipGetLastError();
+}
+
+int64_t tiles_of(const TileArgs &a, int bm, int bn) {
+  int64_t t = 0;
+  for (int i = 0; i < a.n; ++i)
+    t += (int64_t)((a.p[i].M + bm - 1) / bm) * ((a.p[i].N + bn - 1) / bn);
+  return t;
+}
+
+template <bool AKC, bool BKC, int OUT>
+hipError_t launch_tiles(const TileArgs &a, hipStream_t stream) {
+  const int half = OUT == OUT_GATE ? 2 : 1;
+  if (tiles_of(a, 128, 128 / half) >= 256)
+    return launch_ring<128, 128, 3, AKC, BKC, OUT>(a, stream);
+  return launch_ring<64, 64, 3, AKC, BKC, OUT>(a, stream);
+}
+
+// K slices of a plain product with too few tiles to fill the CUs.
+int plan_splits(int64_t M, int64_t N, int64_t stages) {
+  const int64_t tiles = ((M + 63) / 64) * ((N + 63) / 64);
+  int s = 1;
+  while (s < 16 && tiles * s * 2 <= 512 && stages / (s * 2) >= 8) s *= 2;
+  return s;
+}
+
+// A plain product, its K split where that fills the CUs.
+template <bool AKC, bool BKC>
+hipError_t launch_plain(TileArgs a, float *part, hipStream_t stream) {
+  const TileProb &p = a.p[0];
+  const int s = plan_splits(p.M, p.N, (int64_t)((p.K + kBK - 1) / kBK) * p.segs);
+  if (s == 1) return launch_tiles<AKC, BKC, OUT_STORE>(a, stream);
+  a.splits = s;
+  a.p[0].part = part;
+  if (hipError_t e = launch_ring<64, 64, 3, AKC, BKC, OUT_PART>(a, stream); e != hipSuccess)
+    return e;
+  const int64_t n = (int64_t)p.M * p.N;
+  hipLaunchKernelGGL(mlp_reduce_kernel, dim3((unsigned)((n / 8 + 255) / 256)), dim3(256), 0, stream,
+                     part, p.C, n, s);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward) {
+  const int64_t stages = (I + kBK - 1) / kBK * (backward ? 2 : 1), N = backward ? K : H;
+  const int s = plan_splits(M, N, stages);
+  return s > 1 ? s * M * N : 0;
+}
+
+hipError_t launch_gated_mlp(const GatedMlp &q, hipStream_t stream) {
+  TileArgs a;
+  a.act = q.act;
+  TileProb &p = a.p[0];
+  p.A[0] = q.x, p.lda = q.K;
+  p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
+  p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.K;
+  p.C = q.h, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
+  if (hipError_t e = launch_tiles<true, true, OUT_GATE>(a, stream); e != hipSuccess) return e;
+  TileArgs b;
+  TileProb &d = b.p[0];
+  d.A[0] = q.h, d.lda = q.I;
+  d.B[0] = q.wd, d.ldb = q.I;
+  d.M = (int)q.M, d.N = (int)q.H, d.K = (int)q.I;
+  d.C = q.y, d.ldc = q.H;
+  return launch_plain<true, true>(b, q.part, stream);
+}
+
+hipError_t launch_gated_mlp_bwd(const GatedMlp &q, const GatedMlpGrad &o, hipStream_t stream) {
+  if (o.dx || o.dwg || o.dwu) {
+    TileArgs a;
+    a.act = q.act;
+    TileProb &p = a.p[0];
+    p.A[0] = o.dy, p.lda = q.H;
+    p.B[0] = q.wd, p.ldb = q.I;
+    p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.H;
+    p.C = o.dg, p.C2 = o.du, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
+    if (hipError_t e = launch_tiles<true, false, OUT_DGATE>(a, stream); e != hipSuccess) return e;
+  }
+  if (o.dx) {
+    TileArgs a;
+    TileProb &p = a.p[0];
+    p.A[0] = o.dg, p.A[1] = o.du, p.lda = q.I;
+    p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
+    p.M = (int)q.M, p.N = (int)q.K, p.K = (int)q.I, p.segs = 2;
+    p.C = o.dx, p.ldc = q.K;
+    if (hipError_t e = launch_plain<true, false>(a, q.part, stream); e != hipSuccess) return e;
+  }
+  TileArgs w;
+  w.n = 0;
+  auto add = [&](const uint16_t *A, int64_t rows, const uint16_t *B, int64_t cols, uint16_t *C) {
+    if (!C) return;
+    TileProb &p = w.p[w.n++];
+    p.A[0] = A, p.lda = rows;
+    p.B[0] = B, p.ldb = cols;
+    p.M = (int)rows, p.N = (int)cols, p.K = (int)q.M;
+    p.C = C, p.ldc = cols;
+  };
+  add(o.dg, q.I, q.x, q.K, o.dwg);
+  add(o.du, q.I, q.x, q.K, o.dwu);
+  add(o.dy, q.H, q.h, q.I, o.dwd);
+  return w.n ? launch_tiles<false, false, OUT_STORE>(w, stream) : hipSuccess;
+}
+
+hipError_t launch_gate_f32(int act, const float *g, const float *u, float *h, int64_t n,
+                           hipStream_t stream) {
+  if (n <= 0) return hipSuccess;
+  const int64_t grid = (n + 1023) / 1024;
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(gate_f32_kernel, dim3((unsigned)grid), dim3(256), 0, stream, act, g, u, h, n);
+  return hipGetLastError();
+}
+
+hipError_t launch_gate_bwd_f32(int act, const float *g, const float *u, const float *dh, float *dg,
+                               float *du, int64_t n, hipStream_t stream) {
+  if (n <= 0) return hipSuccess;
+  const int64_t grid = (n + 1023) / 1024;
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(gate_bwd_f32_kernel, dim3((unsigned)grid), dim3(256), 0, stream, act, g, u, dh,
+                     dg, du, n);
+  return hipGetLastError();
+}
+
+}  // namespace mj

@@ -42,11 +42,10 @@
 #include <type_traits>
 
 #include "common.h"
+#include "gemm_tile.h"
 #include "launch.h"
 
 namespace mj {
-
-constexpr int kBK = 64;  // K per pipeline stage
 
 // int8 x16 (one 16-byte word) -> 16 bf16 (exact), as two 16-byte words.
 __device__ __forceinline__ void i8x16_to_bf16x16(const uint4 &q, uint4 &lo, uint4 &hi) {
@@ -243,12 +242,6 @@ __device__ __forceinline__ void store_part8(const GemmNT &p, const f32x4 (&acc)[
       }
     }
   }
-}
-
-typedef __attribute__((address_space(3))) void lds_void;
-
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint16_t *lds_dst, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)lds_dst, 16, off, 0, 0, 0);
 }
 
 // IGLP asks the compiler to interleave the stage's MFMAs with its LDS reads
@@ -652,10 +645,6 @@ __global__ __launch_bounds__(256) void gemm_nt_ring_kernel(GemmNT p) {
 //    last stages, whose loads reach past K, take a per-load zero-fill select.
 //    The scalar offset stays below 2^31 and an out-of-range row offset plus it
 //    cannot wrap for K < 2^30, which the launchers check.
-__device__ __forceinline__ void dma16s(__amdgpu_buffer_rsrc_t r, uint16_t *lds_dst,
-                                       uint32_t voff, uint32_t soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)lds_dst, 16, voff, soff, 0, 0);
-}
 
 // Epilogue of a full, 16-byte aligned tile straight from the accumulators:
 // blocks j and j+1 of a lane row are exchanged with v_permlane16_swap so that
@@ -714,17 +703,6 @@ __device__ __forceinline__ void store_tile_direct(const GemmNT &p, const f32x4 (
                                                            pack_bf16x2(x[2], x[3]));
     }
   }
-}
-
-// s_waitcnt lgkmcnt(0) as the builtin (vmcnt and expcnt left open): unlike the
-// same text in inline asm, the compiler's wait-count pass sees it, so it does
-// not add a wait of its own for fragments this one already covered (such a
-// wait, placed after the next step's first read, stalled every stage for a
-// full LDS round trip).
-constexpr int kLgkm0 = 0xC07F;
-
-__device__ __forceinline__ void mfma_16x16x32_tied(f32x4 &acc, const bf16x8 &a, const bf16x8 &b) {
-  asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
 // bf16 256 x 256 tiles with two waves per SIMD: 8 waves laid out 2 x 4, each

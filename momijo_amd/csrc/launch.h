@@ -240,4 +240,72 @@ hipError_t launch_gemm_i8_literal(const int8_t *A, const int8_t *B, int32_t *C, 
                                   const float *b, int64_t M, int64_t N, int64_t K,
                                   hipStream_t stream);
 
+// ---- dropout.hip, residual_norm.hip ----------------------------------------
+// thr: an element is dropped where its 16 random bits are below it; 0 = no
+// dropout, 65536 = all dropped.  scale = 65536 / (65536 - thr), the reciprocal of
+// the share that is kept, so the kept values' mean has no bias.
+struct Dropout {
+  uint32_t thr = 0;
+  float scale = 1.0f;
+  uint64_t seed = 0, counter = 0;
+  const uint64_t *state = nullptr;  // device {seed, counter} in place of seed; counter is added
+};
+hipError_t launch_dropout(bool bf16, const void *x, void *y, int64_t n, const Dropout &d,
+                          hipStream_t stream);
+
+// y = scale x + drop(gate (norm(b) wp + bp)), n = norm(y) wn + bn; x, b, gate, y, n
+// in the activations' type, the vectors fp32; every pointer but x may be null.
+struct ResNorm {
+  const void *x = nullptr, *b = nullptr, *gate = nullptr;
+  const float *scale = nullptr, *wp = nullptr, *bp = nullptr, *wn = nullptr, *bn = nullptr;
+  void *y = nullptr, *n = nullptr;
+  float *stats = nullptr;  // [4][rows]: post mean, post 1 / std, next mean, next 1 / std
+  int64_t rows = 0, dim = 0;
+  int64_t per = 1;         // rows of x for each row of gate
+  float eps = 0.0f;
+  int layer = 0;           // 0 rms, 1 layer
+  Dropout drop;
+};
+struct ResNormGrad {
+  const void *dy = nullptr, *dn = nullptr;
+  void *dx = nullptr, *db = nullptr, *dgate = nullptr;
+  float *dscale = nullptr, *dwp = nullptr, *dbp = nullptr, *dwn = nullptr, *dbn = nullptr;
+  float *part = nullptr;   // residual_norm_part_floats
+  // the walk of plan_residual_norm_bwd
+  int64_t groups = 1, segs = 1, seg_rows = 0, groups_per_team = 1, teams = 0;
+};
+constexpr int64_t kResNormMaxDim = 16384;
+void plan_residual_norm_bwd(const ResNorm &p, ResNormGrad &g);
+int64_t residual_norm_part_floats(const ResNormGrad &g, int64_t dim);
+hipError_t launch_residual_norm(bool bf16, const ResNorm &p, hipStream_t stream);
+hipError_t launch_residual_norm_bwd(bool bf16, const ResNorm &p, const ResNormGrad &g,
+                                    hipStream_t stream);
+
+// ---- gated_mlp.hip ---------------------------------------------------------
+// bf16 [tokens, K] -> [tokens, H] through I gated features; K, I, H multiples of
+// 8, 16-byte aligned arrays, rows contiguous.
+struct GatedMlp {
+  const uint16_t *x = nullptr, *wg = nullptr, *wu = nullptr, *wd = nullptr;
+  int act = 0;
+  uint16_t *h = nullptr;                 // [M, I]
+  float *g = nullptr, *u = nullptr;      // [M, I] fp32 projections kept for the backward, or null
+  uint16_t *y = nullptr;                 // [M, H]
+  int64_t M = 0, K = 0, I = 0, H = 0;
+  float *part = nullptr;                 // split-K partials (gated_mlp_part_floats)
+};
+struct GatedMlpGrad {
+  const uint16_t *dy = nullptr;
+  uint16_t *dg = nullptr, *du = nullptr;  // [M, I] scratch: gradients of g and u
+  uint16_t *dx = nullptr, *dwg = nullptr, *dwu = nullptr, *dwd = nullptr;  // each may be null
+};
+int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward);
+hipError_t launch_gated_mlp(const GatedMlp &p, hipStream_t stream);
+hipError_t launch_gated_mlp_bwd(const GatedMlp &p, const GatedMlpGrad &d, hipStream_t stream);
+// The elementwise halves of the fp32 block: h = act(g) u, and in place dg = dh u
+// act'(g), du = dh act(g) over n elements.
+hipError_t launch_gate_f32(int act, const float *g, const float *u, float *h, int64_t n,
+                           hipStream_t stream);
+hipError_t launch_gate_bwd_f32(int act, const float *g, const float *u, const float *dh, float *dg,
+                               float *du, int64_t n, hipStream_t stream);
+
 }  // namespace mj

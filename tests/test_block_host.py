@@ -1,0 +1,89 @@
+"""Host-side checks of the feed-forward block's operators: the generator's plain form
+against its published vectors, and the C ABI's refusals, before any device work."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import _block as plain
+from momijo_amd import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def test_philox_published_vectors():
+    """Philox4x32-10 for the zero and the all-ones counter and key."""
+    got = plain.philox4x32(np.array([0], np.uint64), 0, 0)
+    assert [hex(v) for v in got[0]] == ["0x6627e8d5", "0xe169c58d", "0xbc57ac4c", "0x9b00dbd8"]
+    ones = (1 << 64) - 1
+    got = plain.philox4x32(np.array([ones], np.uint64), ones, ones)
+    assert [hex(v) for v in got[0]] == ["0x408f276d", "0x41c83b0e", "0xa20bc7c6", "0x6d5451fd"]
+
+
+def test_dropout_status_codes(lib):
+    p = ctypes.c_void_p(16)  # never dereferenced
+    assert lib.mj_dropout(7, p, p, 4, 0.1, 0, 0, None, None) == _lib.MJ_ERR_ARG
+    assert lib.mj_dropout(0, p, p, -1, 0.1, 0, 0, None, None) == _lib.MJ_ERR_ARG
+    assert lib.mj_dropout(0, p, p, 4, 1.1, 0, 0, None, None) == _lib.MJ_ERR_ARG
+    assert lib.mj_dropout(0, None, p, 4, 0.1, 0, 0, None, None) == _lib.MJ_ERR_ARG
+    assert lib.mj_dropout(0, None, None, 0, 0.1, 0, 0, None, None) == _lib.MJ_OK
+
+
+def _norm(lib, **kw):
+    a = dict(dtype=0, norm=0, x=16, b=16, gate=None, gate_rows=0, scale=None, wp=None, bp=None,
+             wn=None, bn=None, eps=1e-6, p=0.0, seed=0, counter=0, state=None, y=16, n=None,
+             stats=None, rows=4, dim=8, stream=None)
+    a.update(kw)
+    return lib.mj_residual_norm(*a.values())
+
+
+def test_residual_norm_status_codes(lib):
+    assert _norm(lib, dtype=3) == _lib.MJ_ERR_ARG
+    assert _norm(lib, norm=2) == _lib.MJ_ERR_ARG
+    assert _norm(lib, rows=-1) == _lib.MJ_ERR_ARG
+    assert _norm(lib, dim=16385) == _lib.MJ_ERR_UNSUPPORTED
+    assert _norm(lib, x=None) == _lib.MJ_ERR_ARG
+    assert _norm(lib, b=None, wp=16) == _lib.MJ_ERR_ARG
+    assert _norm(lib, bp=16) == _lib.MJ_ERR_ARG
+    assert _norm(lib, eps=-1.0) == _lib.MJ_ERR_ARG
+    assert _norm(lib, gate=16, gate_rows=3) == _lib.MJ_ERR_SHAPE
+    assert _norm(lib, gate=16, gate_rows=0) == _lib.MJ_ERR_SHAPE
+    assert _norm(lib, y=None) == _lib.MJ_ERR_ARG
+    assert _norm(lib, n=16) == _lib.MJ_ERR_ARG
+    assert _norm(lib, rows=0) == _lib.MJ_OK and _norm(lib, dim=0) == _lib.MJ_OK
+
+
+def test_residual_norm_backward_needs_its_work(lib):
+    need = lib.mj_residual_norm_work_bytes(100, 64, 4)
+    assert need > 0 and need % (64 * 4) == 0
+    assert lib.mj_residual_norm_work_bytes(100, 64, 3) == 0
+    assert lib.mj_residual_norm_work_bytes(0, 64, 0) == 0
+    args = [0, 0, 16, 16, None, 0, None, None, None, None, 0.0, 0, 0, None, 16, 16, None, 16, 16,
+            None, None, None, None, None, None, 100, 64]
+    assert lib.mj_residual_norm_backward(*args, 16, need - 1, None) == _lib.MJ_ERR_ARG
+    assert lib.mj_residual_norm_backward(*args, None, need, None) == _lib.MJ_ERR_ARG
+    args[14] = None  # no stats
+    assert lib.mj_residual_norm_backward(*args, 16, need, None) == _lib.MJ_ERR_ARG
+
+
+def test_gated_mlp_status_codes(lib):
+    p = ctypes.c_void_p(16)
+    big = 1 << 40
+    fwd = lambda act, m, k, i, h, x=p, g=None: lib.mj_gated_mlp_bf16(  # noqa: E731
+        x, p, p, p, act, p, g, None, p, m, k, i, h, p, big, None)
+    assert fwd(4, 4, 8, 8, 8) == _lib.MJ_ERR_UNSUPPORTED      # no gradient for the approximations
+    assert fwd(42, 4, 8, 8, 8) == _lib.MJ_ERR_ARG
+    assert fwd(3, -1, 8, 8, 8) == _lib.MJ_ERR_ARG
+    assert fwd(3, 4, 12, 8, 8) == _lib.MJ_ERR_UNSUPPORTED
+    assert fwd(3, 4, 8, 8, 1 << 22) == _lib.MJ_ERR_UNSUPPORTED
+    assert fwd(3, 4, 8, 8, 8, ctypes.c_void_p(8)) == _lib.MJ_ERR_UNSUPPORTED
+    assert fwd(3, 4, 8, 8, 8, None) == _lib.MJ_ERR_ARG
+    assert fwd(3, 4, 8, 8, 8, p, p) == _lib.MJ_ERR_ARG        # g without u
+    assert fwd(3, 0, 8, 8, 8) == _lib.MJ_OK
+    need = lib.mj_gated_mlp_work_bytes(64, 512, 4096, 64, 0)
+    assert need > 0
+    assert lib.mj_gated_mlp_bf16(p, p, p, p, 3, p, None, None, p, 64, 512, 4096, 64, p, need - 1,
+                                 None) == _lib.MJ_ERR_ARG
