@@ -82,6 +82,15 @@ __device__ __forceinline__ float2 act_grad_b16(int act, float g) {
   return make_float2(g, 1.0f);
 }
 
+// Four k of one column for each lane of 16: lanes 4 r + c of a group read 8 bytes each
+// (columns 4 c on of row r) and get column (lane % 16) of the group's four rows.  The
+// restrict on the address gives the read alias information of its own; without any,
+// the compiler holds it to depend on every direct load into LDS in flight and waits
+// for them all (a whole memory latency a fragment).
+__device__ __forceinline__ bf16x4 read_tr(const uint16_t *__restrict__ p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)p);
+}
+
 // One operand of a tile: BR rows of a 64-deep stage, NW waves loading 1 KB each a
 // load, LOADS loads a wave.
 //
@@ -98,64 +107,95 @@ template <int BR, int NW, bool KC>
 struct Operand {
   static constexpr int LOADS = BR / (8 * NW);
   static constexpr int STAGE = BR * kBK;  // elements of a stage buffer
-  static constexpr int READS = KC ? 1 : 2;
-  uint32_t off[LOADS];
-  int kc[LOADS];  // KC: the first k of this lane's chunk
+  static constexpr int UNIT = KC ? 8 : 512 / BR;  // LDS rows of a load
+  uint32_t off;  // this lane's byte offset from the load's first row
+  int kc;        // KC: the first k of this lane's chunk
 
   static __device__ __forceinline__ int piece(int k) {
     return BR == 64 ? ((k >> 1) & 1) | ((k >> 2) & 2) : (k & 3) | ((k >> 1) & 4);
   }
 
-  // row(r): the memory row of tile row r relative to the resource's base, or -1.
-  template <typename Row>
-  __device__ __forceinline__ void init(int64_t ld, int wave, int lane, Row row) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int blk = i * NW + wave;
-      if constexpr (KC) {
-        const int r = blk * 8 + (lane >> 3);
-        kc[i] = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
-        const int src = row(r);
-        off[i] = src >= 0 ? (uint32_t)(src * ld + kc[i]) * 2 : kOobOffset;
-      } else {
-        constexpr int CH = BR / 8;  // 16-byte chunks of an LDS row
-        const int k = blk * (512 / BR) + lane / CH, c = lane % CH;
-        kc[i] = 0;
-        off[i] = (uint32_t)(k * ld + ((((c >> 1) ^ piece(k)) << 1) | (c & 1)) * 8) * 2;
-      }
+  // The swizzles repeat after the NW loads of a round, so a lane's offset is the
+  // same for all its loads; what differs is uniform and goes into the resource.
+  __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
+    if constexpr (KC) {
+      kc = ((lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7)) * 8;
+      off = (uint32_t)((lane >> 3) * ld + kc) * 2;
+    } else {
+      constexpr int CH = BR / 8;  // 16-byte chunks of an LDS row
+      const int k = lane / CH, c = lane % CH;
+      kc = 0;
+      off = (uint32_t)(k * ld + ((((c >> 1) ^ piece(wave * UNIT + k)) << 1) | (c & 1)) * 8) * 2;
     }
+  }
+
+  // First LDS row of load i.
+  static __device__ __forceinline__ int row_of(int i, int wave) { return (i * NW + wave) * UNIT; }
+
+  // The resource of a load from `rows` memory rows (clamped to the load's own; none:
+  // it reads zeros) whose first begins at p, `skip` elements into its row.
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const uint16_t *p, int rows, int ld,
+                                                                int skip) {
+    rows = rows < 0 ? 0 : rows > UNIT ? UNIT : rows;
+    const int bytes = rows == 0 ? 0 : (rows * ld - skip) * 2;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), (short)0, bytes, 0x00020000);
   }
 
   static __device__ __forceinline__ uint16_t *dst(uint16_t *stage, int i, int wave) {
     return stage + (i * NW + wave) * 512;
   }
 
-  // The lane's part of a fragment's LDS address, in elements of the stage: block j
-  // of 16 rows at base ^ (j * 16) (K-strided; j < 8 and base's bits of j clear
-  // before the XOR with the piece) or base + j * 1024 (KC), step ks of 32 k.
+  // The lane's part of a fragment's LDS address in bytes: block j of 16 rows at base +
+  // j * 2048 (KC) or base ^ (j * 32) (K-strided: j < 8, and the bits of j are clear in
+  // base before the XOR with the piece), step ks of 32 k.
   static __device__ __forceinline__ int lane_base(int row0, int ks, int lane) {
     const int fr = lane & 15, fh = lane >> 4;
-    if constexpr (KC) return (row0 + fr) * kBK + (((ks * 4 + fh) ^ ((fr >> 1) & 7)) * 8);
+    if constexpr (KC) return (row0 + fr) * 128 + (((ks * 4 + fh) ^ ((fr >> 1) & 7)) * 16);
     const int k = 8 * fh + (fr >> 2);
-    return (ks * 32 + k) * BR + ((row0 >> 4) ^ piece(k)) * 16 + (fr & 3) * 4;
+    return (ks * 32 + k) * (2 * BR) + ((row0 >> 4) ^ piece(k)) * 32 + (fr & 3) * 8;
   }
 
-  // Half h of block j's fragment (KC: the whole of it, h = 0).
-  static __device__ __forceinline__ void read(bf16x8 &f, const uint16_t *stage, int base, int j,
-                                              int h) {
+  // Block j's fragment.  The K-strided address is formed where it is used (in asm, which
+  // the compiler cannot move out of the loop): eight of them kept in registers spill.
+  static __device__ __forceinline__ void read(bf16x8 &f, const uint16_t *stage, int base, int j) {
+    const char *s = (const char *)stage;
     if constexpr (KC) {
-      f = *(const bf16x8 *)(stage + base + j * 16 * kBK);
+      f = *(const bf16x8 *)(s + base + j * 2048);
     } else {
-      const bf16x4 v =
-          __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4 *)(stage + (base ^ (j * 16)) + h * 4 * BR));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[4 * h + i] = v[i];
+      int at;
+      asm volatile("v_xor_b32 %0, %1, %2" : "=v"(at) : "i"(j * 32), "v"(base));
+      const bf16x4 lo = read_tr((const uint16_t *)(s + at));
+      const bf16x4 hi = read_tr((const uint16_t *)(s + at + 8 * BR));
+      f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
 };
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_from(const uint16_t *p, int64_t elems) {
-  return make_rsrc(p, elems > 0 ? elems * 2 : 0);
+// Load i of an operand's stage at k0 (of K segment seg) of the tile rows from row0 of
+// R into LDS.  FAST: the stage is whole; else chunks past K read zeros, and all do
+// where !in.  PAIR (gate/up): tile rows are WN / 2 of P0's, then the same WN / 2 of
+// P1's, in turn.
+template <typename O, bool KC, bool FAST, bool PAIR, int WN = 1>
+__device__ __forceinline__ void load_block(const O &o, const uint16_t *P0, const uint16_t *P1, int ld,
+                                           int row0, int R, int K, int seg, int k0, bool in,
+                                           uint16_t *dst, int i, int wave) {
+  int r = O::row_of(i, wave);
+  if constexpr (KC) {
+    bool second = seg != 0;
+    if constexpr (PAIR) {
+      second = r % WN >= WN / 2;
+      r = (r / WN) * (WN / 2) + r % (WN / 2);
+    }
+    const uint16_t *p = (second ? P1 : P0) + (int64_t)(row0 + r) * ld + k0;
+    if constexpr (FAST) {
+      dma16(O::rsrc(p, R - row0 - r, ld, k0), dst, o.off);
+    } else {
+      dma16(O::rsrc(p, in ? R - row0 - r : 0, ld, k0), dst, k0 + o.kc < K ? o.off : kOobOffset);
+    }
+  } else {
+    const uint16_t *p = (seg ? P1 : P0) + (int64_t)(k0 + r) * ld + row0;
+    dma16(O::rsrc(p, FAST || in ? K - k0 - r : 0, ld, row0), dst, o.off);
+  }
 }
 
 // Which problem, K slice and tile a workgroup computes.  The problems' tiles form
@@ -348,47 +388,22 @@ __global__ __launch_bounds__(256) void mlp_ring_kernel(TileArgs args) {
   const int kt0 = at.split * per, kt1 = std::min(kt0 + per, stages);
 
   OA oa;
-  oa.init(p.lda, wave, lane, [&](int r) { return m0 + r < p.M ? r : -1; });
+  oa.init(p.lda, wave, lane);
   OB ob;
-  ob.init(p.ldb, wave, lane, [&](int r) {
-    if constexpr (OUT == OUT_GATE) r = (r / WN) * (WN / 2) + r % (WN / 2);
-    return n0 + r < p.N ? r : -1;
-  });
-  // whether load i of this wave fetches up rows (gate/up tiles)
-  auto is_up = [&](int i) { return OUT == OUT_GATE && ((i * NW + wave) * 8) % WN >= WN / 2; };
+  ob.init(p.ldb, wave, lane);
   // stage kt into its ring buffer; past the slice it reads zeros
   auto issue = [&](int kt) __attribute__((always_inline)) {
     const int seg = kt >= nk ? 1 : 0, k0 = (kt - seg * nk) * kBK;
     const bool in = kt < kt1;
     uint16_t *as = lds + (kt % S) * (OA::STAGE + OB::STAGE), *bs = as + OA::STAGE;
-    const int ks = OUT == OUT_GATE ? 0 : seg;
-    if constexpr (AKC) {
-      const auto r = rsrc_from(p.A[seg] + (size_t)m0 * p.lda, in ? (int64_t)(p.M - m0) * p.lda : 0);
 #pragma unroll
-      for (int i = 0; i < OA::LOADS; ++i)
-        dma16(r, OA::dst(as, i, wave), k0 + oa.kc[i] < p.K ? oa.off[i] + k0 * 2 : kOobOffset);
-    } else {
-      const auto r = rsrc_from(p.A[seg] + (size_t)k0 * p.lda + m0,
-                               in ? (int64_t)(p.K - k0) * p.lda - m0 : 0);
+    for (int i = 0; i < OA::LOADS; ++i)
+      load_block<OA, AKC, false, false>(oa, p.A[0], p.A[1], (int)p.lda, m0, p.M, p.K, seg, k0, in,
+                                        OA::dst(as, i, wave), i, wave);
 #pragma unroll
-      for (int i = 0; i < OA::LOADS; ++i) dma16(r, OA::dst(as, i, wave), oa.off[i]);
-    }
-    if constexpr (BKC) {
-      const int64_t left = in ? (int64_t)(p.N - n0) * p.ldb : 0;
-      const auto r = rsrc_from(p.B[ks] + (size_t)n0 * p.ldb, left);
-      const auto r2 = rsrc_from(p.B[OUT == OUT_GATE ? 1 : ks] + (size_t)n0 * p.ldb, left);
-#pragma unroll
-      for (int i = 0; i < OB::LOADS; ++i) {
-        const uint32_t o = k0 + ob.kc[i] < p.K ? ob.off[i] + k0 * 2 : kOobOffset;
-        if (is_up(i)) dma16(r2, OB::dst(bs, i, wave), o);
-        else dma16(r, OB::dst(bs, i, wave), o);
-      }
-    } else {
-      const auto r = rsrc_from(p.B[ks] + (size_t)k0 * p.ldb + n0,
-                               in ? (int64_t)(p.K - k0) * p.ldb - n0 : 0);
-#pragma unroll
-      for (int i = 0; i < OB::LOADS; ++i) dma16(r, OB::dst(bs, i, wave), ob.off[i]);
-    }
+    for (int i = 0; i < OB::LOADS; ++i)
+      load_block<OB, BKC, false, OUT == OUT_GATE, WN>(ob, p.B[0], p.B[1], (int)p.ldb, n0, p.N, p.K,
+                                                      seg, k0, in, OB::dst(bs, i, wave), i, wave);
   };
   f32x4 acc[TM][TN];
 #pragma unroll
@@ -405,13 +420,9 @@ __global__ __launch_bounds__(256) void mlp_ring_kernel(TileArgs args) {
   auto read_frags = [&](int kt, int ks) __attribute__((always_inline)) {
     const uint16_t *as = lds + (kt % S) * (OA::STAGE + OB::STAGE), *bs = as + OA::STAGE;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < TM; ++i) OA::read(fa[ks][i], as, abase[ks], i);
 #pragma unroll
-      for (int h = 0; h < OA::READS; ++h) OA::read(fa[ks][i], as, abase[ks], i, h);
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int h = 0; h < OB::READS; ++h) OB::read(fb[ks][j], bs, bbase[ks], j, h);
+    for (int j = 0; j < TN; ++j) OB::read(fb[ks][j], bs, bbase[ks], j);
   };
   auto mma = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
@@ -445,6 +456,145 @@ __global__ __launch_bounds__(256) void mlp_ring_kernel(TileArgs args) {
   // loads past the slice must not land in a later workgroup's LDS
   __builtin_amdgcn_s_waitcnt(0x0F70);
   tile_out<OUT, TM, TN, WM, WN>(args, p, acc, m0, n0, wm, wn, lane, at.split);
+}
+
+// 256 x 256 tiles with two waves per SIMD: 8 waves laid out 2 x 4, each owning 128 x
+// 64 outputs (gate/up: 32 columns of g and of u), on the pipeline of the framework's
+// large bf16 product (gemm_nt_w8_kernel): two A and three B stage buffers (all 160 KB
+// of LDS), a stage of two 32-deep steps with one barrier between them, each step's
+// fragment reads for the next spread between its MFMAs, four direct loads a step for
+// the stage after next.  A K-strided operand has two 8-byte transposed reads a
+// fragment in place of one of 16 bytes; its resource moves along K with the stage, so
+// its loads need no bounds selects at any K.
+template <bool AKC, bool BKC, int OUT>
+__global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
+  constexpr int BM = 256, BN = 256, NW = 8, WM = 128, WN = 64, TM = 8, TN = 4;
+  constexpr int BN_OUT = OUT == OUT_GATE ? BN / 2 : BN;
+  using OA = Operand<BM, NW, AKC>;
+  using OB = Operand<BN, NW, BKC>;
+  constexpr int DPO = 4;  // direct loads per wave per operand per stage
+  static_assert(OA::LOADS == DPO && OB::LOADS == DPO, "loads per stage");
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+  uint16_t *As = lds;                   // stage kt in buffer kt % 2
+  uint16_t *Bs = lds + 2 * OA::STAGE;   // stage kt in buffer kt % 3
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const TileAt at = locate(args);
+  const TileProb &p = args.p[at.prob];
+  const int m0 = at.m * BM, n0 = at.n * BN_OUT;
+  const int M = p.M, N = p.N, K = p.K;
+  const int lda = (int)p.lda, ldb = (int)p.ldb;
+  const uint16_t *const A0 = p.A[0], *const A1 = p.A[1], *const B0 = p.B[0], *const B1 = p.B[1];
+  const int nk = (K + kBK - 1) / kBK, stages = nk * p.segs;
+
+  OA oa;
+  oa.init(lda, wave, lane);
+  OB ob;
+  ob.init(ldb, wave, lane);
+  // direct load d of stage kt into buffer buf: d < 4 is A block d, else B block d - 4
+  auto load = [&](auto fast, int kt, int buf, int d) __attribute__((always_inline)) {
+    constexpr bool FAST = decltype(fast)::value;
+    const int seg = kt >= nk ? 1 : 0, k0 = (kt - seg * nk) * kBK;
+    const bool in = kt < stages;
+    const int i = d & 3;
+    if (d < DPO)
+      load_block<OA, AKC, FAST, false>(oa, A0, A1, lda, m0, M, K, seg, k0, in,
+                                       OA::dst(As + buf * OA::STAGE, i, wave), i, wave);
+    else
+      load_block<OB, BKC, FAST, OUT == OUT_GATE, WN>(ob, B0, B1, ldb, n0, N, K, seg, k0, in,
+                                                     OB::dst(Bs + buf * OB::STAGE, i, wave), i,
+                                                     wave);
+  };
+
+  int abase[2], bbase[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    abase[ks] = OA::lane_base(wm * WM, ks, lane);
+    bbase[ks] = OB::lane_base(wn * WN, ks, lane);
+  }
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  bf16x8 fa[2][TM], fb[2][TN];
+  // the 12 fragments of a step: A's blocks, then B's, three a group
+  constexpr int PER = (TM + TN) / TN;
+  auto read_frag = [&](int t, int dst, int abuf, int bbuf) __attribute__((always_inline)) {
+    if (t < TM) OA::read(fa[dst][t], As + abuf * OA::STAGE, abase[dst], t);
+    else OB::read(fb[dst][t - TM], Bs + bbuf * OB::STAGE, bbase[dst], t - TM);
+  };
+
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int d = 0; d < 2 * DPO; ++d) load(std::false_type(), s, s, d);
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * DPO));  // stage 0
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int t = 0; t < TM + TN; ++t) read_frag(t, 0, 0, 0);
+  __builtin_amdgcn_s_waitcnt(kLgkm0);
+  asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");  // zero fill -> first MFMAs
+
+  auto stage = [&](auto ab_c, auto bb_c, auto fast, int kt) __attribute__((always_inline)) {
+    constexpr int AB = decltype(ab_c)::value;
+    constexpr int BB = decltype(bb_c)::value;
+    auto group = [&](int j, int src, int dst, int abuf, int bbuf, int load_d,
+                     int load_buf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        __builtin_amdgcn_sched_barrier(0);
+        read_frag(PER * j + u, dst, abuf, bbuf);
+        __builtin_amdgcn_sched_barrier(0);
+        mfma_16x16x32_tied(acc[u][j], fb[src][j], fa[src][u]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load(fast, kt + 2, load_buf, load_d);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = PER; i < TM; ++i) mfma_16x16x32_tied(acc[i][j], fb[src][j], fa[src][i]);
+    };
+    // step 0; B loads of stage kt+2 into B buffer (BB + 2) % 3
+#pragma unroll
+    for (int j = 0; j < TN; ++j) group(j, 0, 1, AB, BB, DPO + j, (BB + 2) % 3);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kLgkm0);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | DPO);  // all but this step's B loads
+    asm volatile("s_barrier" ::: "memory");
+    // step 1; A loads of stage kt+2 into A buffer AB
+#pragma unroll
+    for (int j = 0; j < TN; ++j) group(j, 1, 0, AB ^ 1, (BB + 1) % 3, j, AB);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kLgkm0);
+  };
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using F = std::true_type;
+  using S = std::false_type;
+  // stages up to here are whole; K-strided operands end by their resource alone
+  const int whole = K % kBK == 0 ? stages : (p.segs == 1 ? K / kBK : 0);
+  int kt = 0;
+  for (; kt + 8 <= whole; kt += 6) {
+    stage(I0(), I0(), F(), kt);
+    stage(I1(), I1(), F(), kt + 1);
+    stage(I0(), I2(), F(), kt + 2);
+    stage(I1(), I0(), F(), kt + 3);
+    stage(I0(), I1(), F(), kt + 4);
+    stage(I1(), I2(), F(), kt + 5);
+  }
+  for (; kt < stages; kt += 6) {
+    stage(I0(), I0(), S(), kt);
+    if (kt + 1 < stages) stage(I1(), I1(), S(), kt + 1);
+    if (kt + 2 < stages) stage(I0(), I2(), S(), kt + 2);
+    if (kt + 3 < stages) stage(I1(), I0(), S(), kt + 3);
+    if (kt + 4 < stages) stage(I0(), I1(), S(), kt + 4);
+    if (kt + 5 < stages) stage(I1(), I2(), S(), kt + 5);
+  }
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  tile_out<OUT, TM, TN, WM, WN>(args, p, acc, m0, n0, wm, wn, lane, 0);
 }
 
 // C = bf16(sum of the K slices' partials, in slice order), 8 elements a thread.
@@ -553,6 +703,18 @@ hipError_t launch_ring(TileArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <bool AKC, bool BKC, int OUT>
+hipError_t launch_w8(TileArgs a, hipStream_t stream) {
+  constexpr size_t lds = size_t(2 * 256 + 3 * 256) * kBK * sizeof(uint16_t);  // 160 KB
+  auto kern = mlp_w8_kernel<AKC, BKC, OUT>;
+  static std::atomic<uint64_t> done{0};
+  if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
+  set_tiles(a, 256, OUT == OUT_GATE ? 128 : 256);
+  if (a.tiles == 0) return hipSuccess;
+  hipLaunchKernelGGL(kern, dim3((unsigned)a.tiles), dim3(512), lds, stream, a);
+  return hipGetLastError();
+}
+
 int64_t tiles_of(const TileArgs &a, int bm, int bn) {
   int64_t t = 0;
   for (int i = 0; i < a.n; ++i)
@@ -563,6 +725,7 @@ int64_t tiles_of(const TileArgs &a, int bm, int bn) {
 template <bool AKC, bool BKC, int OUT>
 hipError_t launch_tiles(const TileArgs &a, hipStream_t stream) {
   const int half = OUT == OUT_GATE ? 2 : 1;
+  if (tiles_of(a, 256, 256 / half) >= 160) return launch_w8<AKC, BKC, OUT>(a, stream);
   if (tiles_of(a, 128, 128 / half) >= 256)
     return launch_ring<128, 128, 3, AKC, BKC, OUT>(a, stream);
   return launch_ring<64, 64, 3, AKC, BKC, OUT>(a, stream);

@@ -55,7 +55,7 @@ def mlp(x, wg, wu, wd, dy, name, unit, e32):
     is the relative error of a rounding to the operands' type (2^-8 for bf16's 8
     significant bits: h, dg, du and the outputs), e32 the relative error of an fp32 sum
     against the sum of its terms' magnitudes."""
-    x, wg, wu, wd, dy = (t.double().cpu() for t in (x, wg, wu, wd, dy))
+    x, wg, wu, wd, dy = (t.double() for t in (x, wg, wu, wd, dy))
     g, u, dh = x @ wg.t(), x @ wu.t(), dy @ wd
     eg, eu = e32 * (x.abs() @ wg.abs().t()), e32 * (x.abs() @ wu.abs().t())
     edh = e32 * (dy.abs() @ wd.abs())

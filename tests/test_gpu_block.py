@@ -32,7 +32,7 @@ def _gen(*key):
 
 
 def _close(got, want, bound, name):
-    got = got.double().cpu()
+    got = got.to(want.device, torch.float64)
     assert got.shape == want.shape, (name, got.shape, want.shape)
     bad = ~((got - want).abs() <= bound)
     assert not bool(bad.any()), (
@@ -42,11 +42,12 @@ def _close(got, want, bound, name):
 
 # ------------------------------------------------------------------ gated MLP
 # tokens, K, I, H: one token, decode sizes, widths below and across a tile, tokens
-# across 16 / 64 / 128 / 256 rows, odd widths (padded in bf16)
+# across 16 / 64 / 128 / 256 rows, odd widths (padded in bf16); the last two fill the
+# chip with 256 x 256 tiles in every product, with and without K edges
 _MLP = [(1, 64, 64, 64), (1, 1024, 2816, 1024), (2, 8, 8, 8), (3, 1, 1, 1), (5, 33, 47, 29),
         (16, 256, 704, 256), (17, 520, 264, 136), (48, 512, 1376, 512), (65, 96, 200, 328),
         (129, 264, 520, 72), (200, 1001, 999, 77), (257, 128, 1000, 640), (300, 640, 1728, 640),
-        (700, 520, 1400, 520)]
+        (700, 520, 1400, 520), (4001, 2600, 5000, 2568), (4096, 2560, 5120, 2560)]
 
 
 def _mlp_inputs(m, k, i, h, dt):
