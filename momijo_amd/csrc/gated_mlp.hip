@@ -383,27 +383,70 @@ __global__ __launch_bounds__(256) void mlp_ring_kernel(TileArgs args) {
   const TileAt at = locate(args);
   const TileProb &p = args.p[at.prob];
   const int m0 = at.m * BM, n0 = at.n * BN_OUT;
-  const int nk = (p.K + kBK - 1) / kBK, stages = nk * p.segs;
+  const int M = p.M, N = p.N, K = p.K;
+  const int lda = (int)p.lda, ldb = (int)p.ldb;
+  const uint16_t *const A0 = p.A[0], *const A1 = p.A[1], *const B0 = p.B[0], *const B1 = p.B[1];
+  const int nk = (K + kBK - 1) / kBK, stages = nk * p.segs;
   const int per = (stages + args.splits - 1) / args.splits;
   const int kt0 = at.split * per, kt1 = std::min(kt0 + per, stages);
 
   OA oa;
-  oa.init(p.lda, wave, lane);
+  oa.init(lda, wave, lane);
   OB ob;
-  ob.init(p.ldb, wave, lane);
+  ob.init(ldb, wave, lane);
+  // byte offsets of each load's rows from the tile's (K-contiguous: rows past the edge
+  // read zeros) or the stage's first
+  uint32_t aoff[OA::LOADS], boff[OB::LOADS];
+#pragma unroll
+  for (int i = 0; i < OA::LOADS; ++i) {
+    const int r = OA::row_of(i, wave);
+    aoff[i] = !AKC || m0 + r + (lane >> 3) < M ? oa.off + (uint32_t)r * lda * 2 : kOobOffset;
+  }
+#pragma unroll
+  for (int i = 0; i < OB::LOADS; ++i) {
+    int r = OB::row_of(i, wave);
+    if constexpr (OUT == OUT_GATE) r = (r / WN) * (WN / 2) + r % (WN / 2);
+    boff[i] = !BKC || n0 + r + (lane >> 3) < N ? ob.off + (uint32_t)r * ldb * 2 : kOobOffset;
+  }
+  // whether load i fetches up rows (gate/up tiles)
+  auto is_up = [&](int i) { return OUT == OUT_GATE && OB::row_of(i, wave) % WN >= WN / 2; };
+  auto tile_rsrc = [&](const uint16_t *P, int row0, int R, int ld) {
+    return make_rsrc(P + (size_t)row0 * ld, (int64_t)(R - row0) * ld * 2);
+  };
+  auto stage_rsrc = [&](const uint16_t *P, int row0, int k0, int left, int ld) {
+    const int rows = left < 0 ? 0 : left > kBK ? kBK : left;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(P + (int64_t)k0 * ld + row0),
+                                             (short)0, rows ? (rows * ld - row0) * 2 : 0, 0x00020000);
+  };
   // stage kt into its ring buffer; past the slice it reads zeros
   auto issue = [&](int kt) __attribute__((always_inline)) {
     const int seg = kt >= nk ? 1 : 0, k0 = (kt - seg * nk) * kBK;
-    const bool in = kt < kt1;
+    const int Kin = kt < kt1 ? K : 0;
     uint16_t *as = lds + (kt % S) * (OA::STAGE + OB::STAGE), *bs = as + OA::STAGE;
+    if constexpr (AKC) {
+      const auto r = tile_rsrc(seg ? A1 : A0, m0, M, lda);
 #pragma unroll
-    for (int i = 0; i < OA::LOADS; ++i)
-      load_block<OA, AKC, false, false>(oa, p.A[0], p.A[1], (int)p.lda, m0, p.M, p.K, seg, k0, in,
-                                        OA::dst(as, i, wave), i, wave);
+      for (int i = 0; i < OA::LOADS; ++i)
+        dma16(r, OA::dst(as, i, wave), k0 + oa.kc < Kin ? aoff[i] + k0 * 2 : kOobOffset);
+    } else {
+      const auto r = stage_rsrc(seg ? A1 : A0, m0, k0, Kin - k0, lda);
 #pragma unroll
-    for (int i = 0; i < OB::LOADS; ++i)
-      load_block<OB, BKC, false, OUT == OUT_GATE, WN>(ob, p.B[0], p.B[1], (int)p.ldb, n0, p.N, p.K,
-                                                      seg, k0, in, OB::dst(bs, i, wave), i, wave);
+      for (int i = 0; i < OA::LOADS; ++i) dma16(r, OA::dst(as, i, wave), aoff[i]);
+    }
+    if constexpr (BKC) {
+      const auto r = tile_rsrc(OUT != OUT_GATE && seg ? B1 : B0, n0, N, ldb);
+      const auto r2 = tile_rsrc(OUT == OUT_GATE ? B1 : B0, n0, N, ldb);
+#pragma unroll
+      for (int i = 0; i < OB::LOADS; ++i) {
+        const uint32_t o = k0 + ob.kc < Kin ? boff[i] + k0 * 2 : kOobOffset;
+        if (is_up(i)) dma16(r2, OB::dst(bs, i, wave), o);
+        else dma16(r, OB::dst(bs, i, wave), o);
+      }
+    } else {
+      const auto r = stage_rsrc(seg ? B1 : B0, n0, k0, Kin - k0, ldb);
+#pragma unroll
+      for (int i = 0; i < OB::LOADS; ++i) dma16(r, OB::dst(bs, i, wave), boff[i]);
+    }
   };
   f32x4 acc[TM][TN];
 #pragma unroll
@@ -487,6 +530,8 @@ __global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
   const int lda = (int)p.lda, ldb = (int)p.ldb;
   const uint16_t *const A0 = p.A[0], *const A1 = p.A[1], *const B0 = p.B[0], *const B1 = p.B[1];
   const int nk = (K + kBK - 1) / kBK, stages = nk * p.segs;
+  const int per = (stages + args.splits - 1) / args.splits;
+  const int kt0 = at.split * per, kt1 = std::min(kt0 + per, stages);
 
   OA oa;
   oa.init(lda, wave, lane);
@@ -496,7 +541,7 @@ __global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
   auto load = [&](auto fast, int kt, int buf, int d) __attribute__((always_inline)) {
     constexpr bool FAST = decltype(fast)::value;
     const int seg = kt >= nk ? 1 : 0, k0 = (kt - seg * nk) * kBK;
-    const bool in = kt < stages;
+    const bool in = kt < kt1;
     const int i = d & 3;
     if (d < DPO)
       load_block<OA, AKC, FAST, false>(oa, A0, A1, lda, m0, M, K, seg, k0, in,
@@ -529,7 +574,7 @@ __global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int d = 0; d < 2 * DPO; ++d) load(std::false_type(), s, s, d);
+    for (int d = 0; d < 2 * DPO; ++d) load(std::false_type(), kt0 + s, s, d);
   __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * DPO));  // stage 0
   asm volatile("s_barrier" ::: "memory");
 #pragma unroll
@@ -574,8 +619,8 @@ __global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
   using F = std::true_type;
   using S = std::false_type;
   // stages up to here are whole; K-strided operands end by their resource alone
-  const int whole = K % kBK == 0 ? stages : (p.segs == 1 ? K / kBK : 0);
-  int kt = 0;
+  const int whole = std::min(kt1, K % kBK == 0 ? stages : (p.segs == 1 ? K / kBK : 0));
+  int kt = kt0;
   for (; kt + 8 <= whole; kt += 6) {
     stage(I0(), I0(), F(), kt);
     stage(I1(), I1(), F(), kt + 1);
@@ -584,17 +629,17 @@ __global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
     stage(I0(), I1(), F(), kt + 4);
     stage(I1(), I2(), F(), kt + 5);
   }
-  for (; kt < stages; kt += 6) {
+  for (; kt < kt1; kt += 6) {
     stage(I0(), I0(), S(), kt);
-    if (kt + 1 < stages) stage(I1(), I1(), S(), kt + 1);
-    if (kt + 2 < stages) stage(I0(), I2(), S(), kt + 2);
-    if (kt + 3 < stages) stage(I1(), I0(), S(), kt + 3);
-    if (kt + 4 < stages) stage(I0(), I1(), S(), kt + 4);
-    if (kt + 5 < stages) stage(I1(), I2(), S(), kt + 5);
+    if (kt + 1 < kt1) stage(I1(), I1(), S(), kt + 1);
+    if (kt + 2 < kt1) stage(I0(), I2(), S(), kt + 2);
+    if (kt + 3 < kt1) stage(I1(), I0(), S(), kt + 3);
+    if (kt + 4 < kt1) stage(I0(), I1(), S(), kt + 4);
+    if (kt + 5 < kt1) stage(I1(), I2(), S(), kt + 5);
   }
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0F70);
-  tile_out<OUT, TM, TN, WM, WN>(args, p, acc, m0, n0, wm, wn, lane, 0);
+  tile_out<OUT, TM, TN, WM, WN>(args, p, acc, m0, n0, wm, wn, lane, at.split);
 }
 
 // C = bf16(sum of the K slices' partials, in slice order), 8 elements a thread.
@@ -711,9 +756,29 @@ hipError_t launch_w8(TileArgs a, hipStream_t stream) {
   if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
   set_tiles(a, 256, OUT == OUT_GATE ? 128 : 256);
   if (a.tiles == 0) return hipSuccess;
-  hipLaunchKernelGGL(kern, dim3((unsigned)a.tiles), dim3(512), lds, stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.splits)), dim3(512), lds, stream, a);
   return hipGetLastError();
 }
+
+// The tile kernels' times on MI355X (us): a launch, then for each round of workgroups
+// that the CUs hold (per_cu each) the stages at the time of a 64-deep stage with 1, 2,
+// .. workgroups per CU and the fixed part of a round (first loads and, by kind,
+// output).  Fits to products of 48 to 4096 rows, widths 512 to 11008, e.g. h of 512
+// rows (K = 4096, 11008 columns): 256 x 256 97, 128 x 64 147, 64 x 64 160; of 300 rows
+// (K = 1024, 2816 columns) 35, 16.7, 13.1; of 48 rows (11008) 82, 45, and 64 x 64
+// 40.2 with three stages, 34.1 with five (one or two workgroups a CU wait on memory).
+enum : int { T_256 = 0, T_64S3, T_64S5, T_128X64, T_COUNT };
+struct TileCost {
+  int bm, bn, per_cu;
+  double stage[3], fixed[4];  // fixed by OUT_*
+};
+constexpr TileCost kTileCost[T_COUNT] = {
+    {256, 256, 1, {1.47, 0, 0}, {7, 7, 8, 14}},
+    {64, 64, 3, {0.48, 0.52, 0.62}, {2.1, 2.1, 3, 4}},
+    {64, 64, 2, {0.31, 0.48, 0}, {2.1, 2.1, 3, 4}},
+    {128, 64, 2, {0.45, 0.70, 0}, {2.5, 2.5, 4, 6}},
+};
+constexpr int64_t kCUs = 256;
 
 int64_t tiles_of(const TileArgs &a, int bm, int bn) {
   int64_t t = 0;
@@ -722,45 +787,104 @@ int64_t tiles_of(const TileArgs &a, int bm, int bn) {
   return t;
 }
 
+double tile_time_us(const TileCost &c, int out, int64_t wgs, int64_t stages) {
+  const int64_t slots = kCUs * c.per_cu, rest = wgs % slots;
+  double us = 3.0 + (double)(wgs / slots) * (c.fixed[out] + (double)stages * c.stage[c.per_cu - 1]);
+  if (rest) us += c.fixed[out] + (double)stages * c.stage[(rest + kCUs - 1) / kCUs - 1];
+  return us;
+}
+
+struct TilePlan {
+  int tile = T_64S3, splits = 1;
+};
+
+// The tile, and for a plain product the K slices, of the least predicted time.  The
+// slices' partials (fp32, written and read once, and their launch) pay where the
+// tiles leave CUs idle: 512 x 4096 with K = 11008 is 32 tiles of 256 x 256, 58 us in 8
+// slices; 67 on 128 x 64 tiles in 2, the best of the smaller tiles.
+TilePlan plan_tiles(const TileArgs &a, int out) {
+  TilePlan best;
+  double best_us = 1e30;
+  const TileProb &p = a.p[0];
+  const int64_t stages = (int64_t)((p.K + kBK - 1) / kBK) * p.segs;
+  for (int t = 0; t < T_COUNT; ++t) {
+    const TileCost &c = kTileCost[t];
+    const int64_t tiles = tiles_of(a, c.bm, out == OUT_GATE ? c.bn / 2 : c.bn);
+    for (int s = 1; s <= (out == OUT_STORE && a.n == 1 ? 16 : 1); s *= 2) {
+      if (s > 1 && (stages / s < 4 || tiles * s > 2 * kCUs * c.per_cu)) break;
+      double us = tile_time_us(c, s > 1 ? OUT_PART : out, tiles * s, (stages + s - 1) / s);
+      if (s > 1) us += 2.5 + (8.0 * s + 2.0) * (double)p.M * (double)p.N / 8.0e6;
+      if (us < best_us) {
+        best_us = us;
+        best.tile = t;
+        best.splits = s;
+      }
+    }
+  }
+  return best;
+}
+
+template <bool AKC, bool BKC, int OUT>
+hipError_t launch_tile_kernel(int tile, const TileArgs &a, hipStream_t stream) {
+  switch (tile) {
+    case T_256: return launch_w8<AKC, BKC, OUT>(a, stream);
+    case T_64S3: return launch_ring<64, 64, 3, AKC, BKC, OUT>(a, stream);
+    case T_64S5: return launch_ring<64, 64, 5, AKC, BKC, OUT>(a, stream);
+    default: return launch_ring<128, 64, 3, AKC, BKC, OUT>(a, stream);
+  }
+}
+
 template <bool AKC, bool BKC, int OUT>
 hipError_t launch_tiles(const TileArgs &a, hipStream_t stream) {
-  const int half = OUT == OUT_GATE ? 2 : 1;
-  if (tiles_of(a, 256, 256 / half) >= 160) return launch_w8<AKC, BKC, OUT>(a, stream);
-  if (tiles_of(a, 128, 128 / half) >= 256)
-    return launch_ring<128, 128, 3, AKC, BKC, OUT>(a, stream);
-  return launch_ring<64, 64, 3, AKC, BKC, OUT>(a, stream);
+  return launch_tile_kernel<AKC, BKC, OUT>(plan_tiles(a, OUT).tile, a, stream);
 }
 
-// K slices of a plain product with too few tiles to fill the CUs.
-int plan_splits(int64_t M, int64_t N, int64_t stages) {
-  const int64_t tiles = ((M + 63) / 64) * ((N + 63) / 64);
-  int s = 1;
-  while (s < 16 && tiles * s * 2 <= 512 && stages / (s * 2) >= 8) s *= 2;
-  return s;
-}
-
-// A plain product, its K split where that fills the CUs.
+// A plain product, its K split where the plan says; `part` holds splits * M * N floats.
 template <bool AKC, bool BKC>
 hipError_t launch_plain(TileArgs a, float *part, hipStream_t stream) {
   const TileProb &p = a.p[0];
-  const int s = plan_splits(p.M, p.N, (int64_t)((p.K + kBK - 1) / kBK) * p.segs);
-  if (s == 1) return launch_tiles<AKC, BKC, OUT_STORE>(a, stream);
-  a.splits = s;
+  if (p.M == 0 || p.N == 0) return hipSuccess;
+  const TilePlan pl = plan_tiles(a, OUT_STORE);
+  if (pl.splits == 1) return launch_tile_kernel<AKC, BKC, OUT_STORE>(pl.tile, a, stream);
+  a.splits = pl.splits;
   a.p[0].part = part;
-  if (hipError_t e = launch_ring<64, 64, 3, AKC, BKC, OUT_PART>(a, stream); e != hipSuccess)
+  if (hipError_t e = launch_tile_kernel<AKC, BKC, OUT_PART>(pl.tile, a, stream); e != hipSuccess)
     return e;
   const int64_t n = (int64_t)p.M * p.N;
   hipLaunchKernelGGL(mlp_reduce_kernel, dim3((unsigned)((n / 8 + 255) / 256)), dim3(256), 0, stream,
-                     part, p.C, n, s);
+                     part, p.C, n, pl.splits);
   return hipGetLastError();
+}
+
+// The plain products that may split K: y, and dx with its two segments.
+TileArgs down_args(const GatedMlp &q) {
+  TileArgs a;
+  TileProb &p = a.p[0];
+  p.A[0] = q.h, p.lda = q.I;
+  p.B[0] = q.wd, p.ldb = q.I;
+  p.M = (int)q.M, p.N = (int)q.H, p.K = (int)q.I;
+  p.C = q.y, p.ldc = q.H;
+  return a;
+}
+
+TileArgs dx_args(const GatedMlp &q, const GatedMlpGrad &o) {
+  TileArgs a;
+  TileProb &p = a.p[0];
+  p.A[0] = o.dg, p.A[1] = o.du, p.lda = q.I;
+  p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
+  p.M = (int)q.M, p.N = (int)q.K, p.K = (int)q.I, p.segs = 2;
+  p.C = o.dx, p.ldc = q.K;
+  return a;
 }
 
 }  // namespace
 
 int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward) {
-  const int64_t stages = (I + kBK - 1) / kBK * (backward ? 2 : 1), N = backward ? K : H;
-  const int s = plan_splits(M, N, stages);
-  return s > 1 ? s * M * N : 0;
+  GatedMlp q;
+  q.M = M, q.K = K, q.I = I, q.H = H;
+  const TileArgs a = backward ? dx_args(q, GatedMlpGrad()) : down_args(q);
+  const int s = plan_tiles(a, OUT_STORE).splits;
+  return s > 1 ? (int64_t)s * a.p[0].M * a.p[0].N : 0;
 }
 
 hipError_t launch_gated_mlp(const GatedMlp &q, hipStream_t stream) {
@@ -772,13 +896,7 @@ hipError_t launch_gated_mlp(const GatedMlp &q, hipStream_t stream) {
   p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.K;
   p.C = q.h, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
   if (hipError_t e = launch_tiles<true, true, OUT_GATE>(a, stream); e != hipSuccess) return e;
-  TileArgs b;
-  TileProb &d = b.p[0];
-  d.A[0] = q.h, d.lda = q.I;
-  d.B[0] = q.wd, d.ldb = q.I;
-  d.M = (int)q.M, d.N = (int)q.H, d.K = (int)q.I;
-  d.C = q.y, d.ldc = q.H;
-  return launch_plain<true, true>(b, q.part, stream);
+  return launch_plain<true, true>(down_args(q), q.part, stream);
 }
 
 hipError_t launch_gated_mlp_bwd(const GatedMlp &q, const GatedMlpGrad &o, hipStream_t stream) {
@@ -792,15 +910,9 @@ hipError_t launch_gated_mlp_bwd(const GatedMlp &q, const GatedMlpGrad &o, hipStr
     p.C = o.dg, p.C2 = o.du, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
     if (hipError_t e = launch_tiles<true, false, OUT_DGATE>(a, stream); e != hipSuccess) return e;
   }
-  if (o.dx) {
-    TileArgs a;
-    TileProb &p = a.p[0];
-    p.A[0] = o.dg, p.A[1] = o.du, p.lda = q.I;
-    p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
-    p.M = (int)q.M, p.N = (int)q.K, p.K = (int)q.I, p.segs = 2;
-    p.C = o.dx, p.ldc = q.K;
-    if (hipError_t e = launch_plain<true, false>(a, q.part, stream); e != hipSuccess) return e;
-  }
+  if (o.dx)
+    if (hipError_t e = launch_plain<true, false>(dx_args(q, o), q.part, stream); e != hipSuccess)
+      return e;
   TileArgs w;
   w.n = 0;
   auto add = [&](const uint16_t *A, int64_t rows, const uint16_t *B, int64_t cols, uint16_t *C) {
