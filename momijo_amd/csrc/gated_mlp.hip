@@ -659,6 +659,103 @@ __global__ __launch_bounds__(256) void mlp_reduce_kernel(const float *part, uint
                                  pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
+// ---------------------------------------------------------------- few rows
+// Products of at most 16 MB rows: bound by reading the weights once.  A workgroup of NW
+// waves owns 16 weight rows (gate/up: 16 of each) and splits K, 64 at a time dealt to
+// the waves in turn, so each 128-byte line of a weight row is read by two loads of one
+// wave; a lane's 16 bytes are a row's 8 k, which is a fragment of
+// v_mfma_f32_16x16x32_bf16 as it is.  x comes from the caches the same way (rows past M
+// are zeros).  DEPTH slices of 64 are in flight a wave; no LDS in the loop.  The waves'
+// sums are added in wave order and act, g, u, h (or y) follow in the same launch.
+struct SkinnyArgs {
+  const uint16_t *x = nullptr, *w = nullptr, *w2 = nullptr;
+  uint16_t *C = nullptr;
+  float *F = nullptr, *F2 = nullptr;
+  int M = 0, N = 0, K = 0, act = 0;
+};
+
+template <bool GATE, int MB, int DEPTH, int NW = 8>
+__global__ __launch_bounds__(NW * 64) void mlp_skinny_kernel(SkinnyArgs p) {
+  constexpr int G = GATE ? 2 : 1;
+  __shared__ float red[NW][G][MB][16][17];
+  const int lane = threadIdx.x & 63, fr = lane & 15, fh = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16, M = p.M, N = p.N, K = p.K;
+  const int rows = N - n0 < 16 ? N - n0 : 16;
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + (size_t)n0 * K, (int64_t)rows * K * 2);
+  const __amdgpu_buffer_rsrc_t rw2 =
+      make_rsrc((GATE ? p.w2 : p.w) + (size_t)n0 * K, (int64_t)rows * K * 2);
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (int64_t)M * K * 2);
+  const uint32_t wo = fr < rows ? (uint32_t)(fr * K) * 2 : kOobOffset;
+  uint32_t xo[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) xo[b] = b * 16 + fr < M ? (uint32_t)((b * 16 + fr) * K) * 2 : kOobOffset;
+  f32x4 acc[G][MB];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) acc[g][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  uint4 wv[DEPTH][2][G], xv[DEPTH][2][MB];
+  auto load = [&](int s, int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = k0 + 32 * h + 8 * fh;
+      const bool in = k < K;
+      wv[s][h][0] = buffer_load16(rw, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
+      if constexpr (GATE)
+        wv[s][h][1] = buffer_load16(rw2, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+        xv[s][h][b] = buffer_load16(rx, in && xo[b] != kOobOffset ? xo[b] + k * 2 : kOobOffset);
+    }
+  };
+  const int step = NW * 64;
+#pragma unroll
+  for (int s = 0; s < DEPTH; ++s) load(s, wave * 64 + s * step);
+  for (int k0 = wave * 64; k0 < K; k0 += DEPTH * step) {
+#pragma unroll
+    for (int s = 0; s < DEPTH; ++s) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int b = 0; b < MB; ++b)
+            acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8, wv[s][h][g]), __builtin_bit_cast(bf16x8, xv[s][h][b]),
+                acc[g][b], 0, 0, 0);
+      load(s, k0 + (DEPTH + s) * step);
+    }
+  }
+  // block (g, b): weight row 4 fh + q, x row 16 b + fr
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) red[wave][g][b][fr][4 * fh + q] = acc[g][b][q];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MB * 256; e += NW * 64) {
+    const int b = e >> 8, r = (e >> 4) & 15, c = e & 15, m = b * 16 + r, n = n0 + c;
+    if (m >= M || n >= N) continue;
+    float v[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      v[g] = red[0][g][b][r][c];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v[g] += red[w][g][b][r][c];
+    }
+    const size_t at = (size_t)m * N + n;
+    if constexpr (GATE) {
+      if (p.F) p.F[at] = v[0], p.F2[at] = v[1];
+      p.C[at] = (uint16_t)f32_to_bf16_bits(act_b16(p.act, v[0]) * v[1]);
+    } else {
+      p.C[at] = (uint16_t)f32_to_bf16_bits(v[0]);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- fp32 block
 __device__ __forceinline__ float2 act_grad_f32(int act, float g) {
   if (act == EPI_SILU) {
@@ -839,6 +936,32 @@ hipError_t launch_tiles(const TileArgs &a, hipStream_t stream) {
   return launch_tile_kernel<AKC, BKC, OUT>(plan_tiles(a, OUT).tile, a, stream);
 }
 
+// Up to 16 rows always; 17 to 32 where the weights are small (one launch instead of a K
+// split's two, and latency counts): K = 1024, 2816 gate/up columns 6.4 us against 8.8 on
+// tiles, K = 1408, 512 columns 5.8 against 7.9; at K = 2048, 5504 columns 18.7 against
+// 13.9 (x is read again for every 16 weight rows).
+bool skinny_takes(int64_t M, int64_t N, int64_t K) {
+  return M <= 16 || (M <= 32 && N * K <= 3000000);
+}
+
+// One slice of 64 k in flight a wave: 4096 x 11008 gate/up of one row 34.6 us (5.2 TB/s)
+// against 36.3, 37.1, 37.5 with two, three, four (a wave's eight slices end sooner, and
+// more workgroups fit a CU).  Sixteen waves for one long row: K = 11008, 4096 columns
+// 20.6 us against 22.2 at one row (256 workgroups, one a CU), but 26.5 against 24.7 at
+// 16 rows and 8.3 against 8.1 at K = 5504.
+template <bool GATE>
+hipError_t launch_skinny(const SkinnyArgs &a, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.N + 15) / 16));
+  if (a.N == 0) return hipSuccess;
+  if (a.M > 16)
+    hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 2, 1, 8>), grid, dim3(512), 0, stream, a);
+  else if (!GATE && a.M <= 4 && a.K >= 8192)
+    hipLaunchKernelGGL((mlp_skinny_kernel<false, 1, 1, 16>), grid, dim3(1024), 0, stream, a);
+  else
+    hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 1, 1, 8>), grid, dim3(512), 0, stream, a);
+  return hipGetLastError();
+}
+
 // A plain product, its K split where the plan says; `part` holds splits * M * N floats.
 template <bool AKC, bool BKC>
 hipError_t launch_plain(TileArgs a, float *part, hipStream_t stream) {
@@ -882,21 +1005,34 @@ TileArgs dx_args(const GatedMlp &q, const GatedMlpGrad &o) {
 int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward) {
   GatedMlp q;
   q.M = M, q.K = K, q.I = I, q.H = H;
+  if (!backward && skinny_takes(M, H, I)) return 0;
   const TileArgs a = backward ? dx_args(q, GatedMlpGrad()) : down_args(q);
   const int s = plan_tiles(a, OUT_STORE).splits;
   return s > 1 ? (int64_t)s * a.p[0].M * a.p[0].N : 0;
 }
 
 hipError_t launch_gated_mlp(const GatedMlp &q, hipStream_t stream) {
-  TileArgs a;
-  a.act = q.act;
-  TileProb &p = a.p[0];
-  p.A[0] = q.x, p.lda = q.K;
-  p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
-  p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.K;
-  p.C = q.h, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
-  if (hipError_t e = launch_tiles<true, true, OUT_GATE>(a, stream); e != hipSuccess) return e;
-  return launch_plain<true, true>(down_args(q), q.part, stream);
+  if (q.M == 0) return hipSuccess;
+  if (skinny_takes(q.M, q.I, q.K)) {
+    SkinnyArgs a;
+    a.x = q.x, a.w = q.wg, a.w2 = q.wu, a.C = q.h, a.F = q.g, a.F2 = q.u;
+    a.M = (int)q.M, a.N = (int)q.I, a.K = (int)q.K, a.act = q.act;
+    if (hipError_t e = launch_skinny<true>(a, stream); e != hipSuccess) return e;
+  } else {
+    TileArgs a;
+    a.act = q.act;
+    TileProb &p = a.p[0];
+    p.A[0] = q.x, p.lda = q.K;
+    p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
+    p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.K;
+    p.C = q.h, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
+    if (hipError_t e = launch_tiles<true, true, OUT_GATE>(a, stream); e != hipSuccess) return e;
+  }
+  if (!skinny_takes(q.M, q.H, q.I)) return launch_plain<true, true>(down_args(q), q.part, stream);
+  SkinnyArgs a;
+  a.x = q.h, a.w = q.wd, a.C = q.y;
+  a.M = (int)q.M, a.N = (int)q.H, a.K = (int)q.I;
+  return launch_skinny<false>(a, stream);
 }
 
 hipError_t launch_gated_mlp_bwd(const GatedMlp &q, const GatedMlpGrad &o, hipStream_t stream) {
