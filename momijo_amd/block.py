@@ -14,6 +14,7 @@ captured into a HIP graph.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -37,11 +38,15 @@ def _check_type(t: torch.Tensor, name: str) -> int:
 
 def _like(t: torch.Tensor, x: torch.Tensor, shape, name: str) -> torch.Tensor:
     """t as a contiguous tensor of x's type and device and the given shape."""
-    if t.dtype != x.dtype or t.device != x.device:
+    if t.dtype is not x.dtype or t.device != x.device:
         raise TypeError(f"{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _scratch(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 # ------------------------------------------------------------------ dropout
@@ -211,6 +216,11 @@ def residual_norm_train(x: torch.Tensor, branch: torch.Tensor | None = None, *,
                           norm, eps, p, seed, counter, True)
 
 
+@functools.lru_cache(maxsize=1024)
+def _norm_work(rows, dim, gate_rows):
+    return _lib.load().mj_residual_norm_work_bytes(rows, dim, gate_rows)
+
+
 def residual_norm_backward(dy: torch.Tensor | None, dn: torch.Tensor | None,
                            saved: ResidualNormSaved) -> dict[str, torch.Tensor]:
     """The gradients of residual_norm's operands, by their names, from the
@@ -240,9 +250,10 @@ def residual_norm_backward(dy: torch.Tensor | None, dn: torch.Tensor | None,
             if name in out:
                 out[name].zero_()
     gate_rows = 0 if s.gate is None else s.gate.numel() // dim
-    nbytes = _lib.load().mj_residual_norm_work_bytes(rows, dim, gate_rows)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    at = lambda k: _ptr(out.get(k))  # noqa: E731
+    nbytes = _norm_work(rows, dim, gate_rows)
+    work = _scratch(nbytes, x.device)
+    ptr = {k: v.data_ptr() for k, v in out.items()}
+    at = ptr.get
     _lib.call("mj_residual_norm_backward", _DTYPES[x.dtype], _NORMS[s.norm], _ptr(x),
               _ptr(s.branch), _ptr(s.gate), gate_rows, _ptr(s.scale), _ptr(s.post_weight),
               _ptr(s.post_bias), _ptr(s.next_weight), s.p, s.seed, s.counter, _ptr(s.state),
@@ -292,24 +303,23 @@ class ResidualNorm:
 # ------------------------------------------------------------------ gated MLP
 class GatedMLPSaved(NamedTuple):
     """What gated_mlp_backward needs: the operands (bf16 of widths that are not
-    multiples of 8: their zero-padded copies), h and the fp32 projections g, u."""
+    multiples of 8: their zero-padded copies) and one buffer with the fp32
+    projections g and u and then h."""
     x: torch.Tensor
     gate: torch.Tensor
     up: torch.Tensor
     down: torch.Tensor
-    h: torch.Tensor
-    g: torch.Tensor
-    u: torch.Tensor
+    buf: torch.Tensor
     act: int
-    rows: tuple   # leading dimensions of x
-    widths: tuple  # K, I, H as given
+    rows: torch.Size  # leading dimensions of x
+    widths: tuple     # K, I, H as given
 
 
 def _pad8(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     """t zero-padded to [rows, cols], at a 16-byte aligned address."""
-    if t.shape == (rows, cols) and t.is_contiguous() and t.data_ptr() % 16 == 0:
+    if t.data_ptr() % 16 == 0 and t.shape == (rows, cols):
         return t
-    out = torch.empty((rows, cols), dtype=t.dtype, device=t.device)
+    out = t.new_empty((rows, cols))
     r, c = t.shape
     if r < rows:
         out[r:].zero_()
@@ -323,53 +333,63 @@ def _cut(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     return t if t.shape == (rows, cols) else t[:rows, :cols].contiguous()
 
 
-def _mlp_operands(x, gate, up, down, act):
-    """x as [M, K] and the weights, checked, contiguous and (bf16) padded."""
+def _mlp_operands(x, gate, up, down):
+    """x as [M, K] and the weights, checked, contiguous and (bf16) padded; K, I, H."""
     code = _check_type(x, "x")
     if x.dim() < 1 or gate.dim() != 2 or down.dim() != 2:
         raise ValueError("x must have a last dimension, and gate, up, down be 2-D")
-    K, (I, Kw), (H, Iw) = x.shape[-1], gate.shape, down.shape
-    if Kw != K or Iw != I:
-        raise ValueError(f"x has {K} features, gate is {list(gate.shape)}, down {list(down.shape)}")
-    gate = _like(gate, x, gate.shape, "gate")
-    up = _like(up, x, gate.shape, "up")
+    K, shape, (H, Iw) = x.shape[-1], gate.shape, down.shape
+    I = shape[0]
+    if shape[1] != K or Iw != I:
+        raise ValueError(f"x has {K} features, gate is {list(shape)}, down {list(down.shape)}")
+    gate = _like(gate, x, shape, "gate")
+    up = _like(up, x, shape, "up")
     down = _like(down, x, down.shape, "down")
-    x2 = x.reshape(-1, K) if K else x.reshape(x.shape[:-1].numel(), 0)
-    x2 = x2 if x2.is_contiguous() else x2.contiguous()
+    x2 = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), K)
+    if not x2.is_contiguous():
+        x2 = x2.contiguous()
     if code == _lib.BF16:
         Kp, Ip, Hp = K + 7 & ~7, I + 7 & ~7, H + 7 & ~7
         x2 = _pad8(x2, x2.shape[0], Kp)
         gate, up, down = _pad8(gate, Ip, Kp), _pad8(up, Ip, Kp), _pad8(down, Hp, Ip)
-    return code, x2, gate, up, down, (K, I, H)
+    return x2, gate, up, down, (K, I, H)
 
 
-def _work(M, K, I, H, backward, device):
-    nbytes = _lib.load().mj_gated_mlp_work_bytes(M, K, I, H, backward)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
+@functools.lru_cache(maxsize=1024)
+def _mlp_work(M, K, I, H, backward):
+    return _lib.load().mj_gated_mlp_work_bytes(M, K, I, H, backward)
 
 
 def _gated_mlp(x, gate, up, down, act, train):
-    code, x2, gate, up, down, widths = _mlp_operands(x, gate, up, down, act)
+    x2, gate, up, down, widths = _mlp_operands(x, gate, up, down)
     M, K = x2.shape
     H, I = down.shape
     dev = x2.device
-    new = lambda cols, dt=x2.dtype: torch.empty((M, cols), dtype=dt, device=dev)  # noqa: E731
-    y, h = new(H), new(I)
-    if code == _lib.F32:
-        g, u = new(I), new(I)
-        _lib.call("mj_gated_mlp_f32", _ptr(x2), _ptr(gate), _ptr(up), _ptr(down), act, _ptr(h),
-                  _ptr(g), _ptr(u), _ptr(y), M, K, I, H, _stream())
+    f32 = x2.dtype == torch.float32
+    y = x2.new_empty((M, H))
+    # g, u [M, I] fp32 (kept for the backward; the fp32 form always writes them), h, and
+    # the workspace last, each on a 16-byte boundary
+    gu = (M * I * 4 + 15) & ~15 if train or f32 else 0
+    hb = (M * I * (4 if f32 else 2) + 15) & ~15
+    nbytes = 0 if f32 else _mlp_work(M, K, I, H, 0)
+    buf = _scratch(2 * gu + hb, dev) if train else _scratch(2 * gu + hb + nbytes, dev)
+    work = _scratch(nbytes, dev) if train and nbytes else None
+    g = buf.data_ptr()
+    h = g + 2 * gu
+    args = (x2.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), act, h)
+    if f32:
+        _lib.call("mj_gated_mlp_f32", *args, g, g + gu, y.data_ptr(), M, K, I, H, _stream())
     else:
-        g, u = (new(I, torch.float32), new(I, torch.float32)) if train else (None, None)
-        work, nbytes = _work(M, K, I, H, 0, dev)
-        _lib.call("mj_gated_mlp_bf16", _ptr(x2), _ptr(gate), _ptr(up), _ptr(down), act, _ptr(h),
-                  _ptr(g), _ptr(u), _ptr(y), M, K, I, H, _ptr(work), nbytes, _stream())
-    y = _cut(y, M, widths[2])
+        w = None if not nbytes else work.data_ptr() if train else h + hb
+        _lib.call("mj_gated_mlp_bf16", *args, g if train else None, g + gu if train else None,
+                  y.data_ptr(), M, K, I, H, w, nbytes, _stream())
+    if H != widths[2]:
+        y = _cut(y, M, widths[2])
     if x.dim() != 2:
         y = y.reshape(*x.shape[:-1], widths[2])
     if not train:
         return y, None
-    return y, GatedMLPSaved(x2, gate, up, down, h, g, u, act, tuple(x.shape[:-1]), widths)
+    return y, GatedMLPSaved(x2, gate, up, down, buf, act, x.shape[:-1], widths)
 
 
 def gated_mlp(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
@@ -394,23 +414,33 @@ def gated_mlp_backward(dy: torch.Tensor, saved: GatedMLPSaved):
     s = saved
     K0, I0, H0 = s.widths
     x, (M, K), (H, I) = s.x, s.x.shape, s.down.shape
-    dy = _like(dy, x, torch.Size((*s.rows, H0)), "dy").reshape(M, H0)
-    dev = x.device
-    new = lambda r, c: torch.empty((r, c), dtype=x.dtype, device=dev)  # noqa: E731
-    dg, du = new(M, I), new(M, I)
-    dx, dgate, dup, ddown = new(M, K), new(I, K), new(I, K), new(H, I)
-    args = [_ptr(t) for t in (x, s.gate, s.up, s.down)] + [s.act] + \
-        [_ptr(t) for t in (s.h, s.g, s.u)]
-    outs = [_ptr(t) for t in (dg, du, dx, dgate, dup, ddown)]
-    if x.dtype == torch.float32:
-        _lib.call("mj_gated_mlp_backward_f32", *args, _ptr(dy), *outs, M, K, I, H, _stream())
-    else:
+    dy = _like(dy, x, s.rows + (H0,), "dy")
+    if dy.dim() != 2:
+        dy = dy.reshape(M, H0)
+    f32 = x.dtype == torch.float32
+    e = 4 if f32 else 2
+    gu, db = (M * I * 4 + 15) & ~15, (M * I * e + 15) & ~15
+    nbytes = 0 if f32 else _mlp_work(M, K, I, H, 1)
+    dx, dgate, dup, ddown = x.new_empty((M, K)), x.new_empty((I, K)), x.new_empty((I, K)), \
+        x.new_empty((H, I))
+    buf = _scratch(2 * db + nbytes, x.device)  # dg, du, the workspace
+    dg, g = buf.data_ptr(), s.buf.data_ptr()
+    if not f32:
         dy = _pad8(dy, M, H)
-        work, nbytes = _work(M, K, I, H, 1, dev)
-        _lib.call("mj_gated_mlp_backward_bf16", *args, _ptr(dy), *outs, M, K, I, H, _ptr(work),
-                  nbytes, _stream())
-    return (_cut(dx, M, K0).reshape(*s.rows, K0), _cut(dgate, I0, K0), _cut(dup, I0, K0),
-            _cut(ddown, H0, I0))
+    args = (x.data_ptr(), s.gate.data_ptr(), s.up.data_ptr(), s.down.data_ptr(), s.act, g + 2 * gu,
+            g, g + gu, dy.data_ptr(), dg, dg + db, dx.data_ptr(), dgate.data_ptr(), dup.data_ptr(),
+            ddown.data_ptr(), M, K, I, H)
+    if f32:
+        _lib.call("mj_gated_mlp_backward_f32", *args, _stream())
+    else:
+        _lib.call("mj_gated_mlp_backward_bf16", *args, dg + 2 * db if nbytes else None, nbytes,
+                  _stream())
+    if (K, I, H) != s.widths:
+        dx, dgate, dup, ddown = _cut(dx, M, K0), _cut(dgate, I0, K0), _cut(dup, I0, K0), \
+            _cut(ddown, H0, I0)
+    if len(s.rows) != 1:
+        dx = dx.reshape(*s.rows, K0)
+    return dx, dgate, dup, ddown
 
 
 class GatedMLP:
