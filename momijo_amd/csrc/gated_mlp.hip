@@ -501,28 +501,31 @@ __global__ __launch_bounds__(256) void mlp_ring_kernel(TileArgs args) {
   tile_out<OUT, TM, TN, WM, WN>(args, p, acc, m0, n0, wm, wn, lane, at.split);
 }
 
-// 256 x 256 tiles with two waves per SIMD: 8 waves laid out 2 x 4, each owning 128 x
-// 64 outputs (gate/up: 32 columns of g and of u), on the pipeline of the framework's
-// large bf16 product (gemm_nt_w8_kernel): two A and three B stage buffers (all 160 KB
-// of LDS), a stage of two 32-deep steps with one barrier between them, each step's
-// fragment reads for the next spread between its MFMAs, four direct loads a step for
-// the stage after next.  A K-strided operand has two 8-byte transposed reads a
-// fragment in place of one of 16 bytes; its resource moves along K with the stage, so
-// its loads need no bounds selects at any K.
-template <bool AKC, bool BKC, int OUT>
-__global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
-  constexpr int BM = 256, BN = 256, NW = 8, WM = 128, WN = 64, TM = 8, TN = 4;
+// The pipelined tiles: 256 x 256 of 8 waves (2 x 4, 128 x 64 outputs each), one
+// workgroup a CU, or 128 x 128 of 4 waves (2 x 2, 64 x 64 each), two a CU, where 256 x
+// 256 tiles leave CUs idle (twice the operand traffic and a third more LDS reads a
+// flop: 0.86 us for two 64-deep stages of 128 x 128, 1.47 for one of 256 x 256, four
+// times the work).  Both put two waves on a SIMD, and run the pipeline of the
+// framework's large bf16 product (gemm_nt_w8_kernel): two A and three B stage buffers,
+// a stage of two 32-deep steps with one barrier between them, each step's fragment
+// reads for the next spread between its MFMAs, four direct loads a step for the stage
+// after next.  A K-strided operand has two 8-byte transposed reads a fragment in place
+// of one of 16 bytes; its resource moves along K with the stage, so its loads need no
+// bounds selects at any K.
+template <int BM, int NW, bool AKC, bool BKC, int OUT>
+__global__ __launch_bounds__(NW * 64, 2) void mlp_tile_kernel(TileArgs args) {
+  constexpr int BN = BM, WGN = NW / 2, WM = BM / 2, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   constexpr int BN_OUT = OUT == OUT_GATE ? BN / 2 : BN;
   using OA = Operand<BM, NW, AKC>;
   using OB = Operand<BN, NW, BKC>;
   constexpr int DPO = 4;  // direct loads per wave per operand per stage
-  static_assert(OA::LOADS == DPO && OB::LOADS == DPO, "loads per stage");
+  static_assert(OA::LOADS == DPO && OB::LOADS == DPO && TN == DPO, "a load per group");
   extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
   uint16_t *As = lds;                   // stage kt in buffer kt % 2
   uint16_t *Bs = lds + 2 * OA::STAGE;   // stage kt in buffer kt % 3
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 2, wn = wave & 3;
+  const int wm = wave / WGN, wn = wave % WGN;
   const TileAt at = locate(args);
   const TileProb &p = args.p[at.prob];
   const int m0 = at.m * BM, n0 = at.n * BN_OUT;
@@ -564,7 +567,7 @@ __global__ __launch_bounds__(512) void mlp_w8_kernel(TileArgs args) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   bf16x8 fa[2][TM], fb[2][TN];
-  // the 12 fragments of a step: A's blocks, then B's, three a group
+  // the fragments of a step: A's blocks, then B's, PER a group
   constexpr int PER = (TM + TN) / TN;
   auto read_frag = [&](int t, int dst, int abuf, int bbuf) __attribute__((always_inline)) {
     if (t < TM) OA::read(fa[dst][t], As + abuf * OA::STAGE, abase[dst], t);
@@ -845,32 +848,34 @@ hipError_t launch_ring(TileArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <bool AKC, bool BKC, int OUT>
-hipError_t launch_w8(TileArgs a, hipStream_t stream) {
-  constexpr size_t lds = size_t(2 * 256 + 3 * 256) * kBK * sizeof(uint16_t);  // 160 KB
-  auto kern = mlp_w8_kernel<AKC, BKC, OUT>;
+template <int BM, int NW, bool AKC, bool BKC, int OUT>
+hipError_t launch_w(TileArgs a, hipStream_t stream) {
+  constexpr size_t lds = size_t(5 * BM) * kBK * sizeof(uint16_t);  // 160 or 80 KB
+  auto kern = mlp_tile_kernel<BM, NW, AKC, BKC, OUT>;
   static std::atomic<uint64_t> done{0};
   if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
-  set_tiles(a, 256, OUT == OUT_GATE ? 128 : 256);
+  set_tiles(a, BM, OUT == OUT_GATE ? BM / 2 : BM);
   if (a.tiles == 0) return hipSuccess;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.splits)), dim3(512), lds, stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.splits)), dim3(NW * 64), lds, stream, a);
   return hipGetLastError();
 }
 
 // The tile kernels' times on MI355X (us): a launch, then for each round of workgroups
 // that the CUs hold (per_cu each) the stages at the time of a 64-deep stage with 1, 2,
 // .. workgroups per CU and the fixed part of a round (first loads and, by kind,
-// output).  Fits to products of 48 to 4096 rows, widths 512 to 11008, e.g. h of 512
-// rows (K = 4096, 11008 columns): 256 x 256 97, 128 x 64 147, 64 x 64 160; of 300 rows
-// (K = 1024, 2816 columns) 35, 16.7, 13.1; of 48 rows (11008) 82, 45, and 64 x 64
-// 40.2 with three stages, 34.1 with five (one or two workgroups a CU wait on memory).
-enum : int { T_256 = 0, T_64S3, T_64S5, T_128X64, T_COUNT };
+// output).  Fits to products of 48 to 4096 rows, widths 512 to 11008, e.g. the gradients
+// dg, du of 4096 rows (K = 4096, 11008 columns): 256 x 256 395, 128 x 128 445, 128 x 64
+// 641, 64 x 64 771; of 512 rows 105, 67, 90, 87; h of 300 rows (K = 1024, 2816
+// columns) 37, 15.3, 16.4, 13.1; of 48 rows (11008) 82, -, 45, and 64 x 64 40.2
+// with three stages, 34.1 with five (one or two workgroups a CU wait on memory).
+enum : int { T_256 = 0, T_128, T_64S3, T_64S5, T_128X64, T_COUNT };
 struct TileCost {
   int bm, bn, per_cu;
   double stage[3], fixed[4];  // fixed by OUT_*
 };
 constexpr TileCost kTileCost[T_COUNT] = {
     {256, 256, 1, {1.47, 0, 0}, {7, 7, 8, 14}},
+    {128, 128, 2, {0.48, 0.86, 0}, {4, 3, 6, 9}},
     {64, 64, 3, {0.48, 0.52, 0.62}, {2.1, 2.1, 3, 4}},
     {64, 64, 2, {0.31, 0.48, 0}, {2.1, 2.1, 3, 4}},
     {128, 64, 2, {0.45, 0.70, 0}, {2.5, 2.5, 4, 6}},
@@ -924,7 +929,8 @@ TilePlan plan_tiles(const TileArgs &a, int out) {
 template <bool AKC, bool BKC, int OUT>
 hipError_t launch_tile_kernel(int tile, const TileArgs &a, hipStream_t stream) {
   switch (tile) {
-    case T_256: return launch_w8<AKC, BKC, OUT>(a, stream);
+    case T_256: return launch_w<256, 8, AKC, BKC, OUT>(a, stream);
+    case T_128: return launch_w<128, 4, AKC, BKC, OUT>(a, stream);
     case T_64S3: return launch_ring<64, 64, 3, AKC, BKC, OUT>(a, stream);
     case T_64S5: return launch_ring<64, 64, 5, AKC, BKC, OUT>(a, stream);
     default: return launch_ring<128, 64, 3, AKC, BKC, OUT>(a, stream);
