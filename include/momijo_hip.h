@@ -571,7 +571,7 @@ int32_t mj_residual_norm_backward(int32_t dtype, int32_t norm, const void *x, co
  *   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
  * x [M,K], Wg and Wu [I,K], Wd [H,I], h [M,I], y [M,H], all contiguous; act is
  * MJ_EPI_NONE, RELU, GELU_TANH or SILU.
- * bf16: K, I, H multiples of 8 (zero-pad other widths), 16-byte aligned arrays;
+ * bf16: K, I, H multiples of 8 (mj_copy_rows_bf16 pads other widths), 16-byte aligned arrays;
  * h is rounded to bf16; g, u fp32 [M,I] are written for the backward, or both NULL;
  * `work` as mj_gated_mlp_work_bytes says (NULL where that is 0).
  * fp32: any widths; h, g, u are required. */
@@ -583,6 +583,14 @@ int32_t mj_gated_mlp_bf16(const uint16_t *x, const uint16_t *Wg, const uint16_t 
 int32_t mj_gated_mlp_f32(const float *x, const float *Wg, const float *Wu, const float *Wd,
                          int32_t act, float *h, float *g, float *u, float *y, int64_t M, int64_t K,
                          int64_t I, int64_t H, void *stream);
+
+/* Row copies between a width and its zero-padded form, n (1..4) matrices in one
+ * launch: dst[i] [dst_rows, dst_cols] (rows dst_ld apart) takes src[i] [rows, cols] (rows
+ * src_ld apart) and zeros where that ends; dst_rows, dst_cols below rows, cols cut.
+ * bf16, any alignment; the arrays of pointers and sizes are host memory, six sizes for
+ * each matrix: rows, cols, src_ld, dst_rows, dst_cols, dst_ld. */
+int32_t mj_copy_rows_bf16(int32_t n, const uint16_t *const *src, uint16_t *const *dst,
+                          const int64_t *sizes, void *stream);
 
 /* Gradients of the gated block from dy [M,H] and the forward's h, g, u:
  *   dh = dy Wd, dg = dh u act'(g), du = dh act(g)

@@ -14,6 +14,7 @@ captured into a HIP graph.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 from typing import NamedTuple
 
@@ -302,45 +303,39 @@ class ResidualNorm:
 
 # ------------------------------------------------------------------ gated MLP
 class GatedMLPSaved(NamedTuple):
-    """What gated_mlp_backward needs: the operands (bf16 of widths that are not
-    multiples of 8: their zero-padded copies) and one buffer with the fp32
-    projections g and u and then h."""
+    """What gated_mlp_backward needs: the operands, and one buffer with the fp32
+    projections g and u, then h, then the zero-padded copies of operands whose widths
+    are not multiples of 8 (bf16); ``ptrs`` is where the kernels read x, gate, up, down."""
     x: torch.Tensor
     gate: torch.Tensor
     up: torch.Tensor
     down: torch.Tensor
     buf: torch.Tensor
+    ptrs: tuple
     act: int
     rows: torch.Size  # leading dimensions of x
-    widths: tuple     # K, I, H as given
 
 
-def _pad8(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
-    """t zero-padded to [rows, cols], at a 16-byte aligned address."""
-    if t.data_ptr() % 16 == 0 and t.shape == (rows, cols):
-        return t
-    out = t.new_empty((rows, cols))
-    r, c = t.shape
-    if r < rows:
-        out[r:].zero_()
-    if c < cols:
-        out[:r, c:].zero_()
-    out[:r, :c].copy_(t)
-    return out
+def _copy_rows(mats) -> None:
+    """mats: (src pointer, dst pointer, rows, cols, src_ld, dst_rows, dst_cols, dst_ld)."""
+    n = len(mats)
+    src = (ctypes.c_void_p * n)(*(m[0] for m in mats))
+    dst = (ctypes.c_void_p * n)(*(m[1] for m in mats))
+    sizes = (ctypes.c_int64 * (6 * n))(*(v for m in mats for v in m[2:]))
+    _lib.call("mj_copy_rows_bf16", n, src, dst, sizes, _stream())
 
 
-def _cut(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
-    return t if t.shape == (rows, cols) else t[:rows, :cols].contiguous()
+def _up16(n: int) -> int:
+    return n + 15 & ~15
 
 
 def _mlp_operands(x, gate, up, down):
-    """x as [M, K] and the weights, checked, contiguous and (bf16) padded; K, I, H."""
-    code = _check_type(x, "x")
+    """x as [M, K] and the weights, checked and contiguous; K, I, H."""
+    _check_type(x, "x")
     if x.dim() < 1 or gate.dim() != 2 or down.dim() != 2:
         raise ValueError("x must have a last dimension, and gate, up, down be 2-D")
     K, shape, (H, Iw) = x.shape[-1], gate.shape, down.shape
-    I = shape[0]
-    if shape[1] != K or Iw != I:
+    if shape[1] != K or Iw != shape[0]:
         raise ValueError(f"x has {K} features, gate is {list(shape)}, down {list(down.shape)}")
     gate = _like(gate, x, shape, "gate")
     up = _like(up, x, shape, "up")
@@ -348,11 +343,7 @@ def _mlp_operands(x, gate, up, down):
     x2 = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), K)
     if not x2.is_contiguous():
         x2 = x2.contiguous()
-    if code == _lib.BF16:
-        Kp, Ip, Hp = K + 7 & ~7, I + 7 & ~7, H + 7 & ~7
-        x2 = _pad8(x2, x2.shape[0], Kp)
-        gate, up, down = _pad8(gate, Ip, Kp), _pad8(up, Ip, Kp), _pad8(down, Hp, Ip)
-    return x2, gate, up, down, (K, I, H)
+    return x2, gate, up, down, K, Iw, H
 
 
 @functools.lru_cache(maxsize=1024)
@@ -360,36 +351,64 @@ def _mlp_work(M, K, I, H, backward):
     return _lib.load().mj_gated_mlp_work_bytes(M, K, I, H, backward)
 
 
+def _padded(mats, at):
+    """Where the kernels read matrices (pointer, rows, cols, padded rows, padded cols):
+    in place, or from ``at`` on for those whose widths or addresses they cannot take;
+    and the copies that brings about, and their bytes."""
+    ptrs, copies, used = [], [], 0
+    for p, r, c, rp, cp in mats:
+        if (r, c) == (rp, cp) and p % 16 == 0:
+            ptrs.append(p)
+        else:
+            ptrs.append(at + used)
+            copies.append((p, at + used, r, c, c, rp, cp, cp))
+            used += _up16(2 * rp * cp)
+    return tuple(ptrs), copies, used
+
+
 def _gated_mlp(x, gate, up, down, act, train):
-    x2, gate, up, down, widths = _mlp_operands(x, gate, up, down)
-    M, K = x2.shape
-    H, I = down.shape
-    dev = x2.device
-    f32 = x2.dtype == torch.float32
+    x2, gate, up, down, K, I, H = _mlp_operands(x, gate, up, down)
+    M, dev = x2.shape[0], x2.device
     y = x2.new_empty((M, H))
-    # g, u [M, I] fp32 (kept for the backward; the fp32 form always writes them), h, and
-    # the workspace last, each on a 16-byte boundary
-    gu = (M * I * 4 + 15) & ~15 if train or f32 else 0
-    hb = (M * I * (4 if f32 else 2) + 15) & ~15
-    nbytes = 0 if f32 else _mlp_work(M, K, I, H, 0)
-    buf = _scratch(2 * gu + hb, dev) if train else _scratch(2 * gu + hb + nbytes, dev)
-    work = _scratch(nbytes, dev) if train and nbytes else None
-    g = buf.data_ptr()
-    h = g + 2 * gu
-    args = (x2.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), act, h)
-    if f32:
-        _lib.call("mj_gated_mlp_f32", *args, g, g + gu, y.data_ptr(), M, K, I, H, _stream())
+    ptrs = (x2.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr())
+    # one buffer: g, u [M, I] fp32 (kept for the backward; the fp32 form always writes
+    # them), h, then in bf16 padded operands, a padded y and the workspace
+    if x2.dtype == torch.float32:
+        gu = _up16(4 * M * I)
+        buf = _scratch(3 * gu, dev)
+        g = buf.data_ptr()
+        _lib.call("mj_gated_mlp_f32", *ptrs, act, g + 2 * gu, g, g + gu, y.data_ptr(), M, K, I, H,
+                  _stream())
     else:
-        w = None if not nbytes else work.data_ptr() if train else h + hb
-        _lib.call("mj_gated_mlp_bf16", *args, g if train else None, g + gu if train else None,
-                  y.data_ptr(), M, K, I, H, w, nbytes, _stream())
-    if H != widths[2]:
-        y = _cut(y, M, widths[2])
+        Kp, Ip, Hp = K + 7 & ~7, I + 7 & ~7, H + 7 & ~7
+        gu = _up16(4 * M * Ip) if train else 0
+        hb = _up16(2 * M * Ip)
+        mats = ((ptrs[0], M, K, M, Kp), (ptrs[1], I, K, Ip, Kp), (ptrs[2], I, K, Ip, Kp),
+                (ptrs[3], H, I, Hp, Ip))
+        pad = 0
+        if Kp != K or Ip != I or Hp != H or any(p % 16 for p in ptrs):
+            pad = _padded(mats, 0)[2]
+        yb = 0 if Hp == H else _up16(2 * M * Hp)
+        nbytes = _mlp_work(M, Kp, Ip, Hp, 0)
+        # a training step keeps the buffer: what only this call needs goes into another
+        buf = _scratch(2 * gu + hb + pad + (0 if train else yb + nbytes), dev)
+        more = _scratch(yb + nbytes, dev) if train and yb + nbytes else None
+        g = buf.data_ptr()
+        h = g + 2 * gu
+        if pad:
+            ptrs, copies, _ = _padded(mats, h + hb)
+            _copy_rows(copies)
+        end = h + hb + pad if more is None else more.data_ptr()
+        _lib.call("mj_gated_mlp_bf16", *ptrs, act, h, g if train else None,
+                  g + gu if train else None, end if yb else y.data_ptr(), M, Kp, Ip, Hp,
+                  end + yb if nbytes else None, nbytes, _stream())
+        if yb:
+            _copy_rows([(end, y.data_ptr(), M, H, Hp, M, H, H)])
     if x.dim() != 2:
-        y = y.reshape(*x.shape[:-1], widths[2])
+        y = y.reshape(*x.shape[:-1], H)
     if not train:
         return y, None
-    return y, GatedMLPSaved(x2, gate, up, down, buf, act, x.shape[:-1], widths)
+    return y, GatedMLPSaved(x2, gate, up, down, buf, ptrs, act, x.shape[:-1])
 
 
 def gated_mlp(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
@@ -412,34 +431,43 @@ def gated_mlp_train(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down:
 def gated_mlp_backward(dy: torch.Tensor, saved: GatedMLPSaved):
     """(dx, dgate, dup, ddown) of gated_mlp from the gradient of y."""
     s = saved
-    K0, I0, H0 = s.widths
     x, (M, K), (H, I) = s.x, s.x.shape, s.down.shape
-    dy = _like(dy, x, s.rows + (H0,), "dy")
-    if dy.dim() != 2:
-        dy = dy.reshape(M, H0)
-    f32 = x.dtype == torch.float32
-    e = 4 if f32 else 2
-    gu, db = (M * I * 4 + 15) & ~15, (M * I * e + 15) & ~15
-    nbytes = 0 if f32 else _mlp_work(M, K, I, H, 1)
-    dx, dgate, dup, ddown = x.new_empty((M, K)), x.new_empty((I, K)), x.new_empty((I, K)), \
+    dy = _like(dy, x, s.rows + (H,), "dy")
+    out = dx, dgate, dup, ddown = x.new_empty((M, K)), x.new_empty((I, K)), x.new_empty((I, K)), \
         x.new_empty((H, I))
-    buf = _scratch(2 * db + nbytes, x.device)  # dg, du, the workspace
-    dg, g = buf.data_ptr(), s.buf.data_ptr()
-    if not f32:
-        dy = _pad8(dy, M, H)
-    args = (x.data_ptr(), s.gate.data_ptr(), s.up.data_ptr(), s.down.data_ptr(), s.act, g + 2 * gu,
-            g, g + gu, dy.data_ptr(), dg, dg + db, dx.data_ptr(), dgate.data_ptr(), dup.data_ptr(),
-            ddown.data_ptr(), M, K, I, H)
-    if f32:
-        _lib.call("mj_gated_mlp_backward_f32", *args, _stream())
+    outs = tuple(t.data_ptr() for t in out)
+    g = s.buf.data_ptr()
+    if x.dtype == torch.float32:
+        gu = _up16(4 * M * I)
+        buf = _scratch(2 * gu, x.device)  # dg, du
+        dg = buf.data_ptr()
+        _lib.call("mj_gated_mlp_backward_f32", *s.ptrs, s.act, g + 2 * gu, g, g + gu, dy.data_ptr(),
+                  dg, dg + gu, *outs, M, K, I, H, _stream())
     else:
-        _lib.call("mj_gated_mlp_backward_bf16", *args, dg + 2 * db if nbytes else None, nbytes,
-                  _stream())
-    if (K, I, H) != s.widths:
-        dx, dgate, dup, ddown = _cut(dx, M, K0), _cut(dgate, I0, K0), _cut(dup, I0, K0), \
-            _cut(ddown, H0, I0)
+        Kp, Ip, Hp = K + 7 & ~7, I + 7 & ~7, H + 7 & ~7
+        gu, db = _up16(4 * M * Ip), _up16(2 * M * Ip)
+        nbytes = _mlp_work(M, Kp, Ip, Hp, 1)
+        mats = ((dy.data_ptr(), M, H, M, Hp),)
+        pad = _padded(mats, 0)[2]
+        grads = ((outs[0], M, K, M, Kp), (outs[1], I, K, Ip, Kp), (outs[2], I, K, Ip, Kp),
+                 (outs[3], H, I, Hp, Ip))
+        cut = (Kp, Ip, Hp) != (K, I, H)
+        cutb = _padded(grads, 0)[2] if cut else 0
+        buf = _scratch(2 * db + nbytes + pad + cutb, x.device)  # dg, du, the workspace, ..
+        dg = buf.data_ptr()
+        at = dg + 2 * db
+        end = at + _up16(nbytes)
+        (dyp,), copies, _ = _padded(mats, end)
+        if copies:
+            _copy_rows(copies)
+        if cut:
+            outs, back, _ = _padded(grads, end + pad)
+        _lib.call("mj_gated_mlp_backward_bf16", *s.ptrs, s.act, g + 2 * gu, g, g + gu, dyp, dg,
+                  dg + db, *outs, M, Kp, Ip, Hp, at if nbytes else None, nbytes, _stream())
+        if cut:
+            _copy_rows([(q, p, r, c, cp, r, c, c) for p, q, r, c, _, rp, cp, _ in back])
     if len(s.rows) != 1:
-        dx = dx.reshape(*s.rows, K0)
+        dx = dx.reshape(*s.rows, K)
     return dx, dgate, dup, ddown
 
 

@@ -185,6 +185,28 @@ int64_t mj_gated_mlp_work_bytes(int64_t M, int64_t K, int64_t I, int64_t H, int3
   return mj::gated_mlp_part_floats(M, K, I, H, backward != 0) * (int64_t)sizeof(float);
 }
 
+int32_t mj_copy_rows_bf16(int32_t n, const uint16_t *const *src, uint16_t *const *dst,
+                          const int64_t *sizes, void *stream) {
+  if (n < 1 || n > 4) return fail(MJ_ERR_ARG, "1 to 4 matrices, got %d", n);
+  if (!src || !dst || !sizes) return fail(MJ_ERR_ARG, "null argument");
+  mj::CopyRows c;
+  c.n = n;
+  for (int i = 0; i < n; ++i) {
+    const int64_t *z = sizes + 6 * i;
+    mj::CopyRows::Mat &m = c.m[i];
+    m.src = src[i], m.dst = dst[i];
+    m.rows = z[0], m.cols = z[1], m.src_ld = z[2];
+    m.dst_rows = z[3], m.dst_cols = z[4], m.dst_ld = z[5];
+    for (int k = 0; k < 6; ++k)
+      if (z[k] < 0) return fail(MJ_ERR_ARG, "negative size");
+    if (m.src_ld < m.cols || m.dst_ld < m.dst_cols)
+      return fail(MJ_ERR_SHAPE, "rows overlap (leading dimension below the width)");
+    if ((m.dst_rows > 0 && m.dst_cols > 0 && !m.dst) || (m.rows > 0 && m.cols > 0 && !m.src))
+      return fail(MJ_ERR_ARG, "null matrix");
+  }
+  return hip_status(mj::launch_copy_rows_bf16(c, S(stream)), "row copy launch");
+}
+
 int32_t mj_gated_mlp_bf16(const uint16_t *x, const uint16_t *Wg, const uint16_t *Wu,
                           const uint16_t *Wd, int32_t act, uint16_t *h, float *g, float *u,
                           uint16_t *y, int64_t M, int64_t K, int64_t I, int64_t H, void *work,

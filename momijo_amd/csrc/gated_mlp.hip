@@ -27,6 +27,7 @@
 #include "common.h"
 #include "gemm_tile.h"
 #include "launch.h"
+#include "philox.h"
 
 namespace mj {
 
@@ -759,6 +760,36 @@ __global__ __launch_bounds__(NW * 64) void mlp_skinny_kernel(SkinnyArgs p) {
   }
 }
 
+// ---------------------------------------------------------------- odd widths
+// 8 columns a thread: 16-byte loads and stores at the elements' own alignment.
+__global__ __launch_bounds__(256) void copy_rows_kernel(CopyRows c) {
+  const CopyRows::Mat &m = c.m[blockIdx.y];
+  const int64_t per_row = (m.dst_cols + 7) / 8, total = m.dst_rows * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row, col = (i - r * per_row) * 8;
+    const int64_t have = r < m.rows ? m.cols - col : 0, want = m.dst_cols - col;
+    uint32_t w[4] = {0, 0, 0, 0};
+    const uint16_t *s = m.src + r * m.src_ld + col;
+    if (have >= 8) {
+      const u32x4_a2 q = *(const u32x4_a2 *)s;
+      w[0] = q[0], w[1] = q[1], w[2] = q[2], w[3] = q[3];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < have) w[j >> 1] |= (uint32_t)s[j] << (16 * (j & 1));
+    }
+    uint16_t *d = m.dst + r * m.dst_ld + col;
+    if (want >= 8) {
+      *(u32x4_a2 *)d = u32x4_a2{w[0], w[1], w[2], w[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < want) d[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
 // ---------------------------------------------------------------- fp32 block
 __device__ __forceinline__ float2 act_grad_f32(int act, float g) {
   if (act == EPI_SILU) {
@@ -1069,6 +1100,17 @@ hipError_t launch_gated_mlp_bwd(const GatedMlp &q, const GatedMlpGrad &o, hipStr
   add(o.du, q.I, q.x, q.K, o.dwu);
   add(o.dy, q.H, q.h, q.I, o.dwd);
   return w.n ? launch_tiles<false, false, OUT_STORE>(w, stream) : hipSuccess;
+}
+
+hipError_t launch_copy_rows_bf16(const CopyRows &c, hipStream_t stream) {
+  int64_t most = 0;
+  for (int i = 0; i < c.n; ++i)
+    most = std::max(most, c.m[i].dst_rows * ((c.m[i].dst_cols + 7) / 8));
+  if (most == 0) return hipSuccess;
+  const int64_t blocks = std::min<int64_t>((most + 255) / 256, 4096);
+  hipLaunchKernelGGL(copy_rows_kernel, dim3((unsigned)blocks, (unsigned)c.n), dim3(256), 0, stream,
+                     c);
+  return hipGetLastError();
 }
 
 hipError_t launch_gate_f32(int act, const float *g, const float *u, float *h, int64_t n,

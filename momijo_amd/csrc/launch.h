@@ -301,6 +301,16 @@ struct GatedMlpGrad {
 int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward);
 hipError_t launch_gated_mlp(const GatedMlp &p, hipStream_t stream);
 hipError_t launch_gated_mlp_bwd(const GatedMlp &p, const GatedMlpGrad &d, hipStream_t stream);
+// dst[r, c] = src[r, c] inside [rows, cols], else 0, for r < dst_rows, c < dst_cols.
+struct CopyRows {
+  struct Mat {
+    const uint16_t *src = nullptr;
+    uint16_t *dst = nullptr;
+    int64_t rows = 0, cols = 0, src_ld = 0, dst_rows = 0, dst_cols = 0, dst_ld = 0;
+  } m[4];
+  int n = 0;
+};
+hipError_t launch_copy_rows_bf16(const CopyRows &c, hipStream_t stream);
 // The elementwise halves of the fp32 block: h = act(g) u, and in place dg = dh u
 // act'(g), du = dh act(g) over n elements.
 hipError_t launch_gate_f32(int act, const float *g, const float *u, float *h, int64_t n,

@@ -87,3 +87,17 @@ def test_gated_mlp_status_codes(lib):
     assert need > 0
     assert lib.mj_gated_mlp_bf16(p, p, p, p, 3, p, None, None, p, 64, 512, 4096, 64, p, need - 1,
                                  None) == _lib.MJ_ERR_ARG
+
+
+def test_copy_rows_status_codes(lib):
+    ptrs = (ctypes.c_void_p * 1)(16)
+    call = lambda n, *z: lib.mj_copy_rows_bf16(n, ptrs, ptrs, (ctypes.c_int64 * 6)(*z), None)  # noqa: E731
+    assert call(0, 1, 1, 1, 1, 1, 1) == _lib.MJ_ERR_ARG
+    assert call(5, 1, 1, 1, 1, 1, 1) == _lib.MJ_ERR_ARG
+    assert call(1, -1, 1, 1, 1, 1, 1) == _lib.MJ_ERR_ARG
+    assert call(1, 2, 4, 3, 2, 4, 4) == _lib.MJ_ERR_SHAPE     # source rows overlap
+    assert call(1, 2, 4, 4, 2, 8, 4) == _lib.MJ_ERR_SHAPE
+    assert lib.mj_copy_rows_bf16(1, None, ptrs, (ctypes.c_int64 * 6)(), None) == _lib.MJ_ERR_ARG
+    null = (ctypes.c_void_p * 1)()
+    assert lib.mj_copy_rows_bf16(1, null, ptrs, (ctypes.c_int64 * 6)(2, 2, 2, 2, 2, 2), None) == _lib.MJ_ERR_ARG
+    assert call(1, 0, 0, 0, 0, 0, 0) == _lib.MJ_OK
