@@ -316,13 +316,17 @@ class GatedMLPSaved(NamedTuple):
     rows: torch.Size  # leading dimensions of x
 
 
+# ctypes makes an array type anew, a cycle for the garbage collector, unless it is kept
+_PTRS = [ctypes.c_void_p * n for n in range(5)]
+_SIZES = [ctypes.c_int64 * (6 * n) for n in range(5)]
+
+
 def _copy_rows(mats) -> None:
     """mats: (src pointer, dst pointer, rows, cols, src_ld, dst_rows, dst_cols, dst_ld)."""
     n = len(mats)
-    src = (ctypes.c_void_p * n)(*(m[0] for m in mats))
-    dst = (ctypes.c_void_p * n)(*(m[1] for m in mats))
-    sizes = (ctypes.c_int64 * (6 * n))(*(v for m in mats for v in m[2:]))
-    _lib.call("mj_copy_rows_bf16", n, src, dst, sizes, _stream())
+    sizes = [v for m in mats for v in m[2:]]
+    _lib.call("mj_copy_rows_bf16", n, _PTRS[n](*[m[0] for m in mats]),
+              _PTRS[n](*[m[1] for m in mats]), _SIZES[n](*sizes), _stream())
 
 
 def _up16(n: int) -> int:
