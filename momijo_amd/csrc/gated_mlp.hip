@@ -842,19 +842,6 @@ __global__ __launch_bounds__(256) void gate_bwd_f32_kernel(int act, const float 
 }
 
 // ---------------------------------------------------------------- launch
-hipError_t raise_lds(const void *kern, size_t bytes, std::atomic<uint64_t> &done) {
-  int dev = 0;
-  if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
-  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
-  if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
-    hipError_t e =
-        hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != hipSuccess) return e;
-    done.fetch_or(bit, std::memory_order_release);
-  }
-  return hipSuccess;
-}
-
 void set_tiles(TileArgs &a, int bm, int bn_out) {
   a.tiles = 0;
   for (int i = 0; i < a.n; ++i) {

@@ -6,7 +6,23 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace mj {
+
+// Raises a kernel's dynamic-LDS limit, once per device it runs on.
+inline hipError_t raise_lds(const void *kern, size_t bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
+    hipError_t e =
+        hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return e;
+    done.fetch_or(bit, std::memory_order_release);
+  }
+  return hipSuccess;
+}
 
 // ---- gemm_nt.hip: bf16 A x (bf16 | int8) B^T on MFMA ---------------------
 enum BKind : int { B_BF16 = 0, B_INT8 = 1 };
@@ -272,10 +288,14 @@ struct ResNormGrad {
   float *dscale = nullptr, *dwp = nullptr, *dbp = nullptr, *dwn = nullptr, *dbn = nullptr;
   float *part = nullptr;   // residual_norm_part_floats
   // the walk of plan_residual_norm_bwd
-  int64_t groups = 1, segs = 1, seg_rows = 0, groups_per_team = 1, teams = 0;
+  int64_t groups = 1;            // gate rows
+  int64_t segs = 1, seg_rows = 0;  // segments of a group, 0: a workgroup takes whole groups
+  int64_t groups_per_block = 1, blocks = 0;
 };
 constexpr int64_t kResNormMaxDim = 16384;
-void plan_residual_norm_bwd(const ResNorm &p, ResNormGrad &g);
+// bias: whether biases or their gradients are there (residual_norm_bias)
+void plan_residual_norm_bwd(const ResNorm &p, ResNormGrad &g, bool bias);
+bool residual_norm_bias(const ResNorm &p, const ResNormGrad &g);
 int64_t residual_norm_part_floats(const ResNormGrad &g, int64_t dim);
 hipError_t launch_residual_norm(bool bf16, const ResNorm &p, hipStream_t stream);
 hipError_t launch_residual_norm_bwd(bool bf16, const ResNorm &p, const ResNormGrad &g,

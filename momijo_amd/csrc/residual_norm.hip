@@ -15,6 +15,8 @@
 // 8 columns (one 16-byte bf16 access) a thread and VPT such chunks, so every
 // value is read once however many sums its row needs.  Teams of one wave to 16
 // by width, so that a row's chunks just fit the team.
+#include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "launch.h"
@@ -137,7 +139,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_kernel(Re
   __shared__ float lds[64];
   int slot = 0;
   const int lane = threadIdx.x % TPR, dim = (int)p.dim;
-  int64_t m = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
+  // (a wave is of one team, so its row is uniform)
+  int64_t m = (int64_t)blockIdx.x * TEAMS + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   // a team past the last row computes it again (its barriers are everyone's) and writes nothing
   const bool live = m < p.rows;
   if (!live) m = p.rows - 1;
@@ -214,45 +217,199 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_kernel(Re
   }
 }
 
-// Backward.  A team walks a segment of consecutive rows with the columns' sums
-// (the gradients of the vectors, and of the gate's row) in its registers:
+// Backward:
 //   dyt = dy + rn (dn wn - yhat mean(dn wn yhat) - [layer] mean(dn wn))
 //   dx = s dyt, ds += x dyt, dz = keep dyt, dgate += dz c, dc = dz g
 //   dwn += dn yhat, dbn += dn, dwp += dc bhat, dbp += dc
 //   db = rp (dc wp - bhat mean(dc wp bhat) - [layer] mean(dc wp))
 // with bhat, c, y and yhat computed again from x, b and the saved statistics, in
-// the forward's order, so y is the unrounded one.  A segment lies inside one gate
-// row's rows (its dgate goes to the partials) or holds whole groups of them
-// (dgate written as it is finished).  No atomics: sums are added in a fixed order.
+// the forward's order, so y is the unrounded one.
+//
+// A workgroup of 512 threads (512 / TPR teams) walks a segment of rows, its teams in
+// turn, with the columns' sums in registers; the teams' sums are added through LDS at
+// the end and the workgroup writes one partial row for each vector.  A segment lies
+// inside one gate row's rows (its dgate goes to the partials too), or, where the groups
+// are small, is a run of whole groups dealt to the teams, which write dgate as they
+// finish one.  No atomics: sums are added in a fixed order.
+//
+// What bounds it is latency (a row's loads, then two sums over it, one after the
+// other) and, near the memory rate, the vector unit (some 60 operations an element).
+// Two workgroups on a CU cover each other's waits, so a thread has 128 registers: they
+// go to the sums; what a row needs again is computed again from its packed values, and
+// the vectors wait in LDS, each thread's own columns in its own slots (no barrier, no
+// bank conflicts).  8192 x 4096 bf16 with dropout and four gate rows: 118 us (402 MB);
+// with the next row's loads ahead 202 (spills at 128 registers) or 141 (one workgroup a
+// CU); with the vectors in registers, one workgroup a CU, 182 (111 since the
+// partials' sums keep eight loads in flight).
 enum : int { SUM_WN = 0, SUM_BN, SUM_S, SUM_WP, SUM_BP, SUM_G, SUMS };
+enum : int { V_WN = 0, V_WP, V_GATE, V_SCALE, V_BP, VECS };
+constexpr int kBwdThreads = 512;
 
-template <typename T, int TPR, int VPT, bool ALIGNED>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kernel(ResNorm p,
-                                                                                  ResNormGrad g) {
-  constexpr int TEAMS = (TPR > 256 ? TPR : 256) / TPR;
+// 8 consecutive elements as they are stored.
+template <typename T>
+struct Pack8;
+template <>
+struct Pack8<uint16_t> {
+  uint32_t w[4];
+  template <bool ALIGNED>
+  __device__ __forceinline__ void load(const uint16_t *p, int n) {
+    if (ALIGNED || n >= 8) {
+      if constexpr (ALIGNED) {
+        const uint4 q = *(const uint4 *)p;
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+      } else {
+        const u32x4_a2 q = *(const u32x4_a2 *)p;
+        w[0] = q[0], w[1] = q[1], w[2] = q[2], w[3] = q[3];
+      }
+    } else {
+      w[0] = w[1] = w[2] = w[3] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    }
+  }
+  __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
+  __device__ __forceinline__ float get(int i) const {
+    return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+  }
+};
+template <>
+struct Pack8<float> {
+  float v[8];
+  template <bool ALIGNED>
+  __device__ __forceinline__ void load(const float *p, int n) { load8<ALIGNED>(p, n, v); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  }
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+};
+
+template <typename T, int VPT>
+struct RowIn {  // x, b, dy, dn of a row's columns
+  Pack8<T> x[VPT], b[VPT], dy[VPT], dn[VPT];
+  float mean_p, rstd_p, mean_n, rstd_n;
+};
+
+// A row's address for a lane: the row uniform, the lane's byte offset 32 bits.
+template <typename T>
+__device__ __forceinline__ T *lane_at(T *row, uint32_t bytes) {
+  return (T *)((char *)row + bytes);
+}
+template <typename T>
+__device__ __forceinline__ const T *lane_at(const T *row, uint32_t bytes) {
+  return (const T *)((const char *)row + bytes);
+}
+
+// The vectors that wait in LDS (slots of 16 KB VPT); the others are read from memory
+// for every row.
+constexpr bool vec_in_lds(int v, int vpt, bool bias) {
+  return v < (vpt == 4 ? 2 : V_BP) || (vpt == 1 && bias);
+}
+constexpr int lds_vecs(int vpt, bool bias) {
+  int n = 0;
+  for (int v = 0; v < VECS; ++v) n += vec_in_lds(v, vpt, bias);
+  return n;
+}
+
+// BIAS: the biases are there (their gradients' sums, and bp in c).
+template <typename T, int TPR, int VPT, bool ALIGNED, bool BIAS>
+__global__ __launch_bounds__(kBwdThreads, (VPT == 1 && !BIAS ? 4 : 2)) void
+residual_norm_bwd_kernel(ResNorm p, ResNormGrad g) {
+  constexpr int TEAMS = kBwdThreads / TPR;
   __shared__ float lds[64];
+  extern __shared__ __attribute__((aligned(16))) float vecs[];
   int slot = 0;
-  const int lane = threadIdx.x % TPR, dim = (int)p.dim;
-  const int64_t team = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TPR;
-  const bool live = team < g.teams;
-  // rows [r0, r1) of groups [g0, g1)
-  const int64_t t = live ? team : 0;
-  const int64_t g0 = (t / g.segs) * g.groups_per_team;
-  int64_t g1 = g0 + g.groups_per_team;
-  if (g1 > g.groups) g1 = g.groups;
-  const int64_t s0 = (t % g.segs) * g.seg_rows;
-  int64_t s1 = s0 + g.seg_rows;
-  if (s1 > p.per) s1 = p.per;
-  const bool post = p.wp != nullptr, has_b = p.b != nullptr;
+  const int tid = threadIdx.x, dim = (int)p.dim;
+  const uint32_t lane = (uint32_t)tid % TPR;
+  const int team = __builtin_amdgcn_readfirstlane(tid / TPR);  // a wave is of one team
+  const bool inside = g.segs > 0;  // segments inside groups, else whole groups
+  // this workgroup's rows [s0, s1) of group g0, or groups [g0, g1)
+  const int per = (int)p.per;
+  int g0, g1, s0, s1, rounds;
+  if (inside) {
+    g0 = (int)(blockIdx.x / (uint32_t)g.segs);
+    g1 = g0 + 1;
+    s0 = (int)((blockIdx.x % (uint32_t)g.segs) * (uint32_t)g.seg_rows);
+    s1 = std::min(s0 + (int)g.seg_rows, per);
+    rounds = ((int)g.seg_rows + TEAMS - 1) / TEAMS;
+  } else {
+    g0 = (int)(blockIdx.x * (uint32_t)g.groups_per_block);
+    g1 = (int)std::min<int64_t>(g0 + g.groups_per_block, g.groups);
+    s0 = 0;
+    s1 = per;
+    rounds = ((int)g.groups_per_block + TEAMS - 1) / TEAMS * per;
+  }
+  const bool post = p.wp != nullptr, has_b = p.b != nullptr, drop = p.drop.thr != 0;
+  const bool next = g.dn != nullptr;
   const float inv = 1.0f / (float)dim;
   uint64_t seed = 0, counter = 0;
-  if (p.drop.thr) dropout_key(p.drop, seed, counter);
+  if (drop) dropout_key(p.drop, seed, counter);
 
-  Cols<VPT> wp, bp, wn, sc, acc[SUMS];
-  load_vec<TPR, VPT, ALIGNED>(wp, p.wp, 1.0f, lane, dim);
-  load_vec<TPR, VPT, ALIGNED>(bp, p.bp, 0.0f, lane, dim);
-  load_vec<TPR, VPT, ALIGNED>(wn, g.dn ? p.wn : nullptr, 0.0f, lane, dim);
-  load_vec<TPR, VPT, ALIGNED>(sc, p.scale, 1.0f, lane, dim);
+  auto col = [&](int u) { return (int)(u * TPR + lane) * 8; };
+  // the vectors: this thread's columns in its own LDS slots
+  auto at = [&](int v, int u, int h) { return vecs + (((v * VPT + u) * 2 + h) * kBwdThreads + tid) * 4; };
+  auto keep_vec = [&](int v, const auto *src, float fill) __attribute__((always_inline)) {
+    if (!vec_in_lds(v, VPT, BIAS)) return;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = fill;
+      if (src && col(u) < dim) load8<ALIGNED>(src + col(u), dim - col(u), t);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *(float4 *)at(v, u, h) = make_float4(t[4 * h], t[4 * h + 1], t[4 * h + 2], t[4 * h + 3]);
+    }
+  };
+  auto get_vec = [&](float (&t)[4], int v, const auto *src, float fill, int u, int h)
+      __attribute__((always_inline)) {
+    if (vec_in_lds(v, VPT, BIAS)) {
+      const float4 q = *(const float4 *)at(v, u, h);
+      t[0] = q.x, t[1] = q.y, t[2] = q.z, t[3] = q.w;
+    } else {
+      float o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = fill;
+      if (src && col(u) < dim) load8<ALIGNED>(src + col(u), dim - col(u), o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = o[4 * h + i];
+    }
+  };
+  const float *const wn = next ? p.wn : nullptr;
+  keep_vec(V_WN, wn, 0.0f);
+  keep_vec(V_WP, p.wp, 1.0f);
+  keep_vec(V_SCALE, p.scale, 1.0f);
+  keep_vec(V_BP, p.bp, 0.0f);
+  if (!p.gate) keep_vec(V_GATE, (const T *)nullptr, 1.0f);
+
+  int gr = inside ? g0 : g0 + team, s = inside ? s0 + team : 0;
+  auto alive = [&](int gr_, int s_) { return gr_ < g1 && s_ < s1; };
+  auto step = [&](int &gr_, int &s_) {
+    if (inside) s_ += TEAMS;
+    else if (++s_ == per) s_ = 0, gr_ += TEAMS;
+  };
+  auto load_row = [&](RowIn<T, VPT> &r, int gr_, int s_) __attribute__((always_inline)) {
+    const int64_t m = alive(gr_, s_) ? (int64_t)gr_ * per + s_ : 0, base = m * dim;
+    const T *x = (const T *)p.x + base, *b = (const T *)p.b + base;
+    const T *dy = (const T *)g.dy + base, *dn = (const T *)g.dn + base;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const uint32_t o = (u * TPR + lane) * 8 * (uint32_t)sizeof(T);
+      const int left = dim - col(u);
+      r.x[u].clear(), r.b[u].clear(), r.dy[u].clear(), r.dn[u].clear();
+      if (left > 0) {
+        r.x[u].template load<ALIGNED>(lane_at(x, o), left);
+        if (has_b) r.b[u].template load<ALIGNED>(lane_at(b, o), left);
+        if (g.dy) r.dy[u].template load<ALIGNED>(lane_at(dy, o), left);
+        if (next) r.dn[u].template load<ALIGNED>(lane_at(dn, o), left);
+      }
+    }
+    r.mean_p = p.stats[m], r.rstd_p = p.stats[p.rows + m];
+    r.mean_n = p.stats[2 * p.rows + m], r.rstd_n = p.stats[3 * p.rows + m];
+  };
+
+  Cols<VPT> acc[SUMS];
 #pragma unroll
   for (int k = 0; k < SUMS; ++k)
 #pragma unroll
@@ -260,80 +417,91 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kerne
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[k].v[u][i] = 0.0f;
 
-  // every team of a workgroup makes the same number of rounds (barriers inside)
-  const int64_t rounds = g.groups_per_team * g.seg_rows;
-  int64_t gr = g0, s = s0;
-  Cols<VPT> gate;
-  load_vec<TPR, VPT, ALIGNED>(gate, nullptr, 1.0f, lane, dim);
   bool fresh = true;
-  for (int64_t k = 0; k < rounds; ++k) {
-    const bool on = live && gr < g1 && s < s1;
-    const int64_t m = on ? gr * p.per + s : 0;
-    if (on && fresh && p.gate)
-      load_cols<TPR, VPT, ALIGNED>(gate, (const T *)p.gate + gr * p.dim, lane, dim);
+  RowIn<T, VPT> r;
+  for (int k = 0; k < rounds; ++k) {
+    const bool on = alive(gr, s);
+    const int64_t m = on ? (int64_t)gr * per + s : 0;
+    const T *const gate = p.gate ? (const T *)p.gate + (int64_t)(on ? gr : 0) * dim : nullptr;
+    if (fresh && gate) keep_vec(V_GATE, gate, 1.0f);
     fresh = false;
-    Cols<VPT> x, b, dy, dn;
-    load_cols<TPR, VPT, ALIGNED>(x, (const T *)p.x + m * p.dim, lane, dim);
-    if (has_b) load_cols<TPR, VPT, ALIGNED>(b, (const T *)p.b + m * p.dim, lane, dim);
-    else load_vec<TPR, VPT, ALIGNED>(b, nullptr, 0.0f, lane, dim);
-    if (g.dy) load_cols<TPR, VPT, ALIGNED>(dy, (const T *)g.dy + m * p.dim, lane, dim);
-    else load_vec<TPR, VPT, ALIGNED>(dy, nullptr, 0.0f, lane, dim);
-    if (g.dn) load_cols<TPR, VPT, ALIGNED>(dn, (const T *)g.dn + m * p.dim, lane, dim);
-    else load_vec<TPR, VPT, ALIGNED>(dn, nullptr, 0.0f, lane, dim);
-    const float mean_p = p.stats[m], rstd_p = p.stats[p.rows + m];
-    const float mean_n = p.stats[2 * p.rows + m], rstd_n = p.stats[3 * p.rows + m];
+    load_row(r, gr, s);
     uint32_t w[VPT][4];
-    if (p.drop.thr) keep_bits<TPR, VPT, ALIGNED>(w, m, lane, dim, seed, counter);
+    if (drop) keep_bits<TPR, VPT, ALIGNED>(w, m, lane, dim, seed, counter);
 
-    // b -> bhat; yhat from x and c
+    // yhat from x and c, four columns at a time (the vectors' registers)
     Cols<VPT> yh;
     float a[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int u = 0; u < VPT; ++u)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float c = b.v[u][i];
-        if (post) {
-          b.v[u][i] = (b.v[u][i] - mean_p) * rstd_p;
-          c = b.v[u][i] * wp.v[u][i] + bp.v[u][i];
+      for (int h = 0; h < 2; ++h) {
+        float vwp[4], vbp[4], vg[4], vs[4], vn[4];
+        get_vec(vwp, V_WP, p.wp, 1.0f, u, h);
+        get_vec(vbp, V_BP, p.bp, 0.0f, u, h);
+        get_vec(vg, V_GATE, gate, 1.0f, u, h);
+        get_vec(vs, V_SCALE, p.scale, 1.0f, u, h);
+        get_vec(vn, V_WN, wn, 0.0f, u, h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * h + j;
+          const float c = (r.b[u].get(i) - r.mean_p) * r.rstd_p * vwp[j] + vbp[j];
+          float z = c * vg[j];
+          if (drop) z = keep_of(w[u], i, p.drop.thr) ? z * p.drop.scale : 0.0f;
+          const float y = r.x[u].get(i) * vs[j] + (has_b ? z : 0.0f);
+          yh.v[u][i] = (y - r.mean_n) * r.rstd_n;
+          const float d = r.dn[u].get(i) * vn[j];
+          a[0] = __builtin_fmaf(d, yh.v[u][i], a[0]);
+          a[1] += d;
         }
-        float z = c * gate.v[u][i];
-        if (p.drop.thr) z = keep_of(w[u], i, p.drop.thr) ? z * p.drop.scale : 0.0f;
-        const float y = x.v[u][i] * sc.v[u][i] + (has_b ? z : 0.0f);
-        yh.v[u][i] = (y - mean_n) * rstd_n;
-        const float d = dn.v[u][i] * wn.v[u][i];
-        a[0] = __builtin_fmaf(d, yh.v[u][i], a[0]);
-        a[1] += d;
+        __builtin_amdgcn_sched_barrier(0);
       }
-    if (g.dn) team_sum<TPR, 2>(a, lds, slot);
+    if (next) team_sum<TPR, 2>(a, lds, slot);
     const float ma = a[0] * inv, mb = p.layer ? a[1] * inv : 0.0f;
     float q[2] = {0.0f, 0.0f};
+    Cols<VPT> e;
+    T *const dx = on && g.dx ? (T *)g.dx + m * dim : nullptr;
 #pragma unroll
-    for (int u = 0; u < VPT; ++u)
+    for (int u = 0; u < VPT; ++u) {
+      const int c0 = col(u);
+      float out[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float d = dy.v[u][i];
-        if (g.dn) d += rstd_n * (dn.v[u][i] * wn.v[u][i] - yh.v[u][i] * ma - mb);
-        if (on) {
-          acc[SUM_WN].v[u][i] = __builtin_fmaf(dn.v[u][i], yh.v[u][i], acc[SUM_WN].v[u][i]);
-          acc[SUM_BN].v[u][i] += dn.v[u][i];
-          acc[SUM_S].v[u][i] = __builtin_fmaf(d, x.v[u][i], acc[SUM_S].v[u][i]);
+      for (int h = 0; h < 2; ++h) {
+        float vwp[4], vbp[4], vg[4], vs[4], vn[4];
+        get_vec(vwp, V_WP, p.wp, 1.0f, u, h);
+        get_vec(vbp, V_BP, p.bp, 0.0f, u, h);
+        get_vec(vg, V_GATE, gate, 1.0f, u, h);
+        get_vec(vs, V_SCALE, p.scale, 1.0f, u, h);
+        get_vec(vn, V_WN, wn, 0.0f, u, h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * h + j;
+          const float dn = r.dn[u].get(i), bh = (r.b[u].get(i) - r.mean_p) * r.rstd_p;
+          float d = r.dy[u].get(i);
+          if (next) d += r.rstd_n * (dn * vn[j] - yh.v[u][i] * ma - mb);
+          out[i] = d * vs[j];
+          float dk = d;
+          if (drop) dk = keep_of(w[u], i, p.drop.thr) ? d * p.drop.scale : 0.0f;
+          const float dc = dk * vg[j];
+          if (on) {
+            acc[SUM_WN].v[u][i] = __builtin_fmaf(dn, yh.v[u][i], acc[SUM_WN].v[u][i]);
+            acc[SUM_S].v[u][i] = __builtin_fmaf(d, r.x[u].get(i), acc[SUM_S].v[u][i]);
+            acc[SUM_G].v[u][i] = __builtin_fmaf(dk, bh * vwp[j] + vbp[j], acc[SUM_G].v[u][i]);
+            acc[SUM_WP].v[u][i] = __builtin_fmaf(dc, bh, acc[SUM_WP].v[u][i]);
+            if constexpr (BIAS) {
+              acc[SUM_BN].v[u][i] += dn;
+              acc[SUM_BP].v[u][i] += dc;
+            }
+          }
+          e.v[u][i] = c0 + i < dim ? dc * vwp[j] : 0.0f;
+          q[0] = __builtin_fmaf(e.v[u][i], c0 + i < dim ? bh : 0.0f, q[0]);
+          q[1] += e.v[u][i];
         }
-        x.v[u][i] = d * sc.v[u][i];  // dx
-        if (p.drop.thr) d = keep_of(w[u], i, p.drop.thr) ? d * p.drop.scale : 0.0f;
-        const float c = post ? b.v[u][i] * wp.v[u][i] + bp.v[u][i] : b.v[u][i];
-        const float dc = d * gate.v[u][i];
-        if (on) {
-          acc[SUM_G].v[u][i] = __builtin_fmaf(d, c, acc[SUM_G].v[u][i]);
-          acc[SUM_WP].v[u][i] = __builtin_fmaf(dc, b.v[u][i], acc[SUM_WP].v[u][i]);
-          acc[SUM_BP].v[u][i] += dc;
-        }
-        dn.v[u][i] = dc * wp.v[u][i];
-        const bool in = (u * TPR + lane) * 8 + i < dim;
-        q[0] = __builtin_fmaf(in ? dn.v[u][i] : 0.0f, in ? b.v[u][i] : 0.0f, q[0]);
-        q[1] += in ? dn.v[u][i] : 0.0f;
+        __builtin_amdgcn_sched_barrier(0);
       }
-    if (on && g.dx) store_cols<TPR, VPT, ALIGNED>(x, (T *)g.dx + m * p.dim, lane, dim);
+      if (dx && c0 < dim)
+        store8<ALIGNED>(lane_at(dx, (uint32_t)c0 * (uint32_t)sizeof(T)), dim - c0, out);
+    }
     if (has_b) {
       if (post) {
         team_sum<TPR, 2>(q, lds, slot);
@@ -341,36 +509,68 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kerne
 #pragma unroll
         for (int u = 0; u < VPT; ++u)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dn.v[u][i] = rstd_p * (dn.v[u][i] - b.v[u][i] * mq - mr);
+          for (int i = 0; i < 8; ++i) {
+            const float bh = (r.b[u].get(i) - r.mean_p) * r.rstd_p;
+            e.v[u][i] = r.rstd_p * (e.v[u][i] - bh * mq - mr);
+          }
       }
-      if (on && g.db) store_cols<TPR, VPT, ALIGNED>(dn, (T *)g.db + m * p.dim, lane, dim);
-    }
-    if (on && ++s == s1) {
-      if (g.dgate && g.segs == 1) {
-        store_cols<TPR, VPT, ALIGNED>(acc[SUM_G], (T *)g.dgate + gr * p.dim, lane, dim);
+      if (on && g.db) {
+        T *const db = (T *)g.db + m * dim;
 #pragma unroll
         for (int u = 0; u < VPT; ++u)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[SUM_G].v[u][i] = 0.0f;
+          if (col(u) < dim)
+            store8<ALIGNED>(lane_at(db, (uint32_t)col(u) * (uint32_t)sizeof(T)), dim - col(u),
+                            e.v[u]);
       }
-      s = s0;
-      ++gr;
+    }
+    if (on && !inside && s == per - 1) {
+      if (g.dgate)
+        store_cols<TPR, VPT, ALIGNED>(acc[SUM_G], (T *)g.dgate + (int64_t)gr * dim, lane, dim);
+#pragma unroll
+      for (int u = 0; u < VPT; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[SUM_G].v[u][i] = 0.0f;
       fresh = true;
     }
+    step(gr, s);
   }
-  if (!live) return;
-  float *out[SUMS] = {g.dwn, g.dbn, g.dscale, g.dwp, g.dbp, g.segs > 1 ? (float *)g.dgate : nullptr};
+  float *const out[SUMS] = {g.dwn, g.dbn, g.dscale, g.dwp, g.dbp, inside ? (float *)g.dgate : nullptr};
 #pragma unroll
-  for (int k = 0; k < SUMS; ++k)
-    if (out[k])
-      store_cols<TPR, VPT, ALIGNED>(acc[k], g.part + ((int64_t)k * g.teams + team) * p.dim, lane,
-                                    dim);
+  for (int k = 0; k < SUMS; ++k) {
+    if (!BIAS && (k == SUM_BN || k == SUM_BP)) continue;
+    if (!out[k]) continue;
+    if constexpr (TEAMS > 1) {
+      // thread tid of team 0 adds its columns of every team
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < VPT; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *(float4 *)at(0, u, h) = make_float4(acc[k].v[u][4 * h], acc[k].v[u][4 * h + 1],
+                                               acc[k].v[u][4 * h + 2], acc[k].v[u][4 * h + 3]);
+      __syncthreads();
+      if (team == 0) {
+#pragma unroll
+        for (int t = 1; t < TEAMS; ++t)
+#pragma unroll
+          for (int u = 0; u < VPT; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float4 f = *(const float4 *)(at(0, u, h) + t * TPR * 4);
+              acc[k].v[u][4 * h] += f.x, acc[k].v[u][4 * h + 1] += f.y;
+              acc[k].v[u][4 * h + 2] += f.z, acc[k].v[u][4 * h + 3] += f.w;
+            }
+      }
+    }
+    if (team == 0)
+      store_cols<TPR, VPT, ALIGNED>(acc[k], g.part + ((int64_t)k * g.blocks + blockIdx.x) * p.dim,
+                                    lane, dim);
+  }
 }
 
-// Column sums of the teams' partials: 64 columns a workgroup, 16 threads a column
-// over the teams in turn, their sums added in order.  blockIdx.y: one of the
-// vectors, or SUM_G + a gate row (that row's `segs` teams).
+// Column sums of the workgroups' partials: 64 columns a workgroup, 16 threads a column
+// over the partials in turn, their sums added in order.  blockIdx.y: one of the
+// vectors, or SUM_G + a gate row (that row's `segs` partials).
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(ResNormGrad g, int64_t dim) {
   __shared__ float red[16][64];
@@ -380,11 +580,20 @@ __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(ResNormGrad g, 
   const int64_t row = (int64_t)blockIdx.y - SUM_G;
   float *const vec[SUM_G] = {g.dwn, g.dbn, g.dscale, g.dwp, g.dbp};
   if (set < SUM_G && !vec[set]) return;
-  const int64_t first = set == SUM_G ? row * g.segs : 0, count = set == SUM_G ? g.segs : g.teams;
-  const float *part = g.part + ((int64_t)set * g.teams + first) * dim + col;
+  const int64_t first = set == SUM_G ? row * g.segs : 0, count = set == SUM_G ? g.segs : g.blocks;
+  const float *part = g.part + ((int64_t)set * g.blocks + first) * dim + col;
   float s = 0.0f;
-  if (col < dim)
-    for (int64_t t = r; t < count; t += 16) s += part[t * dim];
+  if (col < dim) {
+    int64_t t = r;
+    for (; t + 7 * 16 < count; t += 8 * 16) {  // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = part[(t + 16 * k) * dim];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    for (; t < count; t += 16) s += part[t * dim];
+  }
   red[r][c] = s;
   __syncthreads();
   if (r != 0 || col >= dim) return;
@@ -424,19 +633,30 @@ hipError_t launch_fwd(const ResNorm &p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename T, int TPR, int VPT, bool ALIGNED, bool BIAS>
+hipError_t launch_bwd_kernel(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
+  constexpr size_t lds = (size_t)kBwdThreads * 8 * VPT * sizeof(float) * lds_vecs(VPT, BIAS);
+  auto kern = residual_norm_bwd_kernel<T, TPR, VPT, ALIGNED, BIAS>;
+  static std::atomic<uint64_t> done{0};
+  if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
+  hipLaunchKernelGGL(kern, dim3((unsigned)g.blocks), dim3(kBwdThreads), lds, stream, p, g);
+  return hipGetLastError();
+}
+
 template <typename T, int TPR, int VPT>
 hipError_t launch_bwd(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
-  constexpr int NT = TPR > 256 ? TPR : 256;
-  const int64_t grid = (g.teams + NT / TPR - 1) / (NT / TPR);
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
-  const dim3 gr((unsigned)grid), bl(NT);
+  if (g.blocks > INT32_MAX) return hipErrorInvalidValue;
+  const bool bias = residual_norm_bias(p, g);
+  hipError_t e;
   if (all_aligned(p, &g))
-    hipLaunchKernelGGL((residual_norm_bwd_kernel<T, TPR, VPT, true>), gr, bl, 0, stream, p, g);
+    e = bias ? launch_bwd_kernel<T, TPR, VPT, true, true>(p, g, stream)
+             : launch_bwd_kernel<T, TPR, VPT, true, false>(p, g, stream);
   else
-    hipLaunchKernelGGL((residual_norm_bwd_kernel<T, TPR, VPT, false>), gr, bl, 0, stream, p, g);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    e = bias ? launch_bwd_kernel<T, TPR, VPT, false, true>(p, g, stream)
+             : launch_bwd_kernel<T, TPR, VPT, false, false>(p, g, stream);
+  if (e != hipSuccess) return e;
   const bool sums = g.dwn || g.dbn || g.dscale || g.dwp || g.dbp;
-  const bool gates = g.dgate && g.segs > 1;
+  const bool gates = g.dgate && g.segs > 0;
   if (!sums && !gates) return hipSuccess;
   const int64_t ny = SUM_G + (gates ? g.groups : 0);
   hipLaunchKernelGGL(residual_norm_sum_kernel<T>, dim3((unsigned)((p.dim + 63) / 64), (unsigned)ny),
@@ -462,36 +682,52 @@ hipError_t fwd_typed(const ResNorm &p, hipStream_t stream) {
   });
 }
 
+// Backward teams: one to eight waves of a workgroup of 512 threads.
+int bwd_team(int64_t dim) { return dim <= 512 ? 64 : dim <= 1024 ? 128 : dim <= 2048 ? 256 : 512; }
+
 template <typename T>
 hipError_t bwd_typed(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
-  return by_width<T>(p.dim, [&](auto tpr, auto vpt) {
-    return launch_bwd<T, decltype(tpr)::value, decltype(vpt)::value>(p, g, stream);
-  });
+  switch (bwd_team(p.dim)) {
+    case 64: return launch_bwd<T, 64, 1>(p, g, stream);
+    case 128: return launch_bwd<T, 128, 1>(p, g, stream);
+    case 256: return launch_bwd<T, 256, 1>(p, g, stream);
+    default: break;
+  }
+  if (p.dim <= 4096) return launch_bwd<T, 512, 1>(p, g, stream);
+  if (p.dim <= 8192) return launch_bwd<T, 512, 2>(p, g, stream);
+  return launch_bwd<T, 512, 4>(p, g, stream);
 }
 
 }  // namespace
 
-// Segments of rows for about `kTeams` teams: inside a gate row's group of `per`
-// rows where the groups are large, else whole groups.
-void plan_residual_norm_bwd(const ResNorm &p, ResNormGrad &g) {
-  constexpr int64_t kTeams = 512;
+// Rows for about as many workgroups as the chip holds at once (512 where two fit a
+// CU, else 256), a row for each team of one at least: segments inside a gate row's
+// group of `per` rows where the groups are large, else whole groups.  More workgroups
+// mean more partials and a last round half empty, fewer leave waits uncovered: 8192 x
+// 4096 bf16 with 256 / 512 / 1024 138 / 111 / 121 us, 4096 x 1024 fp32 with biases
+// (one a CU) 30 / 35 / 45.
+void plan_residual_norm_bwd(const ResNorm &p, ResNormGrad &g, bool bias) {
+  const int64_t kBlocks = p.dim <= 4096 && !bias ? 512 : 256;
+  const int64_t teams = kBwdThreads / bwd_team(p.dim);
   g.groups = p.rows / p.per;
-  const int64_t want = (p.rows + kTeams - 1) / kTeams;  // rows per team
+  const int64_t want = std::max(teams, (p.rows + kBlocks - 1) / kBlocks);  // rows per workgroup
   if (p.per >= want) {
     g.segs = (p.per + want - 1) / want;
     g.seg_rows = (p.per + g.segs - 1) / g.segs;
-    g.groups_per_team = 1;
-    g.teams = g.groups * g.segs;
+    g.groups_per_block = 1;
+    g.blocks = g.groups * g.segs;
   } else {
-    g.segs = 1;
+    g.segs = 0;
     g.seg_rows = p.per;
-    g.groups_per_team = want / p.per;
-    g.teams = (g.groups + g.groups_per_team - 1) / g.groups_per_team;
+    g.groups_per_block = std::max(teams, want / p.per);
+    g.blocks = (g.groups + g.groups_per_block - 1) / g.groups_per_block;
   }
 }
 
+bool residual_norm_bias(const ResNorm &p, const ResNormGrad &g) { return g.dbn || g.dbp || p.bp; }
+
 int64_t residual_norm_part_floats(const ResNormGrad &g, int64_t dim) {
-  return (int64_t)SUMS * g.teams * dim;
+  return (int64_t)SUMS * g.blocks * dim;
 }
 
 hipError_t launch_residual_norm(bool bf16, const ResNorm &p, hipStream_t stream) {
