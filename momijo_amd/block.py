@@ -53,6 +53,8 @@ def _scratch(nbytes: int, device) -> torch.Tensor:
 # ------------------------------------------------------------------ dropout
 def _seed_args(seed, device):
     """(seed, state) of a call: an integer, or a device int64 tensor {seed, counter}."""
+    if type(seed) is int:
+        return seed & _MASK64, None
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 2 or seed.device != device or \
                 not seed.is_contiguous():
@@ -73,15 +75,16 @@ def dropout(x: torch.Tensor, p: float, seed, counter: int = 0,
     added (a captured graph draws a new mask when the tensor changes).
     ``out`` may be x."""
     code = _check_type(x, "x")
-    x = x if x.is_contiguous() else x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     if out is None:
         out = torch.empty_like(x)
     elif out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous() or \
             out.device != x.device:
         raise ValueError(f"out must be a contiguous {x.dtype} {list(x.shape)} tensor")
     s, state = _seed_args(seed, x.device)
-    _lib.call("mj_dropout", code, _ptr(x), _ptr(out), x.numel(), p, s, int(counter) & _MASK64,
-              _ptr(state), _stream())
+    _lib.call("mj_dropout", code, x.data_ptr(), out.data_ptr(), x.numel(), p, s,
+              int(counter) & _MASK64, _ptr(state), _stream())
     return out
 
 
@@ -115,71 +118,67 @@ class Dropout:
 
 # ------------------------------------------------------------------ residual norm
 class ResidualNormSaved(NamedTuple):
-    """What residual_norm_backward needs: the operands and the rows' statistics."""
+    """What residual_norm_backward needs: the operands, the arguments that the kernels
+    take of them, and the rows' statistics."""
     x: torch.Tensor
     branch: torch.Tensor | None
     gate: torch.Tensor | None
-    scale: torch.Tensor | None
-    post_weight: torch.Tensor | None
-    post_bias: torch.Tensor | None
-    next_weight: torch.Tensor | None
-    next_bias: torch.Tensor | None
-    norm: str
-    p: float
-    seed: int
+    vectors: tuple        # scale, post_weight, post_bias, next_weight, next_bias
+    args: tuple           # type, norm, pointers of the operands
+    drop: tuple           # p, seed, counter, pointer of the state
     state: torch.Tensor | None
-    counter: int
     stats: torch.Tensor
-    gate_shape: tuple
 
 
-def _vector(t, x, dim, name):
+_VECTORS = ("scale", "post_weight", "post_bias", "next_weight", "next_bias")
+
+
+def _vector(t, device, dim, name):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.device != x.device or t.numel() != dim:
-        raise ValueError(f"{name} must be float32 with {dim} elements on {x.device}")
+    if t.dtype is not torch.float32 or t.numel() != dim or t.device != device:
+        raise ValueError(f"{name} must be float32 with {dim} elements on {device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight, next_bias, norm,
                    eps, p, seed, counter, train):
     code = _check_type(x, "x")
-    if norm not in _NORMS:
+    kind = _NORMS.get(norm)
+    if kind is None:
         raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
-    if x.dim() < 1:
+    shape, device = x.shape, x.device
+    if not shape:
         raise ValueError("x must have at least one dimension")
-    x = x if x.is_contiguous() else x.contiguous()
-    dim = x.shape[-1]
+    if not x.is_contiguous():
+        x = x.contiguous()
+    dim = shape[-1]
     rows = x.numel() // dim if dim else 0
     if branch is not None:
-        branch = _like(branch, x, x.shape, "branch")
-    gate_rows, gate_shape = 0, ()
+        branch = _like(branch, x, shape, "branch")
+    gate_rows = 0
     if gate is not None:
-        gate_shape = tuple(gate.shape)
         if gate.dim() not in (1, 2) or gate.shape[-1] != dim:
             raise ValueError(f"gate must be [{dim}] or [groups, {dim}], got {list(gate.shape)}")
         gate = _like(gate, x, gate.shape, "gate")
         gate_rows = 1 if gate.dim() == 1 else gate.shape[0]
-    scale = _vector(scale, x, dim, "scale")
-    post_weight = _vector(post_weight, x, dim, "post_weight")
-    post_bias = _vector(post_bias, x, dim, "post_bias")
-    next_weight = _vector(next_weight, x, dim, "next_weight")
-    next_bias = _vector(next_bias, x, dim, "next_bias")
-    s, state = _seed_args(seed, x.device)
-    counter = int(counter) & _MASK64
+    scale = _vector(scale, device, dim, "scale")
+    wp, bp = _vector(post_weight, device, dim, "post_weight"), _vector(post_bias, device, dim, "post_bias")
+    wn, bn = _vector(next_weight, device, dim, "next_weight"), _vector(next_bias, device, dim, "next_bias")
+    seed, state = _seed_args(seed, device)
     # without a branch and a scale, y is x itself
     y = x if branch is None and scale is None else torch.empty_like(x)
-    n = torch.empty_like(x) if next_weight is not None else None
-    stats = torch.empty((4, rows), dtype=torch.float32, device=x.device) if train else None
+    n = None if wn is None else torch.empty_like(x)
+    stats = torch.empty((4, rows), dtype=torch.float32, device=device) if train else None
+    args = (code, kind, x.data_ptr(), _ptr(branch), _ptr(gate), gate_rows, _ptr(scale), _ptr(wp),
+            _ptr(bp), _ptr(wn))
+    drop = (p, seed, int(counter) & _MASK64, _ptr(state))
     if y is not x or n is not None:
-        _lib.call("mj_residual_norm", code, _NORMS[norm], _ptr(x), _ptr(branch), _ptr(gate),
-                  gate_rows, _ptr(scale), _ptr(post_weight), _ptr(post_bias), _ptr(next_weight),
-                  _ptr(next_bias), eps, p, s, counter, _ptr(state), None if y is x else _ptr(y),
-                  _ptr(n), _ptr(stats), rows, dim, _stream())
+        _lib.call("mj_residual_norm", *args, _ptr(bn), eps, *drop,
+                  None if y is x else y.data_ptr(), _ptr(n), _ptr(stats), rows, dim, _stream())
     if not train:
-        return y, n, None
-    return y, n, ResidualNormSaved(x, branch, gate, scale, post_weight, post_bias, next_weight,
-                                   next_bias, norm, p, s, state, counter, stats, gate_shape)
+        return y, n
+    return y, n, ResidualNormSaved(x, branch, gate, (scale, wp, bp, wn, bn), args, drop, state, stats)
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *,
@@ -199,9 +198,8 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *,
     the first block: y = scale * x.  ``gate`` is [dim] or [groups, dim] with
     consecutive rows of equal number in each group; x, branch and gate are of one
     type, the vectors Float32."""
-    y, n, _ = _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight,
-                             next_bias, norm, eps, p, seed, counter, False)
-    return y, n
+    return _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight, next_bias,
+                          norm, eps, p, seed, counter, False)
 
 
 def residual_norm_train(x: torch.Tensor, branch: torch.Tensor | None = None, *,
@@ -227,40 +225,38 @@ def residual_norm_backward(dy: torch.Tensor | None, dn: torch.Tensor | None,
     """The gradients of residual_norm's operands, by their names, from the
     gradients of y and n (either may be None, for zero).  Those of x, branch and
     gate have their type, those of the vectors are Float32."""
-    s = saved
-    x = s.x
-    dim, rows = x.shape[-1], s.stats.shape[1]
+    x, branch, gate, vectors, args, drop, _, stats = saved
+    shape = x.shape
+    dim, rows = shape[-1], stats.shape[1]
     if dy is not None:
-        dy = _like(dy, x, x.shape, "dy")
+        dy = _like(dy, x, shape, "dy")
     if dn is not None:
-        if s.next_weight is None:
+        if vectors[3] is None:
             raise ValueError("dn given, but the forward had no next norm")
-        dn = _like(dn, x, x.shape, "dn")
+        dn = _like(dn, x, shape, "dn")
     out = {"x": torch.empty_like(x)}
-    if s.branch is not None:
+    if branch is not None:
         out["branch"] = torch.empty_like(x)
-    if s.gate is not None:
-        out["gate"] = torch.empty_like(s.gate)
-    for name in ("scale", "post_weight", "post_bias", "next_weight", "next_bias"):
-        if getattr(s, name) is not None:
-            out[name] = torch.empty_like(getattr(s, name))
+    if gate is not None:
+        out["gate"] = torch.empty_like(gate)
+    for name, v in zip(_VECTORS, vectors):
+        if v is not None:
+            out[name] = torch.empty_like(v)
     if rows == 0 or dim == 0 or (dy is None and dn is None):
         return {k: v.zero_() for k, v in out.items()}
+    at = {k: v.data_ptr() for k, v in out.items()}
     if dn is None:  # nothing reaches the next norm
-        for name in ("next_weight", "next_bias"):
+        for name in _VECTORS[3:]:
             if name in out:
                 out[name].zero_()
-    gate_rows = 0 if s.gate is None else s.gate.numel() // dim
-    nbytes = _norm_work(rows, dim, gate_rows)
+                del at[name]
+    nbytes = _norm_work(rows, dim, args[5])
     work = _scratch(nbytes, x.device)
-    ptr = {k: v.data_ptr() for k, v in out.items()}
-    at = ptr.get
-    _lib.call("mj_residual_norm_backward", _DTYPES[x.dtype], _NORMS[s.norm], _ptr(x),
-              _ptr(s.branch), _ptr(s.gate), gate_rows, _ptr(s.scale), _ptr(s.post_weight),
-              _ptr(s.post_bias), _ptr(s.next_weight), s.p, s.seed, s.counter, _ptr(s.state),
-              _ptr(s.stats), _ptr(dy), _ptr(dn), at("x"), at("branch"), at("gate"), at("scale"),
-              at("post_weight"), at("post_bias"), None if dn is None else at("next_weight"),
-              None if dn is None else at("next_bias"), rows, dim, _ptr(work), nbytes, _stream())
+    get = at.get
+    _lib.call("mj_residual_norm_backward", *args, *drop, stats.data_ptr(), _ptr(dy), _ptr(dn),
+              at["x"], get("branch"), get("gate"), get("scale"), get("post_weight"),
+              get("post_bias"), get("next_weight"), get("next_bias"), rows, dim, work.data_ptr(),
+              nbytes, _stream())
     return out
 
 
