@@ -574,15 +574,17 @@ int32_t mj_residual_norm_backward(int32_t dtype, int32_t norm, const void *x, co
  * bf16: K, I, H multiples of 8 (mj_copy_rows_bf16 pads other widths), 16-byte aligned arrays;
  * h is rounded to bf16; g, u fp32 [M,I] are written for the backward, or both NULL;
  * `work` as mj_gated_mlp_work_bytes says (NULL where that is 0).
- * fp32: any widths; h, g, u are required. */
+ * fp32: any widths; h, g, u are required (u right behind g saves a launch), and `work`
+ * as mj_gated_mlp_f32_work_bytes says; these and y are 16-byte aligned. */
 int64_t mj_gated_mlp_work_bytes(int64_t M, int64_t K, int64_t I, int64_t H, int32_t backward);
 int32_t mj_gated_mlp_bf16(const uint16_t *x, const uint16_t *Wg, const uint16_t *Wu,
                           const uint16_t *Wd, int32_t act, uint16_t *h, float *g, float *u,
                           uint16_t *y, int64_t M, int64_t K, int64_t I, int64_t H, void *work,
                           int64_t work_bytes, void *stream);
+int64_t mj_gated_mlp_f32_work_bytes(int64_t M, int64_t K, int64_t I, int64_t H, int32_t backward);
 int32_t mj_gated_mlp_f32(const float *x, const float *Wg, const float *Wu, const float *Wd,
                          int32_t act, float *h, float *g, float *u, float *y, int64_t M, int64_t K,
-                         int64_t I, int64_t H, void *stream);
+                         int64_t I, int64_t H, void *work, int64_t work_bytes, void *stream);
 
 /* Row copies between a width and its zero-padded form, n (1..4) matrices in one
  * launch: dst[i] [dst_rows, dst_cols] (rows dst_ld apart) takes src[i] [rows, cols] (rows
@@ -596,7 +598,8 @@ int32_t mj_copy_rows_bf16(int32_t n, const uint16_t *const *src, uint16_t *const
  *   dh = dy Wd, dg = dh u act'(g), du = dh act(g)
  *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
  * dg, du [M,I] are scratch (bf16 in the bf16 form); any of dx, dWg, dWu, dWd may be
- * NULL.  relu'(0) = 0. */
+ * NULL.  relu'(0) = 0.  `work` as the forward's, with backward = 1.  fp32: dWu
+ * right behind dWg saves a launch; g, u, dg, du, dx and work are 16-byte aligned. */
 int32_t mj_gated_mlp_backward_bf16(const uint16_t *x, const uint16_t *Wg, const uint16_t *Wu,
                                    const uint16_t *Wd, int32_t act, const uint16_t *h,
                                    const float *g, const float *u, const uint16_t *dy,
@@ -607,7 +610,7 @@ int32_t mj_gated_mlp_backward_f32(const float *x, const float *Wg, const float *
                                   int32_t act, const float *h, const float *g, const float *u,
                                   const float *dy, float *dg, float *du, float *dx, float *dWg,
                                   float *dWu, float *dWd, int64_t M, int64_t K, int64_t I,
-                                  int64_t H, void *stream);
+                                  int64_t H, void *work, int64_t work_bytes, void *stream);
 
 #ifdef __cplusplus
 }

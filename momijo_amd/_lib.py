@@ -126,11 +126,13 @@ SIGNATURES = {
                                   [_F, _U64, _U64] + [_P] * 12 + [_I64, _I64, _P, _I64, _P]),
     "mj_gated_mlp_work_bytes": (_I64, [_I64, _I64, _I64, _I64, _I32]),
     "mj_gated_mlp_bf16": (_I32, [_P] * 4 + [_I32] + [_P] * 4 + [_I64] * 4 + [_P, _I64, _P]),
-    "mj_gated_mlp_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 4 + [_I64] * 4 + [_P]),
+    "mj_gated_mlp_f32_work_bytes": (_I64, [_I64, _I64, _I64, _I64, _I32]),
+    "mj_gated_mlp_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 4 + [_I64] * 4 + [_P, _I64, _P]),
     "mj_copy_rows_bf16": (_I32, [_I32, _P, _P, _P, _P]),
     "mj_gated_mlp_backward_bf16": (_I32, [_P] * 4 + [_I32] + [_P] * 10 + [_I64] * 4 +
                                    [_P, _I64, _P]),
-    "mj_gated_mlp_backward_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 10 + [_I64] * 4 + [_P]),
+    "mj_gated_mlp_backward_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 10 + [_I64] * 4 +
+                                  [_P, _I64, _P]),
 }
 
 _lib = None

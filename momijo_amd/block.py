@@ -347,8 +347,9 @@ def _mlp_operands(x, gate, up, down):
 
 
 @functools.lru_cache(maxsize=1024)
-def _mlp_work(M, K, I, H, backward):
-    return _lib.load().mj_gated_mlp_work_bytes(M, K, I, H, backward)
+def _mlp_work(M, K, I, H, backward, f32=False):
+    lib = _lib.load()
+    return (lib.mj_gated_mlp_f32_work_bytes if f32 else lib.mj_gated_mlp_work_bytes)(M, K, I, H, backward)
 
 
 def _padded(mats, at):
@@ -375,10 +376,13 @@ def _gated_mlp(x, gate, up, down, act, train):
     # them), h, then in bf16 padded operands, a padded y and the workspace
     if x2.dtype == torch.float32:
         gu = _up16(4 * M * I)
-        buf = _scratch(3 * gu, dev)
+        nbytes = _mlp_work(M, K, I, H, 0, True)
+        buf = _scratch(3 * gu + (0 if train else nbytes), dev)
+        more = _scratch(nbytes, dev) if train and nbytes else None
         g = buf.data_ptr()
+        work = None if not nbytes else g + 3 * gu if more is None else more.data_ptr()
         _lib.call("mj_gated_mlp_f32", *ptrs, act, g + 2 * gu, g, g + gu, y.data_ptr(), M, K, I, H,
-                  _stream())
+                  work, nbytes, _stream())
     else:
         Kp, Ip, Hp = K + 7 & ~7, I + 7 & ~7, H + 7 & ~7
         gu = _up16(4 * M * Ip) if train else 0
@@ -433,16 +437,20 @@ def gated_mlp_backward(dy: torch.Tensor, saved: GatedMLPSaved):
     s = saved
     x, (M, K), (H, I) = s.x, s.x.shape, s.down.shape
     dy = _like(dy, x, s.rows + (H,), "dy")
-    out = dx, dgate, dup, ddown = x.new_empty((M, K)), x.new_empty((I, K)), x.new_empty((I, K)), \
-        x.new_empty((H, I))
+    f32 = x.dtype == torch.float32
+    dx, ddown = x.new_empty((M, K)), x.new_empty((H, I))
+    # (fp32: side by side, for one launch)
+    dgate, dup = x.new_empty((2, I, K)).unbind() if f32 else (x.new_empty((I, K)), x.new_empty((I, K)))
+    out = dx, dgate, dup, ddown
     outs = tuple(t.data_ptr() for t in out)
     g = s.buf.data_ptr()
-    if x.dtype == torch.float32:
+    if f32:
         gu = _up16(4 * M * I)
-        buf = _scratch(2 * gu, x.device)  # dg, du
+        nbytes = _mlp_work(M, K, I, H, 1, True)
+        buf = _scratch(2 * gu + nbytes, x.device)  # dg, du, the workspace
         dg = buf.data_ptr()
         _lib.call("mj_gated_mlp_backward_f32", *s.ptrs, s.act, g + 2 * gu, g, g + gu, dy.data_ptr(),
-                  dg, dg + gu, *outs, M, K, I, H, _stream())
+                  dg, dg + gu, *outs, M, K, I, H, dg + 2 * gu if nbytes else None, nbytes, _stream())
     else:
         Kp, Ip, Hp = K + 7 & ~7, I + 7 & ~7, H + 7 & ~7
         gu, db = _up16(4 * M * Ip), _up16(2 * M * Ip)

@@ -70,6 +70,44 @@ int32_t make_dropout(float p, uint64_t seed, uint64_t counter, const uint64_t *s
   return MJ_OK;
 }
 
+// K slices of an fp32 product (`pair`: of two of one shape in one launch): as many as
+// bring its 64 x 64 tiles to four a CU with 512 k each at least.  y of 1024 x 1024 with
+// K = 2752 61 us whole, 48 and 5 for the sum in four slices; dx, two such products,
+// 147 us one after the other, 78 and 5 in one launch of two slices each.
+int64_t f32_slices(int64_t M, int64_t N, int64_t K, int64_t pair) {
+  const int64_t tiles = ((M + 63) / 64) * ((N + 63) / 64) * pair;
+  int64_t s = 1;
+  while (s < 4 && tiles * s * 2 <= 1024 && K % (2 * s) == 0 && K / (2 * s) >= 512) s *= 2;
+  return s;
+}
+
+// Whether two products' results may be slices of one sum: they fill the chip only
+// together (beyond, adding into the first's result moves fewer bytes).
+bool f32_sums_pair(int64_t M, int64_t N) {
+  return ((M + 63) / 64) * ((N + 63) / 64) * 2 <= 1024;
+}
+
+int64_t words_between(const void *a, const void *b) {
+  return ((intptr_t)b - (intptr_t)a) / (intptr_t)sizeof(float);
+}
+
+// `pair` (1 or 2) products of one shape, each in `slices` along K, in one launch: C
+// [pair][slices][M][N]; the second product's operands lie at A1, B1.
+int32_t f32_products(int64_t pair, int64_t slices, int64_t M, int64_t N, int64_t K, const float *A,
+                     const float *A1, int64_t sAm, int64_t sAk, const float *B, const float *B1,
+                     int64_t sBk, int64_t sBn, float *C, hipStream_t st, const char *what) {
+  mj::BatchDesc bd;
+  bd.rank = 2;
+  bd.shape[0] = pair, bd.shape[1] = slices;
+  bd.a_stride[0] = pair > 1 ? words_between(A, A1) : 0;
+  bd.b_stride[0] = pair > 1 ? words_between(B, B1) : 0;
+  const int64_t k = K / slices;
+  bd.a_stride[1] = k * sAk, bd.b_stride[1] = k * sBk;
+  return hip_status(mj::launch_gemm_f32_batched(M, N, k, A, sAm, sAk, B, sBk, sBn, C, bd,
+                                                pair * slices, st),
+                    what);
+}
+
 // The shared arguments of the residual norm and its backward.
 int32_t make_norm(mj::ResNorm &r, int32_t dtype, int32_t norm, const void *x, const void *b,
                   const void *gate, int64_t gate_rows, const float *scale, const float *wp,
@@ -260,30 +298,50 @@ int32_t mj_gated_mlp_backward_bf16(const uint16_t *x, const uint16_t *Wg, const 
   return hip_status(mj::launch_gated_mlp_bwd(q, o, S(stream)), "gated MLP backward launch");
 }
 
+int64_t mj_gated_mlp_f32_work_bytes(int64_t M, int64_t K, int64_t I, int64_t H, int32_t backward) {
+  if (M <= 0 || K <= 0 || I <= 0 || H <= 0) return 0;
+  const int64_t N = backward ? K : H, n = f32_slices(M, N, I, backward ? 2 : 1) * (backward ? 2 : 1);
+  return n == 1 || (backward && !f32_sums_pair(M, N)) ? 0 : n * M * N * (int64_t)sizeof(float);
+}
+
 int32_t mj_gated_mlp_f32(const float *x, const float *Wg, const float *Wu, const float *Wd,
                          int32_t act, float *h, float *g, float *u, float *y, int64_t M, int64_t K,
-                         int64_t I, int64_t H, void *stream) {
+                         int64_t I, int64_t H, void *work, int64_t work_bytes, void *stream) {
   if (int32_t s = check_mlp(act, M, K, I, H)) return s;
   if (M == 0) return MJ_OK;
   if ((H > 0 && !y) || (I > 0 && (!h || !g || !u || (H > 0 && !Wd) || (K > 0 && (!x || !Wg || !Wu)))))
     return fail(MJ_ERR_ARG, "null operand");
-  const void *el[] = {h, g, u};
+  const void *el[] = {h, g, u, y, work};
   for (const void *e : el)
-    if (!aligned16(e)) return fail(MJ_ERR_UNSUPPORTED, "gated MLP: h, g, u must be 16-byte aligned");
+    if (!aligned16(e))
+      return fail(MJ_ERR_UNSUPPORTED, "gated MLP: h, g, u, y and work must be 16-byte aligned");
+  const int64_t need = mj_gated_mlp_f32_work_bytes(M, K, I, H, 0);
+  if (need > 0 && (!work || work_bytes < need))
+    return fail(MJ_ERR_ARG, "gated MLP: work must hold %lld bytes", (long long)need);
   const hipStream_t st = S(stream);
   if (I > 0) {
-    if (int32_t e = mj_linear_f32(x, Wg, nullptr, MJ_EPI_NONE, g, M, K, I, stream)) return e;
-    if (int32_t e = mj_linear_f32(x, Wu, nullptr, MJ_EPI_NONE, u, M, K, I, stream)) return e;
+    // both projections in one launch where u follows g
+    if (K > 0 && u == g + M * I) {
+      if (int32_t e = f32_products(2, 1, M, I, K, x, x, K, 1, Wg, Wu, 1, K, g, st, "gate and up launch"))
+        return e;
+    } else {
+      if (int32_t e = mj_linear_f32(x, Wg, nullptr, MJ_EPI_NONE, g, M, K, I, stream)) return e;
+      if (int32_t e = mj_linear_f32(x, Wu, nullptr, MJ_EPI_NONE, u, M, K, I, stream)) return e;
+    }
     if (int32_t e = hip_status(mj::launch_gate_f32(act, g, u, h, M * I, st), "gate launch")) return e;
   }
-  return mj_linear_f32(h, Wd, nullptr, MJ_EPI_NONE, y, M, I, H, stream);
+  if (need == 0) return mj_linear_f32(h, Wd, nullptr, MJ_EPI_NONE, y, M, I, H, stream);
+  const int64_t s = f32_slices(M, H, I, 1);
+  if (int32_t e = f32_products(1, s, M, H, I, h, h, I, 1, Wd, Wd, 1, I, (float *)work, st, "y launch"))
+    return e;
+  return hip_status(mj::launch_sum_f32((const float *)work, y, M * H, s, st), "y sum launch");
 }
 
 int32_t mj_gated_mlp_backward_f32(const float *x, const float *Wg, const float *Wu, const float *Wd,
                                   int32_t act, const float *h, const float *g, const float *u,
                                   const float *dy, float *dg, float *du, float *dx, float *dWg,
                                   float *dWu, float *dWd, int64_t M, int64_t K, int64_t I,
-                                  int64_t H, void *stream) {
+                                  int64_t H, void *work, int64_t work_bytes, void *stream) {
   if (int32_t s = check_mlp(act, M, K, I, H)) return s;
   const bool inner = M > 0 && I > 0 && (dx || dWg || dWu);
   if (inner && (!dg || !du || !g || !u || (H > 0 && (!dy || !Wd))))
@@ -291,9 +349,13 @@ int32_t mj_gated_mlp_backward_f32(const float *x, const float *Wg, const float *
   if (M > 0 && I > 0 && K > 0 && dx && (!Wg || !Wu)) return fail(MJ_ERR_ARG, "null weights");
   if (M > 0 && I > 0 && K > 0 && (dWg || dWu) && !x) return fail(MJ_ERR_ARG, "null x");
   if (M > 0 && I > 0 && H > 0 && dWd && (!dy || !h)) return fail(MJ_ERR_ARG, "null dy or h");
-  const void *el[] = {g, u, dg, du};
+  const void *el[] = {g, u, dg, du, dx, work};
   for (const void *e : el)
-    if (!aligned16(e)) return fail(MJ_ERR_UNSUPPORTED, "gated MLP: g, u, dg, du must be 16-byte aligned");
+    if (!aligned16(e))
+      return fail(MJ_ERR_UNSUPPORTED, "gated MLP: g, u, dg, du, dx and work must be 16-byte aligned");
+  const int64_t need = dx ? mj_gated_mlp_f32_work_bytes(M, K, I, H, 1) : 0;
+  if (need > 0 && (!work || work_bytes < need))
+    return fail(MJ_ERR_ARG, "gated MLP backward: work must hold %lld bytes", (long long)need);
   const hipStream_t st = S(stream);
   // dh = dy Wd into dg, which the elementwise step then overwrites in place
   if (inner) {
@@ -304,19 +366,35 @@ int32_t mj_gated_mlp_backward_f32(const float *x, const float *Wg, const float *
       return e;
   }
   if (dx && M > 0 && K > 0) {
-    if (int32_t e = mj_matmul_f32(M, K, I, dg, I, 1, Wg, K, 1, nullptr, MJ_EPI_NONE, dx, K, stream))
-      return e;
-    if (int32_t e = hip_status(mj::launch_gemm_f32_accum(M, K, I, du, I, 1, Wu, K, 1, dx, K, 1, st),
-                               "dx launch"))
-      return e;
+    if (need > 0) {
+      const int64_t s = f32_slices(M, K, I, 2);
+      if (int32_t e = f32_products(2, s, M, K, I, dg, du, I, 1, Wg, Wu, K, 1, (float *)work, st,
+                                   "dx launch"))
+        return e;
+      if (int32_t e = hip_status(mj::launch_sum_f32((const float *)work, dx, M * K, 2 * s, st),
+                                 "dx sum launch"))
+        return e;
+    } else {
+      if (int32_t e = mj_matmul_f32(M, K, I, dg, I, 1, Wg, K, 1, nullptr, MJ_EPI_NONE, dx, K, stream))
+        return e;
+      if (int32_t e = hip_status(mj::launch_gemm_f32_accum(M, K, I, du, I, 1, Wu, K, 1, dx, K, 1, st),
+                                 "dx launch"))
+        return e;
+    }
   }
-  // dW = d^T x: the transposes are strides
-  if (dWg)
-    if (int32_t e = mj_matmul_f32(I, K, M, dg, 1, I, x, K, 1, nullptr, MJ_EPI_NONE, dWg, K, stream))
+  // dW = d^T x: the transposes are strides; both projections' in one launch where dWu
+  // follows dWg
+  if (dWg && dWu == dWg + I * K && M > 0 && I > 0 && K > 0) {
+    if (int32_t e = f32_products(2, 1, I, K, M, dg, du, 1, I, x, x, K, 1, dWg, st, "dW launch"))
       return e;
-  if (dWu)
-    if (int32_t e = mj_matmul_f32(I, K, M, du, 1, I, x, K, 1, nullptr, MJ_EPI_NONE, dWu, K, stream))
-      return e;
+  } else {
+    if (dWg)
+      if (int32_t e = mj_matmul_f32(I, K, M, dg, 1, I, x, K, 1, nullptr, MJ_EPI_NONE, dWg, K, stream))
+        return e;
+    if (dWu)
+      if (int32_t e = mj_matmul_f32(I, K, M, du, 1, I, x, K, 1, nullptr, MJ_EPI_NONE, dWu, K, stream))
+        return e;
+  }
   if (dWd)
     if (int32_t e = mj_matmul_f32(H, I, M, dy, 1, H, h, I, 1, nullptr, MJ_EPI_NONE, dWd, I, stream))
       return e;

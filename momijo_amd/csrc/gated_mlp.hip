@@ -219,7 +219,9 @@ __device__ __forceinline__ TileAt locate(const TileArgs &a) {
   return t;
 }
 
-// The columns that a lane's block j (of 16) starts at, in the tile's output.
+// The outputs of a tile.  A lane's block (i, j) holds row 16 i + (lane & 15) at columns
+// 16 j + 4 (lane >> 4) + q; pairs of blocks are traded between lane rows so that a lane
+// stores 16 bytes.
 template <int ACT, int TM, int TN, int WM, int WN>
 __device__ __forceinline__ void out_gate(const TileProb &p, const f32x4 (&acc)[TM][TN], int m0,
                                          int n0, int wm, int wn, int lane) {
@@ -300,8 +302,6 @@ __device__ __forceinline__ void out_dgate(const TileProb &p, const f32x4 (&acc)[
   }
 }
 
-// A lane's block (i, j) holds row 16 i + (lane & 15) at columns 16 j + 4 (lane >> 4)
-// + q; pairs of blocks are traded between lane rows so that a lane stores 16 bytes.
 template <int TM, int TN, int WM, int WN>
 __device__ __forceinline__ void out_store(const TileProb &p, const f32x4 (&acc)[TM][TN], int m0,
                                           int n0, int wm, int wn, int lane) {
@@ -841,6 +841,27 @@ __global__ __launch_bounds__(256) void gate_bwd_f32_kernel(int act, const float 
   }
 }
 
+// The sum of an fp32 product's K slices, in slice order; the buffers are 16-byte aligned
+// where n is a multiple of 4.
+__global__ __launch_bounds__(256) void sum_f32_kernel(const float *part, float *out, int64_t n,
+                                                      int parts) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (n % 4 == 0 && e < n) {
+    float4 s = *(const float4 *)(part + e);
+    for (int k = 1; k < parts; ++k) {
+      const float4 q = *(const float4 *)(part + k * n + e);
+      s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+    }
+    *(float4 *)(out + e) = s;
+  } else {
+    for (int64_t i = e; i < n && i < e + 4; ++i) {
+      float s = part[i];
+      for (int k = 1; k < parts; ++k) s += part[k * n + i];
+      out[i] = s;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- launch
 void set_tiles(TileArgs &a, int bm, int bn_out) {
   a.tiles = 0;
@@ -1106,6 +1127,16 @@ hipError_t launch_gate_f32(int act, const float *g, const float *u, float *h, in
   const int64_t grid = (n + 1023) / 1024;
   if (grid > INT32_MAX) return hipErrorInvalidValue;
   hipLaunchKernelGGL(gate_f32_kernel, dim3((unsigned)grid), dim3(256), 0, stream, act, g, u, h, n);
+  return hipGetLastError();
+}
+
+hipError_t launch_sum_f32(const float *part, float *out, int64_t n, int64_t parts,
+                          hipStream_t stream) {
+  if (n <= 0) return hipSuccess;
+  const int64_t grid = (n + 1023) / 1024;
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(sum_f32_kernel, dim3((unsigned)grid), dim3(256), 0, stream, part, out, n,
+                     (int)parts);
   return hipGetLastError();
 }
 

@@ -335,6 +335,9 @@ hipError_t launch_copy_rows_bf16(const CopyRows &c, hipStream_t stream);
 // act'(g), du = dh act(g) over n elements.
 hipError_t launch_gate_f32(int act, const float *g, const float *u, float *h, int64_t n,
                            hipStream_t stream);
+// out = the sum of `parts` arrays of n floats each, in order.
+hipError_t launch_sum_f32(const float *part, float *out, int64_t n, int64_t parts,
+                          hipStream_t stream);
 hipError_t launch_gate_bwd_f32(int act, const float *g, const float *u, const float *dh, float *dg,
                                float *du, int64_t n, hipStream_t stream);
 

@@ -89,6 +89,49 @@ def test_gated_mlp_status_codes(lib):
                                  None) == _lib.MJ_ERR_ARG
 
 
+def test_gated_mlp_f32_status_codes(lib):
+    p, odd = ctypes.c_void_p(16), ctypes.c_void_p(20)
+    big = 1 << 40
+    fwd = lambda m, k, i, h, g=p, y=p, work=p, nbytes=big, act=3: lib.mj_gated_mlp_f32(  # noqa: E731
+        p, p, p, p, act, p, g, p, y, m, k, i, h, work, nbytes, None)
+    assert fwd(4, 8, 8, 8, act=42) == _lib.MJ_ERR_ARG
+    assert fwd(4, 8, -8, 8) == _lib.MJ_ERR_ARG
+    assert fwd(4, 8, 8, 8, g=None) == _lib.MJ_ERR_ARG
+    assert fwd(4, 8, 8, 8, y=None) == _lib.MJ_ERR_ARG
+    assert fwd(4, 8, 8, 8, g=odd) == _lib.MJ_ERR_UNSUPPORTED
+    assert fwd(4, 8, 8, 8, y=odd) == _lib.MJ_ERR_UNSUPPORTED
+    assert fwd(0, 8, 8, 8) == _lib.MJ_OK
+    need = lib.mj_gated_mlp_f32_work_bytes(64, 64, 4096, 64, 0)
+    assert need > 0
+    assert fwd(64, 64, 4096, 64, work=None) == _lib.MJ_ERR_ARG
+    assert fwd(64, 64, 4096, 64, nbytes=need - 1) == _lib.MJ_ERR_ARG
+    assert lib.mj_gated_mlp_f32_work_bytes(0, 64, 4096, 64, 0) == 0
+
+
+@pytest.mark.parametrize("name", ["mj_gated_mlp_backward_bf16", "mj_gated_mlp_backward_f32"])
+def test_gated_mlp_backward_status_codes(lib, name):
+    p, odd = 16, 20
+    work = lib.mj_gated_mlp_work_bytes if name.endswith("bf16") else lib.mj_gated_mlp_f32_work_bytes
+
+    def bwd(M=64, K=64, I=4096, H=64, act=3, work=p, nbytes=1 << 40, **at):
+        a = dict(x=p, Wg=p, Wu=p, Wd=p, h=p, g=p, u=p, dy=p, dg=p, du=p, dx=p, dWg=p, dWu=p, dWd=p)
+        a.update(at)
+        return getattr(lib, name)(a["x"], a["Wg"], a["Wu"], a["Wd"], act, a["h"], a["g"], a["u"],
+                                  a["dy"], a["dg"], a["du"], a["dx"], a["dWg"], a["dWu"], a["dWd"],
+                                  M, K, I, H, work, nbytes, None)
+
+    assert bwd(act=4) == _lib.MJ_ERR_UNSUPPORTED
+    assert bwd(M=-1) == _lib.MJ_ERR_ARG
+    for operand in ("x", "Wg", "Wd", "g", "dy", "dg", "h"):
+        assert bwd(**{operand: None}) == _lib.MJ_ERR_ARG, operand
+    for operand in ("g", "u", "dg", "du", "dx"):
+        assert bwd(**{operand: odd}) == _lib.MJ_ERR_UNSUPPORTED, operand
+    need = work(64, 64, 4096, 64, 1)
+    assert need > 0
+    assert bwd(work=None) == _lib.MJ_ERR_ARG
+    assert bwd(nbytes=need - 1) == _lib.MJ_ERR_ARG
+
+
 def test_copy_rows_status_codes(lib):
     ptrs = (ctypes.c_void_p * 1)(16)
     call = lambda n, *z: lib.mj_copy_rows_bf16(n, ptrs, ptrs, (ctypes.c_int64 * 6)(*z), None)  # noqa: E731
