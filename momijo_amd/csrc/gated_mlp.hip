@@ -942,7 +942,10 @@ struct TilePlan {
 // The tile, and for a plain product the K slices, of the least predicted time.  The
 // slices' partials (fp32, written and read once, and their launch) pay where the
 // tiles leave CUs idle: 512 x 4096 with K = 11008 is 32 tiles of 256 x 256, 58 us in 8
-// slices; 67 on 128 x 64 tiles in 2, the best of the smaller tiles.
+// slices; 67 on 128 x 64 tiles in 2, the best of the smaller tiles.  A number of slices
+// that is no power of two has to win by 8 %, about what the predictions are off: 200 rows,
+// 2560 and 6912 wide (y and dx in 6 slices, predicted 14 and 19 % below 4 and 8) step
+// 183 -> 177 us, but 48 rows, 4096 and 11008 (y in 12 for 8, by 2 %) forward 73.7 -> 76.7.
 TilePlan plan_tiles(const TileArgs &a, int out) {
   TilePlan best;
   double best_us = 1e30;
@@ -951,10 +954,11 @@ TilePlan plan_tiles(const TileArgs &a, int out) {
   for (int t = 0; t < T_COUNT; ++t) {
     const TileCost &c = kTileCost[t];
     const int64_t tiles = tiles_of(a, c.bm, out == OUT_GATE ? c.bn / 2 : c.bn);
-    for (int s = 1; s <= (out == OUT_STORE && a.n == 1 ? 16 : 1); s *= 2) {
+    for (int s = 1; s <= (out == OUT_STORE && a.n == 1 ? 16 : 1); ++s) {
       if (s > 1 && (stages / s < 4 || tiles * s > 2 * kCUs * c.per_cu)) break;
       double us = tile_time_us(c, s > 1 ? OUT_PART : out, tiles * s, (stages + s - 1) / s);
       if (s > 1) us += 2.5 + (8.0 * s + 2.0) * (double)p.M * (double)p.N / 8.0e6;
+      if (s & (s - 1)) us *= 1.08;
       if (us < best_us) {
         best_us = us;
         best.tile = t;
