@@ -5,7 +5,9 @@ Dense matmul / Linear (fp32 and bf16 on MFMA), the int8 weight path
 QuantLinear on int8 MFMA) and the fused bias + activation epilogue, behind
 the C ABI declared in include/momijo_hip.h.  The Python classes mirror the
 reference's operator surface (Tensor.matmul, Linear, ReLU, QuantLinear, the
-int8 helpers of learn/api/functional.mojo).
+int8 helpers of learn/api/functional.mojo).  `block` adds the operators of a
+transformer's feed-forward block with their gradients: the gated MLP, the norms
+around its residual sum, and dropout.
 """
 from ._lib import (EPI_GELU_TANH, EPI_GELU_TANH_APPROX, EPI_NONE, EPI_RELU, EPI_RELU_UNARY,
                    EPI_SILU, EPI_SILU_APPROX, ROUND_LEGACY, ROUND_RHE, MomijoHipError)

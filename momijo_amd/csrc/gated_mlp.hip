@@ -669,8 +669,9 @@ __global__ __launch_bounds__(256) void mlp_reduce_kernel(const float *part, uint
 // the waves in turn, so each 128-byte line of a weight row is read by two loads of one
 // wave; a lane's 16 bytes are a row's 8 k, which is a fragment of
 // v_mfma_f32_16x16x32_bf16 as it is.  x comes from the caches the same way (rows past M
-// are zeros).  DEPTH slices of 64 are in flight a wave; no LDS in the loop.  The waves'
-// sums are added in wave order and act, g, u, h (or y) follow in the same launch.
+// are zeros).  A wave loads its next slice of 64 as it multiplies one; no LDS in the
+// loop.  The waves' sums are added in wave order and act, g, u, h (or y) follow in the
+// same launch.
 struct SkinnyArgs {
   const uint16_t *x = nullptr, *w = nullptr, *w2 = nullptr;
   uint16_t *C = nullptr;
@@ -678,7 +679,7 @@ struct SkinnyArgs {
   int M = 0, N = 0, K = 0, act = 0;
 };
 
-template <bool GATE, int MB, int DEPTH, int NW = 8>
+template <bool GATE, int MB, int NW = 8>
 __global__ __launch_bounds__(NW * 64) void mlp_skinny_kernel(SkinnyArgs p) {
   constexpr int G = GATE ? 2 : 1;
   __shared__ float red[NW][G][MB][16][17];
@@ -700,37 +701,32 @@ __global__ __launch_bounds__(NW * 64) void mlp_skinny_kernel(SkinnyArgs p) {
 #pragma unroll
     for (int b = 0; b < MB; ++b) acc[g][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  uint4 wv[DEPTH][2][G], xv[DEPTH][2][MB];
-  auto load = [&](int s, int k0) __attribute__((always_inline)) {
+  uint4 wv[2][G], xv[2][MB];
+  auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = k0 + 32 * h + 8 * fh;
       const bool in = k < K;
-      wv[s][h][0] = buffer_load16(rw, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
+      wv[h][0] = buffer_load16(rw, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
       if constexpr (GATE)
-        wv[s][h][1] = buffer_load16(rw2, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
+        wv[h][1] = buffer_load16(rw2, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
 #pragma unroll
       for (int b = 0; b < MB; ++b)
-        xv[s][h][b] = buffer_load16(rx, in && xo[b] != kOobOffset ? xo[b] + k * 2 : kOobOffset);
+        xv[h][b] = buffer_load16(rx, in && xo[b] != kOobOffset ? xo[b] + k * 2 : kOobOffset);
     }
   };
-  const int step = NW * 64;
+  load(wave * 64);
+  for (int k0 = wave * 64; k0 < K; k0 += NW * 64) {
 #pragma unroll
-  for (int s = 0; s < DEPTH; ++s) load(s, wave * 64 + s * step);
-  for (int k0 = wave * 64; k0 < K; k0 += DEPTH * step) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int s = 0; s < DEPTH; ++s) {
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int b = 0; b < MB; ++b)
-            acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8, wv[s][h][g]), __builtin_bit_cast(bf16x8, xv[s][h][b]),
-                acc[g][b], 0, 0, 0);
-      load(s, k0 + (DEPTH + s) * step);
-    }
+        for (int b = 0; b < MB; ++b)
+          acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8, wv[h][g]), __builtin_bit_cast(bf16x8, xv[h][b]), acc[g][b],
+              0, 0, 0);
+    load(k0 + NW * 64);
   }
   // block (g, b): weight row 4 fh + q, x row 16 b + fr
 #pragma unroll
@@ -993,9 +989,9 @@ bool skinny_takes(int64_t M, int64_t N, int64_t K) {
   return M <= 16 || (M <= 32 && N * K <= 3000000);
 }
 
-// One slice of 64 k in flight a wave: 4096 x 11008 gate/up of one row 34.6 us (5.2 TB/s)
-// against 36.3, 37.1, 37.5 with two, three, four (a wave's eight slices end sooner, and
-// more workgroups fit a CU).  Sixteen waves for one long row: K = 11008, 4096 columns
+// Waves: 4096 x 11008 gate/up of one row 34.6 us with eight (5.2 TB/s) and one slice of
+// 64 k in flight each, 36.3, 37.1, 37.5 with two, three, four in flight (a wave's eight
+// slices end sooner with one, and more workgroups fit a CU).  Sixteen waves for one long row: K = 11008, 4096 columns
 // 20.6 us against 22.2 at one row (256 workgroups, one a CU), but 26.5 against 24.7 at
 // 16 rows and 8.3 against 8.1 at K = 5504.
 template <bool GATE>
@@ -1003,11 +999,11 @@ hipError_t launch_skinny(const SkinnyArgs &a, hipStream_t stream) {
   const dim3 grid((unsigned)((a.N + 15) / 16));
   if (a.N == 0) return hipSuccess;
   if (a.M > 16)
-    hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 2, 1, 8>), grid, dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 2>), grid, dim3(512), 0, stream, a);
   else if (!GATE && a.M <= 4 && a.K >= 8192)
-    hipLaunchKernelGGL((mlp_skinny_kernel<false, 1, 1, 16>), grid, dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((mlp_skinny_kernel<false, 1, 16>), grid, dim3(1024), 0, stream, a);
   else
-    hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 1, 1, 8>), grid, dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 1>), grid, dim3(512), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -237,10 +237,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_kernel(Re
 // Two workgroups on a CU cover each other's waits, so a thread has 128 registers: they
 // go to the sums; what a row needs again is computed again from its packed values, and
 // the vectors wait in LDS, each thread's own columns in its own slots (no barrier, no
-// bank conflicts).  8192 x 4096 bf16 with dropout and four gate rows: 118 us (402 MB);
-// with the next row's loads ahead 202 (spills at 128 registers) or 141 (one workgroup a
-// CU); with the vectors in registers, one workgroup a CU, 182 (111 since the
-// partials' sums keep eight loads in flight).
+// bank conflicts).  8192 x 4096 bf16 with dropout and four gate rows: 111 us with the
+// partials' sums (403 MB, 3.6 TB/s).  Built otherwise, while those sums took 7 us more
+// (118): with the next row's loads ahead 202 (spills at 128 registers) or 141 (one
+// workgroup a CU); with the vectors in registers, one workgroup a CU, 182.
 enum : int { SUM_WN = 0, SUM_BN, SUM_S, SUM_WP, SUM_BP, SUM_G, SUMS };
 enum : int { V_WN = 0, V_WP, V_GATE, V_SCALE, V_BP, VECS };
 constexpr int kBwdThreads = 512;
