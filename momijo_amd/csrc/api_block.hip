@@ -181,7 +181,7 @@ int64_t mj_residual_norm_work_bytes(int64_t rows, int64_t dim, int64_t gate_rows
   for (int bias = 0; bias < 2; ++bias) {
     mj::ResNormGrad g;
     mj::plan_residual_norm_bwd(r, g, bias != 0);
-    const int64_t n = mj::residual_norm_part_floats(g, dim);
+    const int64_t n = mj::residual_norm_part_floats(r, g);
     most = n > most ? n : most;
   }
   return most * (int64_t)sizeof(float);
@@ -213,7 +213,7 @@ int32_t mj_residual_norm_backward(int32_t dtype, int32_t norm, const void *x, co
   g.dy = dy, g.dn = dn, g.dx = dx, g.db = db, g.dgate = dgate;
   g.dscale = dscale, g.dwp = dwp, g.dbp = dbp, g.dwn = dwn, g.dbn = dbn;
   mj::plan_residual_norm_bwd(r, g, mj::residual_norm_bias(r, g));
-  const int64_t need = mj::residual_norm_part_floats(g, dim) * (int64_t)sizeof(float);
+  const int64_t need = mj::residual_norm_part_floats(r, g) * (int64_t)sizeof(float);
   if (!work || work_bytes < need || !aligned16(work))
     return fail(MJ_ERR_ARG, "residual norm backward: work must be 16-byte aligned with %lld bytes",
                 (long long)need);

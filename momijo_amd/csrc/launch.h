@@ -296,7 +296,7 @@ constexpr int64_t kResNormMaxDim = 16384;
 // bias: whether biases or their gradients are there (residual_norm_bias)
 void plan_residual_norm_bwd(const ResNorm &p, ResNormGrad &g, bool bias);
 bool residual_norm_bias(const ResNorm &p, const ResNormGrad &g);
-int64_t residual_norm_part_floats(const ResNormGrad &g, int64_t dim);
+int64_t residual_norm_part_floats(const ResNorm &p, const ResNormGrad &g);
 hipError_t launch_residual_norm(bool bf16, const ResNorm &p, hipStream_t stream);
 hipError_t launch_residual_norm_bwd(bool bf16, const ResNorm &p, const ResNormGrad &g,
                                     hipStream_t stream);

@@ -232,6 +232,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_kernel(Re
 // are small, is a run of whole groups dealt to the teams, which write dgate as they
 // finish one.  No atomics: sums are added in a fixed order.
 //
+// Rows of more than 8192 columns have no registers for the columns' sums: there one kernel
+// takes the rows' four means, and a second one, eight columns a thread and nothing to
+// reduce, walks the rows again and does the rest: 2048 x 16384 bf16 with dropout 99 + 98 us
+// and 13 for the partials' sums, 611 with all in one kernel (spills).
+//
 // What bounds it is latency (a row's loads, then two sums over it, one after the
 // other) and, near the memory rate, the vector unit (some 60 operations an element).
 // Two workgroups on a CU cover each other's waits, so a thread has 128 registers: they
@@ -304,7 +309,7 @@ __device__ __forceinline__ const T *lane_at(const T *row, uint32_t bytes) {
 // The vectors that wait in LDS (slots of 16 KB VPT); the others are read from memory
 // for every row.
 constexpr bool vec_in_lds(int v, int vpt, bool bias) {
-  return v < (vpt == 4 ? 2 : V_BP) || (vpt == 1 && bias);
+  return v < V_BP || (vpt == 1 && bias);
 }
 constexpr int lds_vecs(int vpt, bool bias) {
   int n = 0;
@@ -568,6 +573,208 @@ residual_norm_bwd_kernel(ResNorm p, ResNormGrad g) {
   }
 }
 
+// The rows' means of dn wn yhat, dn wn, dc wp bhat and dc wp, [4][rows] behind the partials
+// (rows of more than 8192 columns).
+__device__ __forceinline__ float *row_means(const ResNorm &p, const ResNormGrad &g) {
+  return g.part + (int64_t)SUMS * g.blocks * p.dim;
+}
+
+// A workgroup a row.  The products of the row's columns that both passes need stay in
+// registers (88 of 128 with the gradients).
+template <typename T, bool ALIGNED>
+__global__ __launch_bounds__(1024) void residual_norm_means_kernel(ResNorm p, ResNormGrad g) {
+  constexpr int TPR = 1024, VPT = 2;
+  __shared__ float lds[64];
+  int slot = 0;
+  const int lane = threadIdx.x, dim = (int)p.dim;
+  const int64_t m = blockIdx.x, base = m * dim;
+  const float mean_p = p.stats[m], rstd_p = p.stats[p.rows + m];
+  const float mean_n = p.stats[2 * p.rows + m], rstd_n = p.stats[3 * p.rows + m];
+  const bool drop = p.drop.thr != 0;
+  uint32_t w[VPT][4];
+  if (drop) {
+    uint64_t seed, counter;
+    dropout_key(p.drop, seed, counter);
+    keep_bits<TPR, VPT, ALIGNED>(w, m, lane, dim, seed, counter);
+  }
+  Cols<VPT> yh, bh, gw, t;  // y, then yhat; b, then bhat; gate wp
+  load_cols<TPR, VPT, ALIGNED>(yh, (const T *)p.x + base, lane, dim);
+  load_vec<TPR, VPT, ALIGNED>(t, p.scale, 1.0f, lane, dim);
+#pragma unroll
+  for (int u = 0; u < VPT; ++u)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      yh.v[u][i] *= t.v[u][i];
+      bh.v[u][i] = 0.0f;
+    }
+  load_vec<TPR, VPT, ALIGNED>(gw, p.wp, 1.0f, lane, dim);
+  if (p.b) {
+    Cols<VPT> gate;
+    load_cols<TPR, VPT, ALIGNED>(bh, (const T *)p.b + base, lane, dim);
+    load_vec<TPR, VPT, ALIGNED>(t, p.bp, 0.0f, lane, dim);
+    if (p.gate) {
+      load_cols<TPR, VPT, ALIGNED>(gate, (const T *)p.gate + m / p.per * dim, lane, dim);
+    } else {
+#pragma unroll
+      for (int u = 0; u < VPT; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gate.v[u][i] = 1.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < VPT; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bh.v[u][i] = (bh.v[u][i] - mean_p) * rstd_p;
+        float z = (bh.v[u][i] * gw.v[u][i] + t.v[u][i]) * gate.v[u][i];
+        if (drop) z = keep_of(w[u], i, p.drop.thr) ? z * p.drop.scale : 0.0f;
+        yh.v[u][i] += z;
+        gw.v[u][i] *= gate.v[u][i];
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < VPT; ++u)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) yh.v[u][i] = (yh.v[u][i] - mean_n) * rstd_n;
+  Cols<VPT> d;  // dn wn, then dy of the row's sum
+  float a[2] = {0.0f, 0.0f}, q[2] = {0.0f, 0.0f};
+  const float inv = 1.0f / (float)dim;
+  if (g.dn) {
+    load_cols<TPR, VPT, ALIGNED>(d, (const T *)g.dn + base, lane, dim);
+    load_cols<TPR, VPT, ALIGNED>(t, p.wn, lane, dim);
+#pragma unroll
+    for (int u = 0; u < VPT; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        d.v[u][i] *= t.v[u][i];
+        a[0] = __builtin_fmaf(d.v[u][i], yh.v[u][i], a[0]);
+        a[1] += d.v[u][i];
+      }
+    team_sum<TPR, 2>(a, lds, slot);
+    a[0] *= inv;
+    a[1] = p.layer ? a[1] * inv : 0.0f;
+  }
+  if (p.wp) {
+    if (g.dy) load_cols<TPR, VPT, ALIGNED>(t, (const T *)g.dy + base, lane, dim);
+#pragma unroll
+    for (int u = 0; u < VPT; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float v = g.dy ? t.v[u][i] : 0.0f;
+        if (g.dn) v += rstd_n * (d.v[u][i] - yh.v[u][i] * a[0] - a[1]);
+        if (drop) v = keep_of(w[u], i, p.drop.thr) ? v * p.drop.scale : 0.0f;
+        const bool in = (u * TPR + lane) * 8 + i < dim;
+        const float e = in ? v * gw.v[u][i] : 0.0f;
+        q[0] = __builtin_fmaf(e, in ? bh.v[u][i] : 0.0f, q[0]);
+        q[1] += e;
+      }
+    team_sum<TPR, 2>(q, lds, slot);
+  }
+  if (lane == 0) {
+    float *const means = row_means(p, g);
+    means[m] = a[0];
+    means[p.rows + m] = a[1];
+    means[2 * p.rows + m] = q[0] * inv;
+    means[3 * p.rows + m] = p.layer ? q[1] * inv : 0.0f;
+  }
+}
+
+// Wide rows' gradients and their columns' sums from the rows' means: eight columns a
+// thread, the workgroup's rows in turn (blockIdx.x as in residual_norm_bwd_kernel,
+// blockIdx.y a run of 2048 columns).
+constexpr int kColThreads = 256;
+template <typename T, bool ALIGNED>
+__global__ __launch_bounds__(kColThreads) void residual_norm_cols_kernel(ResNorm p, ResNormGrad g) {
+  const int dim = (int)p.dim, c0 = ((int)blockIdx.y * kColThreads + (int)threadIdx.x) * 8;
+  const int left = dim - c0;
+  if (left <= 0) return;
+  const bool inside = g.segs > 0, has_b = p.b != nullptr, drop = p.drop.thr != 0;
+  const bool next = g.dn != nullptr, post = p.wp != nullptr;
+  int64_t g0, g1, s0, s1;
+  if (inside) {
+    g0 = (int64_t)blockIdx.x / g.segs;
+    g1 = g0 + 1;
+    s0 = (int64_t)blockIdx.x % g.segs * g.seg_rows;
+    s1 = std::min(s0 + g.seg_rows, p.per);
+  } else {
+    g0 = (int64_t)blockIdx.x * g.groups_per_block;
+    g1 = std::min(g0 + g.groups_per_block, g.groups);
+    s0 = 0;
+    s1 = p.per;
+  }
+  uint64_t seed = 0, counter = 0;
+  if (drop) dropout_key(p.drop, seed, counter);
+  const float *const means = row_means(p, g);
+  auto vec = [&](float (&v)[8], const auto *src, float fill) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fill;
+    if (src) load8<ALIGNED>(src + c0, left, v);
+  };
+  float wn[8], wp[8], bp[8], gate[8], acc[SUMS][8];
+  vec(wn, next ? p.wn : nullptr, 0.0f);
+  vec(wp, p.wp, 1.0f);
+  vec(bp, p.bp, 0.0f);
+  float scale[8];
+  vec(scale, p.scale, 1.0f);
+#pragma unroll
+  for (int k = 0; k < SUMS; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[k][i] = 0.0f;
+
+  for (int64_t gr = g0; gr < g1; ++gr) {
+    vec(gate, p.gate ? (const T *)p.gate + gr * dim : nullptr, 1.0f);
+    for (int64_t r = s0; r < s1; ++r) {
+      const int64_t m = gr * p.per + r, base = m * dim + c0;
+      Pack8<T> x, b, dy, dn;
+      b.clear(), dy.clear(), dn.clear();
+      x.template load<ALIGNED>((const T *)p.x + base, left);
+      if (has_b) b.template load<ALIGNED>((const T *)p.b + base, left);
+      if (g.dy) dy.template load<ALIGNED>((const T *)g.dy + base, left);
+      if (next) dn.template load<ALIGNED>((const T *)g.dn + base, left);
+      uint32_t w[4];
+      if (drop) draws8<ALIGNED>((uint64_t)base, counter, seed, w);
+      const float mean_p = p.stats[m], rstd_p = p.stats[p.rows + m];
+      const float mean_n = p.stats[2 * p.rows + m], rstd_n = p.stats[3 * p.rows + m];
+      const float ma = means[m], mb = means[p.rows + m];
+      const float mq = means[2 * p.rows + m], mr = means[3 * p.rows + m];
+      float dx[8], db[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool kept = !drop || keep_of(w, i, p.drop.thr);
+        const float bh = (b.get(i) - mean_p) * rstd_p, c = bh * wp[i] + bp[i];
+        float z = c * gate[i];
+        if (drop) z = kept ? z * p.drop.scale : 0.0f;
+        const float y = x.get(i) * scale[i] + (has_b ? z : 0.0f);
+        const float yh = (y - mean_n) * rstd_n;
+        float d = dy.get(i);
+        if (next) d += rstd_n * (dn.get(i) * wn[i] - yh * ma - mb);
+        float dk = d;
+        if (drop) dk = kept ? d * p.drop.scale : 0.0f;
+        const float dc = dk * gate[i], e = dc * wp[i];
+        dx[i] = d * scale[i];
+        db[i] = post ? rstd_p * (e - bh * mq - mr) : e;
+        acc[SUM_WN][i] = __builtin_fmaf(dn.get(i), yh, acc[SUM_WN][i]);
+        acc[SUM_BN][i] += dn.get(i);
+        acc[SUM_S][i] = __builtin_fmaf(d, x.get(i), acc[SUM_S][i]);
+        acc[SUM_WP][i] = __builtin_fmaf(dc, bh, acc[SUM_WP][i]);
+        acc[SUM_BP][i] += dc;
+        acc[SUM_G][i] = __builtin_fmaf(dk, c, acc[SUM_G][i]);
+      }
+      if (g.dx) store8<ALIGNED>((T *)g.dx + base, left, dx);
+      if (g.db) store8<ALIGNED>((T *)g.db + base, left, db);
+    }
+    if (!inside) {
+      if (g.dgate) store8<ALIGNED>((T *)g.dgate + gr * dim + c0, left, acc[SUM_G]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[SUM_G][i] = 0.0f;
+    }
+  }
+  float *const out[SUMS] = {g.dwn, g.dbn, g.dscale, g.dwp, g.dbp, inside ? (float *)g.dgate : nullptr};
+#pragma unroll
+  for (int k = 0; k < SUMS; ++k)
+    if (out[k])
+      store8<ALIGNED>(g.part + ((int64_t)k * g.blocks + blockIdx.x) * dim + c0, left, acc[k]);
+}
+
 // Column sums of the workgroups' partials: 64 columns a workgroup, 16 threads a column
 // over the partials in turn, their sums added in order.  blockIdx.y: one of the
 // vectors, or SUM_G + a gate row (that row's `segs` partials).
@@ -643,6 +850,17 @@ hipError_t launch_bwd_kernel(const ResNorm &p, const ResNormGrad &g, hipStream_t
   return hipGetLastError();
 }
 
+template <typename T>
+hipError_t launch_bwd_sums(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
+  const bool sums = g.dwn || g.dbn || g.dscale || g.dwp || g.dbp;
+  const bool gates = g.dgate && g.segs > 0;
+  if (!sums && !gates) return hipSuccess;
+  const int64_t ny = SUM_G + (gates ? g.groups : 0);
+  hipLaunchKernelGGL(residual_norm_sum_kernel<T>, dim3((unsigned)((p.dim + 63) / 64), (unsigned)ny),
+                     dim3(1024), 0, stream, g, p.dim);
+  return hipGetLastError();
+}
+
 template <typename T, int TPR, int VPT>
 hipError_t launch_bwd(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
   if (g.blocks > INT32_MAX) return hipErrorInvalidValue;
@@ -654,14 +872,19 @@ hipError_t launch_bwd(const ResNorm &p, const ResNormGrad &g, hipStream_t stream
   else
     e = bias ? launch_bwd_kernel<T, TPR, VPT, false, true>(p, g, stream)
              : launch_bwd_kernel<T, TPR, VPT, false, false>(p, g, stream);
-  if (e != hipSuccess) return e;
-  const bool sums = g.dwn || g.dbn || g.dscale || g.dwp || g.dbp;
-  const bool gates = g.dgate && g.segs > 0;
-  if (!sums && !gates) return hipSuccess;
-  const int64_t ny = SUM_G + (gates ? g.groups : 0);
-  hipLaunchKernelGGL(residual_norm_sum_kernel<T>, dim3((unsigned)((p.dim + 63) / 64), (unsigned)ny),
-                     dim3(1024), 0, stream, g, p.dim);
-  return hipGetLastError();
+  return e != hipSuccess ? e : launch_bwd_sums<T>(p, g, stream);
+}
+
+template <typename T, bool ALIGNED>
+hipError_t launch_bwd_wide(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
+  if (g.blocks > INT32_MAX || p.rows > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((residual_norm_means_kernel<T, ALIGNED>), dim3((unsigned)p.rows), dim3(1024), 0,
+                     stream, p, g);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  const dim3 grid((unsigned)g.blocks, (unsigned)((p.dim + 8 * kColThreads - 1) / (8 * kColThreads)));
+  hipLaunchKernelGGL((residual_norm_cols_kernel<T, ALIGNED>), grid, dim3(kColThreads), 0, stream, p, g);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  return launch_bwd_sums<T>(p, g, stream);
 }
 
 // The team that a row's chunks of 8 fit.
@@ -695,7 +918,8 @@ hipError_t bwd_typed(const ResNorm &p, const ResNormGrad &g, hipStream_t stream)
   }
   if (p.dim <= 4096) return launch_bwd<T, 512, 1>(p, g, stream);
   if (p.dim <= 8192) return launch_bwd<T, 512, 2>(p, g, stream);
-  return launch_bwd<T, 512, 4>(p, g, stream);
+  return all_aligned(p, &g) ? launch_bwd_wide<T, true>(p, g, stream)
+                            : launch_bwd_wide<T, false>(p, g, stream);
 }
 
 }  // namespace
@@ -726,8 +950,8 @@ void plan_residual_norm_bwd(const ResNorm &p, ResNormGrad &g, bool bias) {
 
 bool residual_norm_bias(const ResNorm &p, const ResNormGrad &g) { return g.dbn || g.dbp || p.bp; }
 
-int64_t residual_norm_part_floats(const ResNormGrad &g, int64_t dim) {
-  return (int64_t)SUMS * g.blocks * dim;
+int64_t residual_norm_part_floats(const ResNorm &p, const ResNormGrad &g) {
+  return (int64_t)SUMS * g.blocks * p.dim + (p.dim > 8192 ? 4 * p.rows : 0);
 }
 
 hipError_t launch_residual_norm(bool bf16, const ResNorm &p, hipStream_t stream) {

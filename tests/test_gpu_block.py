@@ -264,6 +264,17 @@ def test_residual_norm_parts(dev, on, gates):
     _check_norm(o, "rms", 1e-6, 0.1, 3, 0, torch.bfloat16)
 
 
+@pytest.mark.parametrize("rows,dim,gates,on", [
+    (600, 8200, 600, _FULL), (530, 8201, 265, _FULL), (20, 8193, 0, ("post_weight",)),
+    (20, 12288, 2, ("next_weight", "scale")), (300, 10000, 3, ("post_weight", "next_weight")),
+    (7, 16384, 7, ())])
+def test_residual_norm_wide_rows(dev, rows, dim, gates, on):
+    """Above 8192 columns, where the backward walks the rows twice: a gate row for every
+    row and for two, segments inside groups, each part alone."""
+    o = _norm_ops(rows, dim, gates, torch.bfloat16, on)
+    _check_norm(o, "layer" if rows % 3 else "rms", 1e-3, 0.25, 99, 3, torch.bfloat16)
+
+
 @pytest.mark.parametrize("scale", [False, True])
 def test_residual_norm_without_branch(dev, scale):
     """The norm before the first block; without a scale y is x itself."""
