@@ -73,6 +73,21 @@ def test_gated_mlp(dev, m, k, i, h, dtype):
         _close(got, ref[key][0], ref[key][1] + 1e-30, key)
 
 
+@pytest.mark.parametrize("m,k,i,h", [(200, 2560, 6912, 2560), (1000, 1040, 2808, 1040), (48, 1536, 4160, 1536),
+                                     (130, 2000, 4232, 1800)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_gated_mlp_k_slices(dev, m, k, i, h, dtype):
+    """Few outputs and long sums: y and dx in slices of K, of unequal lengths too."""
+    dt = DT[dtype]
+    x, wg, wu, wd, dy = _mlp_inputs(m, k, i, h, dt)
+    unit, e32 = (2.0 ** -8, 2.0 ** -18) if dtype == "bf16" else (2.0 ** -24, 2.0 ** -20)
+    ref = plain.mlp(x, wg, wu, wd, dy, "silu", unit, e32)
+    y, saved = mj.gated_mlp_train(x, wg, wu, wd)
+    for key, got in zip(("y", "dx", "dgate", "dup", "ddown"),
+                        (y,) + tuple(mj.gated_mlp_backward(dy, saved))):
+        _close(got, ref[key][0], ref[key][1] + 1e-30, key)
+
+
 @pytest.mark.parametrize("name", sorted(ACTS))
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_gated_mlp_activations(dev, name, dtype):
