@@ -909,14 +909,18 @@ hipError_t launch_w(TileArgs a, hipStream_t stream) {
 // 641, 64 x 64 771; of 512 rows 105, 67, 90, 87; h of 300 rows (K = 1024, 2816
 // columns) 37, 15.3, 16.4, 13.1; of 48 rows (11008) 82, -, 45, and 64 x 64 40.2
 // with three stages, 34.1 with five (one or two workgroups a CU wait on memory).
+// 128 x 128 and the fixed part of 256 x 256 gate/up are taken from whole layers, whose power
+// lowers the clock: with 0.48, 0.86 and 8, which products alone give, the forward of 1024
+// rows, 4096 and 11008 wide, took 293 us against 273, of 1536 434 against 401, of 6000, 1500
+// and 4000 wide, 254 against 235; 200 rows, 2560 and 6912 wide, 53.8 against 57.2.
 enum : int { T_256 = 0, T_128, T_64S3, T_64S5, T_128X64, T_COUNT };
 struct TileCost {
   int bm, bn, per_cu;
   double stage[3], fixed[4];  // fixed by OUT_*
 };
 constexpr TileCost kTileCost[T_COUNT] = {
-    {256, 256, 1, {1.47, 0, 0}, {7, 7, 8, 14}},
-    {128, 128, 2, {0.48, 0.86, 0}, {4, 3, 6, 9}},
+    {256, 256, 1, {1.47, 0, 0}, {7, 7, 10, 14}},
+    {128, 128, 2, {0.52, 0.98, 0}, {4, 3, 6, 9}},
     {64, 64, 3, {0.48, 0.52, 0.62}, {2.1, 2.1, 3, 4}},
     {64, 64, 2, {0.31, 0.48, 0}, {2.1, 2.1, 3, 4}},
     {128, 64, 2, {0.45, 0.70, 0}, {2.5, 2.5, 4, 6}},
@@ -946,7 +950,7 @@ struct TilePlan {
 // tiles leave CUs idle: 512 x 4096 with K = 11008 is 32 tiles of 256 x 256, 58 us in 8
 // slices; 67 on 128 x 64 tiles in 2, the best of the smaller tiles.  A number of slices
 // that is no power of two has to win by 8 %, about what the predictions are off: 200 rows,
-// 2560 and 6912 wide (y and dx in 6 slices, predicted 14 and 19 % below 4 and 8) step
+// 2560 and 6912 wide (y and dx in 6 slices, predicted 15 and 21 % below 4) step
 // 183 -> 177 us, but 48 rows, 4096 and 11008 (y in 12 for 8, by 2 %) forward 73.7 -> 76.7.
 TilePlan plan_tiles(const TileArgs &a, int out) {
   TilePlan best;
