@@ -224,7 +224,9 @@ int32_t mj_residual_norm_backward(int32_t dtype, int32_t norm, const void *x, co
 
 // ------------------------------------------------------------------ gated MLP
 int64_t mj_gated_mlp_work_bytes(int64_t M, int64_t K, int64_t I, int64_t H, int32_t backward) {
-  if (M <= 0 || K <= 0 || I <= 0 || H <= 0) return 0;
+  // the sliced product's own sizes alone (y [M, H] or dx [M, K], sums over I): it is planned and
+  // launched whether or not the width that it does not have is zero
+  if (M <= 0 || I <= 0 || (backward ? K : H) <= 0) return 0;
   return mj::gated_mlp_part_floats(M, K, I, H, backward != 0) * (int64_t)sizeof(float);
 }
 

@@ -1024,6 +1024,7 @@ hipError_t launch_plain(TileArgs a, float *part, hipStream_t stream) {
   if (p.M == 0 || p.N == 0) return hipSuccess;
   const TilePlan pl = plan_tiles(a, OUT_STORE);
   if (pl.splits == 1) return launch_tile_kernel<AKC, BKC, OUT_STORE>(pl.tile, a, stream);
+  if (!part) return hipErrorInvalidValue;
   a.splits = pl.splits;
   a.p[0].part = part;
   if (hipError_t e = launch_tile_kernel<AKC, BKC, OUT_PART>(pl.tile, a, stream); e != hipSuccess)

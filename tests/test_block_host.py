@@ -144,3 +144,23 @@ def test_copy_rows_status_codes(lib):
     null = (ctypes.c_void_p * 1)()
     assert lib.mj_copy_rows_bf16(1, null, ptrs, (ctypes.c_int64 * 6)(2, 2, 2, 2, 2, 2), None) == _lib.MJ_ERR_ARG
     assert call(1, 0, 0, 0, 0, 0, 0) == _lib.MJ_OK
+
+
+@pytest.mark.parametrize("M,I,N", [(200, 6912, 2560), (64, 4096, 64), (48, 11008, 4096)])
+def test_gated_mlp_work_of_a_zero_width(lib, M, I, N):
+    """y [M, N] (or dx) is summed in K slices whatever the width it does not depend on:
+    with that width zero it needs the same work, and a call without is refused."""
+    p, big = ctypes.c_void_p(16), 1 << 40
+    need = lib.mj_gated_mlp_work_bytes(M, 64, I, N, 0)
+    assert need > 0
+    assert lib.mj_gated_mlp_work_bytes(M, 0, I, N, 0) == need
+    assert lib.mj_gated_mlp_bf16(None, p, p, p, 3, p, None, None, p, M, 0, I, N, None, 0,
+                                 None) == _lib.MJ_ERR_ARG
+    need = lib.mj_gated_mlp_work_bytes(M, N, I, 64, 1)
+    assert need > 0
+    assert lib.mj_gated_mlp_work_bytes(M, N, I, 0, 1) == need
+    assert lib.mj_gated_mlp_backward_bf16(p, p, p, p, 3, p, p, p, None, p, p, p, p, p, p, M, N, I, 0,
+                                          None, big, None) == _lib.MJ_ERR_ARG
+    for zero in ((0, N, I, N), (M, N, 0, N)):
+        assert lib.mj_gated_mlp_work_bytes(*zero, 0) == lib.mj_gated_mlp_work_bytes(*zero, 1) == 0
+    assert lib.mj_gated_mlp_work_bytes(M, N, I, 0, 0) == lib.mj_gated_mlp_work_bytes(M, 0, I, N, 1) == 0
