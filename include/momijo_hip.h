@@ -556,8 +556,9 @@ int64_t mj_residual_norm_work_bytes(int64_t rows, int64_t dim, int64_t gate_rows
 
 /* Gradients of mj_residual_norm from dy, dn (either may be NULL) and the forward's
  * arguments and stats.  dx, db, dgate have element type dtype; dscale, dwp, dbp,
- * dwn, dbn are fp32 [dim]; any may be NULL.  Sums run in a fixed order: the same
- * inputs give the same bits.  rows == 0 writes nothing. */
+ * dwn, dbn are fp32 [dim]; any may be NULL.  A dropped element of gate c adds nothing to
+ * dgate and its dc is 0, whatever c and the gate hold.  Sums run in a fixed order: the
+ * same inputs give the same bits.  rows == 0 writes nothing. */
 int32_t mj_residual_norm_backward(int32_t dtype, int32_t norm, const void *x, const void *b,
                                   const void *gate, int64_t gate_rows, const float *scale,
                                   const float *wp, const float *bp, const float *wn, float p,

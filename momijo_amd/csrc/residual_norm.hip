@@ -220,6 +220,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_kernel(Re
 // Backward:
 //   dyt = dy + rn (dn wn - yhat mean(dn wn yhat) - [layer] mean(dn wn))
 //   dx = s dyt, ds += x dyt, dz = keep dyt, dgate += dz c, dc = dz g
+//   (a dropped element: dgate and dc take 0 without looking at c and g, which may be inf or NaN)
 //   dwn += dn yhat, dbn += dn, dwp += dc bhat, dbp += dc
 //   db = rp (dc wp - bhat mean(dc wp bhat) - [layer] mean(dc wp))
 // with bhat, c, y and yhat computed again from x, b and the saved statistics, in
@@ -485,13 +486,16 @@ residual_norm_bwd_kernel(ResNorm p, ResNormGrad g) {
           float d = r.dy[u].get(i);
           if (next) d += r.rstd_n * (dn * vn[j] - yh.v[u][i] * ma - mb);
           out[i] = d * vs[j];
+          // a dropped element's gradients are 0 whatever c and the gate hold
           float dk = d;
-          if (drop) dk = keep_of(w[u], i, p.drop.thr) ? d * p.drop.scale : 0.0f;
-          const float dc = dk * vg[j];
+          if (drop) dk = d * p.drop.scale;
+          const bool kept = !drop || keep_of(w[u], i, p.drop.thr);
+          const float dc = kept ? dk * vg[j] : 0.0f;
           if (on) {
             acc[SUM_WN].v[u][i] = __builtin_fmaf(dn, yh.v[u][i], acc[SUM_WN].v[u][i]);
             acc[SUM_S].v[u][i] = __builtin_fmaf(d, r.x[u].get(i), acc[SUM_S].v[u][i]);
-            acc[SUM_G].v[u][i] = __builtin_fmaf(dk, bh * vwp[j] + vbp[j], acc[SUM_G].v[u][i]);
+            if (kept)
+              acc[SUM_G].v[u][i] = __builtin_fmaf(dk, bh * vwp[j] + vbp[j], acc[SUM_G].v[u][i]);
             acc[SUM_WP].v[u][i] = __builtin_fmaf(dc, bh, acc[SUM_WP].v[u][i]);
             if constexpr (BIAS) {
               acc[SUM_BN].v[u][i] += dn;
@@ -661,9 +665,10 @@ __global__ __launch_bounds__(1024) void residual_norm_means_kernel(ResNorm p, Re
       for (int i = 0; i < 8; ++i) {
         float v = g.dy ? t.v[u][i] : 0.0f;
         if (g.dn) v += rstd_n * (d.v[u][i] - yh.v[u][i] * a[0] - a[1]);
-        if (drop) v = keep_of(w[u], i, p.drop.thr) ? v * p.drop.scale : 0.0f;
+        if (drop) v *= p.drop.scale;
         const bool in = (u * TPR + lane) * 8 + i < dim;
-        const float e = in ? v * gw.v[u][i] : 0.0f;
+        const bool kept = !drop || keep_of(w[u], i, p.drop.thr);
+        const float e = in && kept ? v * gw.v[u][i] : 0.0f;
         q[0] = __builtin_fmaf(e, in ? bh.v[u][i] : 0.0f, q[0]);
         q[1] += e;
       }
@@ -747,9 +752,8 @@ __global__ __launch_bounds__(kColThreads) void residual_norm_cols_kernel(ResNorm
         const float yh = (y - mean_n) * rstd_n;
         float d = dy.get(i);
         if (next) d += rstd_n * (dn.get(i) * wn[i] - yh * ma - mb);
-        float dk = d;
-        if (drop) dk = kept ? d * p.drop.scale : 0.0f;
-        const float dc = dk * gate[i], e = dc * wp[i];
+        const float dk = drop ? d * p.drop.scale : d;
+        const float dc = kept ? dk * gate[i] : 0.0f, e = dc * wp[i];
         dx[i] = d * scale[i];
         db[i] = post ? rstd_p * (e - bh * mq - mr) : e;
         acc[SUM_WN][i] = __builtin_fmaf(dn.get(i), yh, acc[SUM_WN][i]);
@@ -757,7 +761,7 @@ __global__ __launch_bounds__(kColThreads) void residual_norm_cols_kernel(ResNorm
         acc[SUM_S][i] = __builtin_fmaf(d, x.get(i), acc[SUM_S][i]);
         acc[SUM_WP][i] = __builtin_fmaf(dc, bh, acc[SUM_WP][i]);
         acc[SUM_BP][i] += dc;
-        acc[SUM_G][i] = __builtin_fmaf(dk, c, acc[SUM_G][i]);
+        if (kept) acc[SUM_G][i] = __builtin_fmaf(dk, c, acc[SUM_G][i]);
       }
       if (g.dx) store8<ALIGNED>((T *)g.dx + base, left, dx);
       if (g.db) store8<ALIGNED>((T *)g.db + base, left, db);

@@ -3,6 +3,7 @@ ordinary (bounds as in test_gpu_block.py)."""
 import pytest
 import torch
 
+import _block as plain
 import momijo_amd as mj
 from test_gpu_block import DT, _gen, _normal
 
@@ -31,3 +32,36 @@ def test_gated_mlp_zero_width(dev, m, i, n, dtype):
     dx, dgate, dup, ddown = mj.gated_mlp_backward(dy, saved)
     assert y.shape == (m, 0) and dx.shape == (m, n) and ddown.shape == (0, i)
     assert not bool(dx.any()) and not bool(dgate.any()) and not bool(dup.any())
+
+
+# ------------------------------------------------------------------ residual norm
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,dim", [(34, 264), (21, 1001), (9, 4100), (5, 8200)])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("bias", [False, True])
+def test_residual_norm_dropped_places(dev, rows, dim, post, bias, dtype):
+    """What a dropped place holds (the gate's value; without a post norm the branch's
+    too: infinite, NaN) is in no output and no gradient: the bits are those of other
+    values there."""
+    dt, p, seed, counter = DT[dtype], 0.5, 21, 4
+    g = _gen("dropped", rows, dim)
+    vec = lambda: _normal(g, (dim,), torch.float32, 0.2, 1.0)  # noqa: E731
+    keep = torch.from_numpy(plain.keep(rows * dim, p, seed, counter)).reshape(rows, dim).to(dev)
+    x, branch, dy, dn = (_normal(g, (rows, dim), dt) for _ in range(4))
+    gate = _normal(g, (rows, dim), dt, 0.3, 0.5)   # a gate row for every row
+    kw = dict(scale=vec(), next_weight=vec(), p=p, seed=seed, counter=counter)
+    if post:
+        kw["post_weight"] = vec()
+    if bias:
+        kw["next_bias"] = vec()
+
+    def step(b, q):
+        y, n, saved = mj.residual_norm_train(x, b, gate=q, **kw)
+        return [y, n] + list(mj.residual_norm_backward(dy, dn, saved).values())
+
+    want = step(branch, gate)
+    bad = torch.tensor([float("inf"), float("nan"), -float("inf")], device=dev, dtype=dt)
+    bad = bad.repeat(rows * dim // 3 + 1)[:rows * dim].reshape(rows, dim)
+    b = branch if post else torch.where(keep, branch, bad)
+    for q in (gate, torch.where(keep, gate, bad)):
+        assert all(torch.equal(a, c) for a, c in zip(step(b, q), want))
