@@ -19,7 +19,7 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T *x, T *y,
                                                                Dropout d) {
   uint64_t seed, counter;
   dropout_key(d, seed, counter);
-  const int64_t first = (int64_t)blockIdx.x * (kDropThreads * kUnroll) + threadIdx.x;
+  const int64_t first = grid_block<kDropThreads>() * (kDropThreads * kUnroll) + threadIdx.x;
   float v[kUnroll][8];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
@@ -43,13 +43,12 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T *x, T *y,
 template <typename T>
 static hipError_t launch_typed(const T *x, T *y, int64_t n, const Dropout &d, hipStream_t stream) {
   constexpr int64_t per = (int64_t)kDropThreads * kUnroll * 8;
-  const int64_t grid = (n + per - 1) / per;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid = grid_rows<kDropThreads>((n + per - 1) / per);
   if ((((uintptr_t)x | (uintptr_t)y) & 15) == 0)
-    hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)grid), dim3(kDropThreads), 0,
+    hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(kDropThreads), 0,
                        stream, x, y, n, d);
   else
-    hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)grid), dim3(kDropThreads), 0,
+    hipLaunchKernelGGL((dropout_kernel<T, false>), grid, dim3(kDropThreads), 0,
                        stream, x, y, n, d);
   return hipGetLastError();
 }

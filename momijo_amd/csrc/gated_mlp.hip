@@ -810,7 +810,7 @@ __device__ __forceinline__ float2 act_grad_f32(int act, float g) {
 // 4 elements a thread; the last few singly.
 __global__ __launch_bounds__(256) void gate_f32_kernel(int act, const float *g, const float *u,
                                                        float *h, int64_t n) {
-  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t e = (grid_block<256>() * 256 + threadIdx.x) * 4;
   if (e + 4 <= n) {
     const float4 a = *(const float4 *)(g + e), b = *(const float4 *)(u + e);
     *(float4 *)(h + e) =
@@ -824,7 +824,7 @@ __global__ __launch_bounds__(256) void gate_f32_kernel(int act, const float *g, 
 __global__ __launch_bounds__(256) void gate_bwd_f32_kernel(int act, const float *g, const float *u,
                                                            const float *dh, float *dg, float *du,
                                                            int64_t n) {
-  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t e = (grid_block<256>() * 256 + threadIdx.x) * 4;
   if (e + 4 <= n) {
     const float4 gv = *(const float4 *)(g + e), uv = *(const float4 *)(u + e),
                  dv = *(const float4 *)(dh + e);
@@ -1135,9 +1135,8 @@ hipError_t launch_copy_rows_bf16(const CopyRows &c, hipStream_t stream) {
 hipError_t launch_gate_f32(int act, const float *g, const float *u, float *h, int64_t n,
                            hipStream_t stream) {
   if (n <= 0) return hipSuccess;
-  const int64_t grid = (n + 1023) / 1024;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(gate_f32_kernel, dim3((unsigned)grid), dim3(256), 0, stream, act, g, u, h, n);
+  hipLaunchKernelGGL(gate_f32_kernel, grid_rows<256>((n + 1023) / 1024), dim3(256), 0, stream, act, g,
+                     u, h, n);
   return hipGetLastError();
 }
 
@@ -1154,10 +1153,8 @@ hipError_t launch_sum_f32(const float *part, float *out, int64_t n, int64_t part
 hipError_t launch_gate_bwd_f32(int act, const float *g, const float *u, const float *dh, float *dg,
                                float *du, int64_t n, hipStream_t stream) {
   if (n <= 0) return hipSuccess;
-  const int64_t grid = (n + 1023) / 1024;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(gate_bwd_f32_kernel, dim3((unsigned)grid), dim3(256), 0, stream, act, g, u, dh,
-                     dg, du, n);
+  hipLaunchKernelGGL(gate_bwd_f32_kernel, grid_rows<256>((n + 1023) / 1024), dim3(256), 0, stream, act,
+                     g, u, dh, dg, du, n);
   return hipGetLastError();
 }
 

@@ -24,6 +24,21 @@ inline hipError_t raise_lds(const void *kern, size_t bytes, std::atomic<uint64_t
   return hipSuccess;
 }
 
+// A dimension of a grid holds fewer than 2^32 threads (a launch of more runs the rest of the
+// division, without an error): workgroups of THREADS in rows of kGridRow (a power of two: the
+// number is a shift away), the last row reaching past the end.
+template <int THREADS>
+constexpr int64_t kGridRow = ((int64_t)1 << 31) / THREADS;
+template <int THREADS>
+dim3 grid_rows(int64_t blocks) {
+  constexpr int64_t row = kGridRow<THREADS>;
+  return blocks <= row ? dim3((unsigned)blocks) : dim3((unsigned)row, (unsigned)((blocks + row - 1) / row));
+}
+template <int THREADS>
+__device__ __forceinline__ int64_t grid_block() {
+  return (int64_t)blockIdx.y * kGridRow<THREADS> + blockIdx.x;
+}
+
 // ---- gemm_nt.hip: bf16 A x (bf16 | int8) B^T on MFMA ---------------------
 enum BKind : int { B_BF16 = 0, B_INT8 = 1 };
 

@@ -135,12 +135,13 @@ __device__ __forceinline__ void keep_bits(uint32_t (&w)[VPT][4], int64_t m, int 
 
 template <typename T, int TPR, int VPT, bool ALIGNED>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_kernel(ResNorm p) {
-  constexpr int TEAMS = (TPR > 256 ? TPR : 256) / TPR;
+  constexpr int NT = TPR > 256 ? TPR : 256, TEAMS = NT / TPR;
   __shared__ float lds[64];
   int slot = 0;
   const int lane = threadIdx.x % TPR, dim = (int)p.dim;
   // (a wave is of one team, so its row is uniform)
-  int64_t m = (int64_t)blockIdx.x * TEAMS + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+  const int64_t first = grid_block<NT>() * TEAMS;
+  int64_t m = first + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   // a team past the last row computes it again (its barriers are everyone's) and writes nothing
   const bool live = m < p.rows;
   if (!live) m = p.rows - 1;
@@ -330,20 +331,23 @@ residual_norm_bwd_kernel(ResNorm p, ResNormGrad g) {
   const uint32_t lane = (uint32_t)tid % TPR;
   const int team = __builtin_amdgcn_readfirstlane(tid / TPR);  // a wave is of one team
   const bool inside = g.segs > 0;  // segments inside groups, else whole groups
-  // this workgroup's rows [s0, s1) of group g0, or groups [g0, g1)
+  // this workgroup's ns rows of group g0, or ng whole groups; row numbers count from m0
+  // (the last segments may lie past their group's end: no rows)
   const int per = (int)p.per;
-  int g0, g1, s0, s1, rounds;
+  int64_t g0, m0;
+  int ng, ns, rounds;
   if (inside) {
-    g0 = (int)(blockIdx.x / (uint32_t)g.segs);
-    g1 = g0 + 1;
-    s0 = (int)((blockIdx.x % (uint32_t)g.segs) * (uint32_t)g.seg_rows);
-    s1 = std::min(s0 + (int)g.seg_rows, per);
+    g0 = blockIdx.x / (uint32_t)g.segs;
+    const uint32_t s0 = (blockIdx.x % (uint32_t)g.segs) * (uint32_t)g.seg_rows;
+    m0 = g0 * per + s0;
+    ng = 1;
+    ns = s0 < (uint32_t)per ? (int)std::min((uint32_t)g.seg_rows, (uint32_t)per - s0) : 0;
     rounds = ((int)g.seg_rows + TEAMS - 1) / TEAMS;
   } else {
-    g0 = (int)(blockIdx.x * (uint32_t)g.groups_per_block);
-    g1 = (int)std::min<int64_t>(g0 + g.groups_per_block, g.groups);
-    s0 = 0;
-    s1 = per;
+    g0 = (int64_t)blockIdx.x * g.groups_per_block;
+    m0 = g0 * per;
+    ng = (int)std::min(g.groups_per_block, g.groups - g0);
+    ns = per;
     rounds = ((int)g.groups_per_block + TEAMS - 1) / TEAMS * per;
   }
   const bool post = p.wp != nullptr, has_b = p.b != nullptr, drop = p.drop.thr != 0;
@@ -389,14 +393,14 @@ residual_norm_bwd_kernel(ResNorm p, ResNormGrad g) {
   keep_vec(V_BP, p.bp, 0.0f);
   if (!p.gate) keep_vec(V_GATE, (const T *)nullptr, 1.0f);
 
-  int gr = inside ? g0 : g0 + team, s = inside ? s0 + team : 0;
-  auto alive = [&](int gr_, int s_) { return gr_ < g1 && s_ < s1; };
+  int gr = inside ? 0 : team, s = inside ? team : 0;
+  auto alive = [&](int gr_, int s_) { return gr_ < ng && s_ < ns; };
   auto step = [&](int &gr_, int &s_) {
     if (inside) s_ += TEAMS;
     else if (++s_ == per) s_ = 0, gr_ += TEAMS;
   };
   auto load_row = [&](RowIn<T, VPT> &r, int gr_, int s_) __attribute__((always_inline)) {
-    const int64_t m = alive(gr_, s_) ? (int64_t)gr_ * per + s_ : 0, base = m * dim;
+    const int64_t m = alive(gr_, s_) ? m0 + gr_ * per + s_ : 0, base = m * dim;
     const T *x = (const T *)p.x + base, *b = (const T *)p.b + base;
     const T *dy = (const T *)g.dy + base, *dn = (const T *)g.dn + base;
 #pragma unroll
@@ -427,8 +431,8 @@ residual_norm_bwd_kernel(ResNorm p, ResNormGrad g) {
   RowIn<T, VPT> r;
   for (int k = 0; k < rounds; ++k) {
     const bool on = alive(gr, s);
-    const int64_t m = on ? (int64_t)gr * per + s : 0;
-    const T *const gate = p.gate ? (const T *)p.gate + (int64_t)(on ? gr : 0) * dim : nullptr;
+    const int64_t m = on ? m0 + gr * per + s : 0;
+    const T *const gate = p.gate ? (const T *)p.gate + (on ? g0 + gr : 0) * dim : nullptr;
     if (fresh && gate) keep_vec(V_GATE, gate, 1.0f);
     fresh = false;
     load_row(r, gr, s);
@@ -534,7 +538,7 @@ residual_norm_bwd_kernel(ResNorm p, ResNormGrad g) {
     }
     if (on && !inside && s == per - 1) {
       if (g.dgate)
-        store_cols<TPR, VPT, ALIGNED>(acc[SUM_G], (T *)g.dgate + (int64_t)gr * dim, lane, dim);
+        store_cols<TPR, VPT, ALIGNED>(acc[SUM_G], (T *)g.dgate + (g0 + gr) * dim, lane, dim);
 #pragma unroll
       for (int u = 0; u < VPT; ++u)
 #pragma unroll
@@ -591,7 +595,8 @@ __global__ __launch_bounds__(1024) void residual_norm_means_kernel(ResNorm p, Re
   __shared__ float lds[64];
   int slot = 0;
   const int lane = threadIdx.x, dim = (int)p.dim;
-  const int64_t m = blockIdx.x, base = m * dim;
+  const int64_t m = grid_block<TPR>(), base = m * dim;
+  if (m >= p.rows) return;
   const float mean_p = p.stats[m], rstd_p = p.stats[p.rows + m];
   const float mean_n = p.stats[2 * p.rows + m], rstd_n = p.stats[3 * p.rows + m];
   const bool drop = p.drop.thr != 0;
@@ -834,9 +839,7 @@ bool all_aligned(const ResNorm &p, const ResNormGrad *g) {
 template <typename T, int TPR, int VPT>
 hipError_t launch_fwd(const ResNorm &p, hipStream_t stream) {
   constexpr int NT = TPR > 256 ? TPR : 256;
-  const int64_t grid = (p.rows + NT / TPR - 1) / (NT / TPR);
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
-  const dim3 gr((unsigned)grid), bl(NT);
+  const dim3 gr = grid_rows<NT>((p.rows + NT / TPR - 1) / (NT / TPR)), bl(NT);
   if (all_aligned(p, nullptr))
     hipLaunchKernelGGL((residual_norm_kernel<T, TPR, VPT, true>), gr, bl, 0, stream, p);
   else
@@ -867,7 +870,6 @@ hipError_t launch_bwd_sums(const ResNorm &p, const ResNormGrad &g, hipStream_t s
 
 template <typename T, int TPR, int VPT>
 hipError_t launch_bwd(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
-  if (g.blocks > INT32_MAX) return hipErrorInvalidValue;
   const bool bias = residual_norm_bias(p, g);
   hipError_t e;
   if (all_aligned(p, &g))
@@ -881,8 +883,7 @@ hipError_t launch_bwd(const ResNorm &p, const ResNormGrad &g, hipStream_t stream
 
 template <typename T, bool ALIGNED>
 hipError_t launch_bwd_wide(const ResNorm &p, const ResNormGrad &g, hipStream_t stream) {
-  if (g.blocks > INT32_MAX || p.rows > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((residual_norm_means_kernel<T, ALIGNED>), dim3((unsigned)p.rows), dim3(1024), 0,
+  hipLaunchKernelGGL((residual_norm_means_kernel<T, ALIGNED>), grid_rows<1024>(p.rows), dim3(1024), 0,
                      stream, p, g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   const dim3 grid((unsigned)g.blocks, (unsigned)((p.dim + 8 * kColThreads - 1) / (8 * kColThreads)));
