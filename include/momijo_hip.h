@@ -572,7 +572,8 @@ int32_t mj_residual_norm_backward(int32_t dtype, int32_t norm, const void *x, co
  *   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
  * x [M,K], Wg and Wu [I,K], Wd [H,I], h [M,I], y [M,H], all contiguous; act is
  * MJ_EPI_NONE, RELU, GELU_TANH or SILU.
- * bf16: K, I, H multiples of 8 (mj_copy_rows_bf16 pads other widths), 16-byte aligned arrays;
+ * bf16: K, I, H multiples of 8 (mj_copy_rows_bf16 pads other widths) below 2^22, M at most 2^31 -
+ * 1024, 16-byte aligned arrays;
  * h is rounded to bf16; g, u fp32 [M,I] are written for the backward, or both NULL;
  * `work` as mj_gated_mlp_work_bytes says (NULL where that is 0).
  * fp32: any widths; h, g, u are required (u right behind g saves a launch), and `work`

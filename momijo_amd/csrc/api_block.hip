@@ -34,15 +34,17 @@ int32_t check_mlp(int32_t act, int64_t M, int64_t K, int64_t I, int64_t H) {
 }
 
 // What the tile kernels need of the bf16 block: 16-byte rows, 32-bit offsets
-// within 256 rows of a tile.
-int32_t check_mlp_bf16(const char *what, int64_t K, int64_t I, int64_t H, const void *const *ptrs,
-                       int n) {
+// within 256 rows of a tile and 32-bit row numbers.
+int32_t check_mlp_bf16(const char *what, int64_t M, int64_t K, int64_t I, int64_t H,
+                       const void *const *ptrs, int n) {
   if (K % 8 || I % 8 || H % 8)
     return fail(MJ_ERR_UNSUPPORTED, "%s: K, I and H must be multiples of 8 (%lld, %lld, %lld)", what,
                 (long long)K, (long long)I, (long long)H);
   const int64_t lim = (int64_t)1 << 22;
   if (K >= lim || I >= lim || H >= lim)
     return fail(MJ_ERR_UNSUPPORTED, "%s: widths must be below 2^22", what);
+  if (M > mj::kMlpMaxRows)
+    return fail(MJ_ERR_UNSUPPORTED, "%s: at most %lld rows", what, (long long)mj::kMlpMaxRows);
   for (int i = 0; i < n; ++i)
     if (!aligned16(ptrs[i]))
       return fail(MJ_ERR_UNSUPPORTED, "%s: every array must be 16-byte aligned", what);
@@ -258,7 +260,7 @@ int32_t mj_gated_mlp_bf16(const uint16_t *x, const uint16_t *Wg, const uint16_t 
                           int64_t work_bytes, void *stream) {
   if (int32_t s = check_mlp(act, M, K, I, H)) return s;
   const void *ptrs[] = {x, Wg, Wu, Wd, h, g, u, y, work};
-  if (int32_t s = check_mlp_bf16("gated MLP", K, I, H, ptrs, 9)) return s;
+  if (int32_t s = check_mlp_bf16("gated MLP", M, K, I, H, ptrs, 9)) return s;
   if (M == 0) return MJ_OK;
   if ((H > 0 && !y) || (I > 0 && (!h || (H > 0 && !Wd) || (K > 0 && (!x || !Wg || !Wu)))))
     return fail(MJ_ERR_ARG, "null operand");
@@ -281,7 +283,7 @@ int32_t mj_gated_mlp_backward_bf16(const uint16_t *x, const uint16_t *Wg, const 
                                    int64_t H, void *work, int64_t work_bytes, void *stream) {
   if (int32_t s = check_mlp(act, M, K, I, H)) return s;
   const void *ptrs[] = {x, Wg, Wu, Wd, h, g, u, dy, dg, du, dx, dWg, dWu, dWd, work};
-  if (int32_t s = check_mlp_bf16("gated MLP backward", K, I, H, ptrs, 15)) return s;
+  if (int32_t s = check_mlp_bf16("gated MLP backward", M, K, I, H, ptrs, 15)) return s;
   if (M > 0 && I > 0 && (dx || dWg || dWu) &&
       (!dg || !du || !g || !u || (H > 0 && (!dy || !Wd))))
     return fail(MJ_ERR_ARG, "null operand");

@@ -885,6 +885,7 @@ hipError_t launch_ring(TileArgs a, hipStream_t stream) {
   set_tiles(a, BM, OUT == OUT_GATE ? BN / 2 : BN);
   const int64_t grid = (int64_t)a.tiles * a.splits;
   if (grid == 0) return hipSuccess;
+  if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, a);
   return hipGetLastError();
 }
@@ -896,8 +897,10 @@ hipError_t launch_w(TileArgs a, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
   set_tiles(a, BM, OUT == OUT_GATE ? BM / 2 : BM);
-  if (a.tiles == 0) return hipSuccess;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.splits)), dim3(NW * 64), lds, stream, a);
+  const int64_t grid = (int64_t)a.tiles * a.splits;
+  if (grid == 0) return hipSuccess;
+  if (!grid_fits(grid, NW * 64)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(NW * 64), lds, stream, a);
   return hipGetLastError();
 }
 
@@ -915,15 +918,15 @@ hipError_t launch_w(TileArgs a, hipStream_t stream) {
 // and 4000 wide, 254 against 235; 200 rows, 2560 and 6912 wide, 53.8 against 57.2.
 enum : int { T_256 = 0, T_128, T_64S3, T_64S5, T_128X64, T_COUNT };
 struct TileCost {
-  int bm, bn, per_cu;
+  int bm, bn, threads, per_cu;
   double stage[3], fixed[4];  // fixed by OUT_*
 };
 constexpr TileCost kTileCost[T_COUNT] = {
-    {256, 256, 1, {1.47, 0, 0}, {7, 7, 10, 14}},
-    {128, 128, 2, {0.52, 0.98, 0}, {4, 3, 6, 9}},
-    {64, 64, 3, {0.48, 0.52, 0.62}, {2.1, 2.1, 3, 4}},
-    {64, 64, 2, {0.31, 0.48, 0}, {2.1, 2.1, 3, 4}},
-    {128, 64, 2, {0.45, 0.70, 0}, {2.5, 2.5, 4, 6}},
+    {256, 256, 512, 1, {1.47, 0, 0}, {7, 7, 10, 14}},
+    {128, 128, 256, 2, {0.52, 0.98, 0}, {4, 3, 6, 9}},
+    {64, 64, 256, 3, {0.48, 0.52, 0.62}, {2.1, 2.1, 3, 4}},
+    {64, 64, 256, 2, {0.31, 0.48, 0}, {2.1, 2.1, 3, 4}},
+    {128, 64, 256, 2, {0.45, 0.70, 0}, {2.5, 2.5, 4, 6}},
 };
 constexpr int64_t kCUs = 256;
 
@@ -960,6 +963,7 @@ TilePlan plan_tiles(const TileArgs &a, int out) {
   for (int t = 0; t < T_COUNT; ++t) {
     const TileCost &c = kTileCost[t];
     const int64_t tiles = tiles_of(a, c.bm, out == OUT_GATE ? c.bn / 2 : c.bn);
+    if (!grid_fits(tiles, c.threads)) continue;
     for (int s = 1; s <= (out == OUT_STORE && a.n == 1 ? 16 : 1); ++s) {
       if (s > 1 && (stages / s < 4 || tiles * s > 2 * kCUs * c.per_cu)) break;
       double us = tile_time_us(c, s > 1 ? OUT_PART : out, tiles * s, (stages + s - 1) / s);

@@ -34,6 +34,8 @@ dim3 grid_rows(int64_t blocks) {
   constexpr int64_t row = kGridRow<THREADS>;
   return blocks <= row ? dim3((unsigned)blocks) : dim3((unsigned)row, (unsigned)((blocks + row - 1) / row));
 }
+// Whether one dimension holds them.
+constexpr bool grid_fits(int64_t blocks, int threads) { return blocks * threads < ((int64_t)1 << 32); }
 template <int THREADS>
 __device__ __forceinline__ int64_t grid_block() {
   return (int64_t)blockIdx.y * kGridRow<THREADS> + blockIdx.x;
@@ -333,6 +335,9 @@ struct GatedMlpGrad {
   uint16_t *dg = nullptr, *du = nullptr;  // [M, I] scratch: gradients of g and u
   uint16_t *dx = nullptr, *dwg = nullptr, *dwu = nullptr, *dwd = nullptr;  // each may be null
 };
+// The rows that the tiles' 32-bit row and stage numbers take, with room for the rows and the
+// stages that they look ahead.
+constexpr int64_t kMlpMaxRows = ((int64_t)1 << 31) - 1024;
 int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward);
 hipError_t launch_gated_mlp(const GatedMlp &p, hipStream_t stream);
 hipError_t launch_gated_mlp_bwd(const GatedMlp &p, const GatedMlpGrad &d, hipStream_t stream);

@@ -164,3 +164,13 @@ def test_gated_mlp_work_of_a_zero_width(lib, M, I, N):
     for zero in ((0, N, I, N), (M, N, 0, N)):
         assert lib.mj_gated_mlp_work_bytes(*zero, 0) == lib.mj_gated_mlp_work_bytes(*zero, 1) == 0
     assert lib.mj_gated_mlp_work_bytes(M, N, I, 0, 0) == lib.mj_gated_mlp_work_bytes(M, 0, I, N, 1) == 0
+
+
+def test_gated_mlp_most_rows(lib):
+    """Beyond 2^31 - 1024 rows the tiles' row numbers would overflow: refused."""
+    p = ctypes.c_void_p(16)
+    for m, status in (((1 << 31) - 1023, _lib.MJ_ERR_UNSUPPORTED), ((1 << 31) - 1, _lib.MJ_ERR_UNSUPPORTED),
+                      (0, _lib.MJ_OK)):
+        assert lib.mj_gated_mlp_bf16(p, p, p, p, 3, p, None, None, p, m, 8, 8, 8, None, 0, None) == status
+        assert lib.mj_gated_mlp_backward_bf16(p, p, p, p, 3, p, p, p, p, p, p, None, None, None, None, m, 8,
+                                              8, 8, None, 0, None) == status

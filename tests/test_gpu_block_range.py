@@ -1,4 +1,4 @@
-"""The residual norm over more rows than one dimension of a grid holds (2^32 threads), up to
+"""The residual norm and the gated MLP over more rows than one dimension of a grid holds (2^32 threads), up to
 the last that the ABI takes (bounds as in test_gpu_block.py).  Only the last rows hold
 anything: the others' outputs are zeros."""
 import pytest
@@ -93,3 +93,19 @@ def test_residual_norm_wide_rows_past_a_grid_dimension(dev, dim, backward):
             err = 2.0 ** -18 * (size[name] + size[name].max(-1, keepdim=True).values)
         u = 2.0 ** -8 if have.dtype == torch.bfloat16 else 2.0 ** -24
         _close(have, want, u * want.abs() * 1.01 + err, name)
+
+
+@pytest.mark.parametrize("rows,k,i,h", [((1 << 30) + 5, 8, 8, 8), ((1 << 29) + 3, 8, 40, 8)])
+def test_gated_mlp_rows_past_a_grid_dimension(dev, rows, k, i, h):
+    """2^30 rows are 2^24 tiles of 64 rows, 2^32 threads: larger tiles take them."""
+    _room(rows * 2 * (k + i + h) + (4 << 30))
+    g = _gen("mlp grid", rows)
+    x = _zeros_but_last(g, rows, k)
+    x[:LAST] = x[-LAST:]
+    wg, wu = (_normal(g, (i, k), torch.bfloat16, k ** -0.5) for _ in range(2))
+    wd = _normal(g, (h, i), torch.bfloat16, i ** -0.5)
+    y = mj.gated_mlp(x, wg, wu, wd)
+    ref = plain.mlp(x[-LAST:], wg, wu, wd, torch.zeros((LAST, h), device=dev), "silu", 2.0 ** -8, 2.0 ** -18)["y"]
+    for part in (y[-LAST:], y[:LAST]):
+        _close(part, ref[0], ref[1] + 1e-30, "y")
+    assert not bool(y[LAST:-LAST].any())
