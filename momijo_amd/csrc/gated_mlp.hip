@@ -1148,7 +1148,7 @@ hipError_t launch_sum_f32(const float *part, float *out, int64_t n, int64_t part
                           hipStream_t stream) {
   if (n <= 0) return hipSuccess;
   const int64_t grid = (n + 1023) / 1024;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(sum_f32_kernel, dim3((unsigned)grid), dim3(256), 0, stream, part, out, n,
                      (int)parts);
   return hipGetLastError();

@@ -593,7 +593,7 @@ static hipError_t launch_fx(int64_t M, int64_t N, int64_t K, const T *A, int64_t
   }
   const int TBs = big ? 128 : (tiny ? 32 : 64);
   const int64_t tiles64 = ((M + TBs - 1) / TBs) * ((N + TBs - 1) / TBs);
-  if (tiles64 > INT32_MAX) return hipErrorInvalidValue;  // grid.x limit
+  if (!grid_fits(tiles64, tiny ? 256 : 512)) return hipErrorInvalidValue;
   const int tiles = (int)tiles64;
   constexpr int64_t kMaxGridY = 65535;
   for (int64_t b0 = 0; b0 < batches; b0 += kMaxGridY) {
@@ -887,7 +887,7 @@ hipError_t launch_conv2d_f32(const float *x, const float *w, const float *b, flo
   if (tile >= 224) {
     const int nbn = tile / 32;
     const int64_t tiles_c = ((M + 63) / 64) * ((Ng + 32 * nbn - 1) / (32 * nbn));
-    if (tiles_c > INT32_MAX) return hipErrorInvalidValue;
+    if (!grid_fits(tiles_c, 512)) return hipErrorInvalidValue;
     for (int64_t b0 = 0; b0 < N; b0 += kMaxGridY) {
       const int64_t nb = N - b0 < kMaxGridY ? N - b0 : kMaxGridY;
       const dim3 g((unsigned)tiles_c, (unsigned)nb);
@@ -914,7 +914,7 @@ hipError_t launch_conv2d_f32(const float *x, const float *w, const float *b, flo
   cv.dky = (int)((BKs % (kH * kW)) / kW);
   cv.dkx = (int)(BKs % kW);
   const int64_t tiles64 = ((M + TBs - 1) / TBs) * ((Ng + TBs - 1) / TBs);
-  if (tiles64 > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(tiles64, tiny ? 256 : 512)) return hipErrorInvalidValue;
   const int tiles = (int)tiles64;
   for (int64_t b0 = 0; b0 < N; b0 += kMaxGridY) {
     const int64_t nb = N - b0 < kMaxGridY ? N - b0 : kMaxGridY;
@@ -1032,6 +1032,7 @@ __global__ __launch_bounds__(256) void matvec_kernel(int M, int N, const T *__re
 
 hipError_t launch_matvec_f32(int64_t M, int64_t N, const float *A, int64_t sAm, int64_t sAn,
                              const float *x, int64_t sx, float *y, hipStream_t stream) {
+  if (!grid_fits((M + 3) / 4, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(matvec_kernel<float>, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, stream,
                      (int)M, (int)N, A, sAm, sAn, x, sx, y);
   return hipGetLastError();
@@ -1039,6 +1040,7 @@ hipError_t launch_matvec_f32(int64_t M, int64_t N, const float *A, int64_t sAm, 
 
 hipError_t launch_matvec_f64(int64_t M, int64_t N, const double *A, int64_t sAm, int64_t sAn,
                              const double *x, int64_t sx, double *y, hipStream_t stream) {
+  if (!grid_fits((M + 3) / 4, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(matvec_kernel<double>, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, stream,
                      (int)M, (int)N, A, sAm, sAn, x, sx, y);
   return hipGetLastError();

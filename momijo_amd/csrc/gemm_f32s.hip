@@ -1046,7 +1046,7 @@ static hipError_t launch_tile_s(F32Args p, int64_t batches, hipStream_t stream) 
     attr_set.fetch_or(bit, std::memory_order_release);
   }
   const int64_t tiles = ((p.M + (int64_t)TM - 1) / TM) * ((p.N + (int64_t)TN - 1) / TN);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;  // grid.x limit
+  if (!grid_fits(tiles, T::NT)) return hipErrorInvalidValue;
   for (int64_t b0 = 0; b0 < batches; b0 += kMaxGridY) {
     const int64_t nb = batches - b0 < kMaxGridY ? batches - b0 : kMaxGridY;
     p.batch0 = b0;
@@ -1060,7 +1060,7 @@ static hipError_t launch_tile_s(F32Args p, int64_t batches, hipStream_t stream) 
 template <int TB, int NW, bool AKF, bool BKF, bool CONV>
 static hipError_t launch_direct_s(F32Args p, int64_t batches, hipStream_t stream) {
   const int64_t tiles = ((p.M + (int64_t)TB - 1) / TB) * ((p.N + (int64_t)TB - 1) / TB);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(tiles, NW * 64)) return hipErrorInvalidValue;
   for (int64_t b0 = 0; b0 < batches; b0 += kMaxGridY) {
     const int64_t nb = batches - b0 < kMaxGridY ? batches - b0 : kMaxGridY;
     p.batch0 = b0;

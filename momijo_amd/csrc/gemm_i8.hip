@@ -146,7 +146,7 @@ static hipError_t launch_i8_tile(const int8_t *A, const int8_t *B, int32_t *C, f
                                  const float *b, int64_t M, int64_t N, int64_t K,
                                  hipStream_t stream) {
   const int64_t tiles = ((M + TB - 1) / TB) * ((N + TB - 1) / TB);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;  // grid.x limit
+  if (!grid_fits(tiles, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((gemm_i8_kernel<TB, ANY>), dim3((unsigned)tiles), dim3(256), 0, stream, A, B,
                      C, y, sf, b, (int)M, (int)N, (int)K);
   return hipGetLastError();
@@ -194,6 +194,7 @@ __global__ __launch_bounds__(256) void gemm_i8_literal_kernel(const int8_t *__re
 hipError_t launch_gemm_i8_literal(const int8_t *A, const int8_t *B, int32_t *C, float *y, float sf,
                                   const float *b, int64_t M, int64_t N, int64_t K,
                                   hipStream_t stream) {
+  if (!grid_fits((M * N + 255) / 256, 256)) return hipErrorInvalidValue;
   const unsigned blocks = (unsigned)((M * N + 255) / 256);
   hipLaunchKernelGGL(gemm_i8_literal_kernel, dim3(blocks), dim3(256), 0, stream, A, B, C, y, sf, b,
                      M, N, K);

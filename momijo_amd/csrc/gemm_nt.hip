@@ -903,7 +903,7 @@ static hipError_t launch_w8(const GemmNT &p, hipStream_t stream) {
     attr_set.fetch_or(bit, std::memory_order_release);
   }
   const int64_t grid = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(grid, 512)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(gemm_nt_w8_kernel, dim3((unsigned)grid), dim3(512), lds, stream, p);
   return hipGetLastError();
 }
@@ -1328,7 +1328,7 @@ static hipError_t launch_i8_w4(const GemmI8 &p, hipStream_t stream) {
   }
   const int64_t tiles256 = ((p.M + 255) / 256) * ((p.N + 255) / 256);
   const int64_t tiles128 = ((p.M + 255) / 256) * ((p.N + 127) / 128);
-  if (tiles128 > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(tiles128, 256)) return hipErrorInvalidValue;
   if (tiles256 >= 192)
     hipLaunchKernelGGL((gemm_i8_w4_kernel<256, MODE>), dim3((unsigned)tiles256), dim3(256), lds256,
                        stream, p);
@@ -2048,7 +2048,7 @@ static hipError_t launch_tile(const GemmNT &p, hipStream_t stream) {
     attr_set.fetch_or(bit, std::memory_order_release);
   }
   const int64_t grid = ((p.M + BM - 1) / BM) * ((p.N + BN_OUT - 1) / BN_OUT) * p.splits;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;  // grid.x limit
+  if (!grid_fits(grid, NW * 64)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(NW * 64), lds, stream, p);
   return hipGetLastError();
 }
@@ -2071,7 +2071,7 @@ static hipError_t launch_ring(const GemmNT &p, hipStream_t stream) {
     attr_set.fetch_or(bit, std::memory_order_release);
   }
   const int64_t grid = ((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  if (grid > INT32_MAX) return hipErrorInvalidValue;  // grid.x limit
+  if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, p);
   return hipGetLastError();
 }
@@ -2104,7 +2104,7 @@ static hipError_t launch_w4i8(const GemmNT &p, hipStream_t stream) {
     attr_set.fetch_or(bit, std::memory_order_release);
   }
   const int64_t grid = ((p.M + BM - 1) / BM) * ((p.N + BN_OUT - 1) / BN_OUT) * p.splits;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, p);
   return hipGetLastError();
 }

@@ -189,6 +189,7 @@ __global__ __launch_bounds__(256) void quantize_rowwise_any(const float *__restr
 
 hipError_t launch_quantize_rowwise(const float *W, int64_t N, int64_t K, int rounding,
                                    int8_t *Q, float *scales, hipStream_t stream) {
+  if (!grid_fits((N + 3) / 4, 256)) return hipErrorInvalidValue;
   const unsigned blocks = (unsigned)((N + 3) / 4);
   const bool aligned = ((uintptr_t)W % 16 == 0) && ((uintptr_t)Q % 4 == 0);
   if (aligned && K % 256 == 0 && K <= 4096) {
@@ -312,6 +313,7 @@ __global__ __launch_bounds__(256) void quantize_rows_bf16_any(const uint16_t *__
 template <int W, int CH>
 static hipError_t launch_rows_reg(const uint16_t *x, int64_t M, int64_t K, int8_t *xq, float *sx,
                                  hipStream_t stream) {
+  if (!grid_fits((M + 4 / W - 1) / (4 / W), 256)) return hipErrorInvalidValue;
   const unsigned blocks = (unsigned)((M + 4 / W - 1) / (4 / W));
   hipLaunchKernelGGL((quantize_rows_bf16_reg<W, CH>), dim3(blocks), dim3(256), 0, stream, x,
                      (int)M, (int)K, xq, sx);
@@ -343,6 +345,7 @@ hipError_t launch_quantize_rows_bf16(const uint16_t *x, int64_t M, int64_t K, in
       default: break;
     }
   }
+  if (!grid_fits((M + 3) / 4, 256)) return hipErrorInvalidValue;
   const unsigned blocks = (unsigned)((M + 3) / 4);
   hipLaunchKernelGGL(quantize_rows_bf16_any, dim3(blocks), dim3(256), 0, stream, x, (int)M,
                      (int)K, xq, sx);

@@ -109,3 +109,23 @@ def test_gated_mlp_rows_past_a_grid_dimension(dev, rows, k, i, h):
     for part in (y[-LAST:], y[:LAST]):
         _close(part, ref[0], ref[1] + 1e-30, "y")
     assert not bool(y[LAST:-LAST].any())
+
+
+def test_products_past_a_grid_dimension_are_refused(dev):
+    """The fp32 tiles of 2^29 rows (512 threads for 64 rows) are 2^32 threads: an error, where
+    a launch of a few more runs those few and leaves the other outputs; 2^28 rows run."""
+    k = 8
+    _room(3 << 35)
+    g = _gen("f32 grid")
+    w = _normal(g, (k, k), torch.float32, k ** -0.5)
+    x = torch.zeros(((1 << 29) + 64, k), device=dev)
+    with pytest.raises(mj.MomijoHipError):
+        mj.gated_mlp(x, w, w, w)
+    x = x[:1 << 28]
+    x[-LAST:] = _normal(g, (LAST, k), torch.float32)
+    y = mj.gated_mlp(x, w, w, w)
+    ref = plain.mlp(x[-LAST:], w, w, w, torch.zeros((LAST, k), device=dev), "silu", 2.0 ** -24, 2.0 ** -20)["y"]
+    _close(y[-LAST:], ref[0], ref[1] + 1e-30, "y")
+    assert not bool(y[:-LAST].any())
+    with pytest.raises(mj.MomijoHipError):   # a wave a row
+        mj.quantize_rowwise_int8(torch.zeros(((1 << 26) + 8, 4), device=dev))
