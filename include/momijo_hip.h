@@ -542,7 +542,8 @@ int32_t mj_dropout(int32_t dtype, const void *x, void *y, int64_t n, float p, ui
  * norm(v) = v / sqrt(mean(v^2) + eps) (MJ_NORM_RMS) or (v - mean) / sqrt(var + eps)
  * (MJ_NORM_LAYER), in fp32.  x, b, gate, y, n have element type dtype; scale, wp,
  * bp, wn, bn are fp32 [dim].  Every operand but x may be NULL (b NULL: y = scale
- * x); gate has gate_rows rows, each for rows / gate_rows rows of x.  y may be NULL.
+ * x); gate has gate_rows rows, each for rows / gate_rows rows of x.  y may be NULL, or
+ * x itself where b and scale are NULL (it is not written then).
  * Dropout as mj_dropout over the [rows, dim] array.  stats (or NULL) takes what the
  * backward needs: fp32 [4][rows]. */
 int32_t mj_residual_norm(int32_t dtype, int32_t norm, const void *x, const void *b,

@@ -173,9 +173,8 @@ def _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight, 
     args = (code, kind, x.data_ptr(), _ptr(branch), _ptr(gate), gate_rows, _ptr(scale), _ptr(wp),
             _ptr(bp), _ptr(wn))
     drop = (p, seed, int(counter) & _MASK64, _ptr(state))
-    if y is not x or n is not None:
-        _lib.call("mj_residual_norm", *args, _ptr(bn), eps, *drop,
-                  None if y is x else y.data_ptr(), _ptr(n), _ptr(stats), rows, dim, _stream())
+    _lib.call("mj_residual_norm", *args, _ptr(bn), eps, *drop, y.data_ptr(), _ptr(n), _ptr(stats),
+              rows, dim, _stream())
     if not train:
         return y, n
     return y, n, ResidualNormSaved(x, branch, gate, (scale, wp, bp, wn, bn), args, drop, state, stats)

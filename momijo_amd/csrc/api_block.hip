@@ -169,6 +169,10 @@ int32_t mj_residual_norm(int32_t dtype, int32_t norm, const void *x, const void 
   if (rows == 0 || dim == 0) return MJ_OK;
   if (!y && !n) return fail(MJ_ERR_ARG, "no output");
   if ((n != nullptr) != (wn != nullptr)) return fail(MJ_ERR_ARG, "n and its weight go together");
+  if (y == x && !b && !scale) {  // y is x: not written
+    if (!n) return MJ_OK;
+    y = nullptr;
+  }
   r.y = y, r.n = n, r.stats = stats;
   return hip_status(mj::launch_residual_norm(dtype == MJ_BF16, r, S(stream)),
                     "residual norm launch");

@@ -174,3 +174,12 @@ def test_gated_mlp_most_rows(lib):
         assert lib.mj_gated_mlp_bf16(p, p, p, p, 3, p, None, None, p, m, 8, 8, 8, None, 0, None) == status
         assert lib.mj_gated_mlp_backward_bf16(p, p, p, p, 3, p, p, p, p, p, p, None, None, None, None, m, 8,
                                               8, 8, None, 0, None) == status
+
+
+def test_residual_norm_of_x_itself(lib):
+    """y = x is no work, but the other arguments are checked as in any call."""
+    alone = dict(b=None, x=16, y=16)
+    assert _norm(lib, **alone) == _lib.MJ_OK
+    for bad in (dict(p=0.5), dict(p=2.0), dict(gate=16, gate_rows=1), dict(wp=16), dict(bp=16), dict(bn=16),
+                dict(eps=-1.0), dict(dim=16385), dict(norm=2), dict(n=16)):
+        assert _norm(lib, **{**alone, **bad}) != _lib.MJ_OK, bad

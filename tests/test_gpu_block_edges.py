@@ -65,3 +65,22 @@ def test_residual_norm_dropped_places(dev, rows, dim, post, bias, dtype):
     b = branch if post else torch.where(keep, branch, bad)
     for q in (gate, torch.where(keep, gate, bad)):
         assert all(torch.equal(a, c) for a, c in zip(step(b, q), want))
+
+
+def test_residual_norm_arguments_without_work(dev):
+    """Where y is x and no norm follows, wrong arguments are refused as elsewhere, and right
+    ones give x and its gradient."""
+    x, w = torch.randn((6, 32), device=dev), torch.ones(32, device=dev)
+    for bad in (dict(p=0.5), dict(gate=torch.ones((2, 32), device=dev)), dict(post_weight=w),
+                dict(next_bias=w), dict(post_bias=w), dict(eps=-1.0), dict(p=float("nan"))):
+        with pytest.raises(mj.MomijoHipError):
+            mj.residual_norm(x, **bad)
+        with pytest.raises(mj.MomijoHipError):
+            mj.residual_norm_train(x, **bad)
+    with pytest.raises(mj.MomijoHipError):
+        mj.residual_norm(torch.zeros((1, 16392), device=dev))
+    y, n, saved = mj.residual_norm_train(x)
+    assert y is x and n is None
+    dy = torch.randn_like(x)
+    assert torch.equal(mj.residual_norm_backward(dy, None, saved)["x"], dy)
+    assert mj.residual_norm(x[:0])[0].shape == (0, 32)
