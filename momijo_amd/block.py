@@ -162,6 +162,8 @@ def _residual_norm(x, branch, gate, scale, post_weight, post_bias, next_weight, 
             raise ValueError(f"gate must be [{dim}] or [groups, {dim}], got {list(gate.shape)}")
         gate = _like(gate, x, gate.shape, "gate")
         gate_rows = 1 if gate.dim() == 1 else gate.shape[0]
+        if gate_rows == 0 and rows:  # (its pointer is null: no gate, to the call below)
+            raise ValueError(f"0 gate rows for {rows} rows")
     scale = _vector(scale, device, dim, "scale")
     wp, bp = _vector(post_weight, device, dim, "post_weight"), _vector(post_bias, device, dim, "post_bias")
     wn, bn = _vector(next_weight, device, dim, "next_weight"), _vector(next_bias, device, dim, "next_bias")

@@ -84,3 +84,15 @@ def test_residual_norm_arguments_without_work(dev):
     dy = torch.randn_like(x)
     assert torch.equal(mj.residual_norm_backward(dy, None, saved)["x"], dy)
     assert mj.residual_norm(x[:0])[0].shape == (0, 32)
+
+
+def test_residual_norm_gate_without_rows(dev):
+    """A gate of no rows is a gate that does not divide the rows; with no rows it fits."""
+    x = torch.zeros((6, 32), dtype=torch.bfloat16, device=dev)
+    with pytest.raises(ValueError):
+        mj.residual_norm(x, x, gate=x[:0])
+    with pytest.raises(ValueError):
+        mj.residual_norm_train(x, x, gate=x[:0])
+    y, _, saved = mj.residual_norm_train(x[:0], x[:0], gate=x[:0])
+    grads = mj.residual_norm_backward(y, None, saved)
+    assert y.shape == grads["gate"].shape == (0, 32)
