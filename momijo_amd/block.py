@@ -96,12 +96,14 @@ def dropout_backward(dy: torch.Tensor, p: float, seed, counter: int = 0,
 
 class Dropout:
     """Dropout(p, seed): each training ``forward`` draws from the next counter;
-    ``backward`` takes the counter that its forward returned."""
+    ``backward`` takes the counter that its forward returned.  ``seed`` is as in
+    ``dropout``: a captured forward draws a new mask when a seed tensor changes."""
 
-    def __init__(self, p: float, seed: int = 0):
+    def __init__(self, p: float, seed=0):
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must be in [0, 1], got {p}")
-        self.p, self.seed, self.counter = float(p), int(seed), 0
+        self.p, self.counter = float(p), 0
+        self.seed = seed if isinstance(seed, torch.Tensor) else int(seed)
         self.training = True
 
     def forward(self, x: torch.Tensor) -> tuple[torch.Tensor, int | None]:

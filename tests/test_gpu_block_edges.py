@@ -96,3 +96,31 @@ def test_residual_norm_gate_without_rows(dev):
     y, _, saved = mj.residual_norm_train(x[:0], x[:0], gate=x[:0])
     grads = mj.residual_norm_backward(y, None, saved)
     assert y.shape == grads["gate"].shape == (0, 32)
+
+
+# ------------------------------------------------------------------ dropout
+def test_dropout_class_with_a_device_seed(dev):
+    """A captured forward and backward draw from the seed tensor: every replay the mask of the
+    counter that it holds then, as the eager call with that counter."""
+    x, dy = (_normal(_gen("class", i), (5000,), torch.bfloat16) for i in range(2))
+    state = torch.tensor([77, 0], dtype=torch.int64, device=dev)
+    layer = mj.Dropout(0.3, state)
+    y, c = layer.forward(x)
+    assert c == 0 and torch.equal(y, mj.dropout(x, 0.3, 77, 0))
+    torch.cuda.synchronize()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        g.capture_begin()
+        y, c = layer.forward(x)
+        dx = layer.backward(dy, c)
+        g.capture_end()
+    assert c == 1
+    for step in (0, 1, 9, 2 ** 40):
+        state[1] = step
+        y.zero_(), dx.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, mj.dropout(x, 0.3, 77, step + c))
+        assert torch.equal(dx, mj.dropout(dy, 0.3, 77, step + c))
+    with pytest.raises(ValueError):
+        mj.Dropout(0.3, state.float()).forward(x)
