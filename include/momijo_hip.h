@@ -589,6 +589,11 @@ int32_t mj_gated_mlp_f32(const float *x, const float *Wg, const float *Wu, const
                          int32_t act, float *h, float *g, float *u, float *y, int64_t M, int64_t K,
                          int64_t I, int64_t H, void *work, int64_t work_bytes, void *stream);
 
+/* The kernel of a product of the bf16 block, by name ("" for an empty or refused one):
+ * product 0 gate and up, 1 y, 2 dg and du, 3 dx, 4 dWg, dWu and dWd.  Host only; for
+ * tests and profiles. */
+const char *mj_gated_mlp_kernel(int64_t M, int64_t K, int64_t I, int64_t H, int32_t product);
+
 /* Row copies between a width and its zero-padded form, n (1..4) matrices in one
  * launch: dst[i] [dst_rows, dst_cols] (rows dst_ld apart) takes src[i] [rows, cols] (rows
  * src_ld apart) and zeros where that ends; dst_rows, dst_cols below rows, cols cut.

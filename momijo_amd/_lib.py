@@ -125,6 +125,7 @@ SIGNATURES = {
     "mj_residual_norm_backward": (_I32, [_I32, _I32, _P, _P, _P, _I64] + [_P] * 4 +
                                   [_F, _U64, _U64] + [_P] * 12 + [_I64, _I64, _P, _I64, _P]),
     "mj_gated_mlp_work_bytes": (_I64, [_I64, _I64, _I64, _I64, _I32]),
+    "mj_gated_mlp_kernel": (ctypes.c_char_p, [_I64] * 4 + [_I32]),
     "mj_gated_mlp_bf16": (_I32, [_P] * 4 + [_I32] + [_P] * 4 + [_I64] * 4 + [_P, _I64, _P]),
     "mj_gated_mlp_f32_work_bytes": (_I64, [_I64, _I64, _I64, _I64, _I32]),
     "mj_gated_mlp_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 4 + [_I64] * 4 + [_P, _I64, _P]),

@@ -236,6 +236,14 @@ int64_t mj_gated_mlp_work_bytes(int64_t M, int64_t K, int64_t I, int64_t H, int3
   return mj::gated_mlp_part_floats(M, K, I, H, backward != 0) * (int64_t)sizeof(float);
 }
 
+const char *mj_gated_mlp_kernel(int64_t M, int64_t K, int64_t I, int64_t H, int32_t product) {
+  const void *none = nullptr;
+  if (M <= 0 || K <= 0 || I <= 0 || H <= 0 || product < 0 || product > 4 ||
+      check_mlp(MJ_EPI_NONE, M, K, I, H) || check_mlp_bf16("gated MLP", M, K, I, H, &none, 1))
+    return "";
+  return mj::gated_mlp_kernel_name(M, K, I, H, product);
+}
+
 int32_t mj_copy_rows_bf16(int32_t n, const uint16_t *const *src, uint16_t *const *dst,
                           const int64_t *sizes, void *stream) {
   if (n < 1 || n > 4) return fail(MJ_ERR_ARG, "1 to 4 matrices, got %d", n);

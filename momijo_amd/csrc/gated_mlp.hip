@@ -1003,6 +1003,9 @@ bool skinny_takes(int64_t M, int64_t N, int64_t K) {
   return M <= 16 || (M <= 32 && N * K <= 3000000);
 }
 
+// Sixteen waves for a long sum of few rows (below).
+bool few_rows_deep(int64_t M, int64_t K) { return M <= 4 && K >= 8192; }
+
 // Waves: 4096 x 11008 gate/up of one row 34.6 us with eight (5.2 TB/s) and one slice of
 // 64 k in flight each, 36.3, 37.1, 37.5 with two, three, four in flight (a wave's eight
 // slices end sooner with one, and more workgroups fit a CU).  Sixteen waves for one long row: K = 11008, 4096 columns
@@ -1014,7 +1017,7 @@ hipError_t launch_skinny(const SkinnyArgs &a, hipStream_t stream) {
   if (a.N == 0) return hipSuccess;
   if (a.M > 16)
     hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 2>), grid, dim3(512), 0, stream, a);
-  else if (!GATE && a.M <= 4 && a.K >= 8192)
+  else if (!GATE && few_rows_deep(a.M, a.K))
     hipLaunchKernelGGL((mlp_skinny_kernel<false, 1, 16>), grid, dim3(1024), 0, stream, a);
   else
     hipLaunchKernelGGL((mlp_skinny_kernel<GATE, 1>), grid, dim3(512), 0, stream, a);
@@ -1039,7 +1042,18 @@ hipError_t launch_plain(TileArgs a, float *part, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// The plain products that may split K: y, and dx with its two segments.
+// The products' operands.  y, and dx with its two segments, may split K.
+TileArgs gate_args(const GatedMlp &q) {
+  TileArgs a;
+  a.act = q.act;
+  TileProb &p = a.p[0];
+  p.A[0] = q.x, p.lda = q.K;
+  p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
+  p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.K;
+  p.C = q.h, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
+  return a;
+}
+
 TileArgs down_args(const GatedMlp &q) {
   TileArgs a;
   TileProb &p = a.p[0];
@@ -1060,7 +1074,61 @@ TileArgs dx_args(const GatedMlp &q, const GatedMlpGrad &o) {
   return a;
 }
 
+TileArgs dgate_args(const GatedMlp &q, const GatedMlpGrad &o) {
+  TileArgs a;
+  a.act = q.act;
+  TileProb &p = a.p[0];
+  p.A[0] = o.dy, p.lda = q.H;
+  p.B[0] = q.wd, p.ldb = q.I;
+  p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.H;
+  p.C = o.dg, p.C2 = o.du, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
+  return a;
+}
+
+// The wanted weight gradients (n: how many).
+TileArgs dw_args(const GatedMlp &q, const GatedMlpGrad &o, bool dwg, bool dwu, bool dwd) {
+  TileArgs w;
+  w.n = 0;
+  auto add = [&](const uint16_t *A, int64_t rows, const uint16_t *B, int64_t cols, uint16_t *C) {
+    TileProb &p = w.p[w.n++];
+    p.A[0] = A, p.lda = rows;
+    p.B[0] = B, p.ldb = cols;
+    p.M = (int)rows, p.N = (int)cols, p.K = (int)q.M;
+    p.C = C, p.ldc = cols;
+  };
+  if (dwg) add(o.dg, q.I, q.x, q.K, o.dwg);
+  if (dwu) add(o.du, q.I, q.x, q.K, o.dwu);
+  if (dwd) add(o.dy, q.H, q.h, q.I, o.dwd);
+  return w;
+}
+
 }  // namespace
+
+const char *gated_mlp_kernel_name(int64_t M, int64_t K, int64_t I, int64_t H, int product) {
+  GatedMlp q;
+  q.M = M, q.K = K, q.I = I, q.H = H;
+  const GatedMlpGrad o;
+  if (product == 0 && skinny_takes(M, I, K)) return M > 16 ? "32 rows" : "16 rows";
+  if (product == 1 && skinny_takes(M, H, I))
+    return M > 16 ? "32 rows" : few_rows_deep(M, I) ? "4 rows, 16 waves" : "16 rows";
+  const bool plain = product == 1 || product == 3;
+  const TileArgs a = product == 0   ? gate_args(q)
+                     : product == 1 ? down_args(q)
+                     : product == 2 ? dgate_args(q, o)
+                     : product == 3 ? dx_args(q, o)
+                                    : dw_args(q, o, true, true, true);
+  const TilePlan pl = plan_tiles(a, plain         ? OUT_STORE
+                                    : product == 0 ? OUT_GATE
+                                    : product == 2 ? OUT_DGATE
+                                                   : OUT_STORE);
+  static const char *const names[T_COUNT][2] = {
+      {"256x256", "256x256, K slices"},
+      {"128x128", "128x128, K slices"},
+      {"64x64, 3 stages", "64x64, 3 stages, K slices"},
+      {"64x64, 5 stages", "64x64, 5 stages, K slices"},
+      {"128x64", "128x64, K slices"}};
+  return names[pl.tile][pl.splits > 1];
+}
 
 int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward) {
   GatedMlp q;
@@ -1079,14 +1147,8 @@ hipError_t launch_gated_mlp(const GatedMlp &q, hipStream_t stream) {
     a.M = (int)q.M, a.N = (int)q.I, a.K = (int)q.K, a.act = q.act;
     if (hipError_t e = launch_skinny<true>(a, stream); e != hipSuccess) return e;
   } else {
-    TileArgs a;
-    a.act = q.act;
-    TileProb &p = a.p[0];
-    p.A[0] = q.x, p.lda = q.K;
-    p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
-    p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.K;
-    p.C = q.h, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
-    if (hipError_t e = launch_tiles<true, true, OUT_GATE>(a, stream); e != hipSuccess) return e;
+    if (hipError_t e = launch_tiles<true, true, OUT_GATE>(gate_args(q), stream); e != hipSuccess)
+      return e;
   }
   if (!skinny_takes(q.M, q.H, q.I)) return launch_plain<true, true>(down_args(q), q.part, stream);
   SkinnyArgs a;
@@ -1096,32 +1158,13 @@ hipError_t launch_gated_mlp(const GatedMlp &q, hipStream_t stream) {
 }
 
 hipError_t launch_gated_mlp_bwd(const GatedMlp &q, const GatedMlpGrad &o, hipStream_t stream) {
-  if (o.dx || o.dwg || o.dwu) {
-    TileArgs a;
-    a.act = q.act;
-    TileProb &p = a.p[0];
-    p.A[0] = o.dy, p.lda = q.H;
-    p.B[0] = q.wd, p.ldb = q.I;
-    p.M = (int)q.M, p.N = (int)q.I, p.K = (int)q.H;
-    p.C = o.dg, p.C2 = o.du, p.F = q.g, p.F2 = q.u, p.ldc = q.I;
-    if (hipError_t e = launch_tiles<true, false, OUT_DGATE>(a, stream); e != hipSuccess) return e;
-  }
+  if (o.dx || o.dwg || o.dwu)
+    if (hipError_t e = launch_tiles<true, false, OUT_DGATE>(dgate_args(q, o), stream); e != hipSuccess)
+      return e;
   if (o.dx)
     if (hipError_t e = launch_plain<true, false>(dx_args(q, o), q.part, stream); e != hipSuccess)
       return e;
-  TileArgs w;
-  w.n = 0;
-  auto add = [&](const uint16_t *A, int64_t rows, const uint16_t *B, int64_t cols, uint16_t *C) {
-    if (!C) return;
-    TileProb &p = w.p[w.n++];
-    p.A[0] = A, p.lda = rows;
-    p.B[0] = B, p.ldb = cols;
-    p.M = (int)rows, p.N = (int)cols, p.K = (int)q.M;
-    p.C = C, p.ldc = cols;
-  };
-  add(o.dg, q.I, q.x, q.K, o.dwg);
-  add(o.du, q.I, q.x, q.K, o.dwu);
-  add(o.dy, q.H, q.h, q.I, o.dwd);
+  const TileArgs w = dw_args(q, o, o.dwg, o.dwu, o.dwd);
   return w.n ? launch_tiles<false, false, OUT_STORE>(w, stream) : hipSuccess;
 }
 

@@ -339,6 +339,8 @@ struct GatedMlpGrad {
 // stages that they look ahead.
 constexpr int64_t kMlpMaxRows = ((int64_t)1 << 31) - 1024;
 int64_t gated_mlp_part_floats(int64_t M, int64_t K, int64_t I, int64_t H, bool backward);
+// product: 0 gate and up, 1 y, 2 dg and du, 3 dx, 4 the weight gradients
+const char *gated_mlp_kernel_name(int64_t M, int64_t K, int64_t I, int64_t H, int product);
 hipError_t launch_gated_mlp(const GatedMlp &p, hipStream_t stream);
 hipError_t launch_gated_mlp_bwd(const GatedMlp &p, const GatedMlpGrad &d, hipStream_t stream);
 // dst[r, c] = src[r, c] inside [rows, cols], else 0, for r < dst_rows, c < dst_cols.
