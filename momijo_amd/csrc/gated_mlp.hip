@@ -701,38 +701,33 @@ __global__ __launch_bounds__(NW * 64) void mlp_skinny_kernel(SkinnyArgs p) {
 #pragma unroll
     for (int b = 0; b < MB; ++b) acc[g][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  constexpr int DEPTH = 1;  // slices of 64 in flight
-  uint4 wv[DEPTH][2][G], xv[DEPTH][2][MB];
-  auto load = [&](int s, int k0) __attribute__((always_inline)) {
+  uint4 wv[2][G], xv[2][MB];  // a slice of 64
+  auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = k0 + 32 * h + 8 * fh;
       const bool in = k < K;
-      wv[s][h][0] = buffer_load16(rw, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
+      wv[h][0] = buffer_load16(rw, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
       if constexpr (GATE)
-        wv[s][h][1] = buffer_load16(rw2, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
+        wv[h][1] = buffer_load16(rw2, in && wo != kOobOffset ? wo + k * 2 : kOobOffset);
 #pragma unroll
       for (int b = 0; b < MB; ++b)
-        xv[s][h][b] = buffer_load16(rx, in && xo[b] != kOobOffset ? xo[b] + k * 2 : kOobOffset);
+        xv[h][b] = buffer_load16(rx, in && xo[b] != kOobOffset ? xo[b] + k * 2 : kOobOffset);
     }
   };
   const int step = NW * 64;
+  load(wave * 64);
+  for (int k0 = wave * 64; k0 < K; k0 += step) {
 #pragma unroll
-  for (int s = 0; s < DEPTH; ++s) load(s, wave * 64 + s * step);
-  for (int k0 = wave * 64; k0 < K; k0 += DEPTH * step) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int s = 0; s < DEPTH; ++s) {
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int b = 0; b < MB; ++b)
-            acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8, wv[s][h][g]), __builtin_bit_cast(bf16x8, xv[s][h][b]),
-                acc[g][b], 0, 0, 0);
-      load(s, k0 + (DEPTH + s) * step);
-    }
+        for (int b = 0; b < MB; ++b)
+          acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[h][g]),
+                                                              __builtin_bit_cast(bf16x8, xv[h][b]),
+                                                              acc[g][b], 0, 0, 0);
+    load(k0 + step);
   }
   // block (g, b): weight row 4 fh + q, x row 16 b + fr
 #pragma unroll

@@ -64,8 +64,8 @@ __device__ __forceinline__ void draws8(uint64_t e, uint64_t counter, uint64_t se
   }
 }
 
-// 0 or scale for each of 8 elements; a dropped element's value is not looked
-// at (0, whatever it holds), so its factor must be selected, not multiplied.
+// Whether element i of the 8 is kept.  A dropped element's value is not looked at (0,
+// whatever it holds): callers select by this, they do not multiply by 0.
 __device__ __forceinline__ bool keep_of(const uint32_t (&w)[4], int i, uint32_t thr) {
   return ((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) >= thr;
 }

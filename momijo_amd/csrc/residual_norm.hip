@@ -121,7 +121,7 @@ __device__ __forceinline__ void row_stats(const Cols<VPT> &v, bool layer, float 
   rstd = 1.0f / sqrtf(q[0] * inv + eps);
 }
 
-// The keep factor (0 or scale) of every column of row m.
+// The 16-bit draws of every column of row m, two a word (keep_of).
 template <int TPR, int VPT, bool ALIGNED>
 __device__ __forceinline__ void keep_bits(uint32_t (&w)[VPT][4], int64_t m, int lane, int dim,
                                           uint64_t seed, uint64_t counter) {
@@ -893,7 +893,7 @@ hipError_t launch_bwd_wide(const ResNorm &p, const ResNormGrad &g, hipStream_t s
 }
 
 // The team that a row's chunks of 8 fit.
-template <typename T, typename F>
+template <typename F>
 hipError_t by_width(int64_t dim, F f) {
   if (dim <= 512) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
   if (dim <= 1024) return f(std::integral_constant<int, 128>(), std::integral_constant<int, 1>());
@@ -905,7 +905,7 @@ hipError_t by_width(int64_t dim, F f) {
 
 template <typename T>
 hipError_t fwd_typed(const ResNorm &p, hipStream_t stream) {
-  return by_width<T>(p.dim, [&](auto tpr, auto vpt) {
+  return by_width(p.dim, [&](auto tpr, auto vpt) {
     return launch_fwd<T, decltype(tpr)::value, decltype(vpt)::value>(p, stream);
   });
 }
