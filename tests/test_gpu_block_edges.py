@@ -67,6 +67,25 @@ def test_residual_norm_dropped_places(dev, rows, dim, post, bias, dtype):
         assert all(torch.equal(a, c) for a, c in zip(step(b, q), want))
 
 
+@pytest.mark.parametrize("dim,bias", [(264, True), (1001, False), (8200, True)])
+def test_residual_norm_all_dropped(dev, dim, bias):
+    """p = 1: the branch is in nothing, whatever it and the gate hold."""
+    rows = 12
+    g = _gen("all", dim)
+    x, dy, dn = (_normal(g, (rows, dim), torch.bfloat16) for _ in range(3))
+    w = _normal(g, (dim,), torch.float32, 0.2, 1.0)
+    kw = dict(next_weight=w, next_bias=w if bias else None)
+    nan = torch.full_like(x, float("nan"))
+    y, n, saved = mj.residual_norm_train(x, nan, gate=nan[:2], p=1.0, seed=1, **kw)
+    grads = mj.residual_norm_backward(dy, dn, saved)
+    y0, n0, saved = mj.residual_norm_train(x, torch.zeros_like(x), gate=torch.ones_like(x[:2]), **kw)
+    want = mj.residual_norm_backward(dy, dn, saved)
+    assert torch.equal(y, x) and torch.equal(y0, x) and torch.equal(n, n0)
+    assert not bool(grads["branch"].any()) and not bool(grads["gate"].any())
+    for name in ("x", "next_weight") + (("next_bias",) if bias else ()):
+        assert torch.equal(grads[name], want[name]), name
+
+
 def test_residual_norm_arguments_without_work(dev):
     """Where y is x and no norm follows, wrong arguments are refused as elsewhere, and right
     ones give x and its gradient."""
