@@ -505,8 +505,8 @@ __global__ __launch_bounds__(256) void mlp_ring_kernel(TileArgs args) {
 // The pipelined tiles: 256 x 256 of 8 waves (2 x 4, 128 x 64 outputs each), one
 // workgroup a CU, or 128 x 128 of 4 waves (2 x 2, 64 x 64 each), two a CU, where 256 x
 // 256 tiles leave CUs idle (twice the operand traffic and a third more LDS reads a
-// flop: 0.86 us for two 64-deep stages of 128 x 128, 1.47 for one of 256 x 256, four
-// times the work).  Both put two waves on a SIMD, and run the pipeline of the
+// flop: in whole layers 0.98 us for two 64-deep stages of 128 x 128, 1.47 for one of 256 x
+// 256, twice the work of the two).  Both put two waves on a SIMD, and run the pipeline of the
 // framework's large bf16 product (gemm_nt_w8_kernel): two A and three B stage buffers,
 // a stage of two 32-deep steps with one barrier between them, each step's fragment
 // reads for the next spread between its MFMAs, four direct loads a step for the stage
