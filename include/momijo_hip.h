@@ -620,6 +620,117 @@ int32_t mj_gated_mlp_backward_f32(const float *x, const float *Wg, const float *
                                   float *dWu, float *dWd, int64_t M, int64_t K, int64_t I,
                                   int64_t H, void *work, int64_t work_bytes, void *stream);
 
+/* ---- mixture of experts --------------------------------------------------
+ * Tokens sorted by expert and back, and the experts' gated blocks over the sorted rows (no
+ * reference counterpart).  Device pointers only; these calls allocate nothing, take no
+ * library workspace and can be captured into a HIP graph.  Nothing is read back: how many
+ * rows an expert has stays on the device.
+ *
+ * `tokens` tokens with `topk` experts each are tokens * topk slots (slot t * topk + j),
+ * at most 2^31 - 1024; 1 to 1024 experts. */
+
+/* The sort: pos [slots] is each slot's row among the rows sorted by expert, in the order of
+ * the slots within an expert; offsets [experts + 1] the experts' first rows.  ids [slots]
+ * are int32 or int64 (id_bytes 4, 8); a slot whose id is outside 0 .. experts - 1 is dropped:
+ * such slots come last, in their order, from row offsets[experts] on. */
+int64_t mj_sort_experts_work_bytes(int64_t slots, int64_t experts);
+int32_t mj_sort_experts(const void *ids, int32_t id_bytes, int64_t slots, int64_t experts, int32_t *pos,
+                        int32_t *offsets, void *work, int64_t work_bytes, void *stream);
+
+/* xs[pos[t, j]] = x[t], zeros for a dropped slot: x [tokens, dim] and xs [slots, dim] of
+ * dtype (MJ_F32, MJ_BF16), any alignment of the elements.  With weights [tokens, topk] their
+ * sorted form goes to ws [slots] (0 for a dropped slot); both NULL: none. */
+int32_t mj_dispatch(int32_t dtype, const void *x, const float *weights, const int32_t *pos,
+                    const int32_t *offsets, int64_t experts, void *xs, float *ws, int64_t tokens,
+                    int64_t topk, int64_t dim, void *stream);
+
+/* y[t] = the sum over j of weights[t, j] ys[pos[t, j]] (weights NULL: ones), in fp32 in the
+ * order of j; dropped slots are left out, whatever they hold.  ys is of dtype, y of y_dtype:
+ * the same, or MJ_BF16 from MJ_F32.  Without weights this is mj_dispatch's gradient. */
+int32_t mj_combine(int32_t dtype, int32_t y_dtype, const void *ys, const float *weights, const int32_t *pos,
+                   const int32_t *offsets, int64_t experts, void *y, int64_t tokens, int64_t topk,
+                   int64_t dim, void *stream);
+
+/* mj_combine's gradients: dys[pos[t, j]] = weights[t, j] dy[t] and dw[t, j] = <dy[t],
+ * ys[pos[t, j]]>, both 0 for a dropped slot. */
+int32_t mj_combine_backward(int32_t dtype, const void *dy, const void *ys, const float *weights,
+                            const int32_t *pos, const int32_t *offsets, int64_t experts, void *dys, float *dw,
+                            int64_t tokens, int64_t topk, int64_t dim, void *stream);
+
+/* The experts' gated blocks over R sorted rows (mj_gated_mlp_bf16 with a matrix for each
+ * expert); row r of expert e:
+ *   g = x Wg_e^T, u = x Wu_e^T, h = weights[r] act(g) u, y = h Wd_e^T
+ * xs [R,K], Wg and Wu [experts,I,K], Wd [experts,H,I], h [R,I], ys [R,H] fp32 (a token's rows
+ * are added before they are rounded), weights [R] fp32 or NULL (ones); g, u fp32 [R,I] are written for the backward, or both NULL.  K, I, H
+ * multiples of 8 below 2^22, arrays 16-byte aligned.  ys's rows from offsets[experts] on
+ * become zeros; h, g and u's stay as they were. */
+int32_t mj_experts_mlp_bf16(const uint16_t *xs, const int32_t *offsets, int64_t experts, const uint16_t *Wg,
+                            const uint16_t *Wu, const uint16_t *Wd, int32_t act, const float *weights,
+                            uint16_t *h, float *g, float *u, float *ys, int64_t R, int64_t K, int64_t I,
+                            int64_t H, void *stream);
+
+/* Its gradients from dys [R,H] and the forward's h, g, u:
+ *   dh = dy Wd_e, dg = weights[r] dh u act'(g), du = weights[r] dh act(g)
+ *   dx = dg Wg_e + du Wu_e, dWg_e = dg^T x, dWu_e = du^T x, dWd_e = dy^T h
+ *   dw[slot] = <dh, act(g) u> of row pos[slot], 0 for a dropped slot
+ * dxs [R,K] is fp32, as ys.  dg, du [R,I] are scratch, and with dw dots of mj_experts_mlp_dots floats; any of dxs, dWg,
+ * dWu, dWd, dw may be NULL.  An expert without rows gets zeros, and so do dxs's rows from
+ * offsets[experts] on. */
+int64_t mj_experts_mlp_dots(int64_t R, int64_t experts, int64_t K, int64_t I, int64_t H);
+int32_t mj_experts_mlp_backward_bf16(const uint16_t *xs, const int32_t *offsets, int64_t experts,
+                                     const uint16_t *Wg, const uint16_t *Wu, const uint16_t *Wd, int32_t act,
+                                     const float *weights, const uint16_t *h, const float *g, const float *u,
+                                     const uint16_t *dys, uint16_t *dg, uint16_t *du, float *dxs,
+                                     uint16_t *dWg, uint16_t *dWu, uint16_t *dWd, const int32_t *pos,
+                                     int64_t slots, float *dots, float *dw, int64_t R, int64_t K, int64_t I,
+                                     int64_t H, void *stream);
+
+/* ---- 8-bit floating point ------------------------------------------------
+ * Products of e4m3 values (largest 448) with a scale for each block of 128 features of a
+ * row (x) or 128 x 128 elements (W), for inference (no reference counterpart).  A block of
+ * largest magnitude m is quantized with a = max(m, 2^-100): scale a * (1 / 448), values
+ * e4m3(v * (448 * (1 / a))) to the nearest even, each operation rounded to fp32.  A NaN stays a NaN; an infinity becomes one, with
+ * an infinite scale.  Widths K are multiples of 16, widths below 2^22, rows at most 2^31 -
+ * 1024, arrays of values 16-byte aligned.  Scales of x lie block by block, [ceil(K / 128)]
+ * [rows], those of W as [ceil(N / 128)][ceil(K / 128)].  Scratch memory is the caller's. */
+int32_t mj_quantize_rows_f8(int32_t dtype, const void *x, uint8_t *q, float *scales, int64_t rows, int64_t K,
+                            void *stream);
+int32_t mj_quantize_blocks_f8(int32_t dtype, const void *W, uint8_t *q, float *scales, int64_t mats, int64_t N,
+                              int64_t K, void *stream);
+
+/* y [M,N] bf16 = act(x W^T + bias); the sum of a block's products is scaled and added in
+ * fp32.  bias fp32 [N] or NULL; act MJ_EPI_NONE, RELU, GELU_TANH or SILU.  mj_linear_f8
+ * quantizes x [M,K] of dtype first. */
+int64_t mj_gemm_f8_work_bytes(int64_t M, int64_t N, int64_t K);
+int32_t mj_gemm_f8(const uint8_t *xq, const float *sx, const uint8_t *Wq, const float *sw, const float *bias,
+                   int32_t act, uint16_t *y, int64_t M, int64_t N, int64_t K, void *work, int64_t work_bytes,
+                   void *stream);
+int64_t mj_linear_f8_work_bytes(int64_t M, int64_t N, int64_t K);
+int32_t mj_linear_f8(int32_t dtype, const void *x, const uint8_t *Wq, const float *sw, const float *bias,
+                     int32_t act, uint16_t *y, int64_t M, int64_t N, int64_t K, void *work, int64_t work_bytes,
+                     void *stream);
+
+/* mj_dispatch of quantized rows: each token's row is quantized once and goes to its topk
+ * sorted rows of q [slots,K], scales [ceil(K / 128)][slots]; zeros for a dropped slot. */
+int32_t mj_dispatch_f8(int32_t dtype, const void *x, const int32_t *pos, const int32_t *offsets,
+                       int64_t experts, uint8_t *q, float *scales, int64_t tokens, int64_t topk, int64_t K,
+                       void *stream);
+
+/* Sorted rows times their expert's matrix: y [R,N] fp32 = x W_e^T, zeros from row
+ * offsets[experts] on.  Wq [experts,N,K], sw [experts][ceil(N / 128)][ceil(K / 128)]. */
+int32_t mj_experts_gemm_f8(const uint8_t *xq, const float *sx, const int32_t *offsets, int64_t experts,
+                           const uint8_t *Wq, const float *sw, float *y, int64_t R, int64_t N, int64_t K,
+                           void *stream);
+
+/* The gated block's first half: h = act(x Wg_e^T) (x Wu_e^T) in fp32, quantized to hq
+ * [R,I], sh [ceil(I / 128)][R] as rows of the next product (zeros from row offsets[experts]
+ * on).  I a multiple of 16. */
+int64_t mj_experts_gate_f8_work_bytes(int64_t R, int64_t experts, int64_t I, int64_t K);
+int32_t mj_experts_gate_f8(const uint8_t *xq, const float *sx, const int32_t *offsets, int64_t experts,
+                           const uint8_t *Wg, const float *sg, const uint8_t *Wu, const float *su, int32_t act,
+                           uint8_t *hq, float *sh, int64_t R, int64_t I, int64_t K, void *work,
+                           int64_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -134,6 +134,28 @@ SIGNATURES = {
                                    [_P, _I64, _P]),
     "mj_gated_mlp_backward_f32": (_I32, [_P] * 4 + [_I32] + [_P] * 10 + [_I64] * 4 +
                                   [_P, _I64, _P]),
+    # mixture of experts
+    "mj_sort_experts_work_bytes": (_I64, [_I64, _I64]),
+    "mj_sort_experts": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P, _I64, _P]),
+    "mj_dispatch": (_I32, [_I32] + [_P] * 4 + [_I64, _P, _P] + [_I64] * 3 + [_P]),
+    "mj_combine": (_I32, [_I32, _I32] + [_P] * 4 + [_I64, _P] + [_I64] * 3 + [_P]),
+    "mj_combine_backward": (_I32, [_I32] + [_P] * 5 + [_I64, _P, _P] + [_I64] * 3 + [_P]),
+    "mj_experts_mlp_bf16": (_I32, [_P, _P, _I64, _P, _P, _P, _I32] + [_P] * 5 + [_I64] * 4 + [_P]),
+    "mj_experts_mlp_dots": (_I64, [_I64] * 5),
+    "mj_experts_mlp_backward_bf16": (_I32, [_P, _P, _I64, _P, _P, _P, _I32] + [_P] * 12 +
+                                     [_I64, _P, _P] + [_I64] * 4 + [_P]),
+    # 8-bit floating point
+    "mj_quantize_rows_f8": (_I32, [_I32, _P, _P, _P, _I64, _I64, _P]),
+    "mj_quantize_blocks_f8": (_I32, [_I32, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "mj_gemm_f8_work_bytes": (_I64, [_I64] * 3),
+    "mj_gemm_f8": (_I32, [_P] * 5 + [_I32, _P] + [_I64] * 3 + [_P, _I64, _P]),
+    "mj_linear_f8_work_bytes": (_I64, [_I64] * 3),
+    "mj_linear_f8": (_I32, [_I32] + [_P] * 4 + [_I32, _P] + [_I64] * 3 + [_P, _I64, _P]),
+    "mj_dispatch_f8": (_I32, [_I32] + [_P] * 3 + [_I64, _P, _P] + [_I64] * 3 + [_P]),
+    "mj_experts_gemm_f8": (_I32, [_P] * 3 + [_I64] + [_P] * 3 + [_I64] * 3 + [_P]),
+    "mj_experts_gate_f8_work_bytes": (_I64, [_I64] * 4),
+    "mj_experts_gate_f8": (_I32, [_P] * 3 + [_I64] + [_P] * 4 + [_I32, _P, _P] + [_I64] * 3 +
+                           [_P, _I64, _P]),
 }
 
 _lib = None

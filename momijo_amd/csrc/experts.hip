@@ -1,0 +1,424 @@
+// Tokens of a mixture of experts, sorted by expert and back.
+//
+// T tokens with k experts each are T k slots, slot t k + j.  The sort is a counting
+// sort, stable in the slots: pos[slot] is its row among the sorted ones, offsets[e] the
+// first row of expert e, and slots whose expert is outside [0, E) come last, from
+// offsets[E] on (dropped).  Then, token by token:
+//
+//   dispatch          xs[pos[t, j]] = x[t]                     (0 for a dropped slot)
+//   combine           y[t] = sum_j w[t, j] ys[pos[t, j]]       (dropped slots left out)
+//   combine backward  dys[pos[t, j]] = w[t, j] dy[t], dw[t, j] = <dy[t], ys[pos[t, j]]>
+//
+// and dispatch's gradient is combine without weights.  All of it is bound by memory:
+// going by tokens, each row of x and dy is read once and written k times, each row of ys
+// read once.  Sums run in fp32 in the order of j (dot products: in a fixed order), so
+// the same inputs give the same bits; there are no atomics.
+#include <algorithm>
+#include <atomic>
+
+#include "common.h"
+#include "launch.h"
+#include "philox.h"  // u32x4_a2
+
+namespace mj {
+
+namespace {
+
+// ---------------------------------------------------------------- sort
+// A workgroup of 16 waves sorts 1024 S consecutive slots, each wave 64 S of them, 64 at a
+// time: the lanes of one key find each other by a ballot for each bit of the key, so a
+// lane's place among its wave's earlier ones needs no atomics, and the order is that of
+// the slots.  Counts stay in LDS for each wave and key.
+//
+// Up to 8192 slots one workgroup does it all (a launch of its own for the counts costs
+// more than it gains there); beyond, the counts of every workgroup are written, summed
+// over the workgroups by one more launch and read again.
+enum : int { SORT_WHOLE = 0, SORT_COUNT, SORT_PLACE };
+
+struct SortArgs {
+  const void *ids = nullptr;
+  int wide = 0;           // ids are int64
+  int64_t slots = 0;
+  int experts = 0, bits = 0;
+  int *pos = nullptr, *offsets = nullptr, *work = nullptr;  // work [blocks + 1][experts + 1]
+  int64_t blocks = 1;
+};
+
+constexpr int kSortWaves = 16;
+
+template <int S, int MODE>
+__global__ __launch_bounds__(1024) void sort_kernel(SortArgs a) {
+  extern __shared__ int lds[];
+  const int E1 = a.experts + 1;
+  int *base = lds, *wsum = lds + E1;
+  volatile uint16_t *hist = (volatile uint16_t *)(wsum + kSortWaves);  // [waves][E1]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t first = (int64_t)blockIdx.x * (1024 * S) + wave * (64 * S) + lane;
+  int key[S], place[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int64_t slot = first + s * 64;
+    int64_t id = -1;
+    if (slot < a.slots) id = a.wide ? ((const int64_t *)a.ids)[slot] : ((const int *)a.ids)[slot];
+    key[s] = id >= 0 && id < a.experts ? (int)id : a.experts;
+  }
+  for (int i = tid; i < kSortWaves * E1; i += 1024) hist[i] = 0;
+  __syncthreads();
+  volatile uint16_t *mine = hist + wave * E1;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const bool in = first + s * 64 < a.slots;
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < a.bits; ++b) {
+      const bool bit = (key[s] >> b) & 1;
+      const uint64_t set = __ballot(bit);
+      same &= bit ? set : ~set;
+    }
+    const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
+    const int before = mine[key[s]];  // read by every lane before its first lane adds to it
+    place[s] = before + rank;
+    __builtin_amdgcn_wave_barrier();
+    if (in && rank == 0) mine[key[s]] = (uint16_t)(before + __popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  // counts -> places within the workgroup; totals of the keys
+  for (int e = tid; e < E1; e += 1024) {
+    int run = 0;
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = hist[w * E1 + e];
+      hist[w * E1 + e] = (uint16_t)run;
+      run += c;
+    }
+    base[e] = run;
+    if (MODE == SORT_COUNT) a.work[(int64_t)blockIdx.x * E1 + e] = run;
+  }
+  if constexpr (MODE == SORT_COUNT) return;
+  __syncthreads();
+  // offsets: an exclusive scan of the keys' totals (one thread each, experts <= 1024)
+  const int *total = MODE == SORT_PLACE ? a.work + a.blocks * E1 : base;
+  const int v = tid < a.experts ? total[tid] : 0;
+  int sum = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(sum, d, 64);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 63) wsum[wave] = sum;
+  __syncthreads();
+  int lower = 0, all = 0;
+  for (int w = 0; w < kSortWaves; ++w) {
+    if (w < wave) lower += wsum[w];
+    all += wsum[w];
+  }
+  const int64_t row = (int64_t)blockIdx.x * E1;
+  if (tid < a.experts) {
+    const int off = lower + sum - v;
+    base[tid] = off + (MODE == SORT_PLACE ? a.work[row + tid] : 0);
+    if (blockIdx.x == 0) a.offsets[tid] = off;
+  }
+  if (tid == 0) {
+    base[a.experts] = all + (MODE == SORT_PLACE ? a.work[row + a.experts] : 0);
+    if (blockIdx.x == 0) a.offsets[a.experts] = all;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (first + s * 64 < a.slots) a.pos[first + s * 64] = base[key[s]] + mine[key[s]] + place[s];
+}
+
+// For each key the counts of the workgroups become sums over the earlier ones; their total
+// goes behind.  One workgroup a key.
+__global__ __launch_bounds__(256) void sort_sums_kernel(int *work, int64_t blocks, int E1) {
+  __shared__ int wsum[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x;
+  int carry = 0;
+  for (int64_t b0 = 0; b0 < blocks; b0 += 256) {
+    const int64_t b = b0 + threadIdx.x;
+    const int v = b < blocks ? work[b * E1 + e] : 0;
+    int sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 63) wsum[wave] = sum;
+    __syncthreads();
+    int lower = carry;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) lower += wsum[w];
+      carry += wsum[w];
+    }
+    if (b < blocks) work[b * E1 + e] = lower + sum - v;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) work[blocks * E1 + e] = carry;
+}
+
+// ---------------------------------------------------------------- rows
+// 16 bytes of a row a thread, at the elements' own alignment; `have` of its elements are
+// inside the row.
+template <bool BF>
+struct Unit {
+  static constexpr int N = BF ? 8 : 4;
+  static constexpr int SIZE = BF ? 2 : 4;
+  u32x4_a2 w;
+  __device__ __forceinline__ void load(const void *row, int64_t e, int have) {
+    const char *p = (const char *)row + e * SIZE;
+    if (have >= N) {
+      w = *(const u32x4_a2 *)p;
+    } else {
+      w = u32x4_a2{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < have) {
+          if constexpr (BF) w[i >> 1] |= (uint32_t)((const uint16_t *)p)[i] << (16 * (i & 1));
+          else w[i] = ((const uint32_t *)p)[i];
+        }
+    }
+  }
+  __device__ __forceinline__ void store(void *row, int64_t e, int have) const {
+    char *p = (char *)row + e * SIZE;
+    if (have >= N) {
+      *(u32x4_a2 *)p = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < have) {
+          if constexpr (BF) ((uint16_t *)p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+          else ((uint32_t *)p)[i] = w[i];
+        }
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (BF) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    else return __uint_as_float(w[i]);
+  }
+  __device__ __forceinline__ void set(const float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (BF) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+      else w[i] = __float_as_uint(v[i]);
+    }
+  }
+};
+
+// The token and the unit of a row that a thread handles; false past the last token.
+__device__ __forceinline__ bool unit_of(int64_t i, int64_t units, int64_t tokens, int64_t &t, int64_t &u) {
+  if (i < ((int64_t)1 << 32)) {  // (a division in 32 bits)
+    t = (uint32_t)i / (uint32_t)units;
+  } else {
+    t = i / units;
+  }
+  u = i - t * units;
+  return t < tokens;
+}
+
+template <bool BF>
+__global__ __launch_bounds__(256) void dispatch_kernel(ExpertRows a) {
+  using U = Unit<BF>;
+  int64_t t, u;
+  if (!unit_of(grid_block<256>() * 256 + threadIdx.x, a.units, a.tokens, t, u)) return;
+  const int64_t e = u * U::N;
+  const int have = (int)std::min<int64_t>(a.dim - e, U::N), kept = *a.kept, k = (int)a.topk;
+  U x, zero;
+  x.load((const char *)a.x + t * a.dim * U::SIZE, e, have);
+  zero.w = u32x4_a2{0, 0, 0, 0};
+  const int *pos = a.pos + t * k;
+#pragma unroll 4
+  for (int j = 0; j < k; ++j) {
+    const int p = pos[j];
+    char *row = (char *)a.xs + (int64_t)p * a.dim * U::SIZE;
+    if (p < kept) x.store(row, e, have);
+    else zero.store(row, e, have);
+    if (a.ws && u == 0) a.ws[p] = p < kept ? a.w[t * k + j] : 0.0f;
+  }
+}
+
+// BI, BO: the rows' and the sum's type; a thread's 16 bytes of the sum are one or two units
+// of a row.
+template <bool BI, bool BO>
+__global__ __launch_bounds__(256) void combine_kernel(ExpertRows a) {
+  using UI = Unit<BI>;
+  using UO = Unit<BO>;
+  constexpr int N = UO::N, P = N / UI::N;
+  int64_t t, u;
+  if (!unit_of(grid_block<256>() * 256 + threadIdx.x, a.units, a.tokens, t, u)) return;
+  const int64_t e = u * N;
+  const int have = (int)std::min<int64_t>(a.dim - e, N), kept = *a.kept, k = (int)a.topk;
+  const int *pos = a.pos + t * k;
+  float acc[N] = {};
+  auto load = [&](UI (&v)[P], int p) __attribute__((always_inline)) {
+    const char *row = (const char *)a.xs + (int64_t)p * a.dim * UI::SIZE;
+#pragma unroll
+    for (int q = 0; q < P; ++q) v[q].load(row, e + q * UI::N, have - q * UI::N);
+  };
+  auto add = [&](const UI (&v)[P], int j) __attribute__((always_inline)) {
+    const float w = a.w ? a.w[t * k + j] : 1.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = __builtin_fmaf(w, v[i / UI::N].get(i % UI::N), acc[i]);
+  };
+  int j = 0;
+  for (; j + 4 <= k; j += 4) {  // four rows' loads in flight
+    UI v[4][P];
+    int p[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) p[q] = pos[j + q];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (p[q] < kept) load(v[q], p[q]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (p[q] < kept) add(v[q], j + q);
+  }
+  for (; j < k; ++j) {
+    const int p = pos[j];
+    if (p >= kept) continue;
+    UI v[P];
+    load(v, p);
+    add(v, j);
+  }
+  UO y;
+  y.set(acc);
+  y.store((char *)a.x + t * a.dim * UO::SIZE, e, have);
+}
+
+// One workgroup a token (one wave where a row is short): for each slot the row of dys and
+// the product of dy with the row of ys, its lanes' and waves' sums added in order.
+constexpr int kDotSlots = 16;  // slots whose sums wait in LDS
+
+template <bool BF, int NW>
+__global__ __launch_bounds__(NW * 64) void combine_bwd_kernel(ExpertRows a) {
+  using U = Unit<BF>;
+  __shared__ float red[kDotSlots][NW];
+  const int64_t t = grid_block<NW * 64>();
+  if (t >= a.tokens) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kept = *a.kept, k = (int)a.topk;
+  const char *dy = (const char *)a.x + t * a.dim * U::SIZE;
+  for (int j0 = 0; j0 < k; j0 += kDotSlots) {
+    const int n = std::min(k - j0, kDotSlots);
+    for (int j = 0; j < n; ++j) {
+      const int p = a.pos[t * k + j0 + j];
+      const bool in = p < kept;
+      const float w = a.w[t * k + j0 + j];
+      const int64_t row = (int64_t)p * a.dim * U::SIZE;
+      float sum = 0.0f;
+      for (int64_t e = (int64_t)threadIdx.x * U::N; e < a.dim; e += NW * 64 * U::N) {
+        const int have = (int)std::min<int64_t>(a.dim - e, U::N);
+        U d, y, o;
+        float v[U::N];
+        d.load(dy, e, have);
+        if (in) {
+          y.load((const char *)a.ys + row, e, have);
+#pragma unroll
+          for (int i = 0; i < U::N; ++i) sum = __builtin_fmaf(d.get(i), y.get(i), sum);
+        }
+#pragma unroll
+        for (int i = 0; i < U::N; ++i) v[i] = in ? w * d.get(i) : 0.0f;
+        o.set(v);
+        if (a.xs) o.store((char *)a.xs + row, e, have);
+      }
+      sum = wave_sum_dpp(sum);
+      if (lane == 0) red[j][wave] = sum;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+      float sum = red[threadIdx.x][0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) sum += red[threadIdx.x][w];
+      a.ws[t * k + j0 + threadIdx.x] = sum;
+    }
+    __syncthreads();
+  }
+}
+
+template <int S>
+hipError_t launch_sort(const SortArgs &a, size_t lds, hipStream_t stream) {
+  if (a.blocks == 1) {
+    hipLaunchKernelGGL((sort_kernel<S, SORT_WHOLE>), dim3(1), dim3(1024), lds, stream, a);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((sort_kernel<S, SORT_COUNT>), dim3((unsigned)a.blocks), dim3(1024), lds, stream, a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  hipLaunchKernelGGL(sort_sums_kernel, dim3((unsigned)(a.experts + 1)), dim3(256), 0, stream, a.work,
+                     a.blocks, a.experts + 1);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  hipLaunchKernelGGL((sort_kernel<S, SORT_PLACE>), dim3((unsigned)a.blocks), dim3(1024), lds, stream, a);
+  return hipGetLastError();
+}
+
+// Slots of a workgroup: few steps where one does them all, else 4096.
+int64_t sort_steps(int64_t slots) { return slots <= 1024 ? 1 : slots <= 4096 ? 4 : slots <= 8192 ? 8 : 4; }
+
+int64_t sort_blocks(int64_t slots) {
+  const int64_t per = 1024 * sort_steps(slots);
+  return (slots + per - 1) / per;
+}
+
+// 16-byte units of a row; one for an empty row (its token's weights are sorted all the same).
+template <bool BF>
+int64_t units_of(int64_t dim) {
+  return std::max<int64_t>((dim + Unit<BF>::N - 1) / Unit<BF>::N, 1);
+}
+
+}  // namespace
+
+int64_t sort_experts_work_ints(int64_t slots, int64_t experts) {
+  const int64_t b = sort_blocks(slots);
+  return b > 1 ? (b + 1) * (experts + 1) : 0;
+}
+
+hipError_t launch_sort_experts(const void *ids, bool wide, int64_t slots, int64_t experts, int *pos,
+                               int *offsets, int *work, hipStream_t stream) {
+  SortArgs a;
+  a.ids = ids, a.wide = wide, a.slots = slots, a.experts = (int)experts;
+  while ((1 << a.bits) < experts + 1) ++a.bits;
+  a.pos = pos, a.offsets = offsets, a.work = work;
+  a.blocks = std::max<int64_t>(sort_blocks(slots), 1);  // (no slots: the offsets are zeros)
+  const size_t lds = (size_t)(experts + 1 + kSortWaves) * 4 + (size_t)kSortWaves * (experts + 1) * 2;
+  switch (sort_steps(slots)) {
+    case 1: return launch_sort<1>(a, lds, stream);
+    case 4: return launch_sort<4>(a, lds, stream);
+    default: return launch_sort<8>(a, lds, stream);
+  }
+}
+
+hipError_t launch_dispatch(bool bf16, ExpertRows a, hipStream_t stream) {
+  a.units = bf16 ? units_of<true>(a.dim) : units_of<false>(a.dim);
+  const int64_t n = a.tokens * a.units;
+  if (n == 0 || a.topk == 0) return hipSuccess;
+  const dim3 grid = grid_rows<256>((n + 255) / 256);
+  if (bf16) hipLaunchKernelGGL(dispatch_kernel<true>, grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL(dispatch_kernel<false>, grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_combine(bool bf16, bool y_bf16, ExpertRows a, hipStream_t stream) {
+  a.units = y_bf16 ? units_of<true>(a.dim) : units_of<false>(a.dim);
+  const int64_t n = a.tokens * a.units;
+  if (n == 0) return hipSuccess;
+  const dim3 grid = grid_rows<256>((n + 255) / 256);
+  if (bf16) hipLaunchKernelGGL((combine_kernel<true, true>), grid, dim3(256), 0, stream, a);
+  else if (y_bf16) hipLaunchKernelGGL((combine_kernel<false, true>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((combine_kernel<false, false>), grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_combine_bwd(bool bf16, const ExpertRows &a, hipStream_t stream) {
+  if (a.tokens == 0 || a.topk == 0) return hipSuccess;
+  const bool one = (bf16 ? units_of<true>(a.dim) : units_of<false>(a.dim)) <= 64;
+  const dim3 grid = one ? grid_rows<64>(a.tokens) : grid_rows<256>(a.tokens);
+#define MJ_BWD(BF, NW) \
+  hipLaunchKernelGGL((combine_bwd_kernel<BF, NW>), grid, dim3(NW * 64), 0, stream, a)
+  if (bf16) {
+    if (one) MJ_BWD(true, 1);
+    else MJ_BWD(true, 4);
+  } else {
+    if (one) MJ_BWD(false, 1);
+    else MJ_BWD(false, 4);
+  }
+#undef MJ_BWD
+  return hipGetLastError();
+}
+
+}  // namespace mj

@@ -1,0 +1,376 @@
+// The gated feed-forward block of a mixture of experts on gfx950 bf16 MFMA, forward and
+// backward, over rows sorted by expert (experts.hip).  Row r of expert e, with weight w_r:
+//
+//   g = x Wg_e^T, u = x Wu_e^T, h = w_r act(g) u, y = h Wd_e^T
+//   dh = dy Wd_e, dg = w_r dh u act'(g), du = w_r dh act(g), dw_r = <dh, act(g) u>
+//   dx = dg Wg_e + du Wu_e, dWg_e = dg^T x, dWu_e = du^T x, dWd_e = dy^T h
+//
+// The weight is applied to h and not to y, so that the layer's output is a plain sum of
+// rows, the backward needs no y (dw comes from the fp32 g and u, with the error of an fp32
+// sum and not of a rounded y), and dy's rows are copies of the tokens' gradients.  y and dx
+// stay in fp32: a token's rows are still to be added, and rounded once then.
+//
+// The tiles are the gated block's (mlp_tile.h).  What differs is where a tile's operands
+// are: the rows of all experts run as one launch, each workgroup finding its expert from
+// the offsets (expert_tile.h).  The weight gradients' K is the expert's rows, so their grid
+// is known; an expert without rows gets zeros.  With few rows an expert the weights' reading
+// bounds, and the few-row kernel takes the segments of 16 rows.
+#include <algorithm>
+#include <atomic>
+
+#include "expert_tile.h"
+#include "launch.h"
+#include "mlp_tile.h"
+
+namespace mj {
+
+namespace {
+
+struct ExpertArgs {
+  TileProb p[3];
+  int64_t b_expert = 0;       // elements of an expert's B matrix (row products)
+  int64_t c_expert[3] = {};   // .. of its gradient (weight gradients)
+  const int *offsets = nullptr;
+  int experts = 0, rows = 0, n = 1, tail = 0, act = 0;
+  int tiles_n = 0;            // row products
+  int tiles = 0;              // weight gradients: of one expert
+};
+
+// A product over the rows: the tile's expert and its operands.  SEGS: two K segments.
+template <int BM, int BN_OUT, int OUT, bool SEGS>
+__device__ __forceinline__ bool row_product(const ExpertArgs &a, TileProb &p, TileAt &at, ExpertTile &t) {
+  if (!expert_tile<true>(a.offsets, a.experts, a.rows, a.tail, BM, a.tiles_n, blockIdx.x, t)) return false;
+  const TileProb &q = a.p[0];
+  const int64_t row = (int64_t)t.row0 * q.lda;
+  const bool none = t.expert == a.experts;  // rows of no expert: zeros
+  const int64_t mat = none ? 0 : t.expert * a.b_expert;
+  p.A[0] = q.A[0] + row;
+  p.A[1] = SEGS ? q.A[1] + row : p.A[0];
+  p.B[0] = q.B[0] + mat;
+  p.B[1] = SEGS || OUT == OUT_GATE ? q.B[1] + mat : p.B[0];
+  p.lda = q.lda, p.ldb = q.ldb;
+  p.M = t.rows, p.N = q.N, p.K = none ? 0 : q.K, p.segs = SEGS ? 2 : 1;
+  at = {0, 0, t.m, t.n};
+  return true;
+}
+
+// Its outputs.
+template <int OUT>
+__device__ __forceinline__ TileProb row_outputs(const ExpertArgs &a, int row0, int rows) {
+  TileProb p = a.p[0];
+  const int64_t at = (int64_t)row0 * p.ldc;
+  p.M = rows;
+  if constexpr (OUT == OUT_PART) {
+    p.part += at;
+    return p;
+  }
+  p.C += at;
+  if constexpr (OUT == OUT_DGATE) {
+    p.C2 += at;
+    if (p.dots) p.dots += (int64_t)row0 * p.dots_ld;
+  }
+  if (p.F) p.F += at, p.F2 += at;
+  if (p.rw) p.rw += row0;
+  return p;
+}
+
+// A weight gradient: expert by expert, its matrices' tiles in turn.
+__device__ __forceinline__ void weight_product(const ExpertArgs &a, TileProb &p, TileAt &at, int &e) {
+  const int total = a.tiles * a.experts, x = blockIdx.x & 7, q = total >> 3, r = total & 7;
+  int logical = x * q + (x < r ? x : r) + ((int)blockIdx.x >> 3);
+  e = logical / a.tiles;
+  logical -= e * a.tiles;
+  at.prob = 0, at.split = 0;
+  if (a.n > 1 && logical >= a.p[1].first) at.prob = 1;
+  if (a.n > 2 && logical >= a.p[2].first) at.prob = 2;
+  const TileProb &s = a.p[at.prob];
+  const int row = a.offsets[e];
+  p.lda = s.lda, p.ldb = s.ldb;
+  p.A[0] = p.A[1] = s.A[0] + row * s.lda;
+  p.B[0] = p.B[1] = s.B[0] + row * s.ldb;
+  p.M = s.M, p.N = s.N, p.K = a.offsets[e + 1] - row, p.segs = 1;
+  group_coords(logical - s.first, s.tiles_m, s.tiles_n, 4, at.m, at.n);
+}
+
+__device__ __forceinline__ TileProb weight_outputs(const ExpertArgs &a, int prob, int e) {
+  TileProb p = a.p[prob];
+  p.C += e * a.c_expert[prob];
+  return p;
+}
+
+template <int BM, int BN, int S, bool AKC, bool BKC, int OUT>
+__global__ __launch_bounds__(256) void experts_ring_kernel(ExpertArgs args) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+  TileProb p;
+  TileAt at;
+  if constexpr (AKC) {
+    ExpertTile t;
+    if (!row_product<BM, OUT == OUT_GATE ? BN / 2 : BN, OUT, OUT == OUT_PART && !BKC>(args, p, at, t)) return;
+    ring_tile<BM, BN, S, AKC, BKC, OUT, true>(lds, p, at, 1, args.act,
+                                              [&]() { return row_outputs<OUT>(args, t.row0, t.rows); });
+  } else {
+    int e;
+    weight_product(args, p, at, e);
+    ring_tile<BM, BN, S, AKC, BKC, OUT, true>(lds, p, at, 1, args.act,
+                                              [&]() { return weight_outputs(args, at.prob, e); });
+  }
+}
+
+template <int BM, int NW, bool AKC, bool BKC, int OUT>
+__global__ __launch_bounds__(NW * 64, 2) void experts_tile_kernel(ExpertArgs args) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+  TileProb p;
+  TileAt at;
+  if constexpr (AKC) {
+    ExpertTile t;
+    if (!row_product<BM, OUT == OUT_GATE ? BM / 2 : BM, OUT, OUT == OUT_PART && !BKC>(args, p, at, t)) return;
+    pipe_tile<BM, NW, AKC, BKC, OUT, true>(lds, p, at, 1, args.act,
+                                           [&]() { return row_outputs<OUT>(args, t.row0, t.rows); });
+  } else {
+    int e;
+    weight_product(args, p, at, e);
+    pipe_tile<BM, NW, AKC, BKC, OUT, true>(lds, p, at, 1, args.act,
+                                           [&]() { return weight_outputs(args, at.prob, e); });
+  }
+}
+
+// Few rows an expert: 16 MB of them and 16 weight rows a workgroup.
+struct ExpertSkinny {
+  SkinnyArgs p;
+  const int *offsets = nullptr;
+  int experts = 0, rows = 0, tail = 0, tiles_n = 0;
+};
+
+template <bool GATE, int MB, int NW>
+__global__ __launch_bounds__(NW * 64) void experts_skinny_kernel(ExpertSkinny a) {
+  __shared__ SkinnySums<GATE, MB, NW> sums;
+  ExpertTile t;
+  if (!expert_tile<false>(a.offsets, a.experts, a.rows, a.tail, 16 * MB, a.tiles_n, blockIdx.x, t)) return;
+  SkinnyArgs p = a.p;
+  const int64_t row = t.row0 + t.m * 16 * MB, weights = (int64_t)p.N * p.K;
+  p.M = t.rows - t.m * 16 * MB;
+  p.x += row * p.K;
+  if (GATE) p.C += row * p.N;
+  if (p.F) p.F += row * p.N;
+  if (GATE && p.F2) p.F2 += row * p.N;
+  if (p.rw) p.rw += row;
+  if (t.expert < a.experts) {
+    p.w += t.expert * weights;
+    if (GATE) p.w2 += t.expert * weights;
+  } else {
+    p.K = 0;
+  }
+  skinny_rows<GATE, MB, NW, true>(sums, p, t.n * 16);
+}
+
+// dw of a slot: its row's parts, one wave a slot, in a fixed order; 0 for a dropped slot.
+__global__ __launch_bounds__(256) void expert_dots_kernel(const int *pos, const int *kept,
+                                                          const float *dots, int ld, float *dw,
+                                                          int64_t slots) {
+  const int64_t slot = grid_block<256>() * 4 + (threadIdx.x >> 6);
+  if (slot >= slots) return;
+  const int lane = threadIdx.x & 63, p = pos[slot];
+  float sum = 0.0f;
+  if (p < *kept)
+    for (int c = lane; c < ld; c += 64) sum += dots[(int64_t)p * ld + c];
+  sum = wave_sum_dpp(sum);
+  if (lane == 0) dw[slot] = sum;
+}
+
+// ---------------------------------------------------------------- launch
+template <int BM, int BN, int S, bool AKC, bool BKC, int OUT>
+hipError_t launch_ring(const ExpertArgs &a, int64_t grid, hipStream_t stream) {
+  constexpr size_t lds = size_t(S) * (BM + BN) * kBK * sizeof(uint16_t);
+  auto kern = experts_ring_kernel<BM, BN, S, AKC, BKC, OUT>;
+  static std::atomic<uint64_t> done{0};
+  if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
+  if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, a);
+  return hipGetLastError();
+}
+
+template <int BM, int NW, bool AKC, bool BKC, int OUT>
+hipError_t launch_pipe(const ExpertArgs &a, int64_t grid, hipStream_t stream) {
+  constexpr size_t lds = size_t(5 * BM) * kBK * sizeof(uint16_t);
+  auto kern = experts_tile_kernel<BM, NW, AKC, BKC, OUT>;
+  static std::atomic<uint64_t> done{0};
+  if (hipError_t e = raise_lds((const void *)kern, lds, done); e != hipSuccess) return e;
+  if (!grid_fits(grid, NW * 64)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(NW * 64), lds, stream, a);
+  return hipGetLastError();
+}
+
+template <bool AKC, bool BKC, int OUT>
+hipError_t launch_kernel(int tile, const ExpertArgs &a, int64_t grid, hipStream_t stream) {
+  if (grid == 0) return hipSuccess;
+  switch (tile) {
+    case T_256: return launch_pipe<256, 8, AKC, BKC, OUT>(a, grid, stream);
+    case T_128: return launch_pipe<128, 4, AKC, BKC, OUT>(a, grid, stream);
+    case T_64S3: return launch_ring<64, 64, 3, AKC, BKC, OUT>(a, grid, stream);
+    case T_64S5: return launch_ring<64, 64, 5, AKC, BKC, OUT>(a, grid, stream);
+    default: return launch_ring<128, 64, 3, AKC, BKC, OUT>(a, grid, stream);
+  }
+}
+
+// The experts that the rows reach, at most; the rows are taken to be spread evenly over
+// them, and each to leave half a tile empty.
+int64_t busy_experts(const ExpertMlp &q) { return std::min(q.R, q.E); }
+
+int64_t even_tiles(const ExpertMlp &q, int64_t bm) {
+  const int64_t b = busy_experts(q), per = (q.R + b - 1) / b;
+  return per <= bm ? b : q.R / bm + (b + 1) / 2;
+}
+
+int plan_rows(const ExpertMlp &q, int64_t N, int64_t stages, int out) {
+  int best = T_64S3;
+  double best_us = 1e30;
+  for (int t = 0; t < T_COUNT; ++t) {
+    const TileCost &c = kTileCost[t];
+    const int64_t bn = out == OUT_GATE ? c.bn / 2 : c.bn, tn = (N + bn - 1) / bn;
+    if (!grid_fits(tn * expert_tiles_most(q.R, q.E + 1, c.bm), c.threads)) continue;
+    const double us = tile_time_us(c, out, tn * even_tiles(q, c.bm), stages);
+    if (us < best_us) best_us = us, best = t;
+  }
+  return best;
+}
+
+template <bool BKC, int OUT>
+hipError_t launch_rows(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream) {
+  TileProb &p = a.p[0];
+  if (q.R == 0 || p.N == 0) return hipSuccess;
+  const int64_t stages = (int64_t)((p.K + kBK - 1) / kBK) * p.segs;
+  const int tile = plan_rows(q, p.N, stages, OUT);
+  const int64_t bm = kTileCost[tile].bm, bn = OUT == OUT_GATE ? kTileCost[tile].bn / 2 : kTileCost[tile].bn;
+  a.offsets = q.offsets, a.experts = (int)q.E, a.rows = (int)q.R, a.act = q.act;
+  a.tiles_n = (int)((p.N + bn - 1) / bn);
+  return launch_kernel<true, BKC, OUT>(tile, a, a.tiles_n * expert_tiles_most(q.R, q.E + a.tail, bm), stream);
+}
+
+hipError_t launch_weights(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream) {
+  if (a.n == 0) return hipSuccess;
+  const int64_t per = q.R / q.E, stages = std::max<int64_t>((per + kBK - 1) / kBK, 1);
+  auto tiles_of = [&](const TileCost &c) {
+    int64_t t = 0;
+    for (int i = 0; i < a.n; ++i)
+      t += (int64_t)((a.p[i].M + c.bm - 1) / c.bm) * ((a.p[i].N + c.bn - 1) / c.bn);
+    return t;
+  };
+  int tile = T_64S3;
+  double best_us = 1e30;
+  for (int t = 0; t < T_COUNT; ++t) {
+    const int64_t wgs = tiles_of(kTileCost[t]) * q.E;
+    if (!grid_fits(wgs, kTileCost[t].threads)) continue;
+    const double us = tile_time_us(kTileCost[t], OUT_STORE, wgs, stages);
+    if (us < best_us) best_us = us, tile = t;
+  }
+  const TileCost &c = kTileCost[tile];
+  for (int i = 0; i < a.n; ++i) {
+    TileProb &p = a.p[i];
+    p.tiles_m = (p.M + c.bm - 1) / c.bm;
+    p.tiles_n = (p.N + c.bn - 1) / c.bn;
+    p.first = a.tiles;
+    a.tiles += p.tiles_m * p.tiles_n;
+  }
+  a.offsets = q.offsets, a.experts = (int)q.E;
+  return launch_kernel<false, false, OUT_STORE>(tile, a, (int64_t)a.tiles * q.E, stream);
+}
+
+// Rows of one expert, if they are even, up to which the few-row kernel is taken.
+bool few_rows(const ExpertMlp &q) { return q.R <= 16 * busy_experts(q); }
+
+template <bool GATE>
+hipError_t launch_few(const ExpertMlp &q, ExpertSkinny &a, hipStream_t stream) {
+  a.offsets = q.offsets, a.experts = (int)q.E, a.rows = (int)q.R;
+  a.tiles_n = (a.p.N + 15) / 16;
+  const int64_t grid = a.tiles_n * expert_tiles_most(q.R, q.E + a.tail, 16);
+  if (grid == 0) return hipSuccess;
+  if (!grid_fits(grid, 512)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((experts_skinny_kernel<GATE, 1, 8>), dim3((unsigned)grid), dim3(512), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t expert_dots_ld(const ExpertMlp &q) {
+  if (q.R == 0 || q.I == 0) return 0;
+  const TileCost &c = kTileCost[plan_rows(q, q.I, (q.H + kBK - 1) / kBK, OUT_DGATE)];
+  const int64_t wn = c.bn == 256 ? 64 : c.bn / 2;  // columns of a wave
+  return (q.I + c.bn - 1) / c.bn * (c.bn / wn);
+}
+
+hipError_t launch_experts_mlp(const ExpertMlp &q, hipStream_t stream) {
+  if (q.R == 0) return hipSuccess;
+  if (few_rows(q)) {
+    ExpertSkinny a;
+    a.p.x = q.xs, a.p.w = q.wg, a.p.w2 = q.wu, a.p.C = q.h, a.p.F = q.g, a.p.F2 = q.u, a.p.rw = q.rw;
+    a.p.N = (int)q.I, a.p.K = (int)q.K, a.p.act = q.act;
+    if (hipError_t e = launch_few<true>(q, a, stream); e != hipSuccess) return e;
+    ExpertSkinny d;
+    d.p.x = q.h, d.p.w = q.wd, d.p.F = q.ys;
+    d.p.N = (int)q.H, d.p.K = (int)q.I, d.tail = 1;
+    return launch_few<false>(q, d, stream);
+  }
+  ExpertArgs a;
+  TileProb &p = a.p[0];
+  p.A[0] = p.A[1] = q.xs, p.lda = q.K;
+  p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
+  p.N = (int)q.I, p.K = (int)q.K;
+  p.C = q.h, p.F = q.g, p.F2 = q.u, p.ldc = q.I, p.rw = q.rw;
+  a.b_expert = q.I * q.K;
+  if (hipError_t e = launch_rows<true, OUT_GATE>(q, a, stream); e != hipSuccess) return e;
+  ExpertArgs d;
+  TileProb &y = d.p[0];
+  y.A[0] = y.A[1] = q.h, y.lda = q.I;
+  y.B[0] = y.B[1] = q.wd, y.ldb = q.I;
+  y.N = (int)q.H, y.K = (int)q.I;
+  y.part = q.ys, y.ldc = q.H;
+  d.b_expert = q.H * q.I, d.tail = 1;
+  return launch_rows<true, OUT_PART>(q, d, stream);
+}
+
+hipError_t launch_experts_mlp_bwd(const ExpertMlp &q, const ExpertMlpGrad &o, hipStream_t stream) {
+  if (o.dxs || o.dwg || o.dwu || o.dw) {
+    ExpertArgs a;
+    TileProb &p = a.p[0];
+    p.A[0] = p.A[1] = o.dys, p.lda = q.H;
+    p.B[0] = p.B[1] = q.wd, p.ldb = q.I;
+    p.N = (int)q.I, p.K = (int)q.H;
+    p.C = o.dg, p.C2 = o.du, p.F = q.g, p.F2 = q.u, p.ldc = q.I, p.rw = q.rw;
+    p.dots = o.dots, p.dots_ld = (int)expert_dots_ld(q);
+    a.b_expert = q.H * q.I;
+    if (hipError_t e = launch_rows<false, OUT_DGATE>(q, a, stream); e != hipSuccess) return e;
+  }
+  if (o.dw && o.slots > 0) {
+    const dim3 grid = grid_rows<256>((o.slots + 3) / 4);
+    hipLaunchKernelGGL(expert_dots_kernel, grid, dim3(256), 0, stream, o.pos, q.offsets + q.E, o.dots,
+                       (int)expert_dots_ld(q), o.dw, o.slots);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  if (o.dxs) {
+    ExpertArgs a;
+    TileProb &p = a.p[0];
+    p.A[0] = o.dg, p.A[1] = o.du, p.lda = q.I;
+    p.B[0] = q.wg, p.B[1] = q.wu, p.ldb = q.K;
+    p.N = (int)q.K, p.K = (int)q.I, p.segs = 2;
+    p.part = o.dxs, p.ldc = q.K;
+    a.b_expert = q.I * q.K, a.tail = 1;
+    if (hipError_t e = launch_rows<false, OUT_PART>(q, a, stream); e != hipSuccess) return e;
+  }
+  ExpertArgs w;
+  w.n = 0;
+  auto add = [&](const uint16_t *A, int64_t rows, const uint16_t *B, int64_t cols, uint16_t *C) {
+    if (!C || rows == 0 || cols == 0) return;
+    w.c_expert[w.n] = rows * cols;
+    TileProb &p = w.p[w.n++];
+    p.A[0] = p.A[1] = A, p.lda = rows;
+    p.B[0] = p.B[1] = B, p.ldb = cols;
+    p.M = (int)rows, p.N = (int)cols;
+    p.C = C, p.ldc = cols;
+  };
+  add(o.dg, q.I, q.xs, q.K, o.dwg);
+  add(o.du, q.I, q.xs, q.K, o.dwu);
+  add(o.dys, q.H, q.h, q.I, o.dwd);
+  return launch_weights(q, w, stream);
+}
+
+}  // namespace mj

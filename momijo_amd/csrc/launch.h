@@ -363,4 +363,90 @@ hipError_t launch_sum_f32(const float *part, float *out, int64_t n, int64_t part
 hipError_t launch_gate_bwd_f32(int act, const float *g, const float *u, const float *dh, float *dg,
                                float *du, int64_t n, hipStream_t stream);
 
+// ---- experts.hip -----------------------------------------------------------
+// Tokens with topk experts each, and their rows sorted by expert.
+constexpr int64_t kMaxExperts = 1024;
+int64_t sort_experts_work_ints(int64_t slots, int64_t experts);
+// ids: int32, or int64 (wide); pos [slots], offsets [experts + 1].
+hipError_t launch_sort_experts(const void *ids, bool wide, int64_t slots, int64_t experts, int *pos,
+                               int *offsets, int *work, hipStream_t stream);
+struct ExpertRows {
+  const int *pos = nullptr, *kept = nullptr;  // [tokens, topk]; rows from *kept on are dropped
+  int64_t tokens = 0, topk = 0, dim = 0;
+  int64_t units = 0;         // set by the launch: 16-byte units of a row
+  void *x = nullptr;         // [tokens, dim]: read, or what combine writes
+  void *xs = nullptr;        // [tokens topk, dim] sorted: written, or what combine reads
+  const void *ys = nullptr;  // combine backward: the forward's sorted rows
+  const float *w = nullptr;  // [tokens, topk], or null for ones (combine)
+  float *ws = nullptr;       // dispatch: the sorted weights, or null; combine backward: dw
+};
+hipError_t launch_dispatch(bool bf16, ExpertRows a, hipStream_t stream);
+// bf16 sums from fp32 or bf16 rows, or fp32 from fp32
+hipError_t launch_combine(bool bf16, bool y_bf16, ExpertRows a, hipStream_t stream);
+hipError_t launch_combine_bwd(bool bf16, const ExpertRows &a, hipStream_t stream);
+
+// ---- experts_mlp.hip -------------------------------------------------------
+// bf16 rows [R, K] sorted by expert -> [R, H] through the expert's I gated features; K, I,
+// H multiples of 8, 16-byte aligned arrays, the experts' matrices one behind the other.
+struct ExpertMlp {
+  const uint16_t *xs = nullptr, *wg = nullptr, *wu = nullptr, *wd = nullptr;
+  const int *offsets = nullptr;          // [E + 1]
+  const float *rw = nullptr;             // [R] weights of h's rows, or null for ones
+  int act = 0;
+  uint16_t *h = nullptr;                 // [R, I]
+  float *g = nullptr, *u = nullptr;      // [R, I] fp32 projections kept for the backward, or null
+  float *ys = nullptr;                   // [R, H]; rows from offsets[E] on are zeros
+  int64_t R = 0, E = 0, K = 0, I = 0, H = 0;
+};
+struct ExpertMlpGrad {
+  const uint16_t *dys = nullptr;
+  uint16_t *dg = nullptr, *du = nullptr;   // [R, I] scratch
+  float *dxs = nullptr;                    // (these may each be null)
+  uint16_t *dwg = nullptr, *dwu = nullptr, *dwd = nullptr;
+  float *dots = nullptr, *dw = nullptr;    // scratch [R, expert_dots_ld], dw [slots]; or null
+  const int *pos = nullptr;                // [slots]
+  int64_t slots = 0;
+};
+int64_t expert_dots_ld(const ExpertMlp &q);
+hipError_t launch_experts_mlp(const ExpertMlp &q, hipStream_t stream);
+hipError_t launch_experts_mlp_bwd(const ExpertMlp &q, const ExpertMlpGrad &o, hipStream_t stream);
+
+// ---- fp8.hip ---------------------------------------------------------------
+// x [tokens, dim] -> q [rows, dim], scales [ceil(dim / 128), rows]; with pos each token's
+// row goes to its topk sorted rows.  dim % 16 == 0, 16-byte aligned arrays.
+struct F8Rows {
+  const void *x = nullptr;
+  uint8_t *q = nullptr;
+  float *scales = nullptr;
+  int64_t tokens = 0, dim = 0, rows = 0, topk = 0;
+  const int *pos = nullptr, *kept = nullptr;
+};
+hipError_t launch_quantize_rows_f8(bool bf16, const F8Rows &a, hipStream_t stream);
+// w [mats, n, k] -> q, scales [mats, ceil(n / 128), ceil(k / 128)]
+struct F8Blocks {
+  const void *w = nullptr;
+  uint8_t *q = nullptr;
+  float *scales = nullptr;
+  int64_t mats = 0, n = 0, k = 0;
+};
+hipError_t launch_quantize_blocks_f8(bool bf16, const F8Blocks &a, hipStream_t stream);
+
+// ---- gemm_f8.hip -----------------------------------------------------------
+// y [M, N] = bf16(epi(x W^T + bias)) from e4m3 x [M, K], W [N, K] and their scales sx
+// [ceil(K / 128), M], sw [ceil(N / 128), ceil(K / 128)].  With offsets: rows sorted by expert
+// and a matrix each, one behind the other; h = x W^T, or with w2 act(x W^T) (x W2^T), in fp32.
+// K % 16 == 0 (h: N too), 16-byte aligned arrays.
+struct F8Product {
+  const uint8_t *x = nullptr, *w = nullptr, *w2 = nullptr;
+  const float *sx = nullptr, *sw = nullptr, *sw2 = nullptr, *bias = nullptr;
+  uint16_t *y = nullptr;
+  float *h = nullptr, *part = nullptr;   // part: gemm_f8_part_floats
+  const int *offsets = nullptr;          // [experts + 1], or null for one matrix
+  int experts = 0, epi = 0;
+  int tail = 0;                          // y's rows from offsets[experts] on become zeros
+  int64_t M = 0, N = 0, K = 0;
+};
+int64_t gemm_f8_part_floats(int64_t M, int64_t N, int64_t K);
+hipError_t launch_gemm_f8(const F8Product &q, hipStream_t stream);
+
 }  // namespace mj

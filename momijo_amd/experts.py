@@ -1,0 +1,306 @@
+"""Mixture of experts: tokens sorted by expert and back, and the experts' gated
+feed-forward blocks over the sorted rows, forward and backward.
+
+``sort_experts`` plans where each slot (token t, its j-th expert) goes;
+``dispatch`` copies the tokens' rows there, ``combine`` sums the experts' rows
+back with the tokens' weights, and each has its ``_backward``.  ``experts_mlp``
+is ``gated_mlp`` of every row's own expert, and ``ExpertsMLP`` the layer from
+tokens to tokens.  A slot whose expert is outside 0 .. E - 1 is dropped: it adds
+nothing to its token.  How many rows an expert has stays on the device: no call
+waits for it, and all can be captured into a HIP graph.
+
+Tensors are on the current device; operands of other strides are copied to
+contiguous ones first.  The kernels run on the current stream and allocate
+through torch only.
+"""
+from __future__ import annotations
+
+import functools
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .block import _DTYPES, _check_type, _like, _scratch, _up16
+from .tensor import _ptr, _stream
+
+
+class ExpertPlan(NamedTuple):
+    """Where the slots go.  pos int32 [tokens, topk]: a slot's row among those sorted by
+    expert (in the order of the slots within an expert, dropped slots last); offsets int32
+    [experts + 1]: the experts' first rows, the last entry the first dropped slot's."""
+    pos: torch.Tensor
+    offsets: torch.Tensor
+
+    @property
+    def experts(self) -> int:
+        return self.offsets.shape[0] - 1
+
+    @property
+    def rows(self) -> int:
+        return self.pos.numel()
+
+
+def _check_device(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on the GPU")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+
+
+def _check_plan(plan: ExpertPlan, device) -> None:
+    pos, offsets = plan
+    if pos.dim() != 2 or pos.dtype is not torch.int32 or offsets.dtype is not torch.int32 or \
+            offsets.dim() != 1 or pos.device != device or offsets.device != device or \
+            not pos.is_contiguous() or not offsets.is_contiguous():
+        raise ValueError(f"the plan must be sort_experts's, on {device}")
+
+
+def _contiguous(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t as a contiguous tensor at a multiple of 16 bytes, as the tile kernels read it."""
+    t = _contiguous(t)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _weights(w: torch.Tensor, plan: ExpertPlan, name: str) -> torch.Tensor:
+    if w.dtype is not torch.float32 or w.shape != plan.pos.shape or w.device != plan.pos.device:
+        raise ValueError(f"{name} must be float32 {list(plan.pos.shape)} on {plan.pos.device}, got "
+                         f"{w.dtype} {list(w.shape)} on {w.device}")
+    return _contiguous(w)
+
+
+@functools.lru_cache(maxsize=1024)
+def _sort_work(slots, experts):
+    return _lib.load().mj_sort_experts_work_bytes(slots, experts)
+
+
+def sort_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
+    """The plan for tokens whose experts are ``experts`` [tokens, topk], int32 or int64;
+    an entry outside 0 .. num_experts - 1 is a dropped slot."""
+    if experts.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"experts must be int32 or int64, got {experts.dtype}")
+    if experts.dim() != 2:
+        raise ValueError(f"experts must be [tokens, topk], got {list(experts.shape)}")
+    _check_device(experts, "experts")
+    ids, device = _contiguous(experts), experts.device
+    slots = ids.numel()
+    nbytes = _sort_work(slots, num_experts)
+    pos = torch.empty(ids.shape, dtype=torch.int32, device=device)
+    offsets = torch.empty(max(num_experts, 0) + 1, dtype=torch.int32, device=device)
+    work = _scratch(nbytes, device) if nbytes else None
+    _lib.call("mj_sort_experts", ids.data_ptr(), ids.element_size(), slots, num_experts,
+              pos.data_ptr(), offsets.data_ptr(), _ptr(work), nbytes, _stream())
+    return ExpertPlan(pos, offsets)
+
+
+def _token_rows(x: torch.Tensor, plan: ExpertPlan, name: str):
+    code = _check_type(x, name)
+    _check_device(x, name)
+    _check_plan(plan, x.device)
+    if x.dim() != 2 or x.shape[0] != plan.pos.shape[0]:
+        raise ValueError(f"{name} must be [{plan.pos.shape[0]}, dim], got {list(x.shape)}")
+    return code, _contiguous(x)
+
+
+def _sorted_rows(xs: torch.Tensor, plan: ExpertPlan, name: str):
+    code = _check_type(xs, name)
+    _check_device(xs, name)
+    _check_plan(plan, xs.device)
+    if xs.dim() != 2 or xs.shape[0] != plan.rows:
+        raise ValueError(f"{name} must be [{plan.rows}, dim], got {list(xs.shape)}")
+    return code, _contiguous(xs)
+
+
+def dispatch(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor | None = None):
+    """xs [tokens * topk, dim] with xs[pos[t, j]] = x[t], zeros for dropped slots; with
+    ``weights`` [tokens, topk] (Float32) also their sorted form: (xs, ws)."""
+    code, x = _token_rows(x, plan, "x")
+    (T, k), dim = plan.pos.shape, x.shape[1]
+    xs = x.new_empty((T * k, dim))
+    ws = None
+    if weights is not None:
+        weights = _weights(weights, plan, "weights")
+        ws = weights.new_empty(T * k)
+    _lib.call("mj_dispatch", code, x.data_ptr(), _ptr(weights), plan.pos.data_ptr(),
+              plan.offsets.data_ptr(), plan.experts, xs.data_ptr(), _ptr(ws), T, k, dim, _stream())
+    return xs if weights is None else (xs, ws)
+
+
+def combine(ys: torch.Tensor, weights: torch.Tensor | None, plan: ExpertPlan,
+            dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y[t] = the sum over j of weights[t, j] ys[pos[t, j]], in Float32 and rounded once to
+    ``dtype`` (ys's by default; Float32 rows can give bfloat16); weights None: ones.  Dropped
+    slots are left out, whatever they hold."""
+    code, ys = _sorted_rows(ys, plan, "ys")
+    dtype = ys.dtype if dtype is None else dtype
+    if dtype is not ys.dtype and (ys.dtype, dtype) != (torch.float32, torch.bfloat16):
+        raise TypeError(f"{ys.dtype} rows cannot be combined to {dtype}")
+    (T, k), dim = plan.pos.shape, ys.shape[1]
+    if weights is not None:
+        weights = _weights(weights, plan, "weights")
+    y = ys.new_empty((T, dim), dtype=dtype)
+    _lib.call("mj_combine", code, _DTYPES[dtype], ys.data_ptr(), _ptr(weights), plan.pos.data_ptr(),
+              plan.offsets.data_ptr(), plan.experts, y.data_ptr(), T, k, dim, _stream())
+    return y
+
+
+def dispatch_backward(dxs: torch.Tensor, plan: ExpertPlan,
+                      dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The gradient of ``dispatch``'s x: dx[t] = the sum over j of dxs[pos[t, j]], rounded as
+    ``combine``'s."""
+    return combine(dxs, None, plan, dtype)
+
+
+def combine_backward(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan):
+    """(dys, dweights) of ``combine``: dys[pos[t, j]] = weights[t, j] dy[t] and dweights[t, j]
+    = <dy[t], ys[pos[t, j]]>, both 0 for dropped slots."""
+    code, dy = _token_rows(dy, plan, "dy")
+    (T, k), dim = plan.pos.shape, dy.shape[1]
+    ys = _like(ys, dy, (T * k, dim), "ys")
+    weights = _weights(weights, plan, "weights")
+    dys, dw = torch.empty_like(ys), torch.empty_like(weights)
+    _lib.call("mj_combine_backward", code, dy.data_ptr(), ys.data_ptr(), weights.data_ptr(),
+              plan.pos.data_ptr(), plan.offsets.data_ptr(), plan.experts, dys.data_ptr(),
+              dw.data_ptr(), T, k, dim, _stream())
+    return dys, dw
+
+
+# ------------------------------------------------------------------ the experts' block
+class ExpertsSaved(NamedTuple):
+    """What experts_mlp_backward needs: the operands, and one buffer with the fp32
+    projections g and u, then h."""
+    xs: torch.Tensor
+    plan: ExpertPlan
+    weights: torch.Tensor | None  # sorted, [rows]
+    gate: torch.Tensor
+    up: torch.Tensor
+    down: torch.Tensor
+    buf: torch.Tensor
+    act: int
+
+
+def _matrices(xs, plan, gate, up, down):
+    E = plan.experts
+    if xs.dtype is not torch.bfloat16:
+        raise TypeError(f"the experts' block takes bfloat16 rows, got {xs.dtype}")
+    if gate.dim() != 3 or down.dim() != 3 or gate.shape[0] != E or down.shape[0] != E or \
+            gate.shape[2] != xs.shape[1] or down.shape[2] != gate.shape[1]:
+        raise ValueError(f"gate {list(gate.shape)} and down {list(down.shape)} do not fit rows of "
+                         f"{xs.shape[1]} features and {E} experts")
+    return [_aligned(_like(t, xs, shape, name)) for t, shape, name in
+            ((gate, gate.shape, "gate"), (up, gate.shape, "up"), (down, down.shape, "down"))]
+
+
+def _experts_mlp(xs, plan, gate, up, down, act, weights, train):
+    _, xs = _sorted_rows(xs, plan, "xs")
+    xs = _aligned(xs)
+    gate, up, down = _matrices(xs, plan, gate, up, down)
+    if weights is not None:
+        if weights.dtype is not torch.float32 or weights.shape != (plan.rows,) or \
+                weights.device != xs.device:
+            raise ValueError(f"weights must be float32 [{plan.rows}] on {xs.device}")
+        weights = _contiguous(weights)
+    R, K = xs.shape
+    I, H = gate.shape[1], down.shape[1]
+    ys = torch.empty((R, H), dtype=torch.float32, device=xs.device)
+    gu = _up16(4 * R * I) if train else 0
+    buf = _scratch(2 * gu + _up16(2 * R * I), xs.device)
+    g = buf.data_ptr()
+    _lib.call("mj_experts_mlp_bf16", xs.data_ptr(), plan.offsets.data_ptr(), plan.experts,
+              gate.data_ptr(), up.data_ptr(), down.data_ptr(), act, _ptr(weights), g + 2 * gu,
+              g if train else None, g + gu if train else None, ys.data_ptr(), R, K, I, H, _stream())
+    return ys, ExpertsSaved(xs, plan, weights, gate, up, down, buf, act) if train else None
+
+
+def experts_mlp(xs: torch.Tensor, plan: ExpertPlan, gate: torch.Tensor, up: torch.Tensor,
+                down: torch.Tensor, act: int = _lib.EPI_SILU,
+                weights: torch.Tensor | None = None) -> torch.Tensor:
+    """ys [rows, H] in Float32: ``gated_mlp`` of each sorted row with its expert's matrices,
+    gate and up [E, I, K], down [E, H, I], all bfloat16 with widths in multiples of 8.
+    ``weights`` [rows] (sorted, as ``dispatch`` gives them) multiply h, and so ys.  Rows of
+    dropped slots are zeros."""
+    return _experts_mlp(xs, plan, gate, up, down, act, weights, False)[0]
+
+
+def experts_mlp_train(xs: torch.Tensor, plan: ExpertPlan, gate: torch.Tensor, up: torch.Tensor,
+                      down: torch.Tensor, act: int = _lib.EPI_SILU,
+                      weights: torch.Tensor | None = None):
+    """(ys, saved): experts_mlp and what its backward needs (h in bfloat16, the two
+    projections in Float32).  The operands are kept, not copied: they must not change before
+    the backward."""
+    return _experts_mlp(xs, plan, gate, up, down, act, weights, True)
+
+
+def experts_mlp_backward(dys: torch.Tensor, saved: ExpertsSaved):
+    """(dxs, dgate, dup, ddown, dweights) of experts_mlp from dys, bfloat16; dxs and dweights
+    are Float32.  An expert without rows gets zeros; dxs's rows of dropped slots are zeros; dweights [tokens, topk] is the gradient of the
+    unsorted weights, or None without weights.  dys's rows of dropped slots are not read."""
+    s = saved
+    xs, plan, dev = s.xs, s.plan, s.xs.device
+    (R, K), (E, I, _), H = xs.shape, s.gate.shape, s.down.shape[1]
+    dys = _aligned(_like(dys, xs, (R, H), "dys"))
+    out = [torch.empty(xs.shape, dtype=torch.float32, device=dev)]
+    out += [torch.empty_like(t) for t in (s.gate, s.up, s.down)]
+    dw, dots = None, 0
+    if s.weights is not None:
+        dw = torch.empty(plan.pos.shape, dtype=torch.float32, device=dev)
+        dots = 4 * _lib.load().mj_experts_mlp_dots(R, E, K, I, H)
+    gu, db = _up16(4 * R * I), _up16(2 * R * I)
+    work = _scratch(2 * db + dots, dev)  # dg, du, the parts of dweights
+    g, dg = s.buf.data_ptr(), work.data_ptr()
+    _lib.call("mj_experts_mlp_backward_bf16", xs.data_ptr(), plan.offsets.data_ptr(), E,
+              s.gate.data_ptr(), s.up.data_ptr(), s.down.data_ptr(), s.act, _ptr(s.weights),
+              g + 2 * gu, g, g + gu, dys.data_ptr(), dg, dg + db, *[t.data_ptr() for t in out],
+              plan.pos.data_ptr(), R if dw is not None else 0, dg + 2 * db if dots else None,
+              _ptr(dw), R, K, I, H, _stream())
+    return (*out, dw)
+
+
+class ExpertsMLP:
+    """ExpertsMLP(gate, up, down, act): the layer of E gated blocks, gate and up [E, I, K],
+    down [E, H, I], bfloat16:
+
+        y[t] = the sum over j of weights[t, j] mlp_e(x[t]) for e = experts[t, j]
+
+    experts [tokens, topk] are int32 or int64 (outside 0 .. E - 1: dropped), weights Float32 of
+    the same shape, x [tokens, K]."""
+
+    def __init__(self, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
+                 act: int = _lib.EPI_SILU):
+        if gate.dim() != 3 or up.shape != gate.shape or down.dim() != 3 or \
+                down.shape[0] != gate.shape[0] or down.shape[2] != gate.shape[1]:
+            raise ValueError(f"gate {list(gate.shape)}, up {list(up.shape)} and down "
+                             f"{list(down.shape)} do not fit each other")
+        self.gate, self.up, self.down, self.act = gate, up, down, act
+
+    def _sorted(self, x, experts, weights):
+        plan = sort_experts(experts, self.gate.shape[0])
+        return plan, *dispatch(x, plan, weights)
+
+    def forward(self, x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+        plan, xs, ws = self._sorted(x, experts, weights)
+        ys = experts_mlp(xs, plan, self.gate, self.up, self.down, self.act, ws)
+        return combine(ys, None, plan, x.dtype)
+
+    def forward_train(self, x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor):
+        """(y, saved)"""
+        plan, xs, ws = self._sorted(x, experts, weights)
+        ys, saved = experts_mlp_train(xs, plan, self.gate, self.up, self.down, self.act, ws)
+        return combine(ys, None, plan, x.dtype), saved
+
+    @staticmethod
+    def backward(dy: torch.Tensor, saved: ExpertsSaved) -> dict[str, torch.Tensor]:
+        """The gradients of x, weights, gate, up and down, by their names."""
+        dys = dispatch(dy, saved.plan)
+        dxs, dgate, dup, ddown, dw = experts_mlp_backward(dys, saved)
+        return dict(x=dispatch_backward(dxs, saved.plan, dy.dtype), weights=dw, gate=dgate, up=dup, down=ddown)
+
+
+__all__ = ["ExpertPlan", "sort_experts", "dispatch", "dispatch_backward", "combine",
+           "combine_backward", "experts_mlp", "experts_mlp_train", "experts_mlp_backward",
+           "ExpertsMLP", "ExpertsSaved"]
