@@ -41,11 +41,16 @@ CFLAGS = [
     "-Wall",
     "-Wno-unused-function",
 ]
+# Flags of single files.  gemm_f8.hip scales every result of the matrix cores on the
+# vector unit: results in vector registers, not in accumulation registers that each
+# have to be moved out first.
+FILE_CFLAGS = {"gemm_f8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _compile(src: str) -> str:
-    obj = os.path.join(BUILD_DIR, os.path.basename(src) + ".o")
-    cmd = [HIPCC, *CFLAGS, "-c", src, "-o", obj]
+    name = os.path.basename(src)
+    obj = os.path.join(BUILD_DIR, name + ".o")
+    cmd = [HIPCC, *CFLAGS, *FILE_CFLAGS.get(name, []), "-c", src, "-o", obj]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}")

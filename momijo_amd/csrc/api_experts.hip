@@ -286,27 +286,41 @@ int32_t mj_gemm_f8(const uint8_t *xq, const float *sx, const uint8_t *Wq, const 
 
 int64_t mj_linear_f8_work_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return up16(M * K) + up16(4 * M * f8_blocks(K)) + mj_gemm_f8_work_bytes(M, N, K);
+  const int64_t part = mj_gemm_f8_work_bytes(M, N, K);
+  return mj::gemm_f8_quantizes(M, N, K) ? part : up16(M * K) + up16(4 * M * f8_blocks(K)) + part;
 }
 
 int32_t mj_linear_f8(int32_t dtype, const void *x, const uint8_t *Wq, const float *sw, const float *bias,
                      int32_t act, uint16_t *y, int64_t M, int64_t N, int64_t K, void *work, int64_t work_bytes,
                      void *stream) {
+  if (int32_t s = check_dtype(dtype)) return s;
+  if (int32_t s = check_act(act)) return s;
+  if (int32_t s = check_rows("fp8 Linear", M)) return s;
+  if (int32_t s = check_width("fp8 Linear", N, 1)) return s;
+  if (int32_t s = check_width("fp8 Linear", K, 16)) return s;
+  const void *ptrs[] = {x, Wq, y, work};
+  if (int32_t s = check_aligned("fp8 Linear", ptrs, 4)) return s;
+  if (M == 0 || N == 0) return MJ_OK;
+  if (!y || (K > 0 && (!x || !Wq || !sw))) return fail(MJ_ERR_ARG, "fp8 Linear: null operand");
   const int64_t need = mj_linear_f8_work_bytes(M, N, K);
-  if (need > 0 && (!work || work_bytes < need || !aligned16(work)))
-    return fail(MJ_ERR_ARG, "fp8 Linear: work must be 16-byte aligned with %lld bytes", (long long)need);
-  uint8_t *q = (uint8_t *)work;
-  float *s = need ? (float *)(q + up16(M * K)) : nullptr;
-  char *rest = need ? (char *)s + up16(4 * M * f8_blocks(K)) : nullptr;
-  // (the product's checks first: nothing is enqueued for arguments that it refuses)
-  mj::F8Product p;
-  if (int32_t e = check_act(act)) return e;
-  if (int32_t e = make_f8("fp8 Linear", p, q, s, Wq, sw, M, N, K, 1)) return e;
-  if (M > 0 && N > 0 && (!y || !aligned16(y)))
-    return fail(y ? MJ_ERR_UNSUPPORTED : MJ_ERR_ARG, "fp8 Linear: y must be 16-byte aligned and not null");
-  if (N > 0)
-    if (int32_t e = mj_quantize_rows_f8(dtype, x, q, s, M, K, stream)) return e;
-  return mj_gemm_f8(q, s, Wq, sw, bias, act, y, M, N, K, rest, mj_gemm_f8_work_bytes(M, N, K), stream);
+  if (need > 0 && (!work || work_bytes < need))
+    return fail(MJ_ERR_ARG, "fp8 Linear: work must hold %lld bytes", (long long)need);
+  mj::F8Product q;
+  q.w = Wq, q.sw = sw, q.bias = bias, q.epi = act, q.y = y, q.M = M, q.N = N, q.K = K;
+  char *rest = (char *)work;
+  if (mj::gemm_f8_quantizes(M, N, K)) {
+    q.xf = x, q.xf_bf16 = dtype == MJ_BF16;
+  } else if (K > 0) {
+    mj::F8Rows a;
+    a.x = x, a.tokens = a.rows = M, a.dim = K;
+    a.q = (uint8_t *)work, a.scales = (float *)(rest + up16(M * K));
+    rest = (char *)a.scales + up16(4 * M * f8_blocks(K));
+    if (int32_t s = hip_status(mj::launch_quantize_rows_f8(dtype == MJ_BF16, a, S(stream)), "fp8 rows launch"))
+      return s;
+    q.x = a.q, q.sx = a.scales;
+  }
+  q.part = (float *)rest;
+  return hip_status(mj::launch_gemm_f8(q, S(stream)), "fp8 Linear launch");
 }
 
 int32_t mj_experts_gemm_f8(const uint8_t *xq, const float *sx, const int32_t *offsets, int64_t experts,
@@ -323,8 +337,11 @@ int32_t mj_experts_gemm_f8(const uint8_t *xq, const float *sx, const int32_t *of
 }
 
 int64_t mj_experts_gate_f8_work_bytes(int64_t R, int64_t experts, int64_t I, int64_t K) {
-  if (R <= 0 || experts < 1 || I <= 0 || K < 0) return 0;
-  return 4 * R * I;
+  if (R <= 0 || experts < 1 || experts > mj::kMaxExperts || I <= 0 || K < 0) return 0;
+  mj::F8Product q;
+  const uint8_t none = 0;
+  q.w2 = &none, q.M = R, q.N = I, q.K = K, q.experts = (int)experts;
+  return mj::gemm_f8_fuses(q) ? 0 : 4 * R * I;
 }
 
 int32_t mj_experts_gate_f8(const uint8_t *xq, const float *sx, const int32_t *offsets, int64_t experts,
@@ -342,9 +359,10 @@ int32_t mj_experts_gate_f8(const uint8_t *xq, const float *sx, const int32_t *of
   const int64_t need = mj_experts_gate_f8_work_bytes(R, experts, I, K);
   if (need > 0 && (!work || work_bytes < need))
     return fail(MJ_ERR_ARG, "fp8 gate: work must hold %lld bytes", (long long)need);
-  q.w2 = Wu, q.sw2 = su, q.epi = act, q.h = (float *)work;
+  q.w2 = Wu, q.sw2 = su, q.epi = act, q.h = (float *)work, q.hq = hq, q.sh = sh;
   q.offsets = offsets, q.experts = (int)experts, q.tail = 1;
   if (int32_t s = hip_status(mj::launch_gemm_f8(q, S(stream)), "fp8 gate launch")) return s;
+  if (need == 0) return MJ_OK;
   return mj_quantize_rows_f8(MJ_F32, work, hq, sh, R, I, stream);
 }
 

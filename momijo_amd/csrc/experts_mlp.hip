@@ -74,21 +74,27 @@ __device__ __forceinline__ TileProb row_outputs(const ExpertArgs &a, int row0, i
   return p;
 }
 
-// A weight gradient: expert by expert, its matrices' tiles in turn.
+// A weight gradient: expert by expert, its matrices' tiles in turn, dealt to the XCDs in runs
+// of 32 (a workgroup for each CU of an XCD, 4 x 8 tiles).  A contiguous eighth for each XCD,
+// as in the row products, would give XCDs experts of different lengths: 8 experts with up
+// to twice the rows of the average took 2285 us against 1310.
 __device__ __forceinline__ void weight_product(const ExpertArgs &a, TileProb &p, TileAt &at, int &e) {
-  const int total = a.tiles * a.experts, x = blockIdx.x & 7, q = total >> 3, r = total & 7;
-  int logical = x * q + (x < r ? x : r) + ((int)blockIdx.x >> 3);
+  const int total = a.tiles * a.experts, b = (int)blockIdx.x;
+  int logical = b;
+  if (b < (total & ~255)) logical = (b & ~255) + (b & 7) * 32 + ((b >> 3) & 31);
   e = logical / a.tiles;
   logical -= e * a.tiles;
   at.prob = 0, at.split = 0;
   if (a.n > 1 && logical >= a.p[1].first) at.prob = 1;
   if (a.n > 2 && logical >= a.p[2].first) at.prob = 2;
   const TileProb &s = a.p[at.prob];
-  const int row = a.offsets[e];
+  // (scalars: loaded values would be kept in vector registers)
+  const int row = __builtin_amdgcn_readfirstlane(a.offsets[e]);
+  const int end = __builtin_amdgcn_readfirstlane(a.offsets[e + 1]);
   p.lda = s.lda, p.ldb = s.ldb;
   p.A[0] = p.A[1] = s.A[0] + row * s.lda;
   p.B[0] = p.B[1] = s.B[0] + row * s.ldb;
-  p.M = s.M, p.N = s.N, p.K = a.offsets[e + 1] - row, p.segs = 1;
+  p.M = s.M, p.N = s.N, p.K = end - row, p.segs = 1;
   group_coords(logical - s.first, s.tiles_m, s.tiles_n, 4, at.m, at.n);
 }
 
@@ -212,13 +218,24 @@ hipError_t launch_kernel(int tile, const ExpertArgs &a, int64_t grid, hipStream_
   }
 }
 
-// The experts that the rows reach, at most; the rows are taken to be spread evenly over
-// them, and each to leave half a tile empty.
+// The experts that the rows reach, at most.
 int64_t busy_experts(const ExpertMlp &q) { return std::min(q.R, q.E); }
 
-int64_t even_tiles(const ExpertMlp &q, int64_t bm) {
-  const int64_t b = busy_experts(q), per = (q.R + b - 1) / b;
-  return per <= bm ? b : q.R / bm + (b + 1) / 2;
+// The tiles of bm rows to expect: an expert's rows are taken to be spread over 0.4 to 1.6 of the
+// average, so one of several tiles leaves half a tile empty, and one of about a tile's
+// rows takes one or two.
+double likely_tiles(const ExpertMlp &q, int64_t bm) {
+  const double b = (double)busy_experts(q), per = (double)q.R / b;
+  if (per >= (double)bm) return (double)q.R / (double)bm + b / 2;
+  return b * (1.0 + std::max(0.0, (1.6 * per - (double)bm) / (1.2 * per)));
+}
+
+// The block's tile costs (mlp_tile.h) hold for the experts too, but for 128 x 128: in the large
+// products of 8192 rows and 8 experts, 4096 and 5504 wide, it fell 8 to 12 % behind its
+// prediction (y 446 us, 408 on 256 x 256; dx 867 and 792; h 901 and 831); 8192 rows of 32
+// experts, 2048 and 1408 wide, h 158 us and 177 on 256 x 256.
+double expert_time_us(int tile, int out, double tiles, int64_t stages) {
+  return tile_time_us(kTileCost[tile], out, (int64_t)(tiles + 0.5), stages) * (tile == T_128 ? 1.08 : 1.0);
 }
 
 int plan_rows(const ExpertMlp &q, int64_t N, int64_t stages, int out) {
@@ -228,7 +245,7 @@ int plan_rows(const ExpertMlp &q, int64_t N, int64_t stages, int out) {
     const TileCost &c = kTileCost[t];
     const int64_t bn = out == OUT_GATE ? c.bn / 2 : c.bn, tn = (N + bn - 1) / bn;
     if (!grid_fits(tn * expert_tiles_most(q.R, q.E + 1, c.bm), c.threads)) continue;
-    const double us = tile_time_us(c, out, tn * even_tiles(q, c.bm), stages);
+    const double us = expert_time_us(t, out, (double)tn * likely_tiles(q, c.bm), stages);
     if (us < best_us) best_us = us, best = t;
   }
   return best;
@@ -260,7 +277,7 @@ hipError_t launch_weights(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream)
   for (int t = 0; t < T_COUNT; ++t) {
     const int64_t wgs = tiles_of(kTileCost[t]) * q.E;
     if (!grid_fits(wgs, kTileCost[t].threads)) continue;
-    const double us = tile_time_us(kTileCost[t], OUT_STORE, wgs, stages);
+    const double us = expert_time_us(t, OUT_STORE, (double)wgs, stages);
     if (us < best_us) best_us = us, tile = t;
   }
   const TileCost &c = kTileCost[tile];

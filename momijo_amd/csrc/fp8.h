@@ -1,4 +1,4 @@
-// The quantization of a block to e4m3 (fp8.hip).
+// The quantization of a block to e4m3 (fp8.hip, gemm_f8.hip).
 #pragma once
 
 #include "common.h"
@@ -25,6 +25,18 @@ __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d,
 
 __device__ __forceinline__ uint2 f8_pack8(const float (&v)[8], float inv) {
   return make_uint2(f8_pack4(v[0], v[1], v[2], v[3], inv), f8_pack4(v[4], v[5], v[6], v[7], inv));
+}
+
+// The largest of 16 lanes (magnitudes), in each of them.
+__device__ __forceinline__ float f8_max16(float v) {
+#define MJ_MAX(ctrl) \
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, false)))
+  MJ_MAX(0xB1);   // quad_perm [1,0,3,2]
+  MJ_MAX(0x4E);   // quad_perm [2,3,0,1]
+  MJ_MAX(0x124);  // row_ror:4
+  MJ_MAX(0x128);  // row_ror:8
+#undef MJ_MAX
+  return v;
 }
 
 }  // namespace mj

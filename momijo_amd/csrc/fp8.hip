@@ -46,18 +46,6 @@ __device__ __forceinline__ float max8(const float (&v)[8]) {
   return a;
 }
 
-// The largest of 16 lanes, in each of them.
-__device__ __forceinline__ float max16(float v) {
-#define MJ_MAX(ctrl) \
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, false)))
-  MJ_MAX(0xB1);   // quad_perm [1,0,3,2]
-  MJ_MAX(0x4E);   // quad_perm [2,3,0,1]
-  MJ_MAX(0x124);  // row_ror:4
-  MJ_MAX(0x128);  // row_ror:8
-#undef MJ_MAX
-  return v;
-}
-
 // 16 lanes a block of a row, 8 elements a lane (K % 16 == 0: a lane has all or none).
 template <bool BF>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(F8Rows a) {
@@ -69,7 +57,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(F8Rows a) {
   const bool in = e < a.dim;
   float v[8] = {};
   if (in) load8<BF>(a.x, t * a.dim + e, v);
-  const F8Scale s = f8_scale(max16(max8(v)));
+  const F8Scale s = f8_scale(f8_max16(max8(v)));
   const uint2 q = f8_pack8(v, s.inv);
   auto put = [&](int64_t p, uint2 w, float scale) __attribute__((always_inline)) {
     if (in) *(uint2 *)(a.q + p * a.dim + e) = w;

@@ -439,14 +439,22 @@ hipError_t launch_quantize_blocks_f8(bool bf16, const F8Blocks &a, hipStream_t s
 struct F8Product {
   const uint8_t *x = nullptr, *w = nullptr, *w2 = nullptr;
   const float *sx = nullptr, *sw = nullptr, *sw2 = nullptr, *bias = nullptr;
+  const void *xf = nullptr;              // x in fp32, or bf16, where gemm_f8_quantizes, in place of x, sx
+  bool xf_bf16 = false;
   uint16_t *y = nullptr;
   float *h = nullptr, *part = nullptr;   // part: gemm_f8_part_floats
+  uint8_t *hq = nullptr;                 // h quantized, where gemm_f8_fuses, with its scales
+  float *sh = nullptr;
   const int *offsets = nullptr;          // [experts + 1], or null for one matrix
   int experts = 0, epi = 0;
   int tail = 0;                          // y's rows from offsets[experts] on become zeros
   int64_t M = 0, N = 0, K = 0;
 };
 int64_t gemm_f8_part_floats(int64_t M, int64_t N, int64_t K);
+// Whether the product of one matrix can quantize x itself.
+bool gemm_f8_quantizes(int64_t M, int64_t N, int64_t K);
+// Whether the gate's product quantizes its h (else it leaves fp32 h).
+bool gemm_f8_fuses(const F8Product &q);
 hipError_t launch_gemm_f8(const F8Product &q, hipStream_t stream);
 
 }  // namespace mj

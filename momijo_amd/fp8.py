@@ -141,9 +141,9 @@ class F8Linear:
         M = x.shape[:-1].numel()
         y = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
         nbytes = _work("mj_linear_f8_work_bytes", M, N, K)
-        work = _scratch(nbytes, x.device)
+        work = _scratch(nbytes, x.device) if nbytes else None
         _lib.call("mj_linear_f8", code, x.data_ptr(), self.q.data_ptr(), self.scales.data_ptr(),
-                  _ptr(self.bias), self.act, y.data_ptr(), M, N, K, work.data_ptr(), nbytes, _stream())
+                  _ptr(self.bias), self.act, y.data_ptr(), M, N, K, _ptr(work), nbytes, _stream())
         return y
 
 
