@@ -25,36 +25,37 @@ from .block import _DTYPES, _check_type, _like, _scratch, _up16
 from .tensor import _ptr, _stream
 
 
-class ExpertPlan(NamedTuple):
-    """Where the slots go.  pos int32 [tokens, topk]: a slot's row among those sorted by
-    expert (in the order of the slots within an expert, dropped slots last); offsets int32
-    [experts + 1]: the experts' first rows, the last entry the first dropped slot's."""
-    pos: torch.Tensor
-    offsets: torch.Tensor
-
-    @property
-    def experts(self) -> int:
-        return self.offsets.shape[0] - 1
-
-    @property
-    def rows(self) -> int:
-        return self.pos.numel()
-
-
 def _check_device(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda:
+    device = t.device
+    if device.type != "cuda":
         raise ValueError(f"{name} must be on the GPU")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is "
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {device}, the current device is "
                          f"cuda:{torch.cuda.current_device()}")
 
 
-def _check_plan(plan: ExpertPlan, device) -> None:
-    pos, offsets = plan
-    if pos.dim() != 2 or pos.dtype is not torch.int32 or offsets.dtype is not torch.int32 or \
-            offsets.dim() != 1 or pos.device != device or offsets.device != device or \
-            not pos.is_contiguous() or not offsets.is_contiguous():
-        raise ValueError(f"the plan must be sort_experts's, on {device}")
+class ExpertPlan:
+    """Where the slots go, as ``sort_experts`` finds it (the kernels trust its entries).  pos
+    int32 [tokens, topk]: a slot's row among those sorted by expert (in the order of the slots
+    within an expert, dropped slots last); offsets int32 [experts + 1]: the experts' first
+    rows, the last entry the first dropped slot's."""
+
+    __slots__ = ("pos", "offsets", "tokens", "topk", "rows", "experts", "device", "_args")
+
+    def __init__(self, pos: torch.Tensor, offsets: torch.Tensor):
+        if pos.dim() != 2 or pos.dtype is not torch.int32 or not pos.is_contiguous() or \
+                offsets.dim() != 1 or offsets.dtype is not torch.int32 or \
+                not offsets.is_contiguous() or offsets.device != pos.device or not len(offsets):
+            raise ValueError("pos must be a contiguous int32 [tokens, topk] tensor, offsets int32 "
+                             "[experts + 1] on its device")
+        self._set(pos, offsets, *pos.shape, offsets.shape[0] - 1, pos.device, pos.data_ptr(),
+                  offsets.data_ptr())
+
+    def _set(self, pos, offsets, tokens, topk, experts, device, p, o):
+        self.pos, self.offsets, self.device = pos, offsets, device
+        self.tokens, self.topk, self.rows, self.experts = tokens, topk, tokens * topk, experts
+        self._args = p, o, experts
+        return self
 
 
 def _contiguous(t: torch.Tensor) -> torch.Tensor:
@@ -67,11 +68,25 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _rows_of(t: torch.Tensor, plan: ExpertPlan, rows: int, name: str):
+    """(type code, t contiguous, its width) of a [rows, dim] operand on the plan's device."""
+    code = _DTYPES.get(t.dtype)
+    if code is None or t.dim() != 2 or t.device != plan.device:
+        _check_type(t, name)
+        _check_device(t, name)
+        raise ValueError(f"{name} must be [{rows}, dim] on {plan.device}, got {list(t.shape)} on {t.device}")
+    _check_device(t, name)
+    n, dim = t.shape
+    if n != rows:
+        raise ValueError(f"{name} must be [{rows}, dim], got {list(t.shape)}")
+    return code, t if t.is_contiguous() else t.contiguous(), dim
+
+
 def _weights(w: torch.Tensor, plan: ExpertPlan, name: str) -> torch.Tensor:
-    if w.dtype is not torch.float32 or w.shape != plan.pos.shape or w.device != plan.pos.device:
-        raise ValueError(f"{name} must be float32 {list(plan.pos.shape)} on {plan.pos.device}, got "
+    if w.dtype is not torch.float32 or w.shape != plan.pos.shape or w.device != plan.device:
+        raise ValueError(f"{name} must be float32 {list(plan.pos.shape)} on {plan.device}, got "
                          f"{w.dtype} {list(w.shape)} on {w.device}")
-    return _contiguous(w)
+    return w if w.is_contiguous() else w.contiguous()
 
 
 @functools.lru_cache(maxsize=1024)
@@ -82,53 +97,38 @@ def _sort_work(slots, experts):
 def sort_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
     """The plan for tokens whose experts are ``experts`` [tokens, topk], int32 or int64;
     an entry outside 0 .. num_experts - 1 is a dropped slot."""
-    if experts.dtype not in (torch.int32, torch.int64):
+    size = 8 if experts.dtype is torch.int64 else 4
+    if size == 4 and experts.dtype is not torch.int32:
         raise TypeError(f"experts must be int32 or int64, got {experts.dtype}")
     if experts.dim() != 2:
         raise ValueError(f"experts must be [tokens, topk], got {list(experts.shape)}")
     _check_device(experts, "experts")
-    ids, device = _contiguous(experts), experts.device
-    slots = ids.numel()
-    nbytes = _sort_work(slots, num_experts)
-    pos = torch.empty(ids.shape, dtype=torch.int32, device=device)
-    offsets = torch.empty(max(num_experts, 0) + 1, dtype=torch.int32, device=device)
-    work = _scratch(nbytes, device) if nbytes else None
-    _lib.call("mj_sort_experts", ids.data_ptr(), ids.element_size(), slots, num_experts,
-              pos.data_ptr(), offsets.data_ptr(), _ptr(work), nbytes, _stream())
-    return ExpertPlan(pos, offsets)
-
-
-def _token_rows(x: torch.Tensor, plan: ExpertPlan, name: str):
-    code = _check_type(x, name)
-    _check_device(x, name)
-    _check_plan(plan, x.device)
-    if x.dim() != 2 or x.shape[0] != plan.pos.shape[0]:
-        raise ValueError(f"{name} must be [{plan.pos.shape[0]}, dim], got {list(x.shape)}")
-    return code, _contiguous(x)
-
-
-def _sorted_rows(xs: torch.Tensor, plan: ExpertPlan, name: str):
-    code = _check_type(xs, name)
-    _check_device(xs, name)
-    _check_plan(plan, xs.device)
-    if xs.dim() != 2 or xs.shape[0] != plan.rows:
-        raise ValueError(f"{name} must be [{plan.rows}, dim], got {list(xs.shape)}")
-    return code, _contiguous(xs)
+    ids = _contiguous(experts)
+    T, k = ids.shape
+    nbytes = _sort_work(T * k, num_experts)
+    pos = ids.new_empty((T, k), dtype=torch.int32)
+    offsets = ids.new_empty(max(num_experts, 0) + 1, dtype=torch.int32)
+    work = _scratch(nbytes, ids.device) if nbytes else None
+    p, o = pos.data_ptr(), offsets.data_ptr()
+    _lib.call("mj_sort_experts", ids.data_ptr(), size, T * k, num_experts, p, o, _ptr(work), nbytes,
+              _stream())
+    return object.__new__(ExpertPlan)._set(pos, offsets, T, k, num_experts, ids.device, p, o)
 
 
 def dispatch(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor | None = None):
     """xs [tokens * topk, dim] with xs[pos[t, j]] = x[t], zeros for dropped slots; with
     ``weights`` [tokens, topk] (Float32) also their sorted form: (xs, ws)."""
-    code, x = _token_rows(x, plan, "x")
-    (T, k), dim = plan.pos.shape, x.shape[1]
-    xs = x.new_empty((T * k, dim))
-    ws = None
-    if weights is not None:
-        weights = _weights(weights, plan, "weights")
-        ws = weights.new_empty(T * k)
-    _lib.call("mj_dispatch", code, x.data_ptr(), _ptr(weights), plan.pos.data_ptr(),
-              plan.offsets.data_ptr(), plan.experts, xs.data_ptr(), _ptr(ws), T, k, dim, _stream())
-    return xs if weights is None else (xs, ws)
+    code, x, dim = _rows_of(x, plan, plan.tokens, "x")
+    xs = x.new_empty((plan.rows, dim))
+    if weights is None:
+        _lib.call("mj_dispatch", code, x.data_ptr(), None, *plan._args, xs.data_ptr(), None,
+                  plan.tokens, plan.topk, dim, _stream())
+        return xs
+    weights = _weights(weights, plan, "weights")
+    ws = weights.new_empty(plan.rows)
+    _lib.call("mj_dispatch", code, x.data_ptr(), weights.data_ptr(), *plan._args, xs.data_ptr(),
+              ws.data_ptr(), plan.tokens, plan.topk, dim, _stream())
+    return xs, ws
 
 
 def combine(ys: torch.Tensor, weights: torch.Tensor | None, plan: ExpertPlan,
@@ -136,16 +136,17 @@ def combine(ys: torch.Tensor, weights: torch.Tensor | None, plan: ExpertPlan,
     """y[t] = the sum over j of weights[t, j] ys[pos[t, j]], in Float32 and rounded once to
     ``dtype`` (ys's by default; Float32 rows can give bfloat16); weights None: ones.  Dropped
     slots are left out, whatever they hold."""
-    code, ys = _sorted_rows(ys, plan, "ys")
-    dtype = ys.dtype if dtype is None else dtype
-    if dtype is not ys.dtype and (ys.dtype, dtype) != (torch.float32, torch.bfloat16):
-        raise TypeError(f"{ys.dtype} rows cannot be combined to {dtype}")
-    (T, k), dim = plan.pos.shape, ys.shape[1]
+    code, ys, dim = _rows_of(ys, plan, plan.rows, "ys")
     if weights is not None:
         weights = _weights(weights, plan, "weights")
-    y = ys.new_empty((T, dim), dtype=dtype)
-    _lib.call("mj_combine", code, _DTYPES[dtype], ys.data_ptr(), _ptr(weights), plan.pos.data_ptr(),
-              plan.offsets.data_ptr(), plan.experts, y.data_ptr(), T, k, dim, _stream())
+    if dtype is None or dtype is ys.dtype:
+        to, y = code, ys.new_empty((plan.tokens, dim))
+    elif ys.dtype is torch.float32 and dtype is torch.bfloat16:
+        to, y = _lib.BF16, ys.new_empty((plan.tokens, dim), dtype=dtype)
+    else:
+        raise TypeError(f"{ys.dtype} rows cannot be combined to {dtype}")
+    _lib.call("mj_combine", code, to, ys.data_ptr(), _ptr(weights), *plan._args, y.data_ptr(),
+              plan.tokens, plan.topk, dim, _stream())
     return y
 
 
@@ -159,14 +160,12 @@ def dispatch_backward(dxs: torch.Tensor, plan: ExpertPlan,
 def combine_backward(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan):
     """(dys, dweights) of ``combine``: dys[pos[t, j]] = weights[t, j] dy[t] and dweights[t, j]
     = <dy[t], ys[pos[t, j]]>, both 0 for dropped slots."""
-    code, dy = _token_rows(dy, plan, "dy")
-    (T, k), dim = plan.pos.shape, dy.shape[1]
-    ys = _like(ys, dy, (T * k, dim), "ys")
+    code, dy, dim = _rows_of(dy, plan, plan.tokens, "dy")
+    ys = _like(ys, dy, (plan.rows, dim), "ys")
     weights = _weights(weights, plan, "weights")
     dys, dw = torch.empty_like(ys), torch.empty_like(weights)
     _lib.call("mj_combine_backward", code, dy.data_ptr(), ys.data_ptr(), weights.data_ptr(),
-              plan.pos.data_ptr(), plan.offsets.data_ptr(), plan.experts, dys.data_ptr(),
-              dw.data_ptr(), T, k, dim, _stream())
+              *plan._args, dys.data_ptr(), dw.data_ptr(), plan.tokens, plan.topk, dim, _stream())
     return dys, dw
 
 
@@ -197,8 +196,7 @@ def _matrices(xs, plan, gate, up, down):
 
 
 def _experts_mlp(xs, plan, gate, up, down, act, weights, train):
-    _, xs = _sorted_rows(xs, plan, "xs")
-    xs = _aligned(xs)
+    xs = _aligned(_rows_of(xs, plan, plan.rows, "xs")[1])
     gate, up, down = _matrices(xs, plan, gate, up, down)
     if weights is not None:
         if weights.dtype is not torch.float32 or weights.shape != (plan.rows,) or \

@@ -19,8 +19,7 @@ import torch
 
 from . import _lib
 from .block import _check_type, _scratch
-from .experts import (ExpertPlan, _aligned, _check_device, _check_plan, _contiguous, _token_rows,
-                      combine, sort_experts)
+from .experts import ExpertPlan, _aligned, _check_device, _contiguous, _rows_of, combine, sort_experts
 from .tensor import _ptr, _stream
 
 _F8 = torch.float8_e4m3fn
@@ -134,12 +133,12 @@ class F8Linear:
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         code = _check_type(x, "x")
         _check_device(x, "x")
-        K, N = self.in_features, self.out_features
-        if x.dim() < 1 or x.shape[-1] != K or x.device != self.q.device:
-            raise ValueError(f"x must be [..., {K}] on {self.q.device}, got {list(x.shape)} on {x.device}")
+        K, N, shape = self.in_features, self.out_features, x.shape
+        if not shape or shape[-1] != K or x.device != self.q.device:
+            raise ValueError(f"x must be [..., {K}] on {self.q.device}, got {list(shape)} on {x.device}")
         x = _aligned(x)
-        M = x.shape[:-1].numel()
-        y = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
+        M = shape[0] if len(shape) == 2 else shape[:-1].numel()
+        y = x.new_empty((*shape[:-1], N), dtype=torch.bfloat16)
         nbytes = _work("mj_linear_f8_work_bytes", M, N, K)
         work = _scratch(nbytes, x.device) if nbytes else None
         _lib.call("mj_linear_f8", code, x.data_ptr(), self.q.data_ptr(), self.scales.data_ptr(),
@@ -151,21 +150,19 @@ class F8Linear:
 def dispatch_fp8(x: torch.Tensor, plan: ExpertPlan) -> tuple[torch.Tensor, torch.Tensor]:
     """(q [rows, K], scales [ceil(K / 128), rows]): each token's row quantized once and copied
     to its slots' sorted rows; zeros for dropped slots."""
-    code, x = _token_rows(x, plan, "x")
+    code, x, K = _rows_of(x, plan, plan.tokens, "x")
     x = _aligned(x)
-    (T, k), K = plan.pos.shape, x.shape[1]
-    q = torch.empty((T * k, K), dtype=_F8, device=x.device)
-    scales = torch.empty((_blocks(K), T * k), dtype=torch.float32, device=x.device)
-    _lib.call("mj_dispatch_f8", code, x.data_ptr(), plan.pos.data_ptr(), plan.offsets.data_ptr(),
-              plan.experts, q.data_ptr(), scales.data_ptr(), T, k, K, _stream())
+    q = torch.empty((plan.rows, K), dtype=_F8, device=x.device)
+    scales = torch.empty((_blocks(K), plan.rows), dtype=torch.float32, device=x.device)
+    _lib.call("mj_dispatch_f8", code, x.data_ptr(), *plan._args, q.data_ptr(), scales.data_ptr(),
+              plan.tokens, plan.topk, K, _stream())
     return q, scales
 
 
 def _expert_operands(q, scales, plan, Wq, Wscales, name):
     Wq, Wscales = _matrix(Wq, Wscales, 3, name)
     q, scales = _rows(q, scales, Wq.shape[2], "x")
-    _check_plan(plan, q.device)
-    if q.shape[0] != plan.rows or Wq.shape[0] != plan.experts or Wq.device != q.device:
+    if q.device != plan.device or q.shape[0] != plan.rows or Wq.shape[0] != plan.experts or Wq.device != q.device:
         raise ValueError(f"{plan.rows} rows and {plan.experts} experts planned, got {q.shape[0]} rows "
                          f"and {Wq.shape[0]} matrices on {Wq.device}")
     return q, scales, Wq, Wscales
