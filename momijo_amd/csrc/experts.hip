@@ -163,10 +163,13 @@ struct Unit {
   static constexpr int N = BF ? 8 : 4;
   static constexpr int SIZE = BF ? 2 : 4;
   u32x4_a2 w;
+  // NT: nontemporal
+  template <bool NT = false>
   __device__ __forceinline__ void load(const void *row, int64_t e, int have) {
     const char *p = (const char *)row + e * SIZE;
     if (have >= N) {
-      w = *(const u32x4_a2 *)p;
+      if constexpr (NT) w = __builtin_nontemporal_load((const u32x4_a2 *)p);
+      else w = *(const u32x4_a2 *)p;
     } else {
       w = u32x4_a2{0, 0, 0, 0};
 #pragma unroll
@@ -177,10 +180,12 @@ struct Unit {
         }
     }
   }
+  template <bool NT = false>
   __device__ __forceinline__ void store(void *row, int64_t e, int have) const {
     char *p = (char *)row + e * SIZE;
     if (have >= N) {
-      *(u32x4_a2 *)p = w;
+      if constexpr (NT) __builtin_nontemporal_store(w, (u32x4_a2 *)p);
+      else *(u32x4_a2 *)p = w;
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -237,7 +242,7 @@ __global__ __launch_bounds__(256) void dispatch_kernel(ExpertRows a) {
 
 // BI, BO: the rows' and the sum's type; a thread's 16 bytes of the sum are one or two units
 // of a row.
-template <bool BI, bool BO>
+template <bool BI, bool BO, bool NT>
 __global__ __launch_bounds__(256) void combine_kernel(ExpertRows a) {
   using UI = Unit<BI>;
   using UO = Unit<BO>;
@@ -251,84 +256,91 @@ __global__ __launch_bounds__(256) void combine_kernel(ExpertRows a) {
   auto load = [&](UI (&v)[P], int p) __attribute__((always_inline)) {
     const char *row = (const char *)a.xs + (int64_t)p * a.dim * UI::SIZE;
 #pragma unroll
-    for (int q = 0; q < P; ++q) v[q].load(row, e + q * UI::N, have - q * UI::N);
+    for (int q = 0; q < P; ++q) v[q].template load<NT>(row, e + q * UI::N, have - q * UI::N);
   };
   auto add = [&](const UI (&v)[P], int j) __attribute__((always_inline)) {
     const float w = a.w ? a.w[t * k + j] : 1.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = __builtin_fmaf(w, v[i / UI::N].get(i % UI::N), acc[i]);
   };
-  int j = 0;
-  for (; j + 4 <= k; j += 4) {  // four rows' loads in flight
-    UI v[4][P];
-    int p[4];
+  constexpr int FLY = 8 / P;  // rows' loads in flight
+  for (int j0 = 0; j0 < k; j0 += FLY) {
+    UI v[FLY][P];
+    int p[FLY];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) p[q] = pos[j + q];
+    for (int q = 0; q < FLY; ++q) p[q] = j0 + q < k ? pos[j0 + q] : 0x7FFFFFFF;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < FLY; ++q)
       if (p[q] < kept) load(v[q], p[q]);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (p[q] < kept) add(v[q], j + q);
-  }
-  for (; j < k; ++j) {
-    const int p = pos[j];
-    if (p >= kept) continue;
-    UI v[P];
-    load(v, p);
-    add(v, j);
+    for (int q = 0; q < FLY; ++q)
+      if (p[q] < kept) add(v[q], j0 + q);
   }
   UO y;
   y.set(acc);
-  y.store((char *)a.x + t * a.dim * UO::SIZE, e, have);
+  y.template store<NT>((char *)a.x + t * a.dim * UO::SIZE, e, have);
 }
 
-// One workgroup a token (one wave where a row is short): for each slot the row of dys and
-// the product of dy with the row of ys, its lanes' and waves' sums added in order.
-constexpr int kDotSlots = 16;  // slots whose sums wait in LDS
+// One workgroup a token (one wave where a row is short), four slots at a time: for each the row
+// of dys and the product of dy with the row of ys, its lanes' and waves' sums added in order.
+constexpr int kDotSlots = 4;
 
 template <bool BF, int NW>
 __global__ __launch_bounds__(NW * 64) void combine_bwd_kernel(ExpertRows a) {
   using U = Unit<BF>;
-  __shared__ float red[kDotSlots][NW];
+  __shared__ float red[2][kDotSlots][NW];
   const int64_t t = grid_block<NW * 64>();
   if (t >= a.tokens) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kept = *a.kept, k = (int)a.topk;
   const char *dy = (const char *)a.x + t * a.dim * U::SIZE;
-  for (int j0 = 0; j0 < k; j0 += kDotSlots) {
+  for (int j0 = 0, half = 0; j0 < k; j0 += kDotSlots, half ^= 1) {
     const int n = std::min(k - j0, kDotSlots);
-    for (int j = 0; j < n; ++j) {
-      const int p = a.pos[t * k + j0 + j];
-      const bool in = p < kept;
-      const float w = a.w[t * k + j0 + j];
-      const int64_t row = (int64_t)p * a.dim * U::SIZE;
-      float sum = 0.0f;
-      for (int64_t e = (int64_t)threadIdx.x * U::N; e < a.dim; e += NW * 64 * U::N) {
-        const int have = (int)std::min<int64_t>(a.dim - e, U::N);
-        U d, y, o;
-        float v[U::N];
-        d.load(dy, e, have);
-        if (in) {
-          y.load((const char *)a.ys + row, e, have);
+    int64_t row[kDotSlots];
+    bool in[kDotSlots];
+    float w[kDotSlots], sum[kDotSlots];
 #pragma unroll
-          for (int i = 0; i < U::N; ++i) sum = __builtin_fmaf(d.get(i), y.get(i), sum);
+    for (int q = 0; q < kDotSlots; ++q) {
+      const int64_t slot = t * k + j0 + (q < n ? q : 0);
+      const int p = a.pos[slot];
+      row[q] = (int64_t)p * a.dim * U::SIZE;
+      in[q] = p < kept;
+      w[q] = a.w[slot];
+      sum[q] = 0.0f;
+    }
+    for (int64_t e = (int64_t)threadIdx.x * U::N; e < a.dim; e += NW * 64 * U::N) {
+      const int have = (int)std::min<int64_t>(a.dim - e, U::N);
+      U d, y[kDotSlots];
+      d.load(dy, e, have);
+#pragma unroll
+      for (int q = 0; q < kDotSlots; ++q)
+        if (q < n && in[q]) y[q].load((const char *)a.ys + row[q], e, have);
+#pragma unroll
+      for (int q = 0; q < kDotSlots; ++q) {
+        if (q >= n) continue;
+        U o;
+        float v[U::N];
+        if (in[q]) {
+#pragma unroll
+          for (int i = 0; i < U::N; ++i) sum[q] = __builtin_fmaf(d.get(i), y[q].get(i), sum[q]);
         }
 #pragma unroll
-        for (int i = 0; i < U::N; ++i) v[i] = in ? w * d.get(i) : 0.0f;
+        for (int i = 0; i < U::N; ++i) v[i] = in[q] ? w[q] * d.get(i) : 0.0f;
         o.set(v);
-        if (a.xs) o.store((char *)a.xs + row, e, have);
+        o.store((char *)a.xs + row[q], e, have);
       }
-      sum = wave_sum_dpp(sum);
-      if (lane == 0) red[j][wave] = sum;
     }
-    __syncthreads();
-    if ((int)threadIdx.x < n) {
-      float sum = red[threadIdx.x][0];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) sum += red[threadIdx.x][w];
-      a.ws[t * k + j0 + threadIdx.x] = sum;
+    for (int q = 0; q < kDotSlots; ++q) {
+      sum[q] = wave_sum_dpp(sum[q]);
+      if (lane == 0) red[half][q][wave] = sum[q];
     }
-    __syncthreads();
+    __syncthreads();  // (two buffers: the next four wait only for these to be read)
+    if ((int)threadIdx.x < n) {
+      float s = red[half][threadIdx.x][0];
+#pragma unroll
+      for (int v = 1; v < NW; ++v) s += red[half][threadIdx.x][v];
+      a.ws[t * k + j0 + threadIdx.x] = s;
+    }
   }
 }
 
@@ -398,9 +410,18 @@ hipError_t launch_combine(bool bf16, bool y_bf16, ExpertRows a, hipStream_t stre
   const int64_t n = a.tokens * a.units;
   if (n == 0) return hipSuccess;
   const dim3 grid = grid_rows<256>((n + 255) / 256);
-  if (bf16) hipLaunchKernelGGL((combine_kernel<true, true>), grid, dim3(256), 0, stream, a);
-  else if (y_bf16) hipLaunchKernelGGL((combine_kernel<false, true>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((combine_kernel<false, false>), grid, dim3(256), 0, stream, a);
+  // Rows that no cache of an XCD holds go past it, both ways: 8 x 8192 rows of 4096 bf16 122 ->
+  // 110 us, right behind the kernel that wrote them 120 -> 85; 3000 x 1001 fp32 5.0 -> 6.0.
+  const bool nt = a.tokens * a.topk * a.dim * (bf16 ? 2 : 4) > (32 << 20);
+#define MJ_COMBINE(BI, BO)                                                                       \
+  do {                                                                                           \
+    if (nt) hipLaunchKernelGGL((combine_kernel<BI, BO, true>), grid, dim3(256), 0, stream, a);   \
+    else hipLaunchKernelGGL((combine_kernel<BI, BO, false>), grid, dim3(256), 0, stream, a);     \
+  } while (0)
+  if (bf16) MJ_COMBINE(true, true);
+  else if (y_bf16) MJ_COMBINE(false, true);
+  else MJ_COMBINE(false, false);
+#undef MJ_COMBINE
   return hipGetLastError();
 }
 
