@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256) void combine_kernel(ExpertRows a) {
 // of dys and the product of dy with the row of ys, its lanes' and waves' sums added in order.
 constexpr int kDotSlots = 4;
 
-template <bool BF, int NW>
+template <bool BF, int NW, bool NT>
 __global__ __launch_bounds__(NW * 64) void combine_bwd_kernel(ExpertRows a) {
   using U = Unit<BF>;
   __shared__ float red[2][kDotSlots][NW];
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(NW * 64) void combine_bwd_kernel(ExpertRows a) {
       d.load(dy, e, have);
 #pragma unroll
       for (int q = 0; q < kDotSlots; ++q)
-        if (q < n && in[q]) y[q].load((const char *)a.ys + row[q], e, have);
+        if (q < n && in[q]) y[q].template load<NT>((const char *)a.ys + row[q], e, have);
 #pragma unroll
       for (int q = 0; q < kDotSlots; ++q) {
         if (q >= n) continue;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(NW * 64) void combine_bwd_kernel(ExpertRows a) {
 #pragma unroll
         for (int i = 0; i < U::N; ++i) v[i] = in[q] ? w[q] * d.get(i) : 0.0f;
         o.set(v);
-        o.store((char *)a.xs + row[q], e, have);
+        o.template store<NT>((char *)a.xs + row[q], e, have);
       }
     }
 #pragma unroll
@@ -373,6 +373,14 @@ int64_t units_of(int64_t dim) {
   return std::max<int64_t>((dim + Unit<BF>::N - 1) / Unit<BF>::N, 1);
 }
 
+// Rows that the XCDs' caches do not hold are read (and written) past them.  Combine, 8 x 8192
+// rows of 4096 bf16: 122 -> 110 us, right behind the kernel that wrote them 120 -> 85; 3000 x
+// 1001 fp32 5.0 -> 6.0.  Its backward 254 -> 235.  Dispatch, which only writes them, loses by it
+// (106 -> 114).
+bool past_caches(bool bf16, const ExpertRows &a) {
+  return a.tokens * a.topk * a.dim * (bf16 ? 2 : 4) > (32 << 20);
+}
+
 }  // namespace
 
 int64_t sort_experts_work_ints(int64_t slots, int64_t experts) {
@@ -410,9 +418,7 @@ hipError_t launch_combine(bool bf16, bool y_bf16, ExpertRows a, hipStream_t stre
   const int64_t n = a.tokens * a.units;
   if (n == 0) return hipSuccess;
   const dim3 grid = grid_rows<256>((n + 255) / 256);
-  // Rows that no cache of an XCD holds go past it, both ways: 8 x 8192 rows of 4096 bf16 122 ->
-  // 110 us, right behind the kernel that wrote them 120 -> 85; 3000 x 1001 fp32 5.0 -> 6.0.
-  const bool nt = a.tokens * a.topk * a.dim * (bf16 ? 2 : 4) > (32 << 20);
+  const bool nt = past_caches(bf16, a);
 #define MJ_COMBINE(BI, BO)                                                                       \
   do {                                                                                           \
     if (nt) hipLaunchKernelGGL((combine_kernel<BI, BO, true>), grid, dim3(256), 0, stream, a);   \
@@ -429,14 +435,17 @@ hipError_t launch_combine_bwd(bool bf16, const ExpertRows &a, hipStream_t stream
   if (a.tokens == 0 || a.topk == 0) return hipSuccess;
   const bool one = (bf16 ? units_of<true>(a.dim) : units_of<false>(a.dim)) <= 64;
   const dim3 grid = one ? grid_rows<64>(a.tokens) : grid_rows<256>(a.tokens);
-#define MJ_BWD(BF, NW) \
-  hipLaunchKernelGGL((combine_bwd_kernel<BF, NW>), grid, dim3(NW * 64), 0, stream, a)
+  const bool nt = past_caches(bf16, a);
+#define MJ_BWD(BF, NW, NT) \
+  hipLaunchKernelGGL((combine_bwd_kernel<BF, NW, NT>), grid, dim3(NW * 64), 0, stream, a)
   if (bf16) {
-    if (one) MJ_BWD(true, 1);
-    else MJ_BWD(true, 4);
+    if (one) MJ_BWD(true, 1, false);
+    else if (nt) MJ_BWD(true, 4, true);
+    else MJ_BWD(true, 4, false);
   } else {
-    if (one) MJ_BWD(false, 1);
-    else MJ_BWD(false, 4);
+    if (one) MJ_BWD(false, 1, false);
+    else if (nt) MJ_BWD(false, 4, true);
+    else MJ_BWD(false, 4, false);
   }
 #undef MJ_BWD
   return hipGetLastError();
