@@ -685,6 +685,11 @@ int32_t mj_experts_mlp_backward_bf16(const uint16_t *xs, const int32_t *offsets,
                                      int64_t slots, float *dots, float *dw, int64_t R, int64_t K, int64_t I,
                                      int64_t H, void *stream);
 
+/* The kernel of a product of the experts' block, by name ("" for an empty or refused one):
+ * product 0 gate and up, 1 y, 2 dg and du, 3 dx, 4 the weight gradients.  Host only; for tests
+ * and profiles. */
+const char *mj_experts_mlp_kernel(int64_t R, int64_t experts, int64_t K, int64_t I, int64_t H, int32_t product);
+
 /* ---- 8-bit floating point ------------------------------------------------
  * Products of e4m3 values (largest 448) with a scale for each block of 128 features of a
  * row (x) or 128 x 128 elements (W), for inference (no reference counterpart).  A block of
@@ -697,6 +702,11 @@ int32_t mj_quantize_rows_f8(int32_t dtype, const void *x, uint8_t *q, float *sca
                             void *stream);
 int32_t mj_quantize_blocks_f8(int32_t dtype, const void *W, uint8_t *q, float *scales, int64_t mats, int64_t N,
                               int64_t K, void *stream);
+
+/* The kernel of an 8-bit product, by name ("" for an empty or refused one): of one matrix
+ * (experts 0), or of sorted rows with their experts' (gate: the gated block's first half).
+ * Host only; for tests and profiles. */
+const char *mj_gemm_f8_kernel(int64_t M, int64_t N, int64_t K, int64_t experts, int32_t gate);
 
 /* y [M,N] bf16 = act(x W^T + bias); the sum of a block's products is scaled and added in
  * fp32.  bias fp32 [N] or NULL; act MJ_EPI_NONE, RELU, GELU_TANH or SILU.  mj_linear_f8

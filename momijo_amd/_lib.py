@@ -144,7 +144,9 @@ SIGNATURES = {
     "mj_experts_mlp_dots": (_I64, [_I64] * 5),
     "mj_experts_mlp_backward_bf16": (_I32, [_P, _P, _I64, _P, _P, _P, _I32] + [_P] * 12 +
                                      [_I64, _P, _P] + [_I64] * 4 + [_P]),
+    "mj_experts_mlp_kernel": (ctypes.c_char_p, [_I64] * 5 + [_I32]),
     # 8-bit floating point
+    "mj_gemm_f8_kernel": (ctypes.c_char_p, [_I64] * 4 + [_I32]),
     "mj_quantize_rows_f8": (_I32, [_I32, _P, _P, _P, _I64, _I64, _P]),
     "mj_quantize_blocks_f8": (_I32, [_I32, _P, _P, _P, _I64, _I64, _I64, _P]),
     "mj_gemm_f8_work_bytes": (_I64, [_I64] * 3),

@@ -216,7 +216,28 @@ int32_t mj_experts_mlp_backward_bf16(const uint16_t *xs, const int32_t *offsets,
   return hip_status(mj::launch_experts_mlp_bwd(q, o, S(stream)), "experts backward launch");
 }
 
+const char *mj_experts_mlp_kernel(int64_t R, int64_t experts, int64_t K, int64_t I, int64_t H, int32_t product) {
+  if (R <= 0 || R > mj::kMlpMaxRows || check_experts(experts) || product < 0 || product > 4) return "";
+  for (int64_t w : {K, I, H})
+    if (w == 0 || check_width("experts", w, 8)) return "";
+  mj::ExpertMlp q;
+  q.R = R, q.E = experts, q.K = K, q.I = I, q.H = H;
+  return mj::experts_kernel_name(q, product);
+}
+
 // ------------------------------------------------------------------ 8-bit floating point
+const char *mj_gemm_f8_kernel(int64_t M, int64_t N, int64_t K, int64_t experts, int32_t gate) {
+  if (M <= 0 || M > mj::kMlpMaxRows || N <= 0 || K <= 0 || check_width("fp8", N, 1) || check_width("fp8", K, 16) ||
+      (experts != 0 && check_experts(experts)) || (gate && experts == 0))
+    return "";
+  mj::F8Product q;
+  const uint8_t none = 0;
+  const int32_t row = 0;
+  q.M = M, q.N = N, q.K = K, q.experts = (int)experts;
+  q.offsets = experts ? &row : nullptr, q.w2 = gate ? &none : nullptr;
+  return mj::gemm_f8_kernel_name(q);
+}
+
 int32_t mj_quantize_rows_f8(int32_t dtype, const void *x, uint8_t *q, float *scales, int64_t rows, int64_t K,
                             void *stream) {
   if (int32_t s = check_dtype(dtype)) return s;

@@ -263,23 +263,25 @@ hipError_t launch_rows(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream) {
   return launch_kernel<true, BKC, OUT>(tile, a, a.tiles_n * expert_tiles_most(q.R, q.E + a.tail, bm), stream);
 }
 
-hipError_t launch_weights(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream) {
-  if (a.n == 0) return hipSuccess;
+int plan_weights(const ExpertMlp &q, const ExpertArgs &a) {
   const int64_t per = q.R / q.E, stages = std::max<int64_t>((per + kBK - 1) / kBK, 1);
-  auto tiles_of = [&](const TileCost &c) {
-    int64_t t = 0;
-    for (int i = 0; i < a.n; ++i)
-      t += (int64_t)((a.p[i].M + c.bm - 1) / c.bm) * ((a.p[i].N + c.bn - 1) / c.bn);
-    return t;
-  };
-  int tile = T_64S3;
+  int best = T_64S3;
   double best_us = 1e30;
   for (int t = 0; t < T_COUNT; ++t) {
-    const int64_t wgs = tiles_of(kTileCost[t]) * q.E;
-    if (!grid_fits(wgs, kTileCost[t].threads)) continue;
-    const double us = expert_time_us(t, OUT_STORE, (double)wgs, stages);
-    if (us < best_us) best_us = us, tile = t;
+    const TileCost &c = kTileCost[t];
+    int64_t tiles = 0;
+    for (int i = 0; i < a.n; ++i)
+      tiles += (int64_t)((a.p[i].M + c.bm - 1) / c.bm) * ((a.p[i].N + c.bn - 1) / c.bn);
+    if (!grid_fits(tiles * q.E, c.threads)) continue;
+    const double us = expert_time_us(t, OUT_STORE, (double)(tiles * q.E), stages);
+    if (us < best_us) best_us = us, best = t;
   }
+  return best;
+}
+
+hipError_t launch_weights(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream) {
+  if (a.n == 0) return hipSuccess;
+  const int tile = plan_weights(q, a);
   const TileCost &c = kTileCost[tile];
   for (int i = 0; i < a.n; ++i) {
     TileProb &p = a.p[i];
@@ -290,6 +292,25 @@ hipError_t launch_weights(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream)
   }
   a.offsets = q.offsets, a.experts = (int)q.E;
   return launch_kernel<false, false, OUT_STORE>(tile, a, (int64_t)a.tiles * q.E, stream);
+}
+
+// The wanted weight gradients.
+ExpertArgs weight_args(const ExpertMlp &q, const ExpertMlpGrad &o, bool dwg, bool dwu, bool dwd) {
+  ExpertArgs w;
+  w.n = 0;
+  auto add = [&](const uint16_t *A, int64_t rows, const uint16_t *B, int64_t cols, uint16_t *C) {
+    if (rows == 0 || cols == 0) return;
+    w.c_expert[w.n] = rows * cols;
+    TileProb &p = w.p[w.n++];
+    p.A[0] = p.A[1] = A, p.lda = rows;
+    p.B[0] = p.B[1] = B, p.ldb = cols;
+    p.M = (int)rows, p.N = (int)cols;
+    p.C = C, p.ldc = cols;
+  };
+  if (dwg) add(o.dg, q.I, q.xs, q.K, o.dwg);
+  if (dwu) add(o.du, q.I, q.xs, q.K, o.dwu);
+  if (dwd) add(o.dys, q.H, q.h, q.I, o.dwd);
+  return w;
 }
 
 // Rows of one expert, if they are even, up to which the few-row kernel is taken.
@@ -307,6 +328,19 @@ hipError_t launch_few(const ExpertMlp &q, ExpertSkinny &a, hipStream_t stream) {
 }
 
 }  // namespace
+
+const char *experts_kernel_name(const ExpertMlp &q, int product) {
+  static const char *const names[T_COUNT] = {"256x256", "128x128", "64x64, 3 stages", "64x64, 5 stages", "128x64"};
+  if (product < 2 && few_rows(q)) return "16 rows";
+  auto stages = [](int64_t k) { return (k + kBK - 1) / kBK; };
+  switch (product) {
+    case 0: return names[plan_rows(q, q.I, stages(q.K), OUT_GATE)];
+    case 1: return names[plan_rows(q, q.H, stages(q.I), OUT_PART)];
+    case 2: return names[plan_rows(q, q.I, stages(q.H), OUT_DGATE)];
+    case 3: return names[plan_rows(q, q.K, 2 * stages(q.I), OUT_PART)];
+    default: return names[plan_weights(q, weight_args(q, ExpertMlpGrad(), true, true, true))];
+  }
+}
 
 int64_t expert_dots_ld(const ExpertMlp &q) {
   if (q.R == 0 || q.I == 0) return 0;
@@ -373,20 +407,7 @@ hipError_t launch_experts_mlp_bwd(const ExpertMlp &q, const ExpertMlpGrad &o, hi
     a.b_expert = q.I * q.K, a.tail = 1;
     if (hipError_t e = launch_rows<false, OUT_PART>(q, a, stream); e != hipSuccess) return e;
   }
-  ExpertArgs w;
-  w.n = 0;
-  auto add = [&](const uint16_t *A, int64_t rows, const uint16_t *B, int64_t cols, uint16_t *C) {
-    if (!C || rows == 0 || cols == 0) return;
-    w.c_expert[w.n] = rows * cols;
-    TileProb &p = w.p[w.n++];
-    p.A[0] = p.A[1] = A, p.lda = rows;
-    p.B[0] = p.B[1] = B, p.ldb = cols;
-    p.M = (int)rows, p.N = (int)cols;
-    p.C = C, p.ldc = cols;
-  };
-  add(o.dg, q.I, q.xs, q.K, o.dwg);
-  add(o.du, q.I, q.xs, q.K, o.dwu);
-  add(o.dys, q.H, q.h, q.I, o.dwd);
+  ExpertArgs w = weight_args(q, o, o.dwg, o.dwu, o.dwd);
   return launch_weights(q, w, stream);
 }
 

@@ -994,6 +994,21 @@ int64_t gemm_f8_part_floats(int64_t M, int64_t N, int64_t K) {
   return s > 1 ? s * M * N : 0;
 }
 
+const char *gemm_f8_kernel_name(const F8Product &q) {
+  static const char *const names[F8_COUNT][2] = {{"256x256", "256x256, K slices"},
+                                                 {"192x256", "192x256, K slices"},
+                                                 {"128x128", "128x128, K slices"},
+                                                 {"64x64", "64x64, K slices"}};
+  if (q.offsets || q.w2) {
+    if (few_rows(q)) return q.M > 8 * std::min<int64_t>(q.M, q.experts) ? "32 rows" : "16 rows";
+    return names[plan_experts(q, q.w2 != nullptr)][0];
+  }
+  if (f8_few_rows(q.M, q.N, q.K))
+    return q.M > 32 ? "64 rows" : q.M > 16 ? "32 rows" : gemm_f8_quantizes(q.M, q.N, q.K) ? "16 rows, quantizing" : "16 rows";
+  const F8Plan pl = plan_f8(q.M, q.N, q.K);
+  return names[pl.tile][pl.splits > 1];
+}
+
 hipError_t launch_gemm_f8(const F8Product &q, hipStream_t stream) {
   if (q.M == 0 || q.N == 0) return hipSuccess;
   F8Tiles a;

@@ -408,6 +408,8 @@ struct ExpertMlpGrad {
   int64_t slots = 0;
 };
 int64_t expert_dots_ld(const ExpertMlp &q);
+// product: 0 gate and up, 1 y, 2 dg and du, 3 dx, 4 the weight gradients
+const char *experts_kernel_name(const ExpertMlp &q, int product);
 hipError_t launch_experts_mlp(const ExpertMlp &q, hipStream_t stream);
 hipError_t launch_experts_mlp_bwd(const ExpertMlp &q, const ExpertMlpGrad &o, hipStream_t stream);
 
@@ -455,6 +457,7 @@ int64_t gemm_f8_part_floats(int64_t M, int64_t N, int64_t K);
 bool gemm_f8_quantizes(int64_t M, int64_t N, int64_t K);
 // Whether the gate's product quantizes its h (else it leaves fp32 h).
 bool gemm_f8_fuses(const F8Product &q);
+const char *gemm_f8_kernel_name(const F8Product &q);
 hipError_t launch_gemm_f8(const F8Product &q, hipStream_t stream);
 
 }  // namespace mj
