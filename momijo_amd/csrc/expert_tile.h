@@ -26,13 +26,22 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+// Which of the tiles a launch takes.  Large tiles leave most CUs idle in a last round of a few,
+// and how many there are the host cannot know: with at most half a round over (CUT_REST_MOST)
+// one launch takes the whole rounds and a second one those tiles in quarters (twice as many
+// rows and columns of tiles of half the sides); with more, the first takes all and the
+// second ends at once.
+enum : int { CUT_NONE = 0, CUT_ROUNDS, CUT_REST };
+constexpr int kTileRound = 256, CUT_REST_MOST = kTileRound / 2;
+
 // The tile of workgroup bid.  tail: the rows from offsets[experts] to `rows` are a group
 // too.  Each wave scans the experts' tile counts, 64 experts at a time.  XCD: neighbouring
 // tiles of one expert go to one XCD (they share its operand panels in its L2), 4 tile rows
-// at a time; without, tiles go column by column in launch order.
+// at a time; without, tiles go column by column in launch order.  CUT_REST: bm and tiles_n are
+// the large tiles', t.m and t.n the quarter's.
 template <bool XCD>
 __device__ __forceinline__ bool expert_tile(const int *offsets, int experts, int rows, bool tail, int bm,
-                                            int tiles_n, int bid, ExpertTile &t) {
+                                            int tiles_n, int bid, ExpertTile &t, int cut = CUT_NONE) {
   const int lane = threadIdx.x & 63, groups = experts + (tail ? 1 : 0);
   auto counts = [&](int g0, int &start, int &n) __attribute__((always_inline)) {
     const int g = g0 + lane;
@@ -43,13 +52,21 @@ __device__ __forceinline__ bool expert_tile(const int *offsets, int experts, int
   int start, n, total_m = 0;
   for (int g0 = 0; g0 < groups; g0 += 64)
     total_m += __builtin_amdgcn_readlane(wave_scan(counts(g0, start, n)), 63);
-  const int total = total_m * tiles_n;
+  int total = total_m * tiles_n, first_tile = 0;
+  if (cut != CUT_NONE) {
+    const int rest = total % kTileRound;
+    const bool split = rest <= CUT_REST_MOST;
+    if (cut == CUT_ROUNDS && split) total -= rest;
+    if (cut == CUT_REST) first_tile = total - rest, total = split ? 4 * rest : 0;
+  }
   if (bid >= total) return false;
   int logical = bid;
   if constexpr (XCD) {
     const int x = bid & 7, q = total >> 3, r = total & 7;
     logical = x * q + (x < r ? x : r) + (bid >> 3);
   }
+  const int quarter = logical & 3;
+  if (cut == CUT_REST) logical = first_tile + (logical >> 2);
   const int lm = logical / tiles_n;
   for (int g0 = 0, before = 0; g0 < groups; g0 += 64) {
     const int c = counts(g0, start, n), sum = wave_scan(c) + before;
@@ -68,6 +85,7 @@ __device__ __forceinline__ bool expert_tile(const int *offsets, int experts, int
         t.m = logical / tiles_n;
         t.n = logical - t.m * tiles_n;
       }
+      if (cut == CUT_REST) t.m = 2 * t.m + (quarter >> 1), t.n = 2 * t.n + (quarter & 1);
       return true;
     }
     before = __builtin_amdgcn_readlane(sum, 63);

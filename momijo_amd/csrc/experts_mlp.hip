@@ -17,6 +17,7 @@
 // bounds, and the few-row kernel takes the segments of 16 rows.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "expert_tile.h"
 #include "launch.h"
@@ -32,15 +33,17 @@ struct ExpertArgs {
   int64_t c_expert[3] = {};   // .. of its gradient (weight gradients)
   const int *offsets = nullptr;
   int experts = 0, rows = 0, n = 1, tail = 0, act = 0;
-  int tiles_n = 0;            // row products
+  int tiles_n = 0, cut = CUT_NONE;  // row products
   int tiles = 0;              // weight gradients: of one expert
 };
 
 // A product over the rows: the tile's expert and its operands.  SEGS: two K segments.
 template <int BM, int BN_OUT, int OUT, bool SEGS>
 __device__ __forceinline__ bool row_product(const ExpertArgs &a, TileProb &p, TileAt &at, ExpertTile &t) {
-  if (!expert_tile<true>(a.offsets, a.experts, a.rows, a.tail, BM, a.tiles_n, blockIdx.x, t)) return false;
   const TileProb &q = a.p[0];
+  const int bm = a.cut == CUT_REST ? 2 * BM : BM;
+  if (!expert_tile<true>(a.offsets, a.experts, a.rows, a.tail, bm, a.tiles_n, blockIdx.x, t, a.cut)) return false;
+  if (a.cut == CUT_REST && (t.m * BM >= t.rows || t.n * BN_OUT >= q.N)) return false;
   const int64_t row = (int64_t)t.row0 * q.lda;
   const bool none = t.expert == a.experts;  // rows of no expert: zeros
   const int64_t mat = none ? 0 : t.expert * a.b_expert;
@@ -238,6 +241,21 @@ double expert_time_us(int tile, int out, double tiles, int64_t stages) {
   return tile_time_us(kTileCost[tile], out, (int64_t)(tiles + 0.5), stages) * (tile == T_128 ? 1.08 : 1.0);
 }
 
+// Whether what 256 x 256 tiles leave over their whole rounds goes to 128 x 128 ones (expert_tile.h).
+// A last round of few tiles takes 1.2 to 1.6 us a stage, the quarters 0.75 to 0.98, and a
+// launch that finds nothing left 3 to 4: 8192 rows of 8 experts, 4096 and 5504 wide, h 826 -> 794
+// us (64 stages), dg, du 515 -> 473, y 403 -> 370 (86), dx 761 -> 721 (172).  With 32 stages (32
+// experts, 2048 and 1408 wide) h took 165 us so, 177 whole and 156 on 128 x 128 alone.
+bool cuts(int tile, int64_t stages) { return tile == T_256 && stages >= 48; }
+
+double rows_time_us(int tile, int out, double tiles, int64_t stages) {
+  if (!cuts(tile, stages)) return expert_time_us(tile, out, tiles, stages);
+  const double rest = tiles - std::floor(tiles / kTileRound) * kTileRound;
+  if (rest > CUT_REST_MOST) return expert_time_us(tile, out, tiles, stages) + 3.0;
+  if (rest < 1) return expert_time_us(tile, out, tiles, stages) + 3.0;
+  return expert_time_us(tile, out, tiles - rest, stages) + expert_time_us(T_128, out, 4 * CUT_REST_MOST, stages);
+}
+
 int plan_rows(const ExpertMlp &q, int64_t N, int64_t stages, int out) {
   int best = T_64S3;
   double best_us = 1e30;
@@ -245,7 +263,7 @@ int plan_rows(const ExpertMlp &q, int64_t N, int64_t stages, int out) {
     const TileCost &c = kTileCost[t];
     const int64_t bn = out == OUT_GATE ? c.bn / 2 : c.bn, tn = (N + bn - 1) / bn;
     if (!grid_fits(tn * expert_tiles_most(q.R, q.E + 1, c.bm), c.threads)) continue;
-    const double us = expert_time_us(t, out, (double)tn * likely_tiles(q, c.bm), stages);
+    const double us = rows_time_us(t, out, (double)tn * likely_tiles(q, c.bm), stages);
     if (us < best_us) best_us = us, best = t;
   }
   return best;
@@ -260,7 +278,12 @@ hipError_t launch_rows(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream) {
   const int64_t bm = kTileCost[tile].bm, bn = OUT == OUT_GATE ? kTileCost[tile].bn / 2 : kTileCost[tile].bn;
   a.offsets = q.offsets, a.experts = (int)q.E, a.rows = (int)q.R, a.act = q.act;
   a.tiles_n = (int)((p.N + bn - 1) / bn);
-  return launch_kernel<true, BKC, OUT>(tile, a, a.tiles_n * expert_tiles_most(q.R, q.E + a.tail, bm), stream);
+  const int64_t most = a.tiles_n * expert_tiles_most(q.R, q.E + a.tail, bm);
+  const bool cut = cuts(tile, stages);
+  a.cut = cut ? CUT_ROUNDS : CUT_NONE;
+  if (hipError_t e = launch_kernel<true, BKC, OUT>(tile, a, most, stream); e != hipSuccess || !cut) return e;
+  a.cut = CUT_REST;
+  return launch_kernel<true, BKC, OUT>(T_128, a, 4 * std::min<int64_t>(most, CUT_REST_MOST), stream);
 }
 
 int plan_weights(const ExpertMlp &q, const ExpertArgs &a) {
@@ -346,7 +369,7 @@ int64_t expert_dots_ld(const ExpertMlp &q) {
   if (q.R == 0 || q.I == 0) return 0;
   const TileCost &c = kTileCost[plan_rows(q, q.I, (q.H + kBK - 1) / kBK, OUT_DGATE)];
   const int64_t wn = c.bn == 256 ? 64 : c.bn / 2;  // columns of a wave
-  return (q.I + c.bn - 1) / c.bn * (c.bn / wn);
+  return (q.I + wn - 1) / wn;
 }
 
 hipError_t launch_experts_mlp(const ExpertMlp &q, hipStream_t stream) {

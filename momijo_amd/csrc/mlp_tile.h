@@ -281,7 +281,7 @@ __device__ __forceinline__ void out_dgate(const TileProb &p, const f32x4 (&acc)[
     if constexpr (EX) {
       dot += __shfl_xor(dot, 16, 64);
       dot += __shfl_xor(dot, 32, 64);
-      if (p.dots && fh == 0 && m < p.M) p.dots[(size_t)m * p.dots_ld + (n0 + wn * WN) / WN] = dot;
+      if (p.dots && fh == 0 && m < p.M && n0 + wn * WN < p.N) p.dots[(size_t)m * p.dots_ld + (n0 + wn * WN) / WN] = dot;
     }
   }
 }

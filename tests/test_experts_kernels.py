@@ -17,6 +17,20 @@ def test_every_kernel_of_the_experts_block(product):
     assert {name(*s, product).decode() for s in sizes} == TILES | ({"16 rows"} if product < 2 else set())
 
 
+@pytest.mark.parametrize("product", range(4))
+def test_rounds_of_the_experts_block(product):
+    """The sizes leave nothing, up to half a round and more than that over their whole rounds."""
+    rests = set()
+    for counts, K, I, H in kernels.ROUNDS:
+        name = _lib.load().mj_experts_mlp_kernel(sum(counts), len(counts) - 1, K, I, H, product)
+        assert name == b"256x256"
+        width, cols = ((I, 128), (H, 256), (I, 256), (K, 256))[product]
+        groups = counts if product % 2 else counts[:-1]  # y and dx have the dropped rows too
+        rests.add(sum(-(-c // 256) for c in groups) * -(-width // cols) % 256)
+    assert any(0 < r <= 128 for r in rests) and any(r > 128 for r in rests)
+    assert product % 2 == 0 or {0, 128} <= rests
+
+
 def test_every_kernel_of_the_8_bit_products():
     name = _lib.load().mj_gemm_f8_kernel
     tiles = {"256x256", "192x256", "128x128", "64x64"}

@@ -31,7 +31,11 @@ def _normal(g, shape, dt=torch.float32, std=1.0):
 
 def _ids(g, T, k, E, kind="even"):
     """Experts of T tokens: even, all of one expert (one), half of them dropped (drop), all
-    dropped (none), or each token's the same one k times (same)."""
+    dropped (none), each token's the same one k times (same), or so many of each expert and,
+    last, so many dropped (a tuple)."""
+    if isinstance(kind, tuple):
+        all_ids = torch.repeat_interleave(torch.arange(E + 1), torch.tensor(kind)).to("cuda")
+        return all_ids[torch.randperm(T * k, generator=g, device="cuda")].reshape(T, k)
     ids = torch.randint(0, E, (T, k), generator=g, device="cuda")
     if kind == "one":
         ids.fill_(E // 2)

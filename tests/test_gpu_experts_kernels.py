@@ -25,6 +25,16 @@ EXPERTS = [(3519, 1, 2, 208, 560, 128), (4457, 1, 2, 120, 352, 96), (3529, 1, 2,
            (3844, 1, 2, 144, 2592, 96), (1945, 1, 2, 2056, 96, 128), (2551, 1, 2, 1192, 112, 168),
            (4963, 1, 3, 1816, 96, 128), (59, 3, 24, 944, 96, 144), (95, 5, 22, 280, 152, 96),
            (494, 2, 7, 2440, 136, 176), (139, 1, 26, 200, 104, 104), (4001, 2, 4, 1032, 3000, 1096)]
+# rows of each expert, dropped rows, then K, I, H: what the whole rounds of 256 x 256 tiles leave over,
+# in quarters (up to half a round: one tile, quarters past the rows and the columns) or in whole tiles
+ROUNDS = [((1500, 2050, 1300, 250), 3376, 3376, 3376), ((4090, 1, 2049, 900), 4088, 4088, 4088),
+          ((1400, 2600, 2060, 10), 3240, 3304, 3240), ((1400, 2600, 1290, 10), 4088, 3376, 4088),
+          ((2000, 2600, 3000, 250), 4088, 3376, 4088)]
+
+
+@pytest.mark.parametrize("counts,K,I,H", ROUNDS)
+def test_rounds_of_experts(dev, counts, K, I, H):
+    experts.test_experts(dev, sum(counts), 1, len(counts) - 1, K, I, H, counts)
 
 
 @pytest.mark.parametrize("M,N,K", LINEAR)
