@@ -632,7 +632,8 @@ int32_t mj_gated_mlp_backward_f32(const float *x, const float *Wg, const float *
 /* The sort: pos [slots] is each slot's row among the rows sorted by expert, in the order of
  * the slots within an expert; offsets [experts + 1] the experts' first rows.  ids [slots]
  * are int32 or int64 (id_bytes 4, 8); a slot whose id is outside 0 .. experts - 1 is dropped:
- * such slots come last, in their order, from row offsets[experts] on. */
+ * such slots come last, in their order, from row offsets[experts] on.  (The entry points that
+ * take pos and offsets keep inside their arrays whatever these hold.) */
 int64_t mj_sort_experts_work_bytes(int64_t slots, int64_t experts);
 int32_t mj_sort_experts(const void *ids, int32_t id_bytes, int64_t slots, int64_t experts, int32_t *pos,
                         int32_t *offsets, void *work, int64_t work_bytes, void *stream);
@@ -661,9 +662,9 @@ int32_t mj_combine_backward(int32_t dtype, const void *dy, const void *ys, const
  * expert); row r of expert e:
  *   g = x Wg_e^T, u = x Wu_e^T, h = weights[r] act(g) u, y = h Wd_e^T
  * xs [R,K], Wg and Wu [experts,I,K], Wd [experts,H,I], h [R,I], ys [R,H] fp32 (a token's rows
- * are added before they are rounded), weights [R] fp32 or NULL (ones); g, u fp32 [R,I] are written for the backward, or both NULL.  K, I, H
- * multiples of 8 below 2^22, arrays 16-byte aligned.  ys's rows from offsets[experts] on
- * become zeros; h, g and u's stay as they were. */
+ * are added before they are rounded), weights [R] fp32 or NULL (ones); g, u fp32 [R,I] are
+ * written for the backward, or both NULL.  K, I, H multiples of 8 below 2^22, arrays 16-byte
+ * aligned.  ys's rows from offsets[experts] on become zeros; h, g and u's stay as they were. */
 int32_t mj_experts_mlp_bf16(const uint16_t *xs, const int32_t *offsets, int64_t experts, const uint16_t *Wg,
                             const uint16_t *Wu, const uint16_t *Wd, int32_t act, const float *weights,
                             uint16_t *h, float *g, float *u, float *ys, int64_t R, int64_t K, int64_t I,
@@ -673,9 +674,9 @@ int32_t mj_experts_mlp_bf16(const uint16_t *xs, const int32_t *offsets, int64_t 
  *   dh = dy Wd_e, dg = weights[r] dh u act'(g), du = weights[r] dh act(g)
  *   dx = dg Wg_e + du Wu_e, dWg_e = dg^T x, dWu_e = du^T x, dWd_e = dy^T h
  *   dw[slot] = <dh, act(g) u> of row pos[slot], 0 for a dropped slot
- * dxs [R,K] is fp32, as ys.  dg, du [R,I] are scratch, and with dw dots of mj_experts_mlp_dots floats; any of dxs, dWg,
- * dWu, dWd, dw may be NULL.  An expert without rows gets zeros, and so do dxs's rows from
- * offsets[experts] on. */
+ * dxs [R,K] is fp32, as ys.  dg, du [R,I] are scratch, and with dw dots of
+ * mj_experts_mlp_dots floats; any of dxs, dWg, dWu, dWd, dw may be NULL.  An expert without
+ * rows gets zeros, and so do dxs's rows from offsets[experts] on. */
 int64_t mj_experts_mlp_dots(int64_t R, int64_t experts, int64_t K, int64_t I, int64_t H);
 int32_t mj_experts_mlp_backward_bf16(const uint16_t *xs, const int32_t *offsets, int64_t experts,
                                      const uint16_t *Wg, const uint16_t *Wu, const uint16_t *Wd, int32_t act,
@@ -694,10 +695,11 @@ const char *mj_experts_mlp_kernel(int64_t R, int64_t experts, int64_t K, int64_t
  * Products of e4m3 values (largest 448) with a scale for each block of 128 features of a
  * row (x) or 128 x 128 elements (W), for inference (no reference counterpart).  A block of
  * largest magnitude m is quantized with a = max(m, 2^-100): scale a * (1 / 448), values
- * e4m3(v * (448 * (1 / a))) to the nearest even, each operation rounded to fp32.  A NaN stays a NaN; an infinity becomes one, with
- * an infinite scale.  Widths K are multiples of 16, widths below 2^22, rows at most 2^31 -
- * 1024, arrays of values 16-byte aligned.  Scales of x lie block by block, [ceil(K / 128)]
- * [rows], those of W as [ceil(N / 128)][ceil(K / 128)].  Scratch memory is the caller's. */
+ * e4m3(v * (448 * (1 / a))) to the nearest even, each operation rounded to fp32.  A NaN stays a
+ * NaN; an infinity becomes one, with an infinite scale.  Widths K are multiples of 16,
+ * widths below 2^22, rows at most 2^31 - 1024, arrays of values 16-byte aligned.  Scales of
+ * x lie block by block, [ceil(K / 128)][rows], those of W as [ceil(N / 128)][ceil(K / 128)].
+ * Scratch memory is the caller's. */
 int32_t mj_quantize_rows_f8(int32_t dtype, const void *x, uint8_t *q, float *scales, int64_t rows, int64_t K,
                             void *stream);
 int32_t mj_quantize_blocks_f8(int32_t dtype, const void *W, uint8_t *q, float *scales, int64_t mats, int64_t N,

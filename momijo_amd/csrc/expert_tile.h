@@ -4,6 +4,8 @@
 // and its workgroups past the last tile end at once.
 #pragma once
 
+#include <algorithm>
+
 #include "common.h"
 
 namespace mj {
@@ -12,6 +14,10 @@ struct ExpertTile {
   int expert, row0, rows;  // of the whole expert; expert == experts: the rows behind the last
   int m, n;                // tile
 };
+
+// An entry of the sort's results, kept inside the rows: a plan that is none (a caller's own
+// or overwritten) gives meaningless results, but no access outside the arrays.
+__device__ __forceinline__ int within(int at, int rows) { return std::min(std::max(at, 0), rows); }
 
 // An inclusive sum over a wave's lanes.
 __device__ __forceinline__ int wave_scan(int v) {
@@ -45,8 +51,8 @@ __device__ __forceinline__ bool expert_tile(const int *offsets, int experts, int
   const int lane = threadIdx.x & 63, groups = experts + (tail ? 1 : 0);
   auto counts = [&](int g0, int &start, int &n) __attribute__((always_inline)) {
     const int g = g0 + lane;
-    start = g < groups ? offsets[g] : 0;
-    n = g < groups ? (g < experts ? offsets[g + 1] : rows) - start : 0;
+    start = g < groups ? within(offsets[g], rows) : 0;
+    n = g < groups ? std::max((g < experts ? within(offsets[g + 1], rows) : rows) - start, 0) : 0;
     return (n + bm - 1) / bm;
   };
   int start, n, total_m = 0;
@@ -85,6 +91,7 @@ __device__ __forceinline__ bool expert_tile(const int *offsets, int experts, int
         t.m = logical / tiles_n;
         t.n = logical - t.m * tiles_n;
       }
+      if ((uint32_t)t.m >= (uint32_t)tiles_m || (uint32_t)t.n >= (uint32_t)tiles_n) return false;
       if (cut == CUT_REST) t.m = 2 * t.m + (quarter >> 1), t.n = 2 * t.n + (quarter & 1);
       return true;
     }

@@ -17,6 +17,7 @@
 #include <atomic>
 
 #include "common.h"
+#include "expert_tile.h"  // within
 #include "launch.h"
 #include "philox.h"  // u32x4_a2
 
@@ -219,13 +220,19 @@ __device__ __forceinline__ bool unit_of(int64_t i, int64_t units, int64_t tokens
   return t < tokens;
 }
 
+// The rows of slots that are not dropped.
+__device__ __forceinline__ int kept_rows(const ExpertRows &a) {
+  return within(*a.kept, (int)(a.tokens * a.topk));
+}
+
 template <bool BF>
 __global__ __launch_bounds__(256) void dispatch_kernel(ExpertRows a) {
   using U = Unit<BF>;
   int64_t t, u;
   if (!unit_of(grid_block<256>() * 256 + threadIdx.x, a.units, a.tokens, t, u)) return;
   const int64_t e = u * U::N;
-  const int have = (int)std::min<int64_t>(a.dim - e, U::N), kept = *a.kept, k = (int)a.topk;
+  const int have = (int)std::min<int64_t>(a.dim - e, U::N), kept = kept_rows(a), k = (int)a.topk;
+  const uint32_t rows = (uint32_t)(a.tokens * a.topk);
   U x, zero;
   x.load((const char *)a.x + t * a.dim * U::SIZE, e, have);
   zero.w = u32x4_a2{0, 0, 0, 0};
@@ -233,6 +240,7 @@ __global__ __launch_bounds__(256) void dispatch_kernel(ExpertRows a) {
 #pragma unroll 4
   for (int j = 0; j < k; ++j) {
     const int p = pos[j];
+    if ((uint32_t)p >= rows) continue;
     char *row = (char *)a.xs + (int64_t)p * a.dim * U::SIZE;
     if (p < kept) x.store(row, e, have);
     else zero.store(row, e, have);
@@ -250,7 +258,8 @@ __global__ __launch_bounds__(256) void combine_kernel(ExpertRows a) {
   int64_t t, u;
   if (!unit_of(grid_block<256>() * 256 + threadIdx.x, a.units, a.tokens, t, u)) return;
   const int64_t e = u * N;
-  const int have = (int)std::min<int64_t>(a.dim - e, N), kept = *a.kept, k = (int)a.topk;
+  const int have = (int)std::min<int64_t>(a.dim - e, N), k = (int)a.topk;
+  const uint32_t kept = kept_rows(a);
   const int *pos = a.pos + t * k;
   float acc[N] = {};
   auto load = [&](UI (&v)[P], int p) __attribute__((always_inline)) {
@@ -266,7 +275,7 @@ __global__ __launch_bounds__(256) void combine_kernel(ExpertRows a) {
   constexpr int FLY = 8 / P;  // rows' loads in flight
   for (int j0 = 0; j0 < k; j0 += FLY) {
     UI v[FLY][P];
-    int p[FLY];
+    uint32_t p[FLY];
 #pragma unroll
     for (int q = 0; q < FLY; ++q) p[q] = j0 + q < k ? pos[j0 + q] : 0x7FFFFFFF;
 #pragma unroll
@@ -291,19 +300,21 @@ __global__ __launch_bounds__(NW * 64) void combine_bwd_kernel(ExpertRows a) {
   __shared__ float red[2][kDotSlots][NW];
   const int64_t t = grid_block<NW * 64>();
   if (t >= a.tokens) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kept = *a.kept, k = (int)a.topk;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kept = kept_rows(a), k = (int)a.topk;
+  const uint32_t rows = (uint32_t)(a.tokens * a.topk);
   const char *dy = (const char *)a.x + t * a.dim * U::SIZE;
   for (int j0 = 0, half = 0; j0 < k; j0 += kDotSlots, half ^= 1) {
     const int n = std::min(k - j0, kDotSlots);
     int64_t row[kDotSlots];
-    bool in[kDotSlots];
+    bool in[kDotSlots], is[kDotSlots];
     float w[kDotSlots], sum[kDotSlots];
 #pragma unroll
     for (int q = 0; q < kDotSlots; ++q) {
       const int64_t slot = t * k + j0 + (q < n ? q : 0);
       const int p = a.pos[slot];
       row[q] = (int64_t)p * a.dim * U::SIZE;
-      in[q] = p < kept;
+      is[q] = q < n && (uint32_t)p < rows;
+      in[q] = is[q] && p < kept;
       w[q] = a.w[slot];
       sum[q] = 0.0f;
     }
@@ -313,10 +324,10 @@ __global__ __launch_bounds__(NW * 64) void combine_bwd_kernel(ExpertRows a) {
       d.load(dy, e, have);
 #pragma unroll
       for (int q = 0; q < kDotSlots; ++q)
-        if (q < n && in[q]) y[q].template load<NT>((const char *)a.ys + row[q], e, have);
+        if (in[q]) y[q].template load<NT>((const char *)a.ys + row[q], e, have);
 #pragma unroll
       for (int q = 0; q < kDotSlots; ++q) {
-        if (q >= n) continue;
+        if (!is[q]) continue;
         U o;
         float v[U::N];
         if (in[q]) {

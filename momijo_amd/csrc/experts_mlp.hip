@@ -92,12 +92,12 @@ __device__ __forceinline__ void weight_product(const ExpertArgs &a, TileProb &p,
   if (a.n > 2 && logical >= a.p[2].first) at.prob = 2;
   const TileProb &s = a.p[at.prob];
   // (scalars: loaded values would be kept in vector registers)
-  const int row = __builtin_amdgcn_readfirstlane(a.offsets[e]);
-  const int end = __builtin_amdgcn_readfirstlane(a.offsets[e + 1]);
+  const int row = within(__builtin_amdgcn_readfirstlane(a.offsets[e]), a.rows);
+  const int end = within(__builtin_amdgcn_readfirstlane(a.offsets[e + 1]), a.rows);
   p.lda = s.lda, p.ldb = s.ldb;
   p.A[0] = p.A[1] = s.A[0] + row * s.lda;
   p.B[0] = p.B[1] = s.B[0] + row * s.ldb;
-  p.M = s.M, p.N = s.N, p.K = end - row, p.segs = 1;
+  p.M = s.M, p.N = s.N, p.K = std::max(end - row, 0), p.segs = 1;
   group_coords(logical - s.first, s.tiles_m, s.tiles_n, 4, at.m, at.n);
 }
 
@@ -175,12 +175,12 @@ __global__ __launch_bounds__(NW * 64) void experts_skinny_kernel(ExpertSkinny a)
 // dw of a slot: its row's parts, one wave a slot, in a fixed order; 0 for a dropped slot.
 __global__ __launch_bounds__(256) void expert_dots_kernel(const int *pos, const int *kept,
                                                           const float *dots, int ld, float *dw,
-                                                          int64_t slots) {
+                                                          int64_t slots, int rows) {
   const int64_t slot = grid_block<256>() * 4 + (threadIdx.x >> 6);
   if (slot >= slots) return;
   const int lane = threadIdx.x & 63, p = pos[slot];
   float sum = 0.0f;
-  if (p < *kept)
+  if (p >= 0 && p < within(*kept, rows))
     for (int c = lane; c < ld; c += 64) sum += dots[(int64_t)p * ld + c];
   sum = wave_sum_dpp(sum);
   if (lane == 0) dw[slot] = sum;
@@ -313,7 +313,7 @@ hipError_t launch_weights(const ExpertMlp &q, ExpertArgs &a, hipStream_t stream)
     p.first = a.tiles;
     a.tiles += p.tiles_m * p.tiles_n;
   }
-  a.offsets = q.offsets, a.experts = (int)q.E;
+  a.offsets = q.offsets, a.experts = (int)q.E, a.rows = (int)q.R;
   return launch_kernel<false, false, OUT_STORE>(tile, a, (int64_t)a.tiles * q.E, stream);
 }
 
@@ -417,7 +417,7 @@ hipError_t launch_experts_mlp_bwd(const ExpertMlp &q, const ExpertMlpGrad &o, hi
   if (o.dw && o.slots > 0) {
     const dim3 grid = grid_rows<256>((o.slots + 3) / 4);
     hipLaunchKernelGGL(expert_dots_kernel, grid, dim3(256), 0, stream, o.pos, q.offsets + q.E, o.dots,
-                       (int)expert_dots_ld(q), o.dw, o.slots);
+                       (int)expert_dots_ld(q), o.dw, o.slots, (int)q.R);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (o.dxs) {

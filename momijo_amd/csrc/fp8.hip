@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "expert_tile.h"  // within
 #include "fp8.h"
 #include "launch.h"
 
@@ -67,10 +68,11 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(F8Rows a) {
     put(t, q, s.scale);
     return;
   }
-  const int kept = *a.kept, k = (int)a.topk;
+  const int kept = within(*a.kept, (int)a.rows), k = (int)a.topk;
 #pragma unroll 4
   for (int j = 0; j < k; ++j) {
     const int p = a.pos[t * k + j];
+    if ((uint32_t)p >= (uint32_t)a.rows) continue;
     const bool on = p < kept;
     put(p, on ? q : make_uint2(0, 0), on ? s.scale : 0.0f);
   }

@@ -35,10 +35,11 @@ def _check_device(t: torch.Tensor, name: str) -> None:
 
 
 class ExpertPlan:
-    """Where the slots go, as ``sort_experts`` finds it (the kernels trust its entries).  pos
-    int32 [tokens, topk]: a slot's row among those sorted by expert (in the order of the slots
-    within an expert, dropped slots last); offsets int32 [experts + 1]: the experts' first
-    rows, the last entry the first dropped slot's."""
+    """Where the slots go, as ``sort_experts`` finds it.  pos int32 [tokens, topk]: a slot's row
+    among those sorted by expert (in the order of the slots within an expert, dropped slots
+    last); offsets int32 [experts + 1]: the experts' first rows, the last entry the first
+    dropped slot's.  A plan of other entries gives meaningless rows, but no access outside the
+    tensors."""
 
     __slots__ = ("pos", "offsets", "tokens", "topk", "rows", "experts", "device", "_args")
 
@@ -236,8 +237,9 @@ def experts_mlp_train(xs: torch.Tensor, plan: ExpertPlan, gate: torch.Tensor, up
 
 def experts_mlp_backward(dys: torch.Tensor, saved: ExpertsSaved):
     """(dxs, dgate, dup, ddown, dweights) of experts_mlp from dys, bfloat16; dxs and dweights
-    are Float32.  An expert without rows gets zeros; dxs's rows of dropped slots are zeros; dweights [tokens, topk] is the gradient of the
-    unsorted weights, or None without weights.  dys's rows of dropped slots are not read."""
+    are Float32.  An expert without rows gets zeros, and so do dxs's rows of dropped slots;
+    dweights [tokens, topk] is the gradient of the unsorted weights, or None without weights.
+    dys's rows of dropped slots are not read."""
     s = saved
     xs, plan, dev = s.xs, s.plan, s.xs.device
     (R, K), (E, I, _), H = xs.shape, s.gate.shape, s.down.shape[1]

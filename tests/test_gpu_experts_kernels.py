@@ -94,6 +94,42 @@ def test_no_tokens(dev):
     assert mj.F8Experts.from_float(*m).forward(x, ids, w).shape == (0, 16)
 
 
+@pytest.mark.parametrize("T,k,E,K", [(9, 2, 4, 64), (400, 3, 5, 272), (5000, 1, 3, 1040)])
+def test_plans_that_are_none(dev, T, k, E, K):
+    """A caller's own plan, or one that was overwritten: results mean nothing, but what lies around
+    the sorted rows stays as it was, and so do the operands."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    big = 2 ** 31 - 1
+    rows = T * k
+    pos = torch.randint(-2 * rows, 3 * rows, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    pos[0, 0], pos[-1, -1], pos[1, 0] = big, -big - 1, rows
+    m = [torch.randn(*s, generator=g, device="cuda").bfloat16() for s in ((E, 80, K), (E, 80, K), (E, K, 80))]
+    x, dy = (torch.randn(T, K, generator=g, device="cuda").bfloat16() for _ in range(2))
+    w = torch.rand(T, k, generator=g, device="cuda")
+    before = [t.clone() for t in (x, dy, w, *m)]
+    f8 = mj.F8Experts.from_float(*m)
+    for ends in ([0, big, -5, 7], [rows + 1, rows, 0, -big - 1], [0, rows, 0, rows], [5, 5, 3, big]):
+        offsets = torch.tensor([ends[i % 4] for i in range(E + 1)], dtype=torch.int32, device="cuda")
+        plan = mj.ExpertPlan(pos, offsets)
+        xs, ws = mj.dispatch(x, plan, w)
+        ys, saved = mj.experts_mlp_train(xs, plan, *m, weights=ws)
+        mj.experts_mlp_backward(mj.dispatch(dy, plan), saved)
+        mj.combine(ys, w, plan)
+        mj.combine_backward(dy, xs, w, plan)
+        q, s = mj.dispatch_fp8(x, plan)
+        hq, hs = mj.experts_gate_fp8(q, s, plan, f8.gate, f8.gate_scales, f8.up, f8.up_scales)
+        mj.experts_gemm_fp8(hq, hs, plan, f8.down, f8.down_scales)
+        guard = torch.full((rows + 8, K), 7.0, dtype=torch.bfloat16, device="cuda")
+        wide = torch.full((rows + 8,), 7.0, device="cuda")
+        mj._lib.call("mj_dispatch", 1, x.data_ptr(), w.data_ptr(), *plan._args, guard[4:].data_ptr(),
+                     wide[4:].data_ptr(), T, k, K, None)
+        mj._lib.call("mj_combine_backward", 1, dy.data_ptr(), xs.data_ptr(), w.data_ptr(), *plan._args,
+                     guard[4:].data_ptr(), w.clone().data_ptr(), T, k, K, None)
+        for t in (guard, wide):
+            assert bool((t[:4] == 7).all()) and bool((t[-4:] == 7).all())
+        assert all(torch.equal(a, b) for a, b in zip(before, (x, dy, w, *m)))
+
+
 def test_rows_past_2_32_bytes(dev):
     """Sorted rows of more than 2^32 bytes and 2^31 elements: the last ones are the tokens'."""
     T, k, D = 70000, 4, 8200
