@@ -19,8 +19,9 @@ import torch
 
 from . import _lib
 from .block import _check_type, _scratch
-from .experts import ExpertPlan, _aligned, _check_device, _contiguous, _rows_of, combine, sort_experts
-from .tensor import _ptr, _stream
+from .experts import (ExpertPlan, _aligned, _check_device, _contiguous, _rows_of, _stream, combine,
+                      sort_experts)
+from .tensor import _ptr
 
 _F8 = torch.float8_e4m3fn
 
@@ -40,7 +41,7 @@ def quantize_rows_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     q = torch.empty((M, K), dtype=_F8, device=x.device)
     scales = torch.empty((_blocks(K), M), dtype=torch.float32, device=x.device)
     _lib.call("mj_quantize_rows_f8", code, x.data_ptr(), q.data_ptr(), scales.data_ptr(), M, K,
-              _stream())
+              _stream(x))
     return q, scales
 
 
@@ -56,7 +57,7 @@ def quantize_blocks_fp8(W: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     q = torch.empty(W.shape, dtype=_F8, device=W.device)
     scales = torch.empty((*W.shape[:-2], _blocks(N), _blocks(K)), dtype=torch.float32, device=W.device)
     _lib.call("mj_quantize_blocks_f8", code, W.data_ptr(), q.data_ptr(), scales.data_ptr(), mats, N, K,
-              _stream())
+              _stream(W))
     return q, scales
 
 
@@ -110,7 +111,7 @@ def gemm_fp8_nt(q: torch.Tensor, scales: torch.Tensor, Wq: torch.Tensor, Wscales
     nbytes = _work("mj_gemm_f8_work_bytes", M, N, K)
     work = _scratch(nbytes, q.device) if nbytes else None
     _lib.call("mj_gemm_f8", q.data_ptr(), scales.data_ptr(), Wq.data_ptr(), Wscales.data_ptr(),
-              _ptr(bias), act, y.data_ptr(), M, N, K, _ptr(work), nbytes, _stream())
+              _ptr(bias), act, y.data_ptr(), M, N, K, _ptr(work), nbytes, _stream(q))
     return y
 
 
@@ -142,7 +143,7 @@ class F8Linear:
         nbytes = _work("mj_linear_f8_work_bytes", M, N, K)
         work = _scratch(nbytes, x.device) if nbytes else None
         _lib.call("mj_linear_f8", code, x.data_ptr(), self.q.data_ptr(), self.scales.data_ptr(),
-                  _ptr(self.bias), self.act, y.data_ptr(), M, N, K, _ptr(work), nbytes, _stream())
+                  _ptr(self.bias), self.act, y.data_ptr(), M, N, K, _ptr(work), nbytes, _stream(x))
         return y
 
 
@@ -155,7 +156,7 @@ def dispatch_fp8(x: torch.Tensor, plan: ExpertPlan) -> tuple[torch.Tensor, torch
     q = torch.empty((plan.rows, K), dtype=_F8, device=x.device)
     scales = torch.empty((_blocks(K), plan.rows), dtype=torch.float32, device=x.device)
     _lib.call("mj_dispatch_f8", code, x.data_ptr(), *plan._args, q.data_ptr(), scales.data_ptr(),
-              plan.tokens, plan.topk, K, _stream())
+              plan.tokens, plan.topk, K, _stream(x))
     return q, scales
 
 
@@ -176,7 +177,7 @@ def experts_gemm_fp8(q: torch.Tensor, scales: torch.Tensor, plan: ExpertPlan, Wq
     (R, K), (E, N, _) = q.shape, Wq.shape
     y = torch.empty((R, N), dtype=torch.float32, device=q.device)
     _lib.call("mj_experts_gemm_f8", q.data_ptr(), scales.data_ptr(), plan.offsets.data_ptr(), E,
-              Wq.data_ptr(), Wscales.data_ptr(), y.data_ptr(), R, N, K, _stream())
+              Wq.data_ptr(), Wscales.data_ptr(), y.data_ptr(), R, N, K, _stream(q))
     return y
 
 
@@ -196,7 +197,7 @@ def experts_gate_fp8(q: torch.Tensor, scales: torch.Tensor, plan: ExpertPlan, ga
     work = _scratch(nbytes, q.device) if nbytes else None
     _lib.call("mj_experts_gate_f8", q.data_ptr(), scales.data_ptr(), plan.offsets.data_ptr(), E,
               gate.data_ptr(), gate_scales.data_ptr(), up.data_ptr(), up_scales.data_ptr(), act,
-              hq.data_ptr(), hs.data_ptr(), R, I, K, _ptr(work), nbytes, _stream())
+              hq.data_ptr(), hs.data_ptr(), R, I, K, _ptr(work), nbytes, _stream(q))
     return hq, hs
 
 

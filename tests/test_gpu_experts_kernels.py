@@ -94,6 +94,29 @@ def test_no_tokens(dev):
     assert mj.F8Experts.from_float(*m).forward(x, ids, w).shape == (0, 16)
 
 
+def test_another_current_device(dev, monkeypatch):
+    """Tensors of a device that is not the current one are refused, with saved operands too."""
+    T, k, E, K = 6, 2, 3, 32
+    m = [torch.ones(*s, dtype=torch.bfloat16, device="cuda") for s in ((E, 16, K), (E, 16, K), (E, K, 16))]
+    x, w = torch.ones(T, K, dtype=torch.bfloat16, device="cuda"), torch.ones(T, k, device="cuda")
+    ids = torch.zeros(T, k, dtype=torch.int32, device="cuda")
+    plan = mj.sort_experts(ids, E)
+    xs, ws = mj.dispatch(x, plan, w)
+    ys, saved = mj.experts_mlp_train(xs, plan, *m, weights=ws)
+    f8, (q, s), lin = mj.F8Experts.from_float(*m), mj.dispatch_fp8(x, plan), mj.F8Linear.from_float(m[0][0])
+    rows = mj.quantize_rows_fp8(x)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    for call in (lambda: mj.sort_experts(ids, E), lambda: mj.dispatch(x, plan, w), lambda: mj.combine(ys, w, plan),
+                 lambda: mj.dispatch_backward(ys, plan), lambda: mj.combine_backward(x, xs, w, plan),
+                 lambda: mj.experts_mlp(xs, plan, *m), lambda: mj.experts_mlp_backward(xs, saved),
+                 lambda: mj.quantize_rows_fp8(x), lambda: mj.quantize_blocks_fp8(m[0]), lambda: lin.forward(x),
+                 lambda: mj.gemm_fp8_nt(*rows, lin.q, lin.scales), lambda: mj.dispatch_fp8(x, plan),
+                 lambda: mj.experts_gate_fp8(q, s, plan, f8.gate, f8.gate_scales, f8.up, f8.up_scales),
+                 lambda: mj.experts_gemm_fp8(q, s, plan, f8.gate, f8.gate_scales)):
+        with pytest.raises(ValueError, match="current device"):
+            call()
+
+
 @pytest.mark.parametrize("T,k,E,K", [(9, 2, 4, 64), (400, 3, 5, 272), (5000, 1, 3, 1040)])
 def test_plans_that_are_none(dev, T, k, E, K):
     """A caller's own plan, or one that was overwritten: results mean nothing, but what lies around
