@@ -605,7 +605,7 @@ __global__ __launch_bounds__(256) void f8_sum_kernel(F8Product q, int splits) {
 // weight rows (gate/up: of each) and deals the K blocks to its waves in turn; a lane's 32
 // bytes of a row's 128 are its fragment as they are.  A wave has U blocks' loads in
 // flight.  The waves' sums are added in wave order.  One row, 4096 x 11008 columns, x quantized
-// in it: 9.7 us (4.7 TB/s); 96 rows of 8 experts, 4096 and 11008 wide: h 158 (4.6), y 99 (3.6).
+// in it: 9.7 us (4.7 TB/s); 96 rows of 8 experts, 4096 and 11008 wide: h 158 (4.6), y 90 (4.0).
 //
 // XT: x comes quantized (X_F8), or in its own type: then each workgroup quantizes it into
 // LDS (32 lanes a block) while its first weights are on their way, which saves a launch.
@@ -649,10 +649,15 @@ struct FourOf {
   }
 };
 
+// Weight rows of a workgroup (gate/up: of each).  With 32 rows of x, 32 weight rows: with 16 it
+// reads up to twice as much of x from L2 as of the weights from memory (96 rows of 8 experts,
+// 11008 features, 4096 columns: 90 us, 99 with 16).
+constexpr int skinny_cols(int out, int mb) { return out == F8_ROWS && mb == 2 ? 32 : 16; }
+
 template <int OUT, int MB, int NW, int U, bool EX, int XT>
 __global__ __launch_bounds__(NW * 64) void f8_skinny_kernel(F8Tiles args) {
   constexpr bool GATE = OUT == F8_GATE;
-  constexpr int G = GATE ? 2 : 1;
+  constexpr int COLS = skinny_cols(OUT, MB), G = GATE ? 2 : COLS / 16;
   static_assert(XT == X_F8 || (MB == 1 && !EX), "rows in LDS");
   __shared__ float red[NW][G][MB][16][17];
   extern __shared__ __attribute__((aligned(16))) char xlds[];
@@ -664,16 +669,18 @@ __global__ __launch_bounds__(NW * 64) void f8_skinny_kernel(F8Tiles args) {
                             blockIdx.x, t))
       return;
     f8_operands(args.p, t.expert, t.row0 + t.m * 16 * MB, t.rows - t.m * 16 * MB, p);
-    n0 = t.n * 16;
+    n0 = t.n * COLS;
   } else {
     f8_operands(args.p, 0, 0, (int)args.p.M, p);
-    n0 = blockIdx.x * 16;
+    n0 = blockIdx.x * COLS;
   }
   const int lane = threadIdx.x & 63, fr = lane & 15, fh = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = p.N - n0 < 16 ? p.N - n0 : 16, K = p.K, kbs = p.kbs;
+  // (the second 16: the up projection's, or the next ones)
+  const int rows2 = GATE ? rows : std::min(std::max(p.N - n0 - 16, 0), 16);
   const auto rw = make_rsrc(p.w + (size_t)n0 * K, (int64_t)rows * K);
-  const auto rw2 = make_rsrc(p.w2 + (size_t)n0 * K, (int64_t)rows * K);
+  const auto rw2 = make_rsrc(GATE ? p.w2 + (size_t)n0 * K : p.w + (size_t)(n0 + 16) * K, (int64_t)rows2 * K);
   const int xr = p.M < 16 * MB ? p.M : 16 * MB;
   const auto rx = make_rsrc(p.x, (int64_t)xr * K);
   const int64_t block = (int64_t)(n0 / 128) * kbs;
@@ -695,7 +702,8 @@ __global__ __launch_bounds__(NW * 64) void f8_skinny_kernel(F8Tiles args) {
         const int k = kb * 128 + fh * 32 + h * 16;
         const uint32_t wo = k < K && fr < rows ? (uint32_t)(fr * K + k) : kOobOffset;
         wv[u][0][h] = buffer_load16(rw, wo);
-        if constexpr (GATE) wv[u][1][h] = buffer_load16(rw2, wo);
+        if constexpr (G == 2)
+          wv[u][1][h] = buffer_load16(rw2, k < K && fr < rows2 ? (uint32_t)(fr * K + k) : kOobOffset);
         if constexpr (XT == X_F8) {
 #pragma unroll
           for (int b = 0; b < MB; ++b)
@@ -705,6 +713,7 @@ __global__ __launch_bounds__(NW * 64) void f8_skinny_kernel(F8Tiles args) {
       const uint32_t so = kb < kbs ? (uint32_t)kb * 4 : kOobOffset;
       ws[u][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, so, 0, 0));
       if constexpr (GATE) ws[u][1] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs2, so, 0, 0));
+      else if constexpr (G == 2) ws[u][1] = ws[u][0];  // (32 columns from a multiple of 32: one block)
       if constexpr (XT == X_F8) {
 #pragma unroll
         for (int b = 0; b < MB; ++b)
@@ -772,7 +781,7 @@ __global__ __launch_bounds__(NW * 64) void f8_skinny_kernel(F8Tiles args) {
   __syncthreads();
   for (int e = threadIdx.x; e < MB * 256; e += NW * 64) {
     const int b = e >> 8, r = (e >> 4) & 15, c = e & 15, m = b * 16 + r, n = n0 + c;
-    if (m >= p.M || n >= p.N) continue;
+    if (m >= p.M || n >= p.N) continue;  // (N ends the second 16 in the store)
     float v[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -785,6 +794,7 @@ __global__ __launch_bounds__(NW * 64) void f8_skinny_kernel(F8Tiles args) {
       args.p.h[o] = apply_epi_b16(args.p.epi, v[0]) * v[1];
     } else if constexpr (OUT == F8_ROWS) {
       args.p.h[o] = v[0];
+      if (G == 2 && n + 16 < p.N) args.p.h[o + 16] = v[G - 1];
     } else {
       const float y = v[0] + (args.p.bias ? args.p.bias[n] : 0.0f);
       args.p.y[o] = (uint16_t)f32_to_bf16_bits(apply_epi_b16(args.p.epi, y));
@@ -950,8 +960,10 @@ template <int OUT>
 hipError_t launch_few_rows(F8Tiles &a, hipStream_t stream) {
   const F8Product &q = a.p;
   const int64_t groups = q.experts + q.tail;
-  a.tiles_n = (int)((q.N + 15) / 16);
-  if (q.M > 8 * std::min<int64_t>(q.M, q.experts))
+  const bool two = q.M > 8 * std::min<int64_t>(q.M, q.experts);
+  const int cols = skinny_cols(OUT, two ? 2 : 1);
+  a.tiles_n = (int)((q.N + cols - 1) / cols);
+  if (two)
     return launch_skinny<OUT, 2, 8, 1, true, X_F8>(a, a.tiles_n * expert_tiles_most(q.M, groups, 32), stream);
   return launch_skinny<OUT, 1, 8, 1, true, X_F8>(a, a.tiles_n * expert_tiles_most(q.M, groups, 16), stream);
 }
