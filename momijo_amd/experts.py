@@ -16,6 +16,7 @@ through torch only.
 from __future__ import annotations
 
 import functools
+import operator
 from typing import NamedTuple
 
 import torch
@@ -47,9 +48,12 @@ class ExpertPlan:
     among those sorted by expert (in the order of the slots within an expert, dropped slots
     last); offsets int32 [experts + 1]: the experts' first rows, the last entry the first
     dropped slot's.  A plan of other entries gives meaningless rows, but no access outside the
-    tensors."""
+    tensors.  A plan's tensors and sizes belong together and cannot be replaced."""
 
-    __slots__ = ("pos", "offsets", "tokens", "topk", "rows", "experts", "device", "_index", "_args")
+    __slots__ = ("_pos", "_offsets", "_tokens", "_topk", "_rows", "_experts", "_device", "_index")
+    pos, offsets, tokens, topk, rows, experts, device = (
+        property(operator.attrgetter("_" + name))
+        for name in ("pos", "offsets", "tokens", "topk", "rows", "experts", "device"))
 
     def __init__(self, pos: torch.Tensor, offsets: torch.Tensor):
         if pos.dim() != 2 or pos.dtype is not torch.int32 or not pos.is_contiguous() or \
@@ -57,14 +61,19 @@ class ExpertPlan:
                 not offsets.is_contiguous() or offsets.device != pos.device or not len(offsets):
             raise ValueError("pos must be a contiguous int32 [tokens, topk] tensor, offsets int32 "
                              "[experts + 1] on its device")
-        self._set(pos, offsets, *pos.shape, offsets.shape[0] - 1, pos.device, pos.data_ptr(),
-                  offsets.data_ptr())
+        self._set(pos, offsets, *pos.shape, offsets.shape[0] - 1, pos.device)
 
-    def _set(self, pos, offsets, tokens, topk, experts, device, p, o):
-        self.pos, self.offsets, self.device = pos, offsets, device
-        self.tokens, self.topk, self.rows, self.experts = tokens, topk, tokens * topk, experts
-        self._index, self._args = pos.get_device(), (p, o, experts)
+    def _set(self, pos, offsets, tokens, topk, experts, device):
+        self._pos, self._offsets, self._device = pos, offsets, device
+        self._tokens, self._topk, self._rows, self._experts = tokens, topk, tokens * topk, experts
+        self._index = pos.get_device()
         return self
+
+    @property
+    def _args(self):
+        """The sort's arguments of a library call (addresses taken now: a copied plan has tensors
+        of its own)."""
+        return self._pos.data_ptr(), self._offsets.data_ptr(), self._experts
 
 
 def _contiguous(t: torch.Tensor) -> torch.Tensor:
@@ -83,7 +92,7 @@ def _rows_of(t: torch.Tensor, plan: ExpertPlan, rows: int, name: str):
     if code is None or t.dim() != 2 or t.get_device() != plan._index:
         _check_type(t, name)
         _check_device(t, name)
-        raise ValueError(f"{name} must be [{rows}, dim] on {plan.device}, got {list(t.shape)} on {t.device}")
+        raise ValueError(f"{name} must be [{rows}, dim] on {plan._device}, got {list(t.shape)} on {t.device}")
     _check_device(t, name)
     n, dim = t.shape
     if n != rows:
@@ -92,8 +101,8 @@ def _rows_of(t: torch.Tensor, plan: ExpertPlan, rows: int, name: str):
 
 
 def _weights(w: torch.Tensor, plan: ExpertPlan, name: str) -> torch.Tensor:
-    if w.dtype is not torch.float32 or w.shape != plan.pos.shape or w.get_device() != plan._index:
-        raise ValueError(f"{name} must be float32 {list(plan.pos.shape)} on {plan.device}, got "
+    if w.dtype is not torch.float32 or w.shape != plan._pos.shape or w.get_device() != plan._index:
+        raise ValueError(f"{name} must be float32 {list(plan._pos.shape)} on {plan._device}, got "
                          f"{w.dtype} {list(w.shape)} on {w.device}")
     return w if w.is_contiguous() else w.contiguous()
 
@@ -118,25 +127,24 @@ def sort_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
     pos = ids.new_empty((T, k), dtype=torch.int32)
     offsets = ids.new_empty(max(num_experts, 0) + 1, dtype=torch.int32)
     work = _scratch(nbytes, ids.device) if nbytes else None
-    p, o = pos.data_ptr(), offsets.data_ptr()
-    _lib.call("mj_sort_experts", ids.data_ptr(), size, T * k, num_experts, p, o, _ptr(work), nbytes,
-              _stream(ids))
-    return object.__new__(ExpertPlan)._set(pos, offsets, T, k, num_experts, ids.device, p, o)
+    _lib.call("mj_sort_experts", ids.data_ptr(), size, T * k, num_experts, pos.data_ptr(),
+              offsets.data_ptr(), _ptr(work), nbytes, _stream(ids))
+    return object.__new__(ExpertPlan)._set(pos, offsets, T, k, num_experts, ids.device)
 
 
 def dispatch(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor | None = None):
     """xs [tokens * topk, dim] with xs[pos[t, j]] = x[t], zeros for dropped slots; with
     ``weights`` [tokens, topk] (Float32) also their sorted form: (xs, ws)."""
-    code, x, dim = _rows_of(x, plan, plan.tokens, "x")
-    xs = x.new_empty((plan.rows, dim))
+    code, x, dim = _rows_of(x, plan, plan._tokens, "x")
+    xs = x.new_empty((plan._rows, dim))
     if weights is None:
         _lib.call("mj_dispatch", code, x.data_ptr(), None, *plan._args, xs.data_ptr(), None,
-                  plan.tokens, plan.topk, dim, _stream(xs))
+                  plan._tokens, plan._topk, dim, _stream(xs))
         return xs
     weights = _weights(weights, plan, "weights")
-    ws = weights.new_empty(plan.rows)
+    ws = weights.new_empty(plan._rows)
     _lib.call("mj_dispatch", code, x.data_ptr(), weights.data_ptr(), *plan._args, xs.data_ptr(),
-              ws.data_ptr(), plan.tokens, plan.topk, dim, _stream(xs))
+              ws.data_ptr(), plan._tokens, plan._topk, dim, _stream(xs))
     return xs, ws
 
 
@@ -145,17 +153,17 @@ def combine(ys: torch.Tensor, weights: torch.Tensor | None, plan: ExpertPlan,
     """y[t] = the sum over j of weights[t, j] ys[pos[t, j]], in Float32 and rounded once to
     ``dtype`` (ys's by default; Float32 rows can give bfloat16); weights None: ones.  Dropped
     slots are left out, whatever they hold."""
-    code, ys, dim = _rows_of(ys, plan, plan.rows, "ys")
+    code, ys, dim = _rows_of(ys, plan, plan._rows, "ys")
     if weights is not None:
         weights = _weights(weights, plan, "weights")
     if dtype is None or dtype is ys.dtype:
-        to, y = code, ys.new_empty((plan.tokens, dim))
+        to, y = code, ys.new_empty((plan._tokens, dim))
     elif ys.dtype is torch.float32 and dtype is torch.bfloat16:
-        to, y = _lib.BF16, ys.new_empty((plan.tokens, dim), dtype=dtype)
+        to, y = _lib.BF16, ys.new_empty((plan._tokens, dim), dtype=dtype)
     else:
         raise TypeError(f"{ys.dtype} rows cannot be combined to {dtype}")
     _lib.call("mj_combine", code, to, ys.data_ptr(), _ptr(weights), *plan._args, y.data_ptr(),
-              plan.tokens, plan.topk, dim, _stream(ys))
+              plan._tokens, plan._topk, dim, _stream(ys))
     return y
 
 
@@ -169,12 +177,12 @@ def dispatch_backward(dxs: torch.Tensor, plan: ExpertPlan,
 def combine_backward(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan):
     """(dys, dweights) of ``combine``: dys[pos[t, j]] = weights[t, j] dy[t] and dweights[t, j]
     = <dy[t], ys[pos[t, j]]>, both 0 for dropped slots."""
-    code, dy, dim = _rows_of(dy, plan, plan.tokens, "dy")
-    ys = _like(ys, dy, (plan.rows, dim), "ys")
+    code, dy, dim = _rows_of(dy, plan, plan._tokens, "dy")
+    ys = _like(ys, dy, (plan._rows, dim), "ys")
     weights = _weights(weights, plan, "weights")
     dys, dw = torch.empty_like(ys), torch.empty_like(weights)
     _lib.call("mj_combine_backward", code, dy.data_ptr(), ys.data_ptr(), weights.data_ptr(),
-              *plan._args, dys.data_ptr(), dw.data_ptr(), plan.tokens, plan.topk, dim, _stream(ys))
+              *plan._args, dys.data_ptr(), dw.data_ptr(), plan._tokens, plan._topk, dim, _stream(ys))
     return dys, dw
 
 
@@ -193,7 +201,7 @@ class ExpertsSaved(NamedTuple):
 
 
 def _matrices(xs, plan, gate, up, down):
-    E = plan.experts
+    E = plan._experts
     if xs.dtype is not torch.bfloat16:
         raise TypeError(f"the experts' block takes bfloat16 rows, got {xs.dtype}")
     if gate.dim() != 3 or down.dim() != 3 or gate.shape[0] != E or down.shape[0] != E or \
@@ -205,12 +213,12 @@ def _matrices(xs, plan, gate, up, down):
 
 
 def _experts_mlp(xs, plan, gate, up, down, act, weights, train):
-    xs = _aligned(_rows_of(xs, plan, plan.rows, "xs")[1])
+    xs = _aligned(_rows_of(xs, plan, plan._rows, "xs")[1])
     gate, up, down = _matrices(xs, plan, gate, up, down)
     if weights is not None:
-        if weights.dtype is not torch.float32 or weights.shape != (plan.rows,) or \
+        if weights.dtype is not torch.float32 or weights.shape != (plan._rows,) or \
                 weights.device != xs.device:
-            raise ValueError(f"weights must be float32 [{plan.rows}] on {xs.device}")
+            raise ValueError(f"weights must be float32 [{plan._rows}] on {xs.device}")
         weights = _contiguous(weights)
     R, K = xs.shape
     I, H = gate.shape[1], down.shape[1]
@@ -218,7 +226,7 @@ def _experts_mlp(xs, plan, gate, up, down, act, weights, train):
     gu = _up16(4 * R * I) if train else 0
     buf = _scratch(2 * gu + _up16(2 * R * I), xs.device)
     g = buf.data_ptr()
-    _lib.call("mj_experts_mlp_bf16", xs.data_ptr(), plan.offsets.data_ptr(), plan.experts,
+    _lib.call("mj_experts_mlp_bf16", xs.data_ptr(), plan._offsets.data_ptr(), plan._experts,
               gate.data_ptr(), up.data_ptr(), down.data_ptr(), act, _ptr(weights), g + 2 * gu,
               g if train else None, g + gu if train else None, ys.data_ptr(), R, K, I, H, _stream(xs))
     return ys, ExpertsSaved(xs, plan, weights, gate, up, down, buf, act) if train else None
@@ -257,15 +265,15 @@ def experts_mlp_backward(dys: torch.Tensor, saved: ExpertsSaved):
     out += [torch.empty_like(t) for t in (s.gate, s.up, s.down)]
     dw, dots = None, 0
     if s.weights is not None:
-        dw = torch.empty(plan.pos.shape, dtype=torch.float32, device=dev)
+        dw = torch.empty(plan._pos.shape, dtype=torch.float32, device=dev)
         dots = 4 * _lib.load().mj_experts_mlp_dots(R, E, K, I, H)
     gu, db = _up16(4 * R * I), _up16(2 * R * I)
     work = _scratch(2 * db + dots, dev)  # dg, du, the parts of dweights
     g, dg = s.buf.data_ptr(), work.data_ptr()
-    _lib.call("mj_experts_mlp_backward_bf16", xs.data_ptr(), plan.offsets.data_ptr(), E,
+    _lib.call("mj_experts_mlp_backward_bf16", xs.data_ptr(), plan._offsets.data_ptr(), E,
               s.gate.data_ptr(), s.up.data_ptr(), s.down.data_ptr(), s.act, _ptr(s.weights),
               g + 2 * gu, g, g + gu, dys.data_ptr(), dg, dg + db, *[t.data_ptr() for t in out],
-              plan.pos.data_ptr(), R if dw is not None else 0, dg + 2 * db if dots else None,
+              plan._pos.data_ptr(), R if dw is not None else 0, dg + 2 * db if dots else None,
               _ptr(dw), R, K, I, H, _stream(xs))
     return (*out, dw)
 

@@ -151,20 +151,20 @@ class F8Linear:
 def dispatch_fp8(x: torch.Tensor, plan: ExpertPlan) -> tuple[torch.Tensor, torch.Tensor]:
     """(q [rows, K], scales [ceil(K / 128), rows]): each token's row quantized once and copied
     to its slots' sorted rows; zeros for dropped slots."""
-    code, x, K = _rows_of(x, plan, plan.tokens, "x")
+    code, x, K = _rows_of(x, plan, plan._tokens, "x")
     x = _aligned(x)
-    q = torch.empty((plan.rows, K), dtype=_F8, device=x.device)
-    scales = torch.empty((_blocks(K), plan.rows), dtype=torch.float32, device=x.device)
+    q = torch.empty((plan._rows, K), dtype=_F8, device=x.device)
+    scales = torch.empty((_blocks(K), plan._rows), dtype=torch.float32, device=x.device)
     _lib.call("mj_dispatch_f8", code, x.data_ptr(), *plan._args, q.data_ptr(), scales.data_ptr(),
-              plan.tokens, plan.topk, K, _stream(x))
+              plan._tokens, plan._topk, K, _stream(x))
     return q, scales
 
 
 def _expert_operands(q, scales, plan, Wq, Wscales, name):
     Wq, Wscales = _matrix(Wq, Wscales, 3, name)
     q, scales = _rows(q, scales, Wq.shape[2], "x")
-    if q.device != plan.device or q.shape[0] != plan.rows or Wq.shape[0] != plan.experts or Wq.device != q.device:
-        raise ValueError(f"{plan.rows} rows and {plan.experts} experts planned, got {q.shape[0]} rows "
+    if q.device != plan._device or q.shape[0] != plan._rows or Wq.shape[0] != plan._experts or Wq.device != q.device:
+        raise ValueError(f"{plan._rows} rows and {plan._experts} experts planned, got {q.shape[0]} rows "
                          f"and {Wq.shape[0]} matrices on {Wq.device}")
     return q, scales, Wq, Wscales
 
@@ -176,7 +176,7 @@ def experts_gemm_fp8(q: torch.Tensor, scales: torch.Tensor, plan: ExpertPlan, Wq
     q, scales, Wq, Wscales = _expert_operands(q, scales, plan, Wq, Wscales, "W")
     (R, K), (E, N, _) = q.shape, Wq.shape
     y = torch.empty((R, N), dtype=torch.float32, device=q.device)
-    _lib.call("mj_experts_gemm_f8", q.data_ptr(), scales.data_ptr(), plan.offsets.data_ptr(), E,
+    _lib.call("mj_experts_gemm_f8", q.data_ptr(), scales.data_ptr(), plan._offsets.data_ptr(), E,
               Wq.data_ptr(), Wscales.data_ptr(), y.data_ptr(), R, N, K, _stream(q))
     return y
 
@@ -195,7 +195,7 @@ def experts_gate_fp8(q: torch.Tensor, scales: torch.Tensor, plan: ExpertPlan, ga
     hs = torch.empty((_blocks(I), R), dtype=torch.float32, device=q.device)
     nbytes = _work("mj_experts_gate_f8_work_bytes", R, E, I, K)
     work = _scratch(nbytes, q.device) if nbytes else None
-    _lib.call("mj_experts_gate_f8", q.data_ptr(), scales.data_ptr(), plan.offsets.data_ptr(), E,
+    _lib.call("mj_experts_gate_f8", q.data_ptr(), scales.data_ptr(), plan._offsets.data_ptr(), E,
               gate.data_ptr(), gate_scales.data_ptr(), up.data_ptr(), up_scales.data_ptr(), act,
               hq.data_ptr(), hs.data_ptr(), R, I, K, _ptr(work), nbytes, _stream(q))
     return hq, hs
