@@ -117,7 +117,8 @@ def gemm_fp8_nt(q: torch.Tensor, scales: torch.Tensor, Wq: torch.Tensor, Wscales
 
 class F8Linear:
     """F8Linear(q, scales, bias, act): y = act(x W^T + bias) in bfloat16 for x [..., K],
-    bfloat16 or Float32, quantized in the call; q [N, K] float8_e4m3fn with its block scales."""
+    bfloat16 or Float32, quantized in the call; q [N, K] float8_e4m3fn with its block scales.
+    q, scales and bias can be replaced by others of their shapes on the same device."""
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,
                  act: int = _lib.EPI_NONE):
@@ -125,6 +126,21 @@ class F8Linear:
         self.out_features, self.in_features = self.q.shape
         self.bias = _bias(bias, self.out_features, self.q.device)
         self.act = act
+
+    def __setattr__(self, name, value):
+        held = self.__dict__
+        if name in held:  # (a forward goes by the constructor's checks and sizes)
+            if name in ("in_features", "out_features"):
+                raise AttributeError(f"{name} is q's")
+            if name in ("q", "scales") and value.shape != held[name].shape:
+                raise ValueError(f"{name} must be {list(held[name].shape)}, got {list(value.shape)}")
+            if name == "q":
+                value, _ = _matrix(value, self.scales, 2, name)
+            elif name == "scales":
+                _, value = _matrix(self.q, value, 2, "q")
+            elif name == "bias":
+                value = _bias(value, self.out_features, self.q.device)
+        held[name] = value
 
     @classmethod
     def from_float(cls, W: torch.Tensor, bias: torch.Tensor | None = None,
