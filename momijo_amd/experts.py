@@ -50,10 +50,10 @@ class ExpertPlan:
     dropped slot's.  A plan of other entries gives meaningless rows, but no access outside the
     tensors.  A plan's tensors and sizes belong together and cannot be replaced."""
 
-    __slots__ = ("_pos", "_offsets", "_tokens", "_topk", "_rows", "_experts", "_device", "_index")
+    __slots__ = ("_pos", "_offsets", "_tokens", "_topk", "_rows", "_experts", "_index")
     pos, offsets, tokens, topk, rows, experts, device = (
-        property(operator.attrgetter("_" + name))
-        for name in ("pos", "offsets", "tokens", "topk", "rows", "experts", "device"))
+        property(operator.attrgetter(name))
+        for name in ("_pos", "_offsets", "_tokens", "_topk", "_rows", "_experts", "_pos.device"))
 
     def __init__(self, pos: torch.Tensor, offsets: torch.Tensor):
         if pos.dim() != 2 or pos.dtype is not torch.int32 or not pos.is_contiguous() or \
@@ -61,18 +61,19 @@ class ExpertPlan:
                 not offsets.is_contiguous() or offsets.device != pos.device or not len(offsets):
             raise ValueError("pos must be a contiguous int32 [tokens, topk] tensor, offsets int32 "
                              "[experts + 1] on its device")
-        self._set(pos, offsets, *pos.shape, offsets.shape[0] - 1, pos.device)
+        self._set(pos, offsets, *pos.shape, offsets.shape[0] - 1, pos.get_device())
 
-    def _set(self, pos, offsets, tokens, topk, experts, device):
-        self._pos, self._offsets, self._device = pos, offsets, device
-        self._tokens, self._topk, self._rows, self._experts = tokens, topk, tokens * topk, experts
-        self._index = pos.get_device()
+    def _set(self, pos, offsets, tokens, topk, experts, index):
+        self._pos, self._offsets, self._experts, self._index = pos, offsets, experts, index
+        self._tokens, self._topk, self._rows = tokens, topk, tokens * topk
         return self
+
+    def __reduce__(self):
+        return ExpertPlan, (self._pos, self._offsets)
 
     @property
     def _args(self):
-        """The sort's arguments of a library call (addresses taken now: a copied plan has tensors
-        of its own)."""
+        """The plan's part of a library call's arguments, with the addresses of now."""
         return self._pos.data_ptr(), self._offsets.data_ptr(), self._experts
 
 
@@ -88,12 +89,13 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _rows_of(t: torch.Tensor, plan: ExpertPlan, rows: int, name: str):
     """(type code, t contiguous, its width) of a [rows, dim] operand on the plan's device."""
-    code = _DTYPES.get(t.dtype)
-    if code is None or t.dim() != 2 or t.get_device() != plan._index:
+    code, index = _DTYPES.get(t.dtype), t.get_device()
+    if code is None or t.dim() != 2 or index != plan._index:
         _check_type(t, name)
         _check_device(t, name)
-        raise ValueError(f"{name} must be [{rows}, dim] on {plan._device}, got {list(t.shape)} on {t.device}")
-    _check_device(t, name)
+        raise ValueError(f"{name} must be [{rows}, dim] on {plan.device}, got {list(t.shape)} on {t.device}")
+    if index != torch._C._cuda_getDevice():
+        _check_device(t, name)
     n, dim = t.shape
     if n != rows:
         raise ValueError(f"{name} must be [{rows}, dim], got {list(t.shape)}")
@@ -102,7 +104,7 @@ def _rows_of(t: torch.Tensor, plan: ExpertPlan, rows: int, name: str):
 
 def _weights(w: torch.Tensor, plan: ExpertPlan, name: str) -> torch.Tensor:
     if w.dtype is not torch.float32 or w.shape != plan._pos.shape or w.get_device() != plan._index:
-        raise ValueError(f"{name} must be float32 {list(plan._pos.shape)} on {plan._device}, got "
+        raise ValueError(f"{name} must be float32 {list(plan._pos.shape)} on {plan.device}, got "
                          f"{w.dtype} {list(w.shape)} on {w.device}")
     return w if w.is_contiguous() else w.contiguous()
 
@@ -127,9 +129,10 @@ def sort_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
     pos = ids.new_empty((T, k), dtype=torch.int32)
     offsets = ids.new_empty(max(num_experts, 0) + 1, dtype=torch.int32)
     work = _scratch(nbytes, ids.device) if nbytes else None
+    index = ids.get_device()
     _lib.call("mj_sort_experts", ids.data_ptr(), size, T * k, num_experts, pos.data_ptr(),
-              offsets.data_ptr(), _ptr(work), nbytes, _stream(ids))
-    return object.__new__(ExpertPlan)._set(pos, offsets, T, k, num_experts, ids.device)
+              offsets.data_ptr(), _ptr(work), nbytes, torch._C._cuda_getCurrentRawStream(index))
+    return object.__new__(ExpertPlan)._set(pos, offsets, T, k, num_experts, index)
 
 
 def dispatch(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor | None = None):

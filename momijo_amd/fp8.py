@@ -179,7 +179,7 @@ def dispatch_fp8(x: torch.Tensor, plan: ExpertPlan) -> tuple[torch.Tensor, torch
 def _expert_operands(q, scales, plan, Wq, Wscales, name):
     Wq, Wscales = _matrix(Wq, Wscales, 3, name)
     q, scales = _rows(q, scales, Wq.shape[2], "x")
-    if q.device != plan._device or q.shape[0] != plan._rows or Wq.shape[0] != plan._experts or Wq.device != q.device:
+    if q.get_device() != plan._index or q.shape[0] != plan._rows or Wq.shape[0] != plan._experts or Wq.device != q.device:
         raise ValueError(f"{plan._rows} rows and {plan._experts} experts planned, got {q.shape[0]} rows "
                          f"and {Wq.shape[0]} matrices on {Wq.device}")
     return q, scales, Wq, Wscales

@@ -39,6 +39,16 @@ def test_a_copied_plan_has_its_own_tensors(again):
     assert _given(plan) and _given(twin)
     assert torch.equal(twin.pos, plan.pos) and torch.equal(twin.offsets, plan.offsets)
     assert (twin.tokens, twin.topk, twin.rows, twin.experts) == (4, 2, 8, 3) and twin.device == plan.device
+    assert twin._index == twin.pos.get_device()
+
+
+def test_a_plan_loaded_to_another_device(tmp_path):
+    """The device of a plan's tensors is the one that its rows are checked against."""
+    plan = _plan()
+    plan._index = 0  # as of a plan made on the GPU
+    torch.save(plan, tmp_path / "plan")
+    twin = torch.load(tmp_path / "plan", map_location="cpu", weights_only=False)
+    assert twin._index == -1 and _given(twin)
 
 
 def test_a_plan_follows_its_tensors():
