@@ -94,7 +94,7 @@ def _rows_of(t: torch.Tensor, plan: ExpertPlan, rows: int, name: str):
         _check_type(t, name)
         _check_device(t, name)
         raise ValueError(f"{name} must be [{rows}, dim] on {plan.device}, got {list(t.shape)} on {t.device}")
-    if index != torch._C._cuda_getDevice():
+    if index < 0 or index != torch._C._cuda_getDevice():
         _check_device(t, name)
     n, dim = t.shape
     if n != rows:
