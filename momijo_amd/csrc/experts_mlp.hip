@@ -162,7 +162,8 @@ template <bool GATE, int MB, int NW>
 __global__ __launch_bounds__(NW * 64) void experts_skinny_kernel(ExpertSkinny a) {
   __shared__ SkinnySums<GATE, MB, NW> sums;
   ExpertTile t;
-  if (!expert_tile<false>(a.offsets, a.experts, a.rows, a.tail, 16 * MB, a.tiles_n, blockIdx.x, t)) return;
+  const int bid = (int)grid_block<NW * 64>();  // (below 2^30: 2^18 column tiles of 2048 segments)
+  if (!expert_tile<false>(a.offsets, a.experts, a.rows, a.tail, 16 * MB, a.tiles_n, bid, t)) return;
   SkinnyArgs p = a.p;
   const int64_t row = t.row0 + t.m * 16 * MB, weights = (int64_t)p.N * p.K;
   p.M = t.rows - t.m * 16 * MB;
@@ -353,8 +354,7 @@ hipError_t launch_few(const ExpertMlp &q, ExpertSkinny &a, hipStream_t stream) {
   a.tiles_n = (a.p.N + 15) / 16;
   const int64_t grid = a.tiles_n * expert_tiles_most(q.R, q.E + a.tail, 16);
   if (grid == 0) return hipSuccess;
-  if (!grid_fits(grid, 512)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((experts_skinny_kernel<GATE, 1, 8>), dim3((unsigned)grid), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL((experts_skinny_kernel<GATE, 1, 8>), grid_rows<512>(grid), dim3(512), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -665,8 +665,9 @@ __global__ __launch_bounds__(NW * 64) void f8_skinny_kernel(F8Tiles args) {
   int n0;
   if constexpr (EX) {
     ExpertTile t;
+    const int bid = (int)grid_block<NW * 64>();  // (below 2^30: 2^18 column tiles of 2048 segments)
     if (!expert_tile<false>(args.p.offsets, args.p.experts, (int)args.p.M, args.p.tail, 16 * MB, args.tiles_n,
-                            blockIdx.x, t))
+                            bid, t))
       return;
     f8_operands(args.p, t.expert, t.row0 + t.m * 16 * MB, t.rows - t.m * 16 * MB, p);
     n0 = t.n * COLS;
@@ -828,9 +829,8 @@ hipError_t launch_pipe(F8Tiles a, int64_t grid, hipStream_t stream) {
 
 template <int OUT, int MB, int NW, int U, bool EX, int XT>
 hipError_t launch_skinny(const F8Tiles &a, int64_t grid, hipStream_t stream) {
-  if (!grid_fits(grid, NW * 64)) return hipErrorInvalidValue;
   const size_t lds = XT == X_F8 ? 0 : few_rows_lds(a.p.M, a.p.K);
-  hipLaunchKernelGGL((f8_skinny_kernel<OUT, MB, NW, U, EX, XT>), dim3((unsigned)grid), dim3(NW * 64), lds, stream,
+  hipLaunchKernelGGL((f8_skinny_kernel<OUT, MB, NW, U, EX, XT>), grid_rows<NW * 64>(grid), dim3(NW * 64), lds, stream,
                      a);
   return hipGetLastError();
 }
