@@ -260,8 +260,7 @@ bool cuts(int tile, int64_t stages) { return tile == T_256 && stages >= 48; }
 double rows_time_us(int tile, int out, double tiles, int64_t stages) {
   if (!cuts(tile, stages)) return expert_time_us(tile, out, tiles, stages);
   const double rest = tiles - std::floor(tiles / kTileRound) * kTileRound;
-  if (rest > CUT_REST_MOST) return expert_time_us(tile, out, tiles, stages) + 3.0;
-  if (rest < 1) return expert_time_us(tile, out, tiles, stages) + 3.0;
+  if (rest < 1 || rest > CUT_REST_MOST) return expert_time_us(tile, out, tiles, stages) + 3.0;
   return expert_time_us(tile, out, tiles - rest, stages) + expert_time_us(T_128, out, 4 * CUT_REST_MOST, stages);
 }
 

@@ -1001,9 +1001,11 @@ bool gemm_f8_fuses(const F8Product &q) {
 // between others) does once: few blocks, fewer where a CU has several workgroups.  11008 x 4096
 // columns, one row 11.8 us, 12.8 with that launch, 4 rows 15.4 and 14.1; 4096 x 4096 4 rows 7.7
 // and 8.1, 8 rows 10.1 and 8.3; 1040 x 3000 8 rows 4.1 and 5.0, 16 rows 5.4 and 5.1.
+constexpr int64_t kQuantizeBlocks = 192;
+static_assert(few_rows_lds(1, 128 * kQuantizeBlocks) + sizeof(float) * 16 * 16 * 17 <= 64 * 1024,
+              "x's blocks and the sums of 16 waves");
 bool gemm_f8_quantizes(int64_t M, int64_t N, int64_t K) {
-  return M <= 16 && few_rows_lds(M, K) <= 46 * 1024 &&
-         M * ((K + 127) / 128) * ((N + 4095) / 4096) <= 192;
+  return M <= 16 && N > 0 && M * ((K + 127) / 128) * ((N + 4095) / 4096) <= kQuantizeBlocks;
 }
 
 int64_t gemm_f8_part_floats(int64_t M, int64_t N, int64_t K) {
