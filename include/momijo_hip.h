@@ -696,10 +696,12 @@ const char *mj_experts_mlp_kernel(int64_t R, int64_t experts, int64_t K, int64_t
  * row (x) or 128 x 128 elements (W), for inference (no reference counterpart).  A block of
  * largest magnitude m is quantized with a = max(m, 2^-100): scale a * (1 / 448), values
  * e4m3(v * (448 * (1 / a))) to the nearest even, each operation rounded to fp32.  A NaN stays a
- * NaN; an infinity becomes one, with an infinite scale.  Widths K are multiples of 16,
- * widths below 2^22, rows at most 2^31 - 1024, arrays of values 16-byte aligned.  Scales of
- * x lie block by block, [ceil(K / 128)][rows], those of W as [ceil(N / 128)][ceil(K / 128)].
- * Scratch memory is the caller's. */
+ * NaN; an infinity becomes one, with an infinite scale.  A block's sum is multiplied by its two
+ * scales' product, rounded to fp32: where the blocks' largest magnitudes multiply to less than
+ * 2^-108 it loses bits, and from 2^145 on it is infinite.  Widths K are multiples of 16, widths
+ * below 2^22, rows at most 2^31 - 1024, arrays of values 16-byte aligned.  Scales of x lie block
+ * by block, [ceil(K / 128)][rows], those of W as [ceil(N / 128)][ceil(K / 128)].  Scratch memory
+ * is the caller's. */
 int32_t mj_quantize_rows_f8(int32_t dtype, const void *x, uint8_t *q, float *scales, int64_t rows, int64_t K,
                             void *stream);
 int32_t mj_quantize_blocks_f8(int32_t dtype, const void *W, uint8_t *q, float *scales, int64_t mats, int64_t N,

@@ -12,7 +12,8 @@
 // and dispatch's gradient is combine without weights.  All of it is bound by memory:
 // going by tokens, each row of x and dy is read once and written k times, each row of ys
 // read once.  Sums run in fp32 in the order of j (dot products: in a fixed order), so
-// the same inputs give the same bits; there are no atomics.
+// the same inputs give the same bits; the only atomics are the sort's counts in LDS, whole
+// numbers whose order changes nothing.
 #include <algorithm>
 #include <atomic>
 
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(256) void combine_kernel(ExpertRows a) {
 // One workgroup a token (one wave where a row is short), four slots at a time: for each the row
 // of dys and the product of dy with the row of ys, its lanes' and waves' sums added in order.
 // dy comes from the caches after the first four.  8192 tokens, 8 experts each, 4096 bf16: 236
-// us, 4.8 TB/s (two reads and a write an element of the sorted rows).
+// us, 4.8 TB/s (a read and a write an element of the sorted rows, and dy once).
 constexpr int kDotSlots = 4;
 
 template <bool BF, int NW, bool NT>

@@ -81,7 +81,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(F8Rows a) {
 
 // One workgroup a 128 x 128 block of one of `mats` matrices [N, K]: 16 lanes a row, 8 rows
 // of each thread in registers, so the matrix is read once.  Not in a model's step: weights
-// are quantized when they are loaded.
+// are quantized when they are loaded.  11008 x 4096 bf16 25 us (5.4 TB/s), 8 x 5504 x 4096 102
+// (5.3), fp32 157 (5.8).
 template <bool BF>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(F8Blocks a) {
   __shared__ float red[4];

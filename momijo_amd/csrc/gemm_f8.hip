@@ -425,7 +425,7 @@ __global__ __launch_bounds__(NW * 64, 2) void f8_tile_kernel(F8Tiles args) {
   o.init(K / 2, wave, lane);
   const int kc = o.kc * 2;  // first byte of this lane's chunk
   // Load i of x or of the weights covers tile rows (i NW + wave) 8 on, at the same offsets in
-  // both; of gate/up tiles, whose rows are 4 NW of the gate's, then 4 NW of the up projection's,
+  // both; of gate/up tiles, whose rows are 8 NW of the gate's, then 8 NW of the up projection's,
   // in turn, i / 2 counts in each.  Rows past the edge lie past the resource's end and read
   // zeros, as do chunks past K.
   uint32_t off[4];
@@ -605,7 +605,9 @@ __global__ __launch_bounds__(256) void f8_sum_kernel(F8Product q, int splits) {
 // weight rows (gate/up: of each) and deals the K blocks to its waves in turn; a lane's 32
 // bytes of a row's 128 are its fragment as they are.  A wave has U blocks' loads in
 // flight.  The waves' sums are added in wave order.  One row, 4096 x 11008 columns, x quantized
-// in it: 9.7 us (4.7 TB/s); 96 rows of 8 experts, 4096 and 11008 wide: h 158 (4.6), y 90 (4.0).
+// in it: 11.8 us (3.8 TB/s) where the weights come from memory, 8.8 (5.1) where the last-level
+// cache holds them, launch behind launch; 96 rows of 8 experts, 4096 and 11008 wide: h 158 (4.6), y
+// 90 (4.0).
 //
 // XT: x comes quantized (X_F8), or in its own type: then each workgroup quantizes it into
 // LDS (32 lanes a block) while its first weights are on their way, which saves a launch.
@@ -838,8 +840,8 @@ hipError_t launch_skinny(const F8Tiles &a, int64_t grid, hipStream_t stream) {
 // At most 16 rows.  The number of waves orders the sums, so it goes by the sizes alone and a
 // product has the same bits whether x was quantized before or by the workgroups.  Those
 // (where gemm_f8_quantizes says) hold one block in flight, on 16 waves where there is much to
-// quantize or K is long (one row, 4096 x 11008: 14.1 us, 17.1 on 8; 11008 x 4096: 12.7 and
-// 11.8).  With x quantized before: as many blocks in flight as a wave has, up to three (16
+// quantize or K is long (one row, K = 11008, 4096 columns: 14.1 us, 17.1 on 8; K = 4096, 11008
+// columns: 12.7 and 11.8).  With x quantized before: as many blocks in flight as a wave has, up to three (16
 // rows, us of both launches with 8 waves and one block, 16 and two, 16 and three: K = 1040,
 // 3000 columns 5.1, 5.7, 6.2; 4096, 11008 17.4, 16.8, -; 11008, 4096 18.2, 17.8, 17.6).
 template <int XT>
@@ -998,9 +1000,9 @@ bool gemm_f8_fuses(const F8Product &q) {
 }
 
 // Every workgroup of the few-row kernel quantizes all of x, which a launch of its own (1.7 us
-// between others) does once: few blocks, fewer where a CU has several workgroups.  11008 x 4096
-// columns, one row 11.8 us, 12.8 with that launch, 4 rows 15.4 and 14.1; 4096 x 4096 4 rows 7.7
-// and 8.1, 8 rows 10.1 and 8.3; 1040 x 3000 8 rows 4.1 and 5.0, 16 rows 5.4 and 5.1.
+// between others) does once: few blocks, fewer where a CU has several workgroups.  K =
+// 4096, 11008 columns, one row 11.8 us, 12.8 with that launch, 4 rows 15.4 and 14.1; 4096, 4096 4
+// rows 7.7 and 8.1, 8 rows 10.1 and 8.3; 1040, 3000 8 rows 4.1 and 5.0, 16 rows 5.4 and 5.1.
 constexpr int64_t kQuantizeBlocks = 192;
 static_assert(few_rows_lds(1, 128 * kQuantizeBlocks) + sizeof(float) * 16 * 16 * 17 <= 64 * 1024,
               "x's blocks and the sums of 16 waves");

@@ -179,7 +179,7 @@ def dispatch_backward(dxs: torch.Tensor, plan: ExpertPlan,
 
 def combine_backward(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan):
     """(dys, dweights) of ``combine``: dys[pos[t, j]] = weights[t, j] dy[t] and dweights[t, j]
-    = <dy[t], ys[pos[t, j]]>, both 0 for dropped slots."""
+    = <dy[t], ys[pos[t, j]]>, both 0 for dropped slots.  dy is of ys's type, and so is dys."""
     code, dy, dim = _rows_of(dy, plan, plan._tokens, "dy")
     ys = _like(ys, dy, (plan._rows, dim), "ys")
     weights = _weights(weights, plan, "weights")

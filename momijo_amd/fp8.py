@@ -5,7 +5,9 @@ activations are quantized at call time, a scale for each 128 features of a row.
 A block of largest magnitude m is quantized with a = max(m, 2^-100): scale
 a * (1 / 448), values e4m3(v * (448 * (1 / a))) to the nearest even, each operation
 rounded to Float32.  Products of a block
-are summed on the matrix cores and added up in Float32 with their scales.
+are summed on the matrix cores, multiplied by the product of their two scales and added
+up in Float32; blocks whose largest magnitudes multiply to less than 2^-108 or to 2^145
+and more leave Float32's range there.
 
 Values are torch.float8_e4m3fn.  Scales of rows lie block by block, Float32
 [ceil(K / 128), rows]; those of a matrix are [ceil(N / 128), ceil(K / 128)].  K is a
