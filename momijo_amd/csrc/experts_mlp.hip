@@ -9,6 +9,9 @@
 // rows, the backward needs no y (dw comes from the fp32 g and u, with the error of an fp32
 // sum and not of a rounded y), and dy's rows are copies of the tokens' gradients.  y and dx
 // stay in fp32: a token's rows are still to be added, and rounded once then.
+// h, dg and du are rounded to bf16, as in the block without experts: they are the next products'
+// operands, and the matrix cores take bf16 at full rate (outputs off by 0.0023 against 64 bits;
+// 0.0017 with these in fp32).
 //
 // The tiles are the gated block's (mlp_tile.h).  What differs is where a tile's operands
 // are: the rows of all experts run as one launch, each workgroup finding its expert from
